@@ -14,6 +14,7 @@ from .ops import (
     device_info, init, q3_pack, bcq_pack, quantize_4bit,
     static_scaled_int8_quant, dynamic_scaled_int8_quant,
     gemv_fp16, gemv_int8, gemv_int4, mxfp4_qdq,
+    prompt_attention, paged_attention, cache_write, cache_step, cache_compact,
 )
 
 __all__ = [
@@ -23,4 +24,5 @@ __all__ = [
     "device_info", "init", "q3_pack", "bcq_pack", "quantize_4bit",
     "static_scaled_int8_quant", "dynamic_scaled_int8_quant",
     "gemv_fp16", "gemv_int8", "gemv_int4", "mxfp4_qdq",
+    "prompt_attention", "paged_attention", "cache_write", "cache_step", "cache_compact",
 ]

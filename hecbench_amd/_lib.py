@@ -52,6 +52,14 @@ _SIGNATURES = {
     "hq_gemv_int4": (_c.c_int, [_c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_int, _c.c_int, _c.c_float,
                                 _c.c_float, _c.c_void_p]),
     "hq_mxfp4_qdq": (_c.c_int, [_c.c_void_p, _c.c_void_p, _c.c_int64, _c.c_int, _c.c_void_p]),
+    "hq_prompt_attention": (_c.c_int, [_c.c_void_p] * 4 + [_c.c_int] + [_c.c_void_p] * 2 + [_c.c_int] + [_c.c_int64] * 2 + [_c.c_int] * 3
+                            + [_c.c_int64] * 3 + [_c.c_float, _c.c_int, _c.c_void_p]),
+    "hq_paged_attention": (_c.c_int, [_c.c_void_p] * 4 + [_c.c_int] + [_c.c_void_p] * 4 + [_c.c_int] * 8
+                           + [_c.c_int64, _c.c_float, _c.c_void_p]),
+    "hq_cache_write": (_c.c_int, [_c.c_void_p] * 4 + [_c.c_int] + [_c.c_void_p] * 3 + [_c.c_int, _c.c_int64] + [_c.c_int] * 5
+                       + [_c.c_int64] * 2 + [_c.c_void_p]),
+    "hq_cache_step": (_c.c_int, [_c.c_void_p, _c.c_int, _c.c_int64] + [_c.c_void_p] * 10 + [_c.c_int] * 4 + [_c.c_void_p]),
+    "hq_cache_compact": (_c.c_int, [_c.c_void_p, _c.c_int, _c.c_int64] + [_c.c_void_p] * 5 + [_c.c_int] * 3 + [_c.c_void_p]),
     "hq_probe_stream": (_c.c_int, [_c.c_int, _c.c_void_p, _c.c_void_p, _c.c_int64, _c.c_void_p]),
     "hq_probe_gather16": (_c.c_int, [_c.c_void_p, _c.c_int64, _c.c_int64, _c.c_void_p, _c.c_void_p]),
     "hq_probe_gather16_count": (_c.c_int64, [_c.c_int64]),

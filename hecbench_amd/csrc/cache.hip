@@ -1,0 +1,403 @@
+// The paged key / value cache: tokens into pages, the page tables from one token to the next, live pages to the front.
+#include <climits>
+
+#include "hq_internal.h"
+
+namespace {
+
+constexpr int kThreads = 256;
+
+// ---- tokens into pages ------------------------------------------------------------------------------------------------
+struct WriteArgs {
+  const hq_u4v *k, *v;
+  hq_u4v *kp, *vp;
+  const int *table, *starts, *cu;
+  int64_t ks, vs;  // 16-byte pieces from one token to the next
+  int rows, tokens, width, pages, page_log, kv_heads, pieces;  // pieces of one head's row
+};
+
+// The first i with bounds[i + 1] > t, n if there is none: a wave halves the range sixty-four-fold a step.
+__device__ __forceinline__ int find_row(const int* bounds, int n, int t) {
+  const int lane = threadIdx.x & 63;
+  int lo = 0;
+  while (n > 0) {
+    const int step = (n + 63) >> 6;
+    const int at = lo + min((lane + 1) * step, n);
+    const int below = __popcll(__ballot(bounds[at] <= t));
+    if (below == 64) return lo + n;
+    lo += below * step;
+    n = min(step, n - below * step) - 1;
+  }
+  return lo;
+}
+
+// One wave a token, keys and values.  Bound by the copy; a short call by three loads one after the other (bounds, table, nothing
+// of which the token's own data wait for) and the launch.
+__global__ __launch_bounds__(kThreads) void write_kernel(WriteArgs a) {
+  const int t = blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if (t >= a.tokens) return;
+  const int row = find_row(a.cu, a.rows, t);
+  if (row >= a.rows || t < a.cu[row]) return;
+  const int64_t p = (int64_t)a.starts[row] + (t - a.cu[row]);
+  if (p < 0 || p >= (int64_t)a.width << a.page_log) return;
+  const int page = a.table[(int64_t)row * a.width + (p >> a.page_log)], at = (int)p & ((1 << a.page_log) - 1);
+  if ((unsigned)page >= (unsigned)a.pages) return;
+  const int n = a.kv_heads * a.pieces;
+  for (int i = lane; i < n; i += 64) {
+    const int head = i / a.pieces, piece = i % a.pieces;
+    const int64_t to = ((((int64_t)page * a.kv_heads + head) << a.page_log) + at) * a.pieces + piece;
+    a.kp[to] = a.k[t * a.ks + i];
+    a.vp[to] = a.v[t * a.vs + i];
+  }
+}
+
+// ---- one step of the page tables ----------------------------------------------------------------------------------------
+struct StepArgs {
+  hq_u4v* pool;
+  const int *table, *lengths, *refs, *parent, *add;
+  int *table_out, *lengths_out, *refs_out, *starts_out, *missing;
+  int *need, *source;    // of each row: pages that it asks for; the half-filled page that it copies, -1 if none
+  int *copies, *ncopies; // {source, target} of the pages to be copied
+  int* list;             // pages handed out
+  int* change;           // of each page's count; zero between calls
+  unsigned* arrived;
+  int64_t page_pieces;   // 16-byte pieces of a page
+  int planes, rows, width, pages, page;
+};
+
+__device__ __forceinline__ void put(int* p, int v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ __forceinline__ int get(const int* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+
+// Sum over the workgroup of the values of the threads before this one, and of all.
+__device__ __forceinline__ int block_scan(int v, int* parts, int* total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int sum = v;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int u = __shfl_up(sum, d);
+    if (lane >= d) sum += u;
+  }
+  __syncthreads();
+  if (lane == 63) parts[wave] = sum;
+  __syncthreads();
+  int before = 0, all = 0;
+  for (int w = 0; w < (int)blockDim.x / 64; ++w) {
+    before += w < wave ? parts[w] : 0;
+    all += parts[w];
+  }
+  *total = all;
+  return before + sum - v;
+}
+
+// One workgroup a row: what it inherits, and how the pages' counts change by it; the last one to arrive hands out pages.
+__global__ __launch_bounds__(kThreads) void step_kernel(StepArgs a) {
+  extern __shared__ int off[];
+  __shared__ int parts[kThreads / 64], flag;
+  const int s = blockIdx.x, tid = threadIdx.x;
+  const int cap = a.width * a.page;
+  auto length_of = [&](int r) { return min(max(a.lengths[r], 0), cap); };
+  auto start_of = [&](int r) {
+    const int p = a.parent[r];
+    return p >= 0 && p < a.rows ? length_of(p) : 0;
+  };
+  auto end_of = [&](int r, int start) { return (int)min((int64_t)start + max(a.add[r], 0), (int64_t)cap); };
+  if (s < a.rows) {
+    const int p = a.parent[s];
+    const bool alive = p >= 0 && p < a.rows;
+    if (tid == 0) flag = 0;
+    __syncthreads();
+    if (alive)
+      for (int i = tid; i < s; i += kThreads)
+        if (a.parent[i] == p) flag = 1;
+    __syncthreads();
+    const bool keeps = !flag;
+    const int start = start_of(s), full = start / a.page, used = (start + a.page - 1) / a.page, end = end_of(s, start);
+    const int last = (end + a.page - 1) / a.page, mine = (length_of(s) + a.page - 1) / a.page;
+    const int tail = used > full ? a.table[(int64_t)p * a.width + full] : -1;
+    const bool copies = alive && used > full && !keeps && (unsigned)tail < (unsigned)a.pages;
+    const int from = copies ? full : used;  // the entries from here to `last` are new
+    const bool same = p == s && keeps;
+    for (int j = tid; j < a.width; j += kThreads) {
+      if (!same && j < mine) {
+        const int old = a.table[(int64_t)s * a.width + j];
+        if ((unsigned)old < (unsigned)a.pages) atomicSub(a.change + old, 1);
+      }
+      int e = -1;
+      if (j < from) {
+        e = a.table[(int64_t)p * a.width + j];
+        if ((unsigned)e >= (unsigned)a.pages) e = -1;
+        else if (!same) atomicAdd(a.change + e, 1);
+      }
+      if (j < from || j >= max(last, used)) a.table_out[(int64_t)s * a.width + j] = e;
+    }
+    if (tid == 0) {
+      put(a.need + s, max(last, used) - from);
+      put(a.source + s, copies ? tail : -1);
+    }
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  if (tid == 0) flag = __hip_atomic_fetch_add(a.arrived, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1;
+  __syncthreads();
+  if (!flag) return;
+
+  // where each row's requests begin in the order of all
+  int total = 0;
+  for (int r0 = 0; r0 < a.rows; r0 += kThreads) {
+    const int r = r0 + tid;
+    int all;
+    const int before = block_scan(r < a.rows ? get(a.need + r) : 0, parts, &all);
+    if (r < a.rows) off[r] = total + before;
+    total += all;
+  }
+  // free pages, lowest first, to the requests in their order
+  int nfree = 0;
+  for (int i0 = 0; i0 < a.pages; i0 += kThreads) {
+    const int i = i0 + tid;
+    int count = 1;
+    if (i < a.pages) {
+      const int d = get(a.change + i);
+      count = a.refs[i] + d;
+      if (d) put(a.change + i, 0);
+    }
+    const bool free = count <= 0;
+    int all;
+    const int rank = nfree + block_scan(free, parts, &all);
+    if (i < a.pages) {
+      const bool taken = free && rank < total;
+      a.refs_out[i] = taken ? 1 : count;
+      if (taken) put(a.list + rank, i);
+    }
+    nfree += all;
+  }
+  if (tid == 0) {
+    *a.missing = max(total - nfree, 0);
+    put((int*)a.arrived, 0);
+    flag = 0;
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  for (int r = tid; r < a.rows; r += kThreads) {
+    const int start = start_of(r), source = get(a.source + r), n = get(a.need + r);
+    const int from = source >= 0 ? start / a.page : (start + a.page - 1) / a.page;
+    int end = end_of(r, start);
+    if (off[r] + n > nfree) end = min(end, (from + max(nfree - off[r], 0)) * a.page);
+    a.lengths_out[r] = end;
+    a.starts_out[r] = min(start, end);
+    if (source >= 0 && off[r] < nfree) {
+      const int at = atomicAdd(&flag, 1);
+      a.copies[2 * at] = source;
+      a.copies[2 * at + 1] = get(a.list + off[r]);
+    }
+  }
+  for (int x = tid; x < total; x += kThreads) {
+    int lo = 0, hi = a.rows - 1;  // the last row whose requests begin at x or before
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (off[mid] <= x) lo = mid;
+      else hi = mid - 1;
+    }
+    const int start = start_of(lo), from = get(a.source + lo) >= 0 ? start / a.page : (start + a.page - 1) / a.page;
+    a.table_out[(int64_t)lo * a.width + from + x - off[lo]] = x < nfree ? get(a.list + x) : -1;
+  }
+  __syncthreads();
+  if (tid == 0) *a.ncopies = flag;
+}
+
+// Pages {source, target} of every plane.
+__device__ __forceinline__ void copy_pages(hq_u4v* pool, const int* pairs, int n, int planes, int pages, int64_t pieces) {
+  for (int64_t x = blockIdx.x; x < (int64_t)n * planes; x += gridDim.x) {
+    const int c = x % n;
+    const int64_t plane = x / n;
+    const hq_u4v* from = pool + (plane * pages + pairs[2 * c]) * pieces;
+    hq_u4v* to = pool + (plane * pages + pairs[2 * c + 1]) * pieces;
+    for (int64_t i = threadIdx.x; i < pieces; i += kThreads) to[i] = from[i];
+  }
+}
+__global__ __launch_bounds__(kThreads) void step_copy_kernel(StepArgs a) {
+  copy_pages(a.pool, a.copies, *a.ncopies, a.planes, a.pages, a.page_pieces);
+}
+
+// ---- live pages to the front ----------------------------------------------------------------------------------------------
+struct CompactArgs {
+  hq_u4v* pool;
+  const int *table, *refs;
+  int *table_out, *refs_out, *live;
+  int *pairs;            // {source, target}
+  int *to;               // of every page that moves: where
+  int* nmoves;
+  int64_t page_pieces;
+  int planes, rows, width, pages;
+};
+
+// The i-th page in use behind the first `live` goes to the i-th hole among them.
+__global__ __launch_bounds__(kThreads) void compact_plan_kernel(CompactArgs a) {
+  __shared__ int parts[kThreads / 64];
+  int live = 0;
+  for (int i0 = 0; i0 < a.pages; i0 += kThreads) {
+    int all;
+    block_scan(i0 + (int)threadIdx.x < a.pages && a.refs[i0 + threadIdx.x] > 0, parts, &all);
+    live += all;
+  }
+  int holes = 0, movers = 0;
+  for (int i0 = 0; i0 < a.pages; i0 += kThreads) {
+    const int i = i0 + threadIdx.x;
+    const int n = i < a.pages ? a.refs[i] : 0;
+    const bool hole = i < live && n <= 0, mover = i >= live && n > 0;
+    int all;
+    int rank = holes + block_scan(hole, parts, &all);
+    if (hole) put(a.pairs + 2 * rank + 1, i);
+    holes += all;
+    rank = movers + block_scan(mover, parts, &all);
+    if (mover) put(a.pairs + 2 * rank, i);
+    movers += all;
+    if (i < a.pages && !hole) a.refs_out[i] = mover ? 0 : n;
+  }
+  if (threadIdx.x == 0) {
+    *a.live = live;
+    *a.nmoves = movers;
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  for (int r = threadIdx.x; r < movers; r += kThreads) {
+    const int from = get(a.pairs + 2 * r), to = get(a.pairs + 2 * r + 1);
+    a.refs_out[to] = a.refs[from];
+    a.to[from] = to;
+  }
+}
+__global__ __launch_bounds__(kThreads) void compact_move_kernel(CompactArgs a) {
+  const int live = *a.live;
+  const int64_t n = (int64_t)a.rows * a.width;
+  for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < n; i += (int64_t)gridDim.x * kThreads) {
+    const int e = a.table[i];
+    a.table_out[i] = e >= live && e < a.pages && a.refs[e] > 0 ? a.to[e] : e;
+  }
+  copy_pages(a.pool, a.pairs, *a.nmoves, a.planes, a.pages, a.page_pieces);
+}
+
+bool meet(const void* a, int64_t na, const void* b, int64_t nb) {
+  const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
+  return na > 0 && nb > 0 && x < y + nb && y < x + na;
+}
+bool pool_bad(const void* pool, int planes, int64_t page_bytes) { return planes > 0 && page_bytes > 0 && !pool; }
+}  // namespace
+
+extern "C" int hq_cache_write(const void* k, const void* v, void* k_pages, void* v_pages, int dtype, const int32_t* table,
+                              const int32_t* starts, const int32_t* cu, int rows, int64_t tokens, int table_width, int num_pages,
+                              int page_size, int kv_heads, int head_dim, int64_t k_stride, int64_t v_stride, void* stream) {
+  if (rows < 0 || tokens < 0 || table_width < 0 || num_pages < 0 || kv_heads < 1 || head_dim < 8 || head_dim % 8) return HQ_ERR_BAD_SHAPE;
+  if (page_size < 1 || page_size > 1024 || (page_size & (page_size - 1))) return HQ_ERR_BAD_SHAPE;
+  if (dtype != HQ_DTYPE_F16 && dtype != HQ_DTYPE_BF16) return HQ_ERR_BAD_ENUM;
+  if (rows == 0 || tokens == 0 || table_width == 0 || num_pages == 0) return HQ_OK;
+  if (!k || !v || !k_pages || !v_pages || !table || !starts || !cu) return HQ_ERR_NULL_POINTER;
+  if (k_stride < (int64_t)kv_heads * head_dim || v_stride < (int64_t)kv_heads * head_dim) return HQ_ERR_BAD_SHAPE;
+  if ((((uintptr_t)k | (uintptr_t)v | (uintptr_t)k_pages | (uintptr_t)v_pages) & 15) || k_stride % 8 || v_stride % 8 ||
+      (((uintptr_t)table | (uintptr_t)starts | (uintptr_t)cu) & 3))
+    return HQ_ERR_MISALIGNED;
+  if (tokens > INT_MAX - 64 || (int64_t)kv_heads * head_dim > INT_MAX) return HQ_ERR_TOO_LARGE;
+  const HqDevice* dev = nullptr;
+  const int rc = hq_current_device(&dev);
+  if (rc != HQ_OK) return rc;
+  const WriteArgs a{(const hq_u4v*)k, (const hq_u4v*)v, (hq_u4v*)k_pages, (hq_u4v*)v_pages, table, starts, cu, k_stride / 8, v_stride / 8, rows,
+                    (int)tokens, table_width, num_pages, __builtin_ctz(page_size), kv_heads, head_dim / 8};
+  return hq_launch_as_is(write_kernel, dim3((unsigned)((tokens + 3) / 4)), dim3(kThreads), 0, (hipStream_t)stream, a);
+}
+
+extern "C" int hq_cache_step(void* pool, int planes, int64_t page_bytes, const int32_t* table, const int32_t* lengths, const int32_t* refs,
+                             const int32_t* parent, const int32_t* add, int32_t* table_out, int32_t* lengths_out, int32_t* refs_out,
+                             int32_t* starts_out, int32_t* missing, int rows, int table_width, int num_pages, int page_size, void* stream) {
+  if (planes < 0 || page_bytes < 0 || page_bytes % 16 || rows < 0 || table_width < 0 || num_pages < 0 || page_size < 1) return HQ_ERR_BAD_SHAPE;
+  if (!missing || (num_pages && (!refs || !refs_out)) || (rows && (!lengths || !parent || !add || !lengths_out || !starts_out)) ||
+      (rows && table_width && (!table || !table_out)) || (num_pages && pool_bad(pool, planes, page_bytes)))
+    return HQ_ERR_NULL_POINTER;
+  if (((uintptr_t)pool & 15) || (((uintptr_t)table | (uintptr_t)lengths | (uintptr_t)refs | (uintptr_t)parent | (uintptr_t)add |
+                                  (uintptr_t)table_out | (uintptr_t)lengths_out | (uintptr_t)refs_out | (uintptr_t)starts_out | (uintptr_t)missing) & 3))
+    return HQ_ERR_MISALIGNED;
+  const int64_t entries = (int64_t)rows * table_width;
+  if (rows > 16384 || (int64_t)table_width * page_size > INT_MAX - 1024 || entries > INT_MAX) return HQ_ERR_TOO_LARGE;
+  const void* ins[] = {table, lengths, refs, parent, add};
+  const int64_t nin[] = {4 * entries, 4 * (int64_t)rows, 4 * (int64_t)num_pages, 4 * (int64_t)rows, 4 * (int64_t)rows};
+  const void* outs[] = {table_out, lengths_out, refs_out, starts_out, missing};
+  const int64_t nout[] = {4 * entries, 4 * (int64_t)rows, 4 * (int64_t)num_pages, 4 * (int64_t)rows, 4};
+  for (int i = 0; i < 5; ++i)
+    for (int j = 0; j < 5; ++j)
+      if (meet(ins[i], nin[i], outs[j], nout[j]) || (i < j && meet(outs[i], nout[i], outs[j], nout[j]))) return HQ_ERR_BAD_SHAPE;
+  const HqDevice* dev = nullptr;
+  int rc = hq_current_device(&dev);
+  if (rc != HQ_OK) return rc;
+  HqWorkspace ws;
+  const int64_t most = entries < num_pages ? entries : num_pages;
+  rc = hq_get_workspace((hipStream_t)stream, (size_t)(4 * (int64_t)rows + 1 + most), (size_t)num_pages + 1, &ws);
+  if (rc != HQ_OK) return rc;
+  StepArgs a{};
+  a.pool = (hq_u4v*)pool;
+  a.table = table;
+  a.lengths = lengths;
+  a.refs = refs;
+  a.parent = parent;
+  a.add = add;
+  a.table_out = table_out;
+  a.lengths_out = lengths_out;
+  a.refs_out = refs_out;
+  a.starts_out = starts_out;
+  a.missing = missing;
+  a.need = (int*)ws.partial;
+  a.source = a.need + rows;
+  a.copies = a.source + rows;
+  a.ncopies = a.copies + 2 * (int64_t)rows;
+  a.list = a.ncopies + 1;
+  a.arrived = ws.counters;
+  a.change = (int*)ws.counters + 1;
+  a.page_pieces = page_bytes / 16;
+  a.planes = planes;
+  a.rows = rows;
+  a.width = table_width;
+  a.pages = num_pages;
+  a.page = page_size;
+  rc = hq_launch_as_is(step_kernel, dim3(rows > 1 ? rows : 1), dim3(kThreads), 4 * (size_t)rows, (hipStream_t)stream, a);
+  if (rc != HQ_OK || rows == 0 || planes == 0 || page_bytes == 0 || num_pages == 0) return rc;
+  const int64_t items = (int64_t)rows * planes, grid = 16 * (int64_t)dev->cus;
+  return hq_launch_as_is(step_copy_kernel, dim3((unsigned)(items < grid ? items : grid)), dim3(kThreads), 0, (hipStream_t)stream, a);
+}
+
+extern "C" int hq_cache_compact(void* pool, int planes, int64_t page_bytes, const int32_t* table, const int32_t* refs, int32_t* table_out,
+                                int32_t* refs_out, int32_t* live, int rows, int table_width, int num_pages, void* stream) {
+  if (planes < 0 || page_bytes < 0 || page_bytes % 16 || rows < 0 || table_width < 0 || num_pages < 0) return HQ_ERR_BAD_SHAPE;
+  const int64_t entries = (int64_t)rows * table_width;
+  if (!live || (num_pages && (!refs || !refs_out)) || (entries && (!table || !table_out)) || (num_pages && pool_bad(pool, planes, page_bytes)))
+    return HQ_ERR_NULL_POINTER;
+  if (((uintptr_t)pool & 15) || (((uintptr_t)table | (uintptr_t)refs | (uintptr_t)table_out | (uintptr_t)refs_out | (uintptr_t)live) & 3))
+    return HQ_ERR_MISALIGNED;
+  if (entries > INT_MAX || num_pages > INT_MAX / 4) return HQ_ERR_TOO_LARGE;
+  const void* ins[] = {table, refs};
+  const int64_t nin[] = {4 * entries, 4 * (int64_t)num_pages};
+  const void* outs[] = {table_out, refs_out, live};
+  const int64_t nout[] = {4 * entries, 4 * (int64_t)num_pages, 4};
+  for (int i = 0; i < 3; ++i)
+    for (int j = 0; j < 3; ++j)
+      if ((i < 2 && meet(ins[i], nin[i], outs[j], nout[j])) || (i < j && meet(outs[i], nout[i], outs[j], nout[j]))) return HQ_ERR_BAD_SHAPE;
+  const HqDevice* dev = nullptr;
+  int rc = hq_current_device(&dev);
+  if (rc != HQ_OK) return rc;
+  HqWorkspace ws;
+  rc = hq_get_workspace((hipStream_t)stream, (size_t)(2 * (int64_t)num_pages + 1), 0, &ws);
+  if (rc != HQ_OK) return rc;
+  CompactArgs a{};
+  a.pool = (hq_u4v*)pool;
+  a.table = table;
+  a.refs = refs;
+  a.table_out = table_out;
+  a.refs_out = refs_out;
+  a.live = live;
+  a.nmoves = (int*)ws.partial;
+  a.to = a.nmoves + 1;
+  a.pairs = a.to + num_pages;  // half of the pages at most move
+  a.page_pieces = page_bytes / 16;
+  a.planes = planes;
+  a.rows = rows;
+  a.width = table_width;
+  a.pages = num_pages;
+  rc = hq_launch_as_is(compact_plan_kernel, dim3(1), dim3(kThreads), 0, (hipStream_t)stream, a);
+  if (rc != HQ_OK || (entries == 0 && (planes == 0 || page_bytes == 0))) return rc;
+  return hq_launch_as_is(compact_move_kernel, dim3(16 * (unsigned)dev->cus), dim3(kThreads), 0, (hipStream_t)stream, a);
+}

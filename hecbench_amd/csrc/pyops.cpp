@@ -16,6 +16,7 @@
 #include <c10/hip/HIPStream.h>
 
 #include <climits>
+#include <cmath>
 #include <cstdint>
 #include <string>
 
@@ -422,6 +423,180 @@ PyObject* mxfp4_qdq(PyObject* const* a) {  // x, out
   return r.release();
 }
 
+// [tokens][heads][head size] that may be a part of wider rows: a fused projection's queries, say.
+struct Rows {
+  const at::Tensor* t;
+  int64_t tokens, heads, size, stride;
+};
+Rows rows_of(PyObject* o, const char* name, unsigned dtypes) {
+  if (o == Py_None || !THPVariable_Check(o)) value_error(std::string(name) + " must be a torch tensor");
+  const at::Tensor& t = THPVariable_Unpack(o);
+  if (!(dtypes & ((unsigned)t.scalar_type() < 32 ? 1u << (unsigned)t.scalar_type() : 0u)))
+    value_error(std::string(name) + " must be " + names_of(dtypes));
+  if (t.dim() != 3) value_error(std::string(name) + " must be [tokens][heads][head size]");
+  Rows r{&t, t.size(0), t.size(1), t.size(2), t.size(1) * t.size(2)};
+  if (t.numel() == 0) return r;
+  if ((r.size > 1 && t.stride(2) != 1) || (r.heads > 1 && t.stride(1) != r.size))
+    value_error(std::string(name) + " must hold the heads of a token one behind the other");
+  if (r.tokens > 1) r.stride = t.stride(0);
+  if (r.stride < r.heads * r.size) value_error(std::string(name) + " must not overlap itself");
+  return r;
+}
+float scale_of(PyObject* o, int64_t head_size) { return o == Py_None ? 1.0f / std::sqrt((float)head_size) : real(o); }
+void same_type(const at::Tensor& like, const at::Tensor& t, const char* name) {
+  if (t.scalar_type() != like.scalar_type()) value_error(std::string(name) + " must have the type of the others");
+}
+
+PyObject* prompt_attention(PyObject* const* a) {  // q, k, v, cu_q, cu_k, causal, scale, out
+  const Rows q = rows_of(a[0], "q", kF16 | kBF16), k = rows_of(a[1], "k", kF16 | kBF16), v = rows_of(a[2], "v", kF16 | kBF16);
+  same_type(*q.t, *k.t, "k");
+  same_type(*q.t, *v.t, "v");
+  if (v.tokens != k.tokens || v.heads != k.heads || v.size != k.size || k.size != q.size) value_error("k and v must be [keys][heads][head size of q]");
+  const at::Tensor* cu_q = tensor(a[3], "cu_q", kI32);
+  const at::Tensor* cu_k = tensor(a[4], "cu_k", kI32, cu_q->numel(), true);
+  if (cu_q->numel() < 1) value_error("cu_q must hold one bound more than there are sequences");
+  if (!cu_k && k.tokens != q.tokens) value_error("cu_k is required where there are other keys than q's tokens");
+  const int causal = PyObject_IsTrue(a[5]);
+  if (causal < 0) throw python_error();
+  const float scale = scale_of(a[6], q.size);
+  const at::Tensor* o = tensor(a[7], "out", dt(q.t->scalar_type()), q.tokens * q.heads * q.size, true);
+  same_device(q.t, k.t, v.t, cu_q, cu_k, o);
+  Result r(a[7], o, *q.t, {q.tokens, q.heads, q.size}, q.t->scalar_type());
+  const int hq = size_of(q.heads), hk = size_of(k.heads), d = size_of(q.size), seqs = size_of(cu_q->numel() - 1);
+  void* st = stream();
+  call("hq_prompt_attention", [&] {
+    return hq_prompt_attention(ptr(q.t), ptr(k.t), ptr(v.t), r.t.data_ptr(), act_dtype(*q.t), in<int32_t>(cu_q), in<int32_t>(cu_k), seqs, q.tokens,
+                               k.tokens, hq, hk, d, q.stride, k.stride, v.stride, scale, causal, st);
+  });
+  return r.release();
+}
+
+PyObject* paged_attention(PyObject* const* a) {  // q, k_pages, v_pages, table, lengths, groups, shared, scale, out
+  const Rows q = rows_of(a[0], "q", kF16 | kBF16);
+  const at::Tensor* k = tensor(a[1], "k_pages", dt(q.t->scalar_type()));
+  if (k->dim() != 4 || k->size(3) != q.size) value_error("k_pages must be [pages][heads][tokens of a page][head size of q]");
+  const at::Tensor* v = tensor(a[2], "v_pages", dt(q.t->scalar_type()), k->numel());
+  if (v->sizes() != k->sizes()) value_error("v_pages must have the shape of k_pages");
+  const at::Tensor* table = tensor(a[3], "table", kI32);
+  if (table->dim() != 2 || table->size(0) != q.tokens) value_error("table must be [requests][pages of a request]");
+  const at::Tensor* lengths = tensor(a[4], "lengths", kI32, q.tokens);
+  const at::Tensor* groups = tensor(a[5], "groups", kI32, -1, true);
+  if (groups && groups->numel() < 1) value_error("groups must hold one bound more than there are groups");
+  if (!groups && a[6] != Py_None) value_error("shared goes with groups");
+  const at::Tensor* shared = groups ? tensor(a[6], "shared", kI32, groups->numel() - 1) : nullptr;
+  const float scale = scale_of(a[7], q.size);
+  const at::Tensor* o = tensor(a[8], "out", dt(q.t->scalar_type()), q.tokens * q.heads * q.size, true);
+  same_device(q.t, k, v, table, lengths, groups, shared, o);
+  Result r(a[8], o, *q.t, {q.tokens, q.heads, q.size}, q.t->scalar_type());
+  const int ng = groups ? size_of(groups->numel() - 1) : 0, batch = size_of(q.tokens), width = size_of(table->size(1)), pages = size_of(k->size(0)),
+            page = size_of(k->size(2)), hq = size_of(q.heads), hk = size_of(k->size(1)), d = size_of(q.size);
+  void* st = stream();
+  call("hq_paged_attention", [&] {
+    return hq_paged_attention(ptr(q.t), ptr(k), ptr(v), r.t.data_ptr(), act_dtype(*q.t), in<int32_t>(table), in<int32_t>(lengths), in<int32_t>(groups),
+                              in<int32_t>(shared), ng, batch, width, pages, page, hq, hk, d, q.stride, scale, st);
+  });
+  return r.release();
+}
+
+PyObject* cache_write(PyObject* const* a) {  // k, v, k_pages, v_pages, table, starts, cu
+  const Rows k = rows_of(a[0], "k", kF16 | kBF16), v = rows_of(a[1], "v", kF16 | kBF16);
+  same_type(*k.t, *v.t, "v");
+  if (v.tokens != k.tokens || v.heads != k.heads || v.size != k.size) value_error("v must have the shape of k");
+  const at::Tensor* kp = tensor(a[2], "k_pages", dt(k.t->scalar_type()));
+  if (kp->dim() != 4 || kp->size(1) != k.heads || kp->size(3) != k.size) value_error("k_pages must be [pages][heads of k][tokens of a page][head size of k]");
+  const at::Tensor* vp = tensor(a[3], "v_pages", dt(k.t->scalar_type()), kp->numel());
+  if (vp->sizes() != kp->sizes()) value_error("v_pages must have the shape of k_pages");
+  const at::Tensor* table = tensor(a[4], "table", kI32);
+  if (table->dim() != 2) value_error("table must be [requests][pages of a request]");
+  const at::Tensor* starts = tensor(a[5], "starts", kI32, table->size(0));
+  const at::Tensor* cu = tensor(a[6], "cu", kI32, table->size(0) + 1);
+  same_device(k.t, v.t, kp, vp, table, starts, cu);
+  const int rows = size_of(table->size(0)), width = size_of(table->size(1)), pages = size_of(kp->size(0)), page = size_of(kp->size(2)),
+            heads = size_of(k.heads), d = size_of(k.size);
+  void* st = stream();
+  call("hq_cache_write", [&] {
+    return hq_cache_write(ptr(k.t), ptr(v.t), kp->data_ptr(), vp->data_ptr(), act_dtype(*k.t), in<int32_t>(table), in<int32_t>(starts), in<int32_t>(cu),
+                          rows, k.tokens, width, pages, page, heads, d, k.stride, v.stride, st);
+  });
+  Py_RETURN_NONE;
+}
+
+// The pool [planes][pages][...]: bytes of a page.
+int64_t page_bytes_of(const at::Tensor& pool, int64_t pages) {
+  if (pool.dim() < 3 || pool.size(1) != pages) value_error("pool must be [planes][pages][...], with a count in refs for every page");
+  int64_t n = pool.element_size();
+  for (int64_t i = 2; i < pool.dim(); ++i) n *= pool.size(i);
+  return n;
+}
+constexpr unsigned kPool = kF32 | kF16 | kBF16 | kU8 | kI8 | kI16 | kI32;
+
+// The i-th of the results that the caller gave, or None.
+struct Given {
+  THPObjectPtr seq;
+  Given(PyObject* o, int n) {
+    if (o == Py_None) return;
+    seq = THPObjectPtr(PySequence_Fast(o, "out must be a sequence of tensors"));
+    if (!seq) throw python_error();
+    if (PySequence_Fast_GET_SIZE(seq.get()) != n) value_error("out must hold " + std::to_string(n) + " tensors");
+  }
+  PyObject* at(int i) const { return seq ? PySequence_Fast_GET_ITEM(const_cast<THPObjectPtr&>(seq).get(), i) : Py_None; }
+};
+
+PyObject* cache_step(PyObject* const* a) {  // pool, page_size, table, lengths, refs, parent, add, out
+  const at::Tensor* pool = tensor(a[0], "pool", kPool);
+  const int page = small_integer(a[1], "page_size");
+  const at::Tensor* table = tensor(a[2], "table", kI32);
+  if (table->dim() != 2) value_error("table must be [requests][pages of a request]");
+  const int64_t rows = table->size(0), width = table->size(1);
+  const at::Tensor* lengths = tensor(a[3], "lengths", kI32, rows);
+  const at::Tensor* refs = tensor(a[4], "refs", kI32);
+  const at::Tensor* parent = tensor(a[5], "parent", kI32, rows);
+  const at::Tensor* add = tensor(a[6], "add", kI32, rows);
+  const int64_t pages = refs->numel(), bytes = page_bytes_of(*pool, pages);
+  const Given given(a[7], 5);
+  const at::Tensor* ot = tensor(given.at(0), "out[0]", kI32, rows * width, true);
+  const at::Tensor* ol = tensor(given.at(1), "out[1]", kI32, rows, true);
+  const at::Tensor* orf = tensor(given.at(2), "out[2]", kI32, pages, true);
+  const at::Tensor* os = tensor(given.at(3), "out[3]", kI32, rows, true);
+  const at::Tensor* om = tensor(given.at(4), "out[4]", kI32, 1, true);
+  same_device(pool, table, lengths, refs, parent, add, ot, ol, orf, os, om);
+  Result rt(given.at(0), ot, *table, {rows, width}, ScalarType::Int), rl(given.at(1), ol, *table, {rows}, ScalarType::Int),
+      rr(given.at(2), orf, *table, {pages}, ScalarType::Int), rs(given.at(3), os, *table, {rows}, ScalarType::Int),
+      rm(given.at(4), om, *table, {1}, ScalarType::Int);
+  const int planes = size_of(pool->size(0)), n = size_of(rows), w = size_of(width), np = size_of(pages);
+  void* st = stream();
+  call("hq_cache_step", [&] {
+    return hq_cache_step(pool->data_ptr(), planes, bytes, in<int32_t>(table), in<int32_t>(lengths), in<int32_t>(refs), in<int32_t>(parent),
+                         in<int32_t>(add), to<int32_t>(rt.t), to<int32_t>(rl.t), to<int32_t>(rr.t), to<int32_t>(rs.t), to<int32_t>(rm.t), n, w, np, page,
+                         st);
+  });
+  THPObjectPtr t(rt.release()), l(rl.release()), r(rr.release()), s(rs.release()), m(rm.release());
+  return PyTuple_Pack(5, t.get(), l.get(), r.get(), s.get(), m.get());
+}
+
+PyObject* cache_compact(PyObject* const* a) {  // pool, table, refs, out
+  const at::Tensor* pool = tensor(a[0], "pool", kPool);
+  const at::Tensor* table = tensor(a[1], "table", kI32);
+  if (table->dim() != 2) value_error("table must be [requests][pages of a request]");
+  const at::Tensor* refs = tensor(a[2], "refs", kI32);
+  const int64_t rows = table->size(0), width = table->size(1), pages = refs->numel(), bytes = page_bytes_of(*pool, pages);
+  const Given given(a[3], 3);
+  const at::Tensor* ot = tensor(given.at(0), "out[0]", kI32, rows * width, true);
+  const at::Tensor* orf = tensor(given.at(1), "out[1]", kI32, pages, true);
+  const at::Tensor* ol = tensor(given.at(2), "out[2]", kI32, 1, true);
+  same_device(pool, table, refs, ot, orf, ol);
+  Result rt(given.at(0), ot, *table, {rows, width}, ScalarType::Int), rr(given.at(1), orf, *table, {pages}, ScalarType::Int),
+      rl(given.at(2), ol, *table, {1}, ScalarType::Int);
+  const int planes = size_of(pool->size(0)), n = size_of(rows), w = size_of(width), np = size_of(pages);
+  void* st = stream();
+  call("hq_cache_compact", [&] {
+    return hq_cache_compact(pool->data_ptr(), planes, bytes, in<int32_t>(table), in<int32_t>(refs), to<int32_t>(rt.t), to<int32_t>(rr.t),
+                            to<int32_t>(rl.t), n, w, np, st);
+  });
+  THPObjectPtr t(rt.release()), r(rr.release()), l(rl.release());
+  return PyTuple_Pack(3, t.get(), r.get(), l.get());
+}
+
 // ---- the module ------------------------------------------------------------------------------------------------------
 template <PyObject* (*F)(PyObject* const*), int NARGS>
 PyObject* method(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
@@ -447,6 +622,11 @@ PyMethodDef kMethods[] = {
     HQ_METHOD("gemv_int8", gemv_int<false>, 5),
     HQ_METHOD("gemv_int4", gemv_int<true>, 5),
     HQ_METHOD("mxfp4_qdq", mxfp4_qdq, 2),
+    HQ_METHOD("prompt_attention", prompt_attention, 8),
+    HQ_METHOD("paged_attention", paged_attention, 9),
+    HQ_METHOD("cache_write", cache_write, 7),
+    HQ_METHOD("cache_step", cache_step, 8),
+    HQ_METHOD("cache_compact", cache_compact, 4),
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_ops", "Host path of the operators over libhq.", -1, kMethods};
 

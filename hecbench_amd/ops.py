@@ -138,3 +138,41 @@ def mxfp4_qdq(x, out=None):
     """mxfp4<T>() of src/mxfp4-hip/main.cu:144-171: microscaling fp4 quantise-dequantise of an fp16 / bf16 tensor
     whose element count is a multiple of 32."""
     return _native.mxfp4_qdq(x, out)
+
+
+def prompt_attention(q, k, v, cu_q, cu_k=None, causal=True, scale=None, out=None):
+    """Attention over packed sequences: tokens cu_q[i] .. cu_q[i + 1] - 1 of q [tokens][heads][64 or 128] are sequence i's and see
+    its keys cu_k[i] .. cu_k[i + 1] - 1 (cu_k: cu_q's) of k and v [keys][kv_heads][head size]; fp16 or bf16, int32 bounds.
+    causal: the last token sees all keys, each one before it a key less; a token that sees none gets zeros.  scale: 1 / sqrt of the
+    head size.  q, k and v may be parts of a fused projection's rows.  Returns [tokens][heads][head size]; tokens of no sequence
+    are left unwritten."""
+    return _native.prompt_attention(q, k, v, cu_q, cu_k, causal, scale, out)
+
+
+def paged_attention(q, k_pages, v_pages, table, lengths, groups=None, shared=None, scale=None, out=None):
+    """Attention of one token per request over a paged cache: q [requests][heads][64 or 128] over the first lengths[s] tokens of
+    row s, token t being token t % page of page table[s][t // page] in k_pages and v_pages [pages][kv_heads][page][head size].
+    groups (int32 [n + 1]) and shared (int32 [n]): the first shared[g] tokens of the requests groups[g] .. groups[g + 1] - 1 are in the
+    same pages, as cache_step leaves them, and are read once for all of them."""
+    return _native.paged_attention(q, k_pages, v_pages, table, lengths, groups, shared, scale, out)
+
+
+def cache_write(k, v, k_pages, v_pages, table, starts, cu):
+    """Tokens cu[s] .. cu[s + 1] - 1 of k and v [tokens][kv_heads][head size] become tokens starts[s] and on of row s of the table;
+    a token without a page is left out."""
+    _native.cache_write(k, v, k_pages, v_pages, table, starts, cu)
+
+
+def cache_step(pool, page_size, table, lengths, refs, parent, add, out=None):
+    """The page tables of the next step: row s goes on from row parent[s] of this one (-1: from nothing) and gets room for add[s]
+    tokens more.  Whole pages are shared, a half-filled one is copied in every plane of pool [planes][pages][...] for each row but the
+    first that goes on from it, new pages are the free ones (refs[p] <= 0), lowest first, to the rows in order.
+    Returns (table, lengths, refs, starts, missing): starts are the lengths before the new tokens, missing (int32 [1]) the pages that
+    there were not - a row ends where its pages end.  out: five tensors for them that share nothing with the arguments."""
+    return _native.cache_step(pool, page_size, table, lengths, refs, parent, add, out)
+
+
+def cache_compact(pool, table, refs, out=None):
+    """Moves the pages in use (refs[p] > 0) behind the first n, n the number of pages in use, into the free ones among those, in order,
+    in every plane of the pool.  Returns (table, refs, n as int32 [1])."""
+    return _native.cache_compact(pool, table, refs, out)

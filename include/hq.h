@@ -47,7 +47,7 @@ extern "C" {
 /* element types of the activation vector / matrix */
 #define HQ_DTYPE_F32 0
 #define HQ_DTYPE_F16 1
-#define HQ_DTYPE_BF16 2 /* accepted by the activation quantisers and hq_mxfp4_qdq only */
+#define HQ_DTYPE_BF16 2 /* accepted by the activation quantisers, hq_mxfp4_qdq, attention and its cache only */
 
 /* flags */
 #define HQ_FLAG_ACCUMULATE 1u /* y += result (reference wrapper semantics) */
@@ -320,6 +320,54 @@ int hq_gemv_int4(const uint8_t* mat_packed, const void* vec_fp16, void* res_fp16
  * (kernel main.cu:109-142), without its timing loop and printing.
  */
 int hq_mxfp4_qdq(const void* in, void* out, int64_t n_elems, int dtype, void* stream);
+
+/*
+ * Attention and its paged key / value cache: what a program that serves the model calls between the products above.  No counterpart
+ * in the reference.  fp16 or bf16 (HQ_DTYPE_F16, HQ_DTYPE_BF16); products and softmax statistics in fp32, the weights rounded to
+ * the data's type for their product with the values, one rounding of the result.  heads = R * kv_heads: query head h reads key /
+ * value head h / R.  head_dim 64 or 128; scale finite and >= 0.  int32 bounds, tables and lengths are device memory, read by the
+ * kernels: numbers out of range are cut to what there is.
+ *
+ * hq_prompt_attention: sequence i is tokens cu_q[i] ... cu_q[i+1]-1 of q and keys cu_k[i] ... cu_k[i+1]-1 of k and v (cu_k NULL: cu_q):
+ *     out[t][h] = sum_j softmax_j(scale * q[t][h] . k[j][h/R]) * v[j][h/R]
+ *   over the sequence's keys; causal != 0: over those with j <= i + (number of keys) - (number of tokens), i and j counted
+ *   within the sequence.  A token that sees no key gets zeros.  A key that a token does not see has no effect on it, whatever it
+ *   holds; a value that is not finite makes the results of the tokens that see it NaN.  q [total_q][heads][head_dim], rows q_stride
+ *   elements apart, k and v [total_k][kv_heads][head_dim] likewise (parts of a fused projection's rows); out contiguous; all 16-byte
+ *   aligned, strides multiples of 8.  Tokens of no sequence are not written.
+ * hq_paged_attention: one query a request.  Token t of request s is token t % page_size of page table[s][t / page_size]
+ *   (table [batch][table_width], pages [num_pages][kv_heads][page_size][head_dim], contiguous); request s sees its first lengths[s] tokens.
+ *   Requests groups[g] ... groups[g+1]-1 (bounds in ascending order) have their first shared[g] tokens, as far as the first one's length reaches, in the same
+ *   pages, which are read once for all of them, from the first one's row; ngroups 0: nothing is shared.  page_size a power of two, 8 ... 1024.  A table entry
+ *   that is needed and no page counts as a page of zeros.  Partial sums of divided keys are in the stream's workspace.
+ * hq_cache_write: tokens cu[s] ... cu[s+1]-1 of k and v [tokens][kv_heads][head_dim] (strides as above) become tokens starts[s], ... of row s
+ *   of the table.  A token whose place is outside its row, or in no page, is left out.
+ * hq_cache_step: from the tables of one step to the next one's.  Row s inherits row parent[s] (of the old tables; any number outside
+ *   0 ... rows-1: nothing) and gets room for add[s] tokens (negative: none) as far as its table_width pages reach.  Whole pages are
+ *   shared; a half-filled one stays with the first row that inherits it and is copied, all page_bytes of it in every one of the
+ *   pool's planes ([planes][num_pages][page_bytes]), for every other.  refs counts the rows that use a page (and whatever else the
+ *   caller counts there); a page with refs <= 0 after the old rows have gone and the new ones come is free, and the pages that are asked for, row by row
+ *   and front to back, are the free ones, lowest first.  Where there are no more, the entry is -1, the row ends before it and
+ *   *missing counts it.  lengths_out: the new lengths, starts_out: the inherited part of them; entries behind a row's last page
+ *   are -1.  Outputs share no memory with inputs (HQ_ERR_BAD_SHAPE).  rows <= 16384.
+ * hq_cache_compact: n pages are in use (refs > 0); those at n and beyond move, in order, into the free ones below n, in every plane;
+ *   table_out and refs_out follow, *live = n.
+ * The last two and hq_paged_attention use the stream's workspace: before a stream is captured, run the largest call once.
+ */
+int hq_prompt_attention(const void* q, const void* k, const void* v, void* out, int dtype, const int32_t* cu_q, const int32_t* cu_k, int seqs,
+                        int64_t total_q, int64_t total_k, int heads, int kv_heads, int head_dim, int64_t q_stride, int64_t k_stride,
+                        int64_t v_stride, float scale, int causal, void* stream);
+int hq_paged_attention(const void* q, const void* k_pages, const void* v_pages, void* out, int dtype, const int32_t* table, const int32_t* lengths,
+                       const int32_t* groups, const int32_t* shared, int ngroups, int batch, int table_width, int num_pages, int page_size,
+                       int heads, int kv_heads, int head_dim, int64_t q_stride, float scale, void* stream);
+int hq_cache_write(const void* k, const void* v, void* k_pages, void* v_pages, int dtype, const int32_t* table, const int32_t* starts,
+                   const int32_t* cu, int rows, int64_t tokens, int table_width, int num_pages, int page_size, int kv_heads, int head_dim,
+                   int64_t k_stride, int64_t v_stride, void* stream);
+int hq_cache_step(void* pool, int planes, int64_t page_bytes, const int32_t* table, const int32_t* lengths, const int32_t* refs,
+                  const int32_t* parent, const int32_t* add, int32_t* table_out, int32_t* lengths_out, int32_t* refs_out, int32_t* starts_out,
+                  int32_t* missing, int rows, int table_width, int num_pages, int page_size, void* stream);
+int hq_cache_compact(void* pool, int planes, int64_t page_bytes, const int32_t* table, const int32_t* refs, int32_t* table_out,
+                     int32_t* refs_out, int32_t* live, int rows, int table_width, int num_pages, void* stream);
 
 /*
  * Memory-system probes for the benchmark report (no counterpart in the reference): the rate this device

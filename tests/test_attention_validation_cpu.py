@@ -1,0 +1,140 @@
+"""What attention and the cache refuse, before any pointer reaches a kernel: no GPU."""
+import pytest
+import torch
+
+import hecbench_amd as hq
+from hecbench_amd import _lib
+
+
+def i32(*shape):
+    return torch.zeros(shape, dtype=torch.int32)
+
+
+def half(*shape):
+    return torch.zeros(shape, dtype=torch.float16)
+
+
+def refuse(match, fn, *args, **kw):
+    with pytest.raises(ValueError, match=match):
+        fn(*args, **kw)
+
+
+def test_prompt_attention():
+    q, k, cu = half(6, 8, 64), half(6, 2, 64), i32(3)
+    f = hq.prompt_attention
+    refuse("device tensors only", f, q, k, k, cu)
+    refuse("device tensors only", f, q, half(9, 2, 64), half(9, 2, 64), cu, i32(3))
+    refuse("q must be float16 or bfloat16", f, q.float(), k, k, cu)
+    refuse("k must have the type", f, q, k.bfloat16(), k, cu)
+    refuse("v must have the type", f, q, k, k.bfloat16(), cu)
+    refuse("must be \\[tokens\\]", f, q.view(6, -1), k, k, cu)
+    refuse("head size of q", f, q, k, half(6, 2, 128), cu)
+    refuse("head size of q", f, q, half(6, 2, 128), half(6, 2, 128), cu)
+    refuse("head size of q", f, q, k, half(5, 2, 64), cu)
+    refuse("cu_q must be int32", f, q, k, k, cu.long())
+    refuse("cu_k must hold 3", f, q, k, k, cu, i32(4))
+    refuse("cu_k is required", f, q, half(9, 2, 64), half(9, 2, 64), cu)
+    refuse("cu_q must hold one", f, q, k, k, i32(0))
+    refuse("one behind the other", f, half(6, 64, 8).transpose(1, 2), k, k, cu)
+    refuse("one behind the other", f, half(8, 6, 64).transpose(0, 1), k, k, cu)
+    refuse("not overlap itself", f, half(6 * 8 * 64).as_strided((6, 8, 64), (64, 64, 1)), k, k, cu)
+    refuse("out must be float16", f, q, k, k, cu, out=torch.zeros(6, 8, 64))
+    refuse("out must hold", f, q, k, k, cu, out=half(5, 8, 64))
+    refuse("device tensors only", f, half(6, 12, 64)[:, :8], half(6, 12, 64)[:, 8:10], half(6, 12, 64)[:, 10:], cu)
+
+
+def test_paged_attention():
+    q, p, table, n = half(3, 8, 64), half(10, 2, 16, 64), i32(3, 4), i32(3)
+    f = hq.paged_attention
+    refuse("device tensors only", f, q, p, p, table, n)
+    refuse("device tensors only", f, q, p, p, table, n, i32(2), i32(1))
+    refuse("k_pages must be float16", f, q, p.bfloat16(), p, table, n)
+    refuse("k_pages must be \\[pages\\]", f, q, half(10, 2, 16, 128), p, table, n)
+    refuse("v_pages must hold", f, q, p, half(9, 2, 16, 64), table, n)
+    refuse("v_pages must have the shape", f, q, p, half(10, 16, 2, 64), table, n)
+    refuse("k_pages must be contiguous", f, q, p.transpose(0, 1), p, table, n)
+    refuse("table must be \\[requests\\]", f, q, p, p, i32(4, 4), n)
+    refuse("lengths must hold 3", f, q, p, p, table, i32(4))
+    refuse("groups must hold one", f, q, p, p, table, n, i32(0), i32(0))
+    refuse("shared is required", f, q, p, p, table, n, i32(2))
+    refuse("shared goes with groups", f, q, p, p, table, n, None, i32(1))
+    refuse("shared must hold 1", f, q, p, p, table, n, i32(2), i32(2))
+
+
+def test_cache():
+    k, p, table, n = half(5, 2, 64), half(10, 2, 16, 64), i32(3, 4), i32(3)
+    refuse("device tensors only", hq.cache_write, k, k, p, p, table, n, i32(4))
+    refuse("v must have the shape", hq.cache_write, k, half(4, 2, 64), p, p, table, n, i32(4))
+    refuse("k_pages must be \\[pages\\]", hq.cache_write, k, k, half(10, 3, 16, 64), p, table, n, i32(4))
+    refuse("cu must hold 4", hq.cache_write, k, k, p, p, table, n, i32(3))
+    refuse("starts must hold 3", hq.cache_write, k, k, p, p, table, i32(4), i32(4))
+    pool, refs = half(4, 10, 32), i32(10)
+    refuse("device tensors only", hq.cache_step, pool, 16, table, n, refs, n, n)
+    refuse("pool must be \\[planes\\]", hq.cache_step, pool, 16, table, n, i32(9), n, n)
+    refuse("pool must be \\[planes\\]", hq.cache_step, half(4, 10), 16, table, n, refs, n, n)
+    refuse("pool must be contiguous", hq.cache_step, half(10, 4, 32).transpose(0, 1), 16, table, n, refs, n, n)
+    refuse("parent must hold 3", hq.cache_step, pool, 16, table, n, refs, i32(2), n)
+    refuse("add must be int32", hq.cache_step, pool, 16, table, n, refs, n, n.float())
+    refuse("out must hold 5", hq.cache_step, pool, 16, table, n, refs, n, n, out=[table])
+    refuse("out\\[2\\] must hold 10", hq.cache_step, pool, 16, table, n, refs, n, n, out=[table, n, i32(9), n, i32(1)])
+    refuse("device tensors only", hq.cache_compact, pool, table, refs)
+    refuse("out must hold 3", hq.cache_compact, pool, table, refs, out=[table, refs])
+
+
+def test_entry_points():
+    """The C entry points' own checks come before any HIP call."""
+    lib = _lib.load()
+
+    def prompt(**kw):
+        a = dict(q=16, k=16, v=16, out=16, dtype=1, cu_q=16, cu_k=16, seqs=1, tq=4, tk=4, heads=8, kv=2, d=64, qs=512, ks=128, vs=128, scale=0.1,
+                 causal=1, stream=None)
+        a.update(kw)
+        return lib.hq_prompt_attention(*a.values())
+
+    assert prompt(q=None) == -1 and prompt(v=None) == -1 and prompt(cu_q=None) == -1 and prompt(cu_k=None, tk=5) == -1
+    assert prompt(heads=7) == -2 and prompt(d=96) == -2 and prompt(seqs=-1) == -2 and prompt(qs=504) == -2 and prompt(kv=0) == -2
+    assert prompt(scale=-1.0) == -2 and prompt(scale=float("nan")) == -2 and prompt(scale=float("inf")) == -2
+    assert prompt(dtype=0) == -3 and prompt(dtype=7) == -3
+    assert prompt(q=24) == -4 and prompt(qs=516) == -4 and prompt(cu_q=18) == -4 and prompt(out=8) == -4
+    assert prompt(tq=2 ** 40) == -6
+    assert prompt(seqs=0, q=None) == 0 and prompt(tq=0, out=None) == 0
+
+    def paged(**kw):
+        a = dict(q=16, k=16, v=16, out=16, dtype=2, table=16, lengths=16, groups=16, shared=16, ngroups=1, batch=2, width=4, pages=9, page=16, heads=8,
+                 kv=2, d=128, qs=1024, scale=0.1, stream=None)
+        a.update(kw)
+        return lib.hq_paged_attention(*a.values())
+
+    assert paged(q=None) == -1 and paged(table=None) == -1 and paged(groups=None) == -1 and paged(k=None) == -1 and paged(lengths=None) == -1
+    assert paged(page=12) == -2 and paged(page=4) == -2 and paged(page=2048) == -2 and paged(d=32) == -2 and paged(heads=9) == -2 and paged(width=-1) == -2
+    assert paged(dtype=0) == -3 and paged(k=8) == -4 and paged(table=2) == -4
+    assert paged(width=2 ** 30) == -6
+    assert paged(batch=0, q=None) == 0
+
+    def write(**kw):
+        a = dict(k=16, v=16, kp=16, vp=16, dtype=1, table=16, starts=16, cu=16, rows=2, tokens=3, width=4, pages=9, page=16, kv=2, d=64, ks=128, vs=128,
+                 stream=None)
+        a.update(kw)
+        return lib.hq_cache_write(*a.values())
+
+    assert write(k=None) == -1 and write(page=0) == -2 and write(d=12) == -2 and write(ks=120) == -2 and write(dtype=0) == -3 and write(kp=8) == -4
+    assert write(tokens=0, k=None) == 0 and write(rows=0) == 0
+
+    def step(**kw):
+        a = dict(pool=16, planes=2, bytes=32, table=1 << 20, lengths=2 << 20, refs=3 << 20, parent=4 << 20, add=5 << 20, to=6 << 20, lo=7 << 20,
+                 ro=8 << 20, so=9 << 20, missing=10 << 20, rows=3, width=4, pages=9, page=16, stream=None)
+        a.update(kw)
+        return lib.hq_cache_step(*a.values())
+
+    assert step(table=None) == -1 and step(missing=None) == -1 and step(pool=None) == -1 and step(refs=None) == -1
+    assert step(bytes=24) == -2 and step(page=0) == -2 and step(rows=-1) == -2
+    assert step(to=(1 << 20) + 8) == -2 and step(ro=3 << 20) == -2 and step(lo=9 << 20) == -2  # results on top of arguments, or of each other
+    assert step(pool=8) == -4 and step(add=(5 << 20) + 1) == -4 and step(rows=20000, width=100) == -6
+
+    def compact(**kw):
+        a = dict(pool=16, planes=2, bytes=32, table=1 << 20, refs=3 << 20, to=6 << 20, ro=8 << 20, live=10 << 20, rows=3, width=4, pages=9, stream=None)
+        a.update(kw)
+        return lib.hq_cache_compact(*a.values())
+
+    assert compact(live=None) == -1 and compact(pool=None) == -1 and compact(to=1 << 20) == -2 and compact(ro=(3 << 20) + 4) == -2
+    assert compact(bytes=8) == -2 and compact(pool=4) == -4
