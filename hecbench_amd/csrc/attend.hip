@@ -47,11 +47,19 @@ __device__ __forceinline__ float pair_sum(float v) {
 }
 __device__ __forceinline__ float finite_or_zero(float m) { return m == -INFINITY ? 0.f : m; }
 
+// A value that is the same in all lanes, in scalar registers.
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+template <typename P>
+__device__ __forceinline__ const P* uniform(const P* p) {
+  const uint64_t x = (uint64_t)p;
+  return (const P*)((uint64_t)(uint32_t)uniform((int)(x >> 32)) << 32 | (uint32_t)uniform((int)x));
+}
+
 constexpr int kThreads = 256, kWaves = 4;
 
 // What one workgroup attends: up to 128 rows (RW = 4 waves of them, all of which see every key of a tile) or up to 32 rows (RW = 1,
 // the waves share the tile's keys among them).
-template <typename T, int D, int RW>
+template <typename T, int D, int RW, bool DIRECT = false>
 struct Attend {
   typedef typename Kind<T>::V8 V8;
   static constexpr int KW = kWaves / RW;            // waves that divide a tile's keys
@@ -60,7 +68,8 @@ struct Attend {
   static constexpr int CH = D / 8;                  // 16-byte pieces of a row
   static constexpr int NL = TILE * CH / kThreads;   // pieces that a thread brings
   static constexpr int STEP = kThreads / CH;        // rows between two of them
-  static constexpr int LDS = 2 * TILE * D * 2;
+  static constexpr int BUF = 2 * TILE * D * 2;      // a tile's keys and values
+  static constexpr int LDS = (DIRECT ? 2 : 1) * BUF;
 
   // A row's pieces are stored in an order that depends on the row, so that the lanes of a read pass meet different banks: the keys'
   // pieces by all bits of the row, which 16 lanes read piece by piece, the values' by the two bits of the four rows that a
@@ -96,6 +105,53 @@ struct Attend {
     }
   }
 
+  // DIRECT: a tile goes from memory into LDS past the registers, its second buffer is filled while the first is worked on, and one barrier
+  // a tile does.  An instruction brings 1 KB, the lanes' pieces one behind the other, so it is the lane's address that follows the
+  // order of the pieces.
+  uint32_t koff[NL], voff[NL];
+  static __device__ __forceinline__ int direct_row(int i) { return ((threadIdx.x >> 6) * NL + i) * (64 / CH) + (threadIdx.x & 63) / CH; }
+  template <typename SRC>
+  __device__ __forceinline__ void direct_offsets(const SRC& src, int rows) {
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      const int row = direct_row(i), r = min(row, rows - 1), ch = threadIdx.x % CH;
+      koff[i] = (uint32_t)(r * (int)src.ks + k_piece(row, ch) * 8) * 2;
+      voff[i] = (uint32_t)(r * (int)src.vs + v_piece(row, ch) * 8) * 2;
+    }
+  }
+  template <typename SRC>
+  __device__ __forceinline__ void direct_load(const SRC& src, int base, char* buf) {
+    const T *kb = uniform(src.k + base * src.ks), *vb = uniform(src.v + base * src.vs);
+    const uint32_t lds = uniform((int)((uint32_t)(uintptr_t)(lds_char*)buf + (threadIdx.x >> 6) * (NL * 1024)));
+#pragma unroll
+    for (int i = 0; i < NL; ++i)
+      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds + i * 1024), "v"(koff[i]), "s"(kb) : "memory");
+#pragma unroll
+    for (int i = 0; i < NL; ++i)
+      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds + TILE * D * 2 + i * 1024), "v"(voff[i]), "s"(vb)
+                   : "memory");
+  }
+  // What store() does on the way, on a tile that is in LDS.
+  __device__ __forceinline__ void clean(uint32_t (&bad)[(NL + 3) / 4]) {
+    hq_u4v* vs = reinterpret_cast<hq_u4v*>(sm + TILE * D * 2) + threadIdx.x;
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      hq_u4v v = vs[i * kThreads];
+      if (i % 4 == 0) bad[i / 4] = 0;
+      uint32_t found = 0;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const uint32_t e = ((v[w] & Kind<T>::kExp) + Kind<T>::kStep) & 0x80008000u;
+        found |= ((e >> 15 & 1u) | (e >> 30 & 2u)) << (2 * w);
+        v[w] &= ~((e >> 15) * 0xffffu);
+      }
+      if (found) {
+        bad[i / 4] |= found << (8 * (i % 4));
+        vs[i * kThreads] = v;
+      }
+    }
+  }
+
   // Into LDS.  In a tile that not every row sees whole, a value that is not finite would reach the rows that do not see it (0 times
   // infinity): it is stored as zero, and the bits returned say which values were.
   __device__ __forceinline__ void store(bool partly, uint32_t (&bad)[(NL + 3) / 4]) {
@@ -125,14 +181,18 @@ struct Attend {
     char* vs = sm + TILE * D * 2;
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
-      const int row = row0 + i * STEP;
       hq_u4v w;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const uint32_t b = bad[i / 4] >> (8 * (i % 4) + 2 * j);
         w[j] = (b & 1 ? Kind<T>::kOne & 0xffffu : 0u) | (b & 2 ? Kind<T>::kOne & 0xffff0000u : 0u);
       }
-      *reinterpret_cast<hq_u4v*>(vs + row * D * 2 + v_piece(row, ch) * 16) = w;
+      if (DIRECT) {
+        reinterpret_cast<hq_u4v*>(vs)[threadIdx.x + i * kThreads] = w;
+      } else {
+        const int row = row0 + i * STEP;
+        *reinterpret_cast<hq_u4v*>(vs + row * D * 2 + v_piece(row, ch) * 16) = w;
+      }
     }
   }
 
@@ -181,13 +241,19 @@ struct Attend {
 #pragma unroll
       for (int r = 0; r < 16; ++r) top = fmaxf(top, s[b][r]);
     top = pair_max(top) * c;
-    const float mn = fmaxf(m, top), ms = finite_or_zero(mn), f = __builtin_amdgcn_exp2f(m - ms);
-    m = mn;
-    l *= f;
+    // A maximum that has grown by less than 2^8 stays: the weights may then be up to 2^8, which neither fp32 sums nor the 16-bit
+    // weights mind, and the sums need no scaling.  The scaling of 64 registers a tile was a fifth of the vector instructions.
+    if (__builtin_amdgcn_ballot_w64(top > m + 8.f)) {
+      const float mn = top > m + 8.f ? top : m;  // each row by its own scores: its bits do not depend on its neighbours
+      const float f = mn == m ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+      m = mn;
+      l *= f;
 #pragma unroll
-    for (int d = 0; d < D / 32; ++d)
+      for (int d = 0; d < D / 32; ++d)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) o[d][r] *= f;
+        for (int r = 0; r < 16; ++r) o[d][r] *= f;
+    }
+    const float ms = finite_or_zero(m);
     V8 p[NB][2];
 #pragma unroll
     for (int b = 0; b < NB; ++b)
@@ -205,7 +271,7 @@ struct Attend {
       for (int b = 0; b < NB; ++b)
 #pragma unroll
         for (int t = 0; t < 2; ++t) o[d] = Kind<T>::mfma(v_operand(key0, b, t, d), p[b][t], o[d]);
-    if (partly && *(volatile int*)poison == tileno) {  // rows that see a value that is not finite
+    if (partly && *(volatile __attribute__((address_space(3))) int*)poison == tileno) {  // rows that see a value that is not finite
       __syncthreads();
       store_bad(bad);
       __syncthreads();
@@ -253,6 +319,38 @@ struct Attend {
     }
     l = pair_sum(l);
   }
+
+  template <typename SRC>
+  __device__ __forceinline__ void run_direct(const SRC& src, int end, int whole, float c) {
+    clear();
+    if (end <= 0) return;
+    uint32_t bad[(NL + 3) / 4] = {};
+    char* const bufs = sm;
+#pragma unroll
+    for (int kk = 0; kk < D / 16; ++kk) asm volatile("" : "+v"(qf[kk]));  // here, not at every tile: the loads in flight then are the next tile's
+    direct_offsets(src, src.n);
+    direct_load(src, 0, bufs);
+    for (int base = 0, tileno = 0; base < end; base += TILE, ++tileno) {
+      const bool partly = base + TILE > whole;
+      sm = bufs + (tileno & 1) * BUF;
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __syncthreads();
+      if (base + TILE < end) {
+        if (base + 2 * TILE > src.n) direct_offsets(src, src.n - base - TILE);
+        direct_load(src, base + TILE, bufs + (~tileno & 1) * BUF);
+      }
+      if (partly) {
+        clean(bad);
+        uint32_t any = 0;
+#pragma unroll
+        for (int i = 0; i < (NL + 3) / 4; ++i) any |= bad[i];
+        if (any) *poison = tileno;
+        __syncthreads();
+      }
+      tile(base, partly, c, tileno, bad);
+    }
+    l = pair_sum(l);
+  }
 };
 
 // Sets up the poison word; a barrier of run() lies between this and its first use.
@@ -284,8 +382,8 @@ __device__ __forceinline__ bool find_tile(const int* bounds, int n, int x, F til
     if (x < total) {
       const unsigned long long past = __ballot(sum > x);
       const int at = __ffsll((unsigned long long)past) - 1;
-      *entry = i0 + at;
-      *which = x - (__shfl(sum, at) - __shfl(t, at));
+      *entry = __builtin_amdgcn_readfirstlane(i0 + at);
+      *which = __builtin_amdgcn_readfirstlane(x - (__shfl(sum, at) - __shfl(t, at)));
       return true;
     }
     x -= total;
@@ -318,7 +416,7 @@ struct PackedKeys {  // of one sequence and one head
 
 template <typename T, int D, int RW>
 __global__ __launch_bounds__(kThreads, 2) void prompt_kernel(PromptArgs a) {
-  typedef Attend<T, D, RW> A;
+  typedef Attend<T, D, RW, true> A;
   typedef typename Kind<T>::V8 V8;
   constexpr int ROWS = 32 * RW;
   extern __shared__ __align__(16) char sm[];
@@ -350,7 +448,7 @@ __global__ __launch_bounds__(kThreads, 2) void prompt_kernel(PromptArgs a) {
   auto limit = [&](int t) { return a.causal ? min(max(t + 1 + nk - nq, 0), nk) : nk; };
   w.lim = limit(token);
   PackedKeys<T> src{(const T*)a.k + (int64_t)k0 * a.ks + head * D, (const T*)a.v + (int64_t)k0 * a.vs + head * D, a.ks, a.vs, nk};
-  w.run(src, 0, limit(last_row / ratio), limit(first_row / ratio), a.c);
+  w.run_direct(src, uniform(limit(last_row / ratio)), uniform(limit(first_row / ratio)), a.c);
   float inv = 1.f / w.l;
   if (w.lim == 0) inv = 0.f;  // sees no key
   if (RW == 4) {
@@ -572,7 +670,7 @@ template <typename T, int D>
 int launch_prompt(const PromptArgs& a, hipStream_t stream) {
   const int64_t items = ((int64_t)a.total_q * a.ratio / 128 + a.seqs) * a.kv_heads;
   if (items > INT_MAX) return HQ_ERR_TOO_LARGE;
-  return hq_launch_as_is(prompt_kernel<T, D, 4>, dim3((unsigned)items), dim3(kThreads), Attend<T, D, 4>::LDS, stream, a);
+  return hq_launch_as_is(prompt_kernel<T, D, 4>, dim3((unsigned)items), dim3(kThreads), Attend<T, D, 4, true>::LDS, stream, a);
 }
 
 template <typename T, int D>
