@@ -8,6 +8,7 @@
 // transposed, S^T = K Q^T: the matrix core leaves a row's scores in one lane and its partner 32 lanes on, so maximum and sum are
 // sums within a lane and one exchange, and the same registers are, rounded, the operand of O^T = V^T P^T without another move: the
 // order of the keys in that sum is free, and the transposing LDS read fetches V's rows in the order in which S^T left them.
+#include <algorithm>
 #include <climits>
 #include <cmath>
 
@@ -57,6 +58,12 @@ __device__ __forceinline__ const P* uniform(const P* p) {
 
 constexpr int kThreads = 256, kWaves = 4;
 
+__device__ __forceinline__ int wave_min(int v) {
+#pragma unroll
+  for (int d = 32; d; d >>= 1) v = min(v, __shfl_xor(v, d));
+  return v;
+}
+
 // What one workgroup attends: up to 128 rows (RW = 4 waves of them, all of which see every key of a tile) or up to 32 rows (RW = 1,
 // the waves share the tile's keys among them).
 template <typename T, int D, int RW, bool DIRECT = false>
@@ -83,9 +90,12 @@ struct Attend {
   f32x16 o[D / 32];
   float m = -INFINITY, l = 0.f;
   hq_u4v kr[NL], vr[NL];
-  int lim;  // keys below this are seen by the lane's row
+  int lim;              // keys below this are seen by the lane's row
+  int all_see, any_sees;  // below the first by all rows of the wave, below the second by one of them
 
   __device__ __forceinline__ void clear() {
+    all_see = uniform(wave_min(lim));
+    any_sees = -uniform(wave_min(-lim));
 #pragma unroll
     for (int d = 0; d < D / 32; ++d)
 #pragma unroll
@@ -134,21 +144,26 @@ struct Attend {
   // What store() does on the way, on a tile that is in LDS.
   __device__ __forceinline__ void clean(uint32_t (&bad)[(NL + 3) / 4]) {
     hq_u4v* vs = reinterpret_cast<hq_u4v*>(sm + TILE * D * 2) + threadIdx.x;
+    hq_u4v v[NL];
+    uint32_t any = 0;
+#pragma unroll
+    for (int i = 0; i < NL; ++i) v[i] = vs[i * kThreads];
+#pragma unroll
+    for (int i = 0; i < NL; ++i)
+#pragma unroll
+      for (int w = 0; w < 4; ++w) any |= (v[i][w] & Kind<T>::kExp) + Kind<T>::kStep;
+#pragma unroll
+    for (int i = 0; i < (NL + 3) / 4; ++i) bad[i] = 0;
+    if (!(any & 0x80008000u)) return;
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
-      hq_u4v v = vs[i * kThreads];
-      if (i % 4 == 0) bad[i / 4] = 0;
-      uint32_t found = 0;
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
-        const uint32_t e = ((v[w] & Kind<T>::kExp) + Kind<T>::kStep) & 0x80008000u;
-        found |= ((e >> 15 & 1u) | (e >> 30 & 2u)) << (2 * w);
-        v[w] &= ~((e >> 15) * 0xffffu);
+        const uint32_t e = ((v[i][w] & Kind<T>::kExp) + Kind<T>::kStep) & 0x80008000u;
+        bad[i / 4] |= ((e >> 15 & 1u) | (e >> 30 & 2u)) << (8 * (i % 4) + 2 * w);
+        v[i][w] &= ~((e >> 15) * 0xffffu);
       }
-      if (found) {
-        bad[i / 4] |= found << (8 * (i % 4));
-        vs[i * kThreads] = v;
-      }
+      vs[i * kThreads] = v[i];
     }
   }
 
@@ -212,10 +227,9 @@ struct Attend {
     return u.v;
   }
 
-  // One tile, keys from `base` on.  partly: not every row of the workgroup sees all of it.
-  __device__ __forceinline__ void tile(int base, bool partly, float c, int tileno, const uint32_t (&bad)[(NL + 3) / 4]) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
-    const int key0 = RW == 4 ? 0 : wave * 32 * NB;
+  // The wave's part of a tile, keys from base + key0 on.
+  __device__ __forceinline__ void attend_tile(int base, int key0, int left, float c) {
+    const int lane = threadIdx.x & 63, half = lane >> 5;
     f32x16 s[NB];
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
@@ -228,8 +242,7 @@ struct Attend {
         s[b] = Kind<T>::mfma(a, qf[kk], s[b]);
       }
     }
-    const int left = lim - base - key0 - 4 * half;  // a key of the registers below it is seen
-    if (partly) {
+    if (base + key0 + 32 * NB > all_see) {
 #pragma unroll
       for (int b = 0; b < NB; ++b)
 #pragma unroll
@@ -271,6 +284,14 @@ struct Attend {
       for (int b = 0; b < NB; ++b)
 #pragma unroll
         for (int t = 0; t < 2; ++t) o[d] = Kind<T>::mfma(v_operand(key0, b, t, d), p[b][t], o[d]);
+  }
+
+  // One tile, keys from `base` on.  partly: not every row of the workgroup sees all of it.
+  __device__ __forceinline__ void tile(int base, bool partly, float c, int tileno, const uint32_t (&bad)[(NL + 3) / 4]) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
+    const int key0 = RW == 4 ? 0 : wave * 32 * NB;
+    const int left = lim - base - key0 - 4 * half;  // a key of the registers below it is seen
+    if (base + key0 < any_sees) attend_tile(base, key0, left, c);
     if (partly && *(volatile __attribute__((address_space(3))) int*)poison == tileno) {  // rows that see a value that is not finite
       __syncthreads();
       store_bad(bad);
@@ -293,6 +314,18 @@ struct Attend {
         for (int r = 0; r < 16; ++r) o[d][r] = n[r] > 0.f ? NAN : o[d][r];
       }
     }
+  }
+
+  // The row's sums as one of several shares; none: the row sees nothing in any of them, which share 0 says by an infinite maximum.
+  __device__ __forceinline__ void put_share(float* po, float* pm, int64_t at, bool none) const {
+    const int half = (threadIdx.x >> 5) & 1;
+    if (m != -INFINITY)  // a share that no key went into is not read
+#pragma unroll
+      for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          *reinterpret_cast<hq_f4v*>(po + at * D + 32 * d + 8 * g + 4 * half) = hq_f4v{o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]};
+    if (half == 0) *reinterpret_cast<float2*>(pm + 2 * at) = float2{none ? INFINITY : m, l};
   }
 
   // Keys [first, end) of src; whole: keys below it are seen by every row of the workgroup.
@@ -321,16 +354,16 @@ struct Attend {
   }
 
   template <typename SRC>
-  __device__ __forceinline__ void run_direct(const SRC& src, int end, int whole, float c) {
+  __device__ __forceinline__ void run_direct(const SRC& src, int first, int end, int whole, float c) {
     clear();
-    if (end <= 0) return;
+    if (first >= end) return;
     uint32_t bad[(NL + 3) / 4] = {};
     char* const bufs = sm;
 #pragma unroll
     for (int kk = 0; kk < D / 16; ++kk) asm volatile("" : "+v"(qf[kk]));  // here, not at every tile: the loads in flight then are the next tile's
-    direct_offsets(src, src.n);
-    direct_load(src, 0, bufs);
-    for (int base = 0, tileno = 0; base < end; base += TILE, ++tileno) {
+    direct_offsets(src, src.n - first);
+    direct_load(src, first, bufs);
+    for (int base = first, tileno = 0; base < end; base += TILE, ++tileno) {
       const bool partly = base + TILE > whole;
       sm = bufs + (tileno & 1) * BUF;
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -358,32 +391,28 @@ __device__ __forceinline__ void set_up(int* poison) {
   if (threadIdx.x == 0) *poison = -1;
 }
 
-__device__ __forceinline__ int wave_min(int v) {
-#pragma unroll
-  for (int d = 32; d; d >>= 1) v = min(v, __shfl_xor(v, d));
-  return v;
-}
-
-// Item x of a list in which entry i has tiles(n_i) tiles, n_i = bounds[i + 1] - bounds[i]: the entry, and which of its tiles.  A wave
-// looks at 64 entries at a time.
+// Item x of a list in which entry i, bounds[i] to bounds[i + 1], cut to 0 ... most, has tiles(its length) tiles: the entry, its begin and
+// length, and which of its tiles.  A wave looks at 64 entries at a time.
 template <typename F>
-__device__ __forceinline__ bool find_tile(const int* bounds, int n, int x, F tiles, int* entry, int* which) {
+__device__ __forceinline__ bool find_tile(const int* bounds, int n, int most, int x, F tiles, int* entry, int* begin, int* length, int* which) {
   const int lane = threadIdx.x & 63;
   for (int i0 = 0; i0 < n; i0 += 64) {
     const int i = i0 + lane;
-    int t = i < n ? tiles(bounds[i], bounds[i + 1]) : 0;
+    const int b = i < n ? min(max(bounds[i], 0), most) : 0, len = i < n ? min(max(bounds[i + 1], b), most) - b : 0;
+    const int t = tiles(len);
     int sum = t;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
       const int u = __shfl_up(sum, d);
       if (lane >= d) sum += u;
     }
-    const int total = __shfl(sum, 63);
+    const int total = __builtin_amdgcn_readlane(sum, 63);
     if (x < total) {
-      const unsigned long long past = __ballot(sum > x);
-      const int at = __ffsll((unsigned long long)past) - 1;
-      *entry = __builtin_amdgcn_readfirstlane(i0 + at);
-      *which = __builtin_amdgcn_readfirstlane(x - (__shfl(sum, at) - __shfl(t, at)));
+      const int at = __ffsll(__ballot(sum > x)) - 1;
+      *entry = i0 + at;
+      *begin = __builtin_amdgcn_readlane(b, at);
+      *length = __builtin_amdgcn_readlane(len, at);
+      *which = x - __builtin_amdgcn_readlane(sum - t, at);
       return true;
     }
     x -= total;
@@ -397,7 +426,8 @@ struct PromptArgs {
   void* out;
   const int *cu_q, *cu_k;
   int64_t qs, ks, vs;  // elements from one token to the next
-  int seqs, total_q, total_k, heads, kv_heads, ratio, causal;
+  float *po, *pm;      // shares of the sums [total_q * heads][shares][D], and {maximum, sum} [total_q * heads][shares]
+  int seqs, total_q, total_k, heads, kv_heads, ratio, causal, shares;
   float c;
 };
 
@@ -414,29 +444,28 @@ struct PackedKeys {  // of one sequence and one head
   }
 };
 
-template <typename T, int D, int RW>
-__global__ __launch_bounds__(kThreads, 2) void prompt_kernel(PromptArgs a) {
-  typedef Attend<T, D, RW, true> A;
+// A workgroup's rows and share of the keys.  Many rows: all keys, and the result; few: the keys are divided among `shares` workgroups.
+template <typename T, int D>
+__global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void prompt_kernel(PromptArgs a) {
+  typedef Attend<T, D, 4, true> A;
   typedef typename Kind<T>::V8 V8;
-  constexpr int ROWS = 32 * RW;
+  constexpr int ROWS = 128;
   extern __shared__ __align__(16) char sm[];
   __shared__ int poison;
-  const int head = blockIdx.x % a.kv_heads;
-  int seq, tile;
-  const int total_q = a.total_q, total_k = a.total_k, ratio = a.ratio;
-  auto tiles = [=](int b, int e) {
-    b = min(max(b, 0), total_q);
-    e = min(max(e, b), total_q);
-    return (int)(((int64_t)(e - b) * ratio + ROWS - 1) / ROWS);
-  };
-  if (!find_tile(a.cu_q, a.seqs, blockIdx.x / a.kv_heads, tiles, &seq, &tile)) return;
-  const int q0 = min(max(a.cu_q[seq], 0), total_q), nq = min(max(a.cu_q[seq + 1], q0), total_q) - q0;
-  const int k0 = min(max(a.cu_k[seq], 0), total_k), nk = min(max(a.cu_k[seq + 1], k0), total_k) - k0;
+  int x = blockIdx.x;
+  const int head = x % a.kv_heads;
+  x /= a.kv_heads;
+  const int share = x % a.shares;
+  x /= a.shares;
+  const int ratio = a.ratio;
+  int seq, tile, q0, nq;
+  if (!find_tile(a.cu_q, a.seqs, a.total_q, x, [=](int n) { return (int)((n * (int64_t)ratio + ROWS - 1) / ROWS); }, &seq, &q0, &nq, &tile)) return;
+  const int k0 = min(max(a.cu_k[seq], 0), a.total_k), nk = min(max(a.cu_k[seq + 1], k0), a.total_k) - k0;
   const int rows = nq * ratio;
   tile = (rows + ROWS - 1) / ROWS - 1 - tile;  // the tiles with most keys come first
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int first_row = tile * ROWS, last_row = min(first_row + ROWS, rows) - 1;
-  const int row = first_row + (RW == 4 ? wave * 32 : 0) + (lane & 31), r = min(row, last_row);
+  const int row = first_row + wave * 32 + (lane & 31), r = min(row, last_row);
   const int token = r / ratio, h = head * ratio + r % ratio;
   A w;
   w.sm = sm;
@@ -448,11 +477,12 @@ __global__ __launch_bounds__(kThreads, 2) void prompt_kernel(PromptArgs a) {
   auto limit = [&](int t) { return a.causal ? min(max(t + 1 + nk - nq, 0), nk) : nk; };
   w.lim = limit(token);
   PackedKeys<T> src{(const T*)a.k + (int64_t)k0 * a.ks + head * D, (const T*)a.v + (int64_t)k0 * a.vs + head * D, a.ks, a.vs, nk};
-  w.run_direct(src, uniform(limit(last_row / ratio)), uniform(limit(first_row / ratio)), a.c);
-  float inv = 1.f / w.l;
-  if (w.lim == 0) inv = 0.f;  // sees no key
-  if (RW == 4) {
-    if (row > last_row) return;
+  const int each = a.shares == 1 ? nk : max(256, ((nk + a.shares - 1) / a.shares + A::TILE - 1) & -A::TILE);
+  const int end = uniform(limit(last_row / ratio)), first = (int)min((int64_t)share * each, (int64_t)end);
+  w.run_direct(src, first, min(end, first + each), uniform(limit(first_row / ratio)), a.c);
+  if (row > last_row) return;
+  if (a.shares == 1) {
+    const float inv = 1.f / w.l;
     T* out = (T*)a.out + ((int64_t)(q0 + token) * a.heads + h) * D + 4 * (lane >> 5);
 #pragma unroll
     for (int d = 0; d < D / 32; ++d)
@@ -461,9 +491,11 @@ __global__ __launch_bounds__(kThreads, 2) void prompt_kernel(PromptArgs a) {
         typedef T T4 __attribute__((ext_vector_type(4)));
         T4 v;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = (T)(w.lim == 0 ? 0.f : w.o[d][4 * g + i] * inv);
+        for (int i = 0; i < 4; ++i) v[i] = (T)(w.lim == 0 ? 0.f : w.o[d][4 * g + i] * inv);  // a token that sees no key
         *reinterpret_cast<T4*>(out + 32 * d + 8 * g) = v;
       }
+  } else {
+    w.put_share(a.po, a.pm, ((int64_t)(q0 + token) * a.heads + h) * a.shares + share, w.lim == 0);
   }
 }
 
@@ -579,17 +611,7 @@ __device__ __forceinline__ void attend_rows(const PagedArgs& a, char* sm, int* p
       }
     }
   } else {
-    if (row > last_row) return;
-#pragma unroll
-    for (int d = 0; d < D / 32; ++d)
-#pragma unroll
-      for (int g = 0; g < 4; ++g)
-        *reinterpret_cast<hq_f4v*>(a.po + at * D + 32 * d + 8 * g + 4 * (lane >> 5)) =
-            hq_f4v{w.o[d][4 * g], w.o[d][4 * g + 1], w.o[d][4 * g + 2], w.o[d][4 * g + 3]};
-    if (lane < 32) {
-      a.pm[2 * at] = w.m;
-      a.pm[2 * at + 1] = w.l;
-    }
+    if (row <= last_row) w.put_share(a.po, a.pm, at, false);
   }
 }
 
@@ -603,15 +625,9 @@ __global__ __launch_bounds__(kThreads, 2) void paged_kernel(PagedArgs a) {
     const int head = x % a.kv_heads;
     x /= a.kv_heads;
     const int share = x % a.np;
-    int g, tile;
-    const int batch = a.batch, ratio = a.ratio;
-    auto tiles = [=](int b, int e) {
-      b = min(max(b, 0), batch);
-      e = min(max(e, b), batch);
-      return (int)(((int64_t)(e - b) * ratio + 127) / 128);
-    };
-    if (!find_tile(a.groups, a.ngroups, x / a.np, tiles, &g, &tile)) return;
-    const int b0 = min(max(a.groups[g], 0), batch), nb = min(max(a.groups[g + 1], b0), batch) - b0;
+    int g, tile, b0, nb;
+    const int ratio = a.ratio;
+    if (!find_tile(a.groups, a.ngroups, a.batch, x / a.np, [=](int n) { return (int)((n * (int64_t)ratio + 127) / 128); }, &g, &b0, &nb, &tile)) return;
     const int n = shared_tokens(a, g);
     int first, end;
     share_of(n, a.np, share, &first, &end);
@@ -636,29 +652,65 @@ __global__ __launch_bounds__(kThreads, 2) void paged_kernel(PagedArgs a) {
   }
 }
 
-// The shares of a row (request, head) together: one wave a row.
+// The shares of a row together, one wave a row: their maxima and sums a lane each, then the sums of the values, 16 bytes a lane,
+// several shares at a time.  first: shares before it were not written.
 template <typename T, int D>
-__global__ __launch_bounds__(kThreads) void join_kernel(PagedArgs a) {
+__device__ __forceinline__ void join_shares(const float* po, const float* pm, int64_t row, int first, int slots, bool none, T* out) {
+  constexpr int LANES = D / 4, AT_ONCE = 64 / LANES;  // lanes of a share, shares of a load
+  const int lane = threadIdx.x & 63, d = (lane % LANES) * 4;
+  const float2* ml = reinterpret_cast<const float2*>(pm) + row * slots;
+  float m = -INFINITY;
+  for (int s = first + lane; s < slots; s += 64) m = fmaxf(m, ml[s].x);
+  m = hq_wave_max(m);
+  const float ms = finite_or_zero(m);
+  float l = 0.f;
+  hq_f4v o = {0.f, 0.f, 0.f, 0.f};
+  for (int s0 = first; s0 < slots; s0 += 64) {
+    const int s = s0 + lane;
+    const float2 mine = s < slots ? ml[s] : float2{-INFINITY, 0.f};
+    const float f = __builtin_amdgcn_exp2f(mine.x - ms);
+    l += mine.y * f;
+    const int n = min(slots - s0, 64);
+#pragma unroll 4
+    for (int i = 0; i < n; i += AT_ONCE) {
+      const int at = i + lane / LANES;
+      const float w = __shfl(f, at & 63);
+      if (at < n && w != 0.f) o += *reinterpret_cast<const hq_f4v*>(po + (row * slots + s0 + at) * D + d) * w;
+    }
+  }
+  l = hq_wave_sum(l);
+#pragma unroll
+  for (int x = LANES; x < 64; x <<= 1)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] += __shfl_xor(o[i], x);
+  if (lane < LANES) {
+    typedef T T4 __attribute__((ext_vector_type(4)));
+    T4 v;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = (T)(none ? 0.f : o[i] / l);
+    *reinterpret_cast<T4*>(out + row * D + d) = v;
+  }
+}
+
+template <typename T, int D>
+__global__ __launch_bounds__(kThreads) void join_paged_kernel(PagedArgs a) {
   const int64_t row = (int64_t)blockIdx.x * kWaves + (threadIdx.x >> 6);
   if (row >= (int64_t)a.batch * a.heads) return;
-  const int lane = threadIdx.x & 63, slots = a.np + a.ns;
-  bool grouped = false;
   const int b = row / a.heads;
+  bool grouped = false;
   for (int g = 0; g < a.ngroups; ++g) grouped |= b >= a.groups[g] && b < a.groups[g + 1];
-  const int s0 = grouped ? 0 : a.np;  // nobody wrote the common shares of a request without a group
-  float m = -INFINITY;
-  for (int s = s0; s < slots; ++s) m = fmaxf(m, a.pm[2 * (row * slots + s)]);
-  const float ms = finite_or_zero(m);
-  float l = 0.f, o[D / 64] = {};
-  for (int s = s0; s < slots; ++s) {
-    const float f = __builtin_amdgcn_exp2f(a.pm[2 * (row * slots + s)] - ms);
-    l += f * a.pm[2 * (row * slots + s) + 1];
-#pragma unroll
-    for (int i = 0; i < D / 64; ++i) o[i] += f * a.po[(row * slots + s) * D + 64 * i + lane];
-  }
-  const bool none = a.lengths[b] <= 0;
-#pragma unroll
-  for (int i = 0; i < D / 64; ++i) ((T*)a.out)[row * D + 64 * i + lane] = (T)(none ? 0.f : o[i] / l);
+  // nobody wrote the common shares of a request without a group
+  join_shares<T, D>(a.po, a.pm, row, grouped ? 0 : a.np, a.np + a.ns, a.lengths[b] <= 0, (T*)a.out);
+}
+
+template <typename T, int D>
+__global__ __launch_bounds__(kThreads) void join_prompt_kernel(PromptArgs a) {
+  const int64_t row = (int64_t)blockIdx.x * kWaves + (threadIdx.x >> 6);
+  if (row >= (int64_t)a.total_q * a.heads) return;
+  const int token = row / a.heads;
+  if (token < a.cu_q[0] || token >= a.cu_q[a.seqs]) return;
+  const float2 first = reinterpret_cast<const float2*>(a.pm)[row * a.shares];
+  join_shares<T, D>(a.po, a.pm, row, 0, a.shares, first.x == INFINITY && first.y == 0.f, (T*)a.out);
 }
 
 // Scores are compared and masked by -infinity before they are scaled: a scale of zero (all keys alike) becomes one that no score notices.
@@ -666,11 +718,25 @@ float exponent_scale(float s) { return s * 1.44269504088896340736f > 1e-30f ? s 
 bool bad_scale(float s) { return !(s >= 0.f) || std::isinf(s); }
 bool misaligned(const void* p, int64_t stride) { return ((uintptr_t)p & 15) || stride % 8; }
 
+// Few rows leave compute units idle, and each of their workgroups with all keys: then the keys are divided, so that there are up to
+// two workgroups a compute unit, each with 256 keys at least.
 template <typename T, int D>
-int launch_prompt(const PromptArgs& a, hipStream_t stream) {
+int launch_prompt(PromptArgs a, int cus, hipStream_t stream) {
   const int64_t items = ((int64_t)a.total_q * a.ratio / 128 + a.seqs) * a.kv_heads;
-  if (items > INT_MAX) return HQ_ERR_TOO_LARGE;
-  return hq_launch_as_is(prompt_kernel<T, D, 4>, dim3((unsigned)items), dim3(kThreads), Attend<T, D, 4, true>::LDS, stream, a);
+  const int64_t want = 2 * (int64_t)cus / items, most = ((int64_t)a.total_k + 255) / 256;
+  a.shares = (int)std::max<int64_t>(1, std::min(want, most));
+  if (items * a.shares > INT_MAX) return HQ_ERR_TOO_LARGE;
+  const int64_t rows = (int64_t)a.total_q * a.heads;
+  if (a.shares > 1) {
+    HqWorkspace ws;
+    const int rc = hq_get_workspace(stream, (size_t)(rows * a.shares * (D + 2)), 0, &ws);
+    if (rc != HQ_OK) return rc;
+    a.po = ws.partial;
+    a.pm = ws.partial + rows * a.shares * D;
+  }
+  const int rc = hq_launch_as_is(prompt_kernel<T, D>, dim3((unsigned)(items * a.shares)), dim3(kThreads), Attend<T, D, 4, true>::LDS, stream, a);
+  if (rc != HQ_OK || a.shares == 1) return rc;
+  return hq_launch_as_is(join_prompt_kernel<T, D>, dim3((unsigned)((rows + kWaves - 1) / kWaves)), dim3(kThreads), 0, stream, a);
 }
 
 template <typename T, int D>
@@ -702,7 +768,7 @@ int launch_paged(PagedArgs a, int cus, hipStream_t stream) {
   if (attr != hipSuccess) return (int)attr;
   int rc = hq_launch_as_is(paged_kernel<T, D>, dim3((unsigned)grid), dim3(kThreads), most_lds, stream, a);
   if (rc != HQ_OK || slots == 1) return rc;
-  return hq_launch_as_is(join_kernel<T, D>, dim3((unsigned)((rows + kWaves - 1) / kWaves)), dim3(kThreads), 0, stream, a);
+  return hq_launch_as_is(join_paged_kernel<T, D>, dim3((unsigned)((rows + kWaves - 1) / kWaves)), dim3(kThreads), 0, stream, a);
 }
 
 // One of the four kernels by type and head size.
@@ -726,13 +792,14 @@ extern "C" int hq_prompt_attention(const void* q, const void* k, const void* v, 
   if (misaligned(q, q_stride) || misaligned(k, k_stride) || misaligned(v, v_stride) || ((uintptr_t)out & 15) ||
       (((uintptr_t)cu_q | (uintptr_t)cu_k) & 3))
     return HQ_ERR_MISALIGNED;
-  if (total_q * (heads / kv_heads) > INT_MAX - 128 || total_k > INT_MAX - 128) return HQ_ERR_TOO_LARGE;
+  if (total_q * (heads / kv_heads) > INT_MAX - 128 || total_k > INT_MAX - 128 || k_stride > 1 << 24 || v_stride > 1 << 24)  // 32-bit offsets in a tile
+    return HQ_ERR_TOO_LARGE;
   const HqDevice* dev = nullptr;
   const int rc = hq_current_device(&dev);
   if (rc != HQ_OK) return rc;
-  const PromptArgs a{q, k, v, out, cu_q, cu_k ? cu_k : cu_q, q_stride, k_stride, v_stride, seqs, (int)total_q, (int)total_k, heads, kv_heads,
-                     heads / kv_heads, causal != 0, exponent_scale(scale)};
-  return HQ_BY_TYPE(launch_prompt, a, (hipStream_t)stream);
+  const PromptArgs a{q, k, v, out, cu_q, cu_k ? cu_k : cu_q, q_stride, k_stride, v_stride, nullptr, nullptr, seqs, (int)total_q, (int)total_k, heads, kv_heads,
+                     heads / kv_heads, causal != 0, 1, exponent_scale(scale)};
+  return HQ_BY_TYPE(launch_prompt, a, dev->cus, (hipStream_t)stream);
 }
 
 extern "C" int hq_paged_attention(const void* q, const void* k_pages, const void* v_pages, void* out, int dtype, const int32_t* table,
