@@ -11,6 +11,7 @@
 #include <algorithm>
 #include <climits>
 #include <cmath>
+#include <type_traits>
 
 #include "hq_internal.h"
 
@@ -94,8 +95,6 @@ struct Attend {
   int all_see, any_sees;  // below the first by all rows of the wave, below the second by one of them
 
   __device__ __forceinline__ void clear() {
-    all_see = uniform(wave_min(lim));
-    any_sees = -uniform(wave_min(-lim));
 #pragma unroll
     for (int d = 0; d < D / 32; ++d)
 #pragma unroll
@@ -119,31 +118,28 @@ struct Attend {
   // a tile does.  An instruction brings 1 KB, the lanes' pieces one behind the other, so it is the lane's address that follows the
   // order of the pieces.
   uint32_t koff[NL], voff[NL];
-  static __device__ __forceinline__ int direct_row(int i) { return ((threadIdx.x >> 6) * NL + i) * (64 / CH) + (threadIdx.x & 63) / CH; }
-  template <typename SRC>
-  __device__ __forceinline__ void direct_offsets(const SRC& src, int rows) {
+  // (Of a thread number that the compiler cannot see through where it happens inside the loop, once: nothing of it is then kept in
+  // registers all along.)
+  template <typename F>
+  static __device__ __forceinline__ void direct_offsets(uint32_t (&off)[NL], int stride, int rows, F piece) {
+    int tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
-      const int row = direct_row(i), r = min(row, rows - 1), ch = threadIdx.x % CH;
-      koff[i] = (uint32_t)(r * (int)src.ks + k_piece(row, ch) * 8) * 2;
-      voff[i] = (uint32_t)(r * (int)src.vs + v_piece(row, ch) * 8) * 2;
+      const int row = ((tid >> 6) * NL + i) * (64 / CH) + (tid & 63) / CH;
+      off[i] = __umul24(min(row, rows - 1), 2 * stride) + piece(row, tid % CH) * 16;
     }
   }
-  template <typename SRC>
-  __device__ __forceinline__ void direct_load(const SRC& src, int base, char* buf) {
-    const T *kb = uniform(src.k + base * src.ks), *vb = uniform(src.v + base * src.vs);
-    const uint32_t lds = uniform((int)((uint32_t)(uintptr_t)(lds_char*)buf + (threadIdx.x >> 6) * (NL * 1024)));
+  static __device__ __forceinline__ void direct_load(const T* from, const uint32_t (&off)[NL], char* to) {
+    from = uniform(from);
+    const uint32_t lds = uniform((int)((uint32_t)(uintptr_t)(lds_char*)to + (threadIdx.x >> 6) * (NL * 1024)));
 #pragma unroll
     for (int i = 0; i < NL; ++i)
-      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds + i * 1024), "v"(koff[i]), "s"(kb) : "memory");
-#pragma unroll
-    for (int i = 0; i < NL; ++i)
-      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds + TILE * D * 2 + i * 1024), "v"(voff[i]), "s"(vb)
-                   : "memory");
+      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds + i * 1024), "v"(off[i]), "s"(from) : "memory");
   }
   // What store() does on the way, on a tile that is in LDS.
-  __device__ __forceinline__ void clean(uint32_t (&bad)[(NL + 3) / 4]) {
-    hq_u4v* vs = reinterpret_cast<hq_u4v*>(sm + TILE * D * 2) + threadIdx.x;
+  static __device__ __forceinline__ void clean(char* values, uint32_t (&bad)[(NL + 3) / 4]) {
+    hq_u4v* vs = reinterpret_cast<hq_u4v*>(values) + threadIdx.x;
     hq_u4v v[NL];
     uint32_t any = 0;
 #pragma unroll
@@ -191,9 +187,8 @@ struct Attend {
     }
   }
   // The same places again, one for each value that was not finite and zero for the others.
-  __device__ __forceinline__ void store_bad(const uint32_t (&bad)[(NL + 3) / 4]) {
+  static __device__ __forceinline__ void store_bad(char* vs, const uint32_t (&bad)[(NL + 3) / 4]) {
     const int ch = threadIdx.x % CH, row0 = threadIdx.x / CH;
-    char* vs = sm + TILE * D * 2;
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
       hq_u4v w;
@@ -212,11 +207,11 @@ struct Attend {
   }
 
   // V^T of 32 elements of the head (block d) and 16 keys (block b, half t) as the matrix core takes it: see the top of the file.
-  __device__ __forceinline__ V8 v_operand(int key0, int b, int t, int d) const {
+  static __device__ __forceinline__ V8 v_operand(const char* values, int key0, int b, int t, int d) {
     const int lane = threadIdx.x & 63;
     const int row = key0 + 32 * b + 16 * t + 4 * (lane >> 5) + ((lane >> 2) & 3);
     const int ch = 4 * d + 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1);
-    lds_char* vs = (lds_char*)sm + TILE * D * 2 + (lane & 1) * 8;
+    lds_char* vs = (lds_char*)values + (lane & 1) * 8;
     typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
     union {
       s16x4 h[2];
@@ -227,10 +222,9 @@ struct Attend {
     return u.v;
   }
 
-  // The wave's part of a tile, keys from base + key0 on.
-  __device__ __forceinline__ void attend_tile(int base, int key0, int left, float c) {
+  // The wave's part of a tile, step by step.  Scores of its rows and the keys from key0 on:
+  __device__ __forceinline__ void scores(f32x16 (&s)[NB], const char* keys, int key0) const {
     const int lane = threadIdx.x & 63, half = lane >> 5;
-    f32x16 s[NB];
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
 #pragma unroll
@@ -238,36 +232,49 @@ struct Attend {
 #pragma unroll
       for (int kk = 0; kk < D / 16; ++kk) {
         const int row = key0 + 32 * b + (lane & 31);
-        const V8 a = *reinterpret_cast<const V8*>(sm + row * D * 2 + k_piece(row, 2 * kk + half) * 16);
+        const V8 a = *reinterpret_cast<const V8*>(keys + row * D * 2 + k_piece(row, 2 * kk + half) * 16);
         s[b] = Kind<T>::mfma(a, qf[kk], s[b]);
       }
     }
-    if (base + key0 + 32 * NB > all_see) {
+  }
+  // Which of the lane's registers are keys that the row sees: the first `left` of the wave's, less 4 in the upper lanes.
+  static __device__ __forceinline__ void mask(f32x16 (&s)[NB], int left) {
 #pragma unroll
-      for (int b = 0; b < NB; ++b)
+    for (int b = 0; b < NB; ++b) {
+      // bit i: key i of the block is seen; a bit field of a sign and a bitwise select cost two instructions a score and no scalar register
+      const int n = left - 32 * b;
+      const int seen = n >= 32 ? -1 : n <= 0 ? 0 : (int)((1u << n) - 1);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[b][r] = 32 * b + 8 * (r / 4) + r % 4 < left ? s[b][r] : -INFINITY;
+      for (int r = 0; r < 16; ++r) {
+        const uint32_t keep = (uint32_t)__builtin_amdgcn_sbfe(seen, 8 * (r / 4) + r % 4, 1);
+        s[b][r] = __uint_as_float((__float_as_uint(s[b][r]) & keep) | (~keep & 0xff800000u));
+      }
     }
-    float top = -INFINITY;
+  }
+  static __device__ __forceinline__ float top_of(const f32x16 (&s)[NB]) {
+    float top = s[0][0];
 #pragma unroll
     for (int b = 0; b < NB; ++b)
 #pragma unroll
       for (int r = 0; r < 16; ++r) top = fmaxf(top, s[b][r]);
-    top = pair_max(top) * c;
-    // A maximum that has grown by less than 2^8 stays: the weights may then be up to 2^8, which neither fp32 sums nor the 16-bit
-    // weights mind, and the sums need no scaling.  The scaling of 64 registers a tile was a fifth of the vector instructions.
-    if (__builtin_amdgcn_ballot_w64(top > m + 8.f)) {
-      const float mn = top > m + 8.f ? top : m;  // each row by its own scores: its bits do not depend on its neighbours
-      const float f = mn == m ? 1.f : __builtin_amdgcn_exp2f(m - mn);
-      m = mn;
-      l *= f;
+    return pair_max(top);
+  }
+  // A maximum that has grown by less than 2^8 stays: the weights may then be up to 2^8, which neither fp32 sums nor the 16-bit
+  // weights mind, and the sums need no scaling.  The scaling of 64 registers a tile was a fifth of the vector instructions.
+  __device__ __forceinline__ void raise(float top) {
+    if (!__builtin_amdgcn_ballot_w64(top > m + 8.f)) return;
+    const float mn = top > m + 8.f ? top : m;  // each row by its own scores: its bits do not depend on its neighbours
+    const float f = mn == m ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+    m = mn;
+    l *= f;
 #pragma unroll
-      for (int d = 0; d < D / 32; ++d)
+    for (int d = 0; d < D / 32; ++d)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) o[d][r] *= f;
-    }
+      for (int r = 0; r < 16; ++r) o[d][r] *= f;
+  }
+  __device__ __forceinline__ void weights(V8 (&p)[NB][2], const f32x16 (&s)[NB], float c) {
     const float ms = finite_or_zero(m);
-    V8 p[NB][2];
+    float sum[2] = {0.f, 0.f};
 #pragma unroll
     for (int b = 0; b < NB; ++b)
 #pragma unroll
@@ -275,45 +282,108 @@ struct Attend {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const float e = __builtin_amdgcn_exp2f(fmaf(s[b][8 * t + i], c, -ms));
-          l += e;
+          sum[i & 1] += e;
           p[b][t][i] = (T)e;  // 2^-9 (bf16) or 2^-12 of a weight at most, to the nearest: as much as the result's own rounding
         }
+    l += sum[0] + sum[1];
+  }
+  __device__ __forceinline__ void values(const V8 (&p)[NB][2], const char* values, int key0) {
 #pragma unroll
     for (int d = 0; d < D / 32; ++d)
 #pragma unroll
       for (int b = 0; b < NB; ++b)
 #pragma unroll
-        for (int t = 0; t < 2; ++t) o[d] = Kind<T>::mfma(v_operand(key0, b, t, d), p[b][t], o[d]);
+        for (int t = 0; t < 2; ++t) o[d] = Kind<T>::mfma(v_operand(values, key0, b, t, d), p[b][t], o[d]);
   }
-
-  // One tile, keys from `base` on.  partly: not every row of the workgroup sees all of it.
-  __device__ __forceinline__ void tile(int base, bool partly, float c, int tileno, const uint32_t (&bad)[(NL + 3) / 4]) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
-    const int key0 = RW == 4 ? 0 : wave * 32 * NB;
-    const int left = lim - base - key0 - 4 * half;  // a key of the registers below it is seen
-    if (base + key0 < any_sees) attend_tile(base, key0, left, c);
-    if (partly && *(volatile __attribute__((address_space(3))) int*)poison == tileno) {  // rows that see a value that is not finite
-      __syncthreads();
-      store_bad(bad);
-      __syncthreads();
+  // scores() of the next tile and weights() of this one, an instruction of the matrix core and its share of the others in turn: left
+  // alone, the compiler moves the reads of all operands to the front and runs out of registers.
+  __device__ __forceinline__ void scores_and_weights(f32x16 (&n)[NB], const char* keys, V8 (&p)[NB][2], const f32x16 (&s)[NB], float c) {
+    const int lane = threadIdx.x & 63, half = lane >> 5;
+    constexpr int STEPS = NB * D / 16, EACH = NB * 16 / STEPS, AHEAD = 4;
+    auto operand = [&](int j) {
+      const int row = 32 * (j / (D / 16)) + (lane & 31);
+      return *reinterpret_cast<const V8*>(keys + row * D * 2 + k_piece(row, 2 * (j % (D / 16)) + half) * 16);
+    };
+    const float ms = finite_or_zero(m);
+    float sum[2] = {0.f, 0.f};
+    V8 a[AHEAD];
+    hq_u4v w[NB][2];
 #pragma unroll
-      for (int d = 0; d < D / 32; ++d) {
-        f32x16 n;
+    for (int j = 0; j < AHEAD; ++j) a[j] = operand(j);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) n[r] = 0.f;
+    for (int b = 0; b < NB; ++b)
 #pragma unroll
-        for (int b = 0; b < NB; ++b)
+      for (int r = 0; r < 16; ++r) n[b][r] = 0.f;
 #pragma unroll
-          for (int t = 0; t < 2; ++t) {
-            V8 seen;
+    for (int j = 0; j < STEPS; ++j) {
+      n[j / (D / 16)] = Kind<T>::mfma(a[j % AHEAD], qf[j % (D / 16)], n[j / (D / 16)]);
+      if (j + AHEAD < STEPS) a[j % AHEAD] = operand(j + AHEAD);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) seen[i] = 32 * b + 16 * t + 8 * (i / 4) + i % 4 < left ? (T)1.f : (T)0.f;
-            n = Kind<T>::mfma(v_operand(key0, b, t, d), seen, n);
-          }
-#pragma unroll
-        for (int r = 0; r < 16; ++r) o[d][r] = n[r] > 0.f ? NAN : o[d][r];
+      for (int i = j * EACH; i < (j + 1) * EACH; i += 2) {
+        const float e0 = __builtin_amdgcn_exp2f(fmaf(s[i / 16][i % 16], c, -ms)), e1 = __builtin_amdgcn_exp2f(fmaf(s[i / 16][i % 16 + 1], c, -ms));
+        sum[0] += e0;
+        sum[1] += e1;
+        typedef T T2 __attribute__((ext_vector_type(2)));
+        uint32_t two = __builtin_bit_cast(uint32_t, T2{(T)e0, (T)e1});
+        asm volatile("" : "+v"(two), "+v"(sum[0]), "+v"(sum[1]));  // here and now
+        w[i / 16][i / 8 % 2][i % 8 / 2] = two;
       }
+      __builtin_amdgcn_sched_barrier(0);
     }
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) p[b][h] = __builtin_bit_cast(V8, w[b][h]);
+    l += sum[0] + sum[1];
+  }
+  // values() of this tile, and the maximum of the next one's scores.
+  __device__ __forceinline__ float values_and_top(const V8 (&p)[NB][2], const char* vs, const f32x16 (&n)[NB]) {
+    constexpr int STEPS = D / 32 * NB * 2, EACH = NB * 16 / STEPS, AHEAD = 4;
+    auto operand = [&](int j) { return v_operand(vs, 0, j / 2 % NB, j % 2, j / (2 * NB)); };
+    V8 a[AHEAD];
+    float top = n[0][0];
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) a[j] = operand(j);
+#pragma unroll
+    for (int j = 0; j < STEPS; ++j) {
+      o[j / (2 * NB)] = Kind<T>::mfma(a[j % AHEAD], p[j / 2 % NB][j % 2], o[j / (2 * NB)]);
+      if (j + AHEAD < STEPS) a[j % AHEAD] = operand(j + AHEAD);
+#pragma unroll
+      for (int i = j * EACH; i < (j + 1) * EACH; ++i) top = fmaxf(top, n[i / 16][i % 16]);
+            asm volatile("" : "+v"(top));
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    return pair_max(top);
+  }
+  // Rows that see a value that is not finite.
+  __device__ __forceinline__ void spoil(char* values, int key0, int left, const uint32_t (&bad)[(NL + 3) / 4]) {
+    __syncthreads();
+    store_bad(values, bad);
+    __syncthreads();
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d) {
+      f32x16 n;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) n[r] = 0.f;
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          V8 seen;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) seen[i] = 32 * b + 16 * t + 8 * (i / 4) + i % 4 < left ? (T)1.f : (T)0.f;
+          n = Kind<T>::mfma(v_operand(values, key0, b, t, d), seen, n);
+        }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[d][r] = n[r] > 0.f ? NAN : o[d][r];
+    }
+  }
+  __device__ __forceinline__ bool spoiled(int tileno) const { return *(volatile __attribute__((address_space(3))) int*)poison == tileno; }
+  __device__ __forceinline__ void note(const uint32_t (&bad)[(NL + 3) / 4], int tileno) {
+    uint32_t any = 0;
+#pragma unroll
+    for (int i = 0; i < (NL + 3) / 4; ++i) any |= bad[i];
+    if (any) *poison = tileno;
   }
 
   // The row's sums as one of several shares; none: the row sees nothing in any of them, which share 0 says by an infinite maximum.
@@ -334,53 +404,110 @@ struct Attend {
     clear();
     if (first >= end) return;
     uint32_t bad[(NL + 3) / 4] = {};
+    char* const vs = sm + TILE * D * 2;
+    const int key0 = RW == 4 ? 0 : (threadIdx.x >> 6) * 32 * NB;
     load(src, first);
-    int tileno = 0;
-    for (int base = first; base < end; base += TILE, ++tileno) {
+    for (int base = first, tileno = 0; base < end; base += TILE, ++tileno) {
       const bool partly = base + TILE > whole;
       __syncthreads();
       store(partly, bad);
-      if (partly) {
-        uint32_t any = 0;
-#pragma unroll
-        for (int i = 0; i < (NL + 3) / 4; ++i) any |= bad[i];
-        if (any) *poison = tileno;
-      }
+      if (partly) note(bad, tileno);
       __syncthreads();
       if (base + TILE < end) load(src, base + TILE);
-      tile(base, partly, c, tileno, bad);
+      const int left = lim - base - key0 - 4 * ((threadIdx.x >> 5) & 1);
+      if (base + key0 < any_sees) {
+        f32x16 s[NB];
+        V8 p[NB][2];
+        scores(s, sm, key0);
+        if (base + key0 + 32 * NB > all_see) mask(s, left);
+        raise(top_of(s) * c);
+        weights(p, s, c);
+        values(p, vs, key0);
+      }
+      if (partly && spoiled(tileno)) spoil(vs, key0, left, bad);
     }
     l = pair_sum(l);
   }
 
+  // The same, DIRECT.  Heads of 128: the scores of the next tile are in the matrix core while the vector unit makes this one's weights
+  // of its own, and the next scores' maximum is taken under this tile's product with the values; the keys so run a tile ahead.  Heads
+  // of 64, where the vector unit is the busier of the two and the registers saved are two waves more: one step after the other
+  // (16384 tokens, heads of 128: 2186 us one after the other, 2130 so; 8192 tokens, heads of 64: 359 and 376).
   template <typename SRC>
   __device__ __forceinline__ void run_direct(const SRC& src, int first, int end, int whole, float c) {
     clear();
     if (first >= end) return;
-    uint32_t bad[(NL + 3) / 4] = {};
-    char* const bufs = sm;
+    constexpr int HALF = TILE * D * 2, K_AHEAD = D == 128;
+    const int nt = (end - first + TILE - 1) / TILE;
+    direct_offsets(koff, (int)src.ks, src.n - first, [](int row, int ch) { return k_piece(row, ch); });
+    direct_offsets(voff, (int)src.vs, src.n - first, [](int row, int ch) { return v_piece(row, ch); });
+    auto load_k = [&](int t, int slot) {
+      const int base = first + t * TILE;
+      if (base + TILE > src.n) direct_offsets(koff, (int)src.ks, src.n - base, [](int row, int ch) { return k_piece(row, ch); });
+      direct_load(src.k + base * src.ks, koff, sm + slot * HALF);
+    };
+    auto load_v = [&](int t, int slot) {
+      const int base = first + t * TILE;
+      if (base + TILE > src.n) direct_offsets(voff, (int)src.vs, src.n - base, [](int row, int ch) { return v_piece(row, ch); });
+      direct_load(src.v + base * src.vs, voff, sm + (2 + slot) * HALF);
+    };
+    const int half4 = 4 * ((threadIdx.x >> 5) & 1);
+    f32x16 s0[NB], s1[NB];
+    float top = 0.f;
+    load_k(0, 0);
+    load_v(0, 0);
 #pragma unroll
     for (int kk = 0; kk < D / 16; ++kk) asm volatile("" : "+v"(qf[kk]));  // here, not at every tile: the loads in flight then are the next tile's
-    direct_offsets(src, src.n - first);
-    direct_load(src, first, bufs);
-    for (int base = first, tileno = 0; base < end; base += TILE, ++tileno) {
-      const bool partly = base + TILE > whole;
-      sm = bufs + (tileno & 1) * BUF;
+    if (K_AHEAD) {
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       __syncthreads();
-      if (base + TILE < end) {
-        if (base + 2 * TILE > src.n) direct_offsets(src, src.n - base - TILE);
-        direct_load(src, base + TILE, bufs + (~tileno & 1) * BUF);
-      }
+      if (nt > 1) load_k(1, 1);
+      scores(s0, sm, 0);
+      if (first + TILE > all_see) mask(s0, lim - first - half4);
+      top = top_of(s0);
+    }
+    // One tile.  K_AHEAD: its scores in s, the next one's go to n (behind the last tile they are of no tile, and not used: one way
+    // through the step, as two ways that both sum into o cost the compiler a second set of its registers).
+    auto step = [&](int t, auto SLOT, f32x16(&s)[NB], f32x16(&n)[NB]) __attribute__((always_inline)) {
+      const int base = first + t * TILE;
+      const bool partly = base + TILE > whole;
+      char* const vs = sm + (2 + SLOT) * HALF;
+      uint32_t bad[(NL + 3) / 4] = {};
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __syncthreads();
+      if (t + 1 + K_AHEAD < nt) load_k(t + 1 + K_AHEAD, (SLOT + 1 + K_AHEAD) % 2);
+      if (t + 1 < nt) load_v(t + 1, 1 - SLOT);
       if (partly) {
-        clean(bad);
-        uint32_t any = 0;
-#pragma unroll
-        for (int i = 0; i < (NL + 3) / 4; ++i) any |= bad[i];
-        if (any) *poison = tileno;
+        clean(vs, bad);
+        note(bad, t);
         __syncthreads();
       }
-      tile(base, partly, c, tileno, bad);
+      if (base < any_sees) {
+        V8 p[NB][2];
+        if (K_AHEAD) {
+          raise(top * c);
+          scores_and_weights(n, sm + (1 - SLOT) * HALF, p, s, c);
+          if (base + 2 * TILE > all_see) mask(n, lim - base - TILE - half4);
+          top = values_and_top(p, vs, n);
+        } else {
+          scores(s, sm + SLOT * HALF, 0);
+          if (base + TILE > all_see) mask(s, lim - base - half4);
+          raise(top_of(s) * c);
+          weights(p, s, c);
+          values(p, vs, 0);
+        }
+      }
+      if (partly && spoiled(t)) spoil(vs, 0, lim - base - half4, bad);
+    };
+    if (K_AHEAD) {
+      int t = 0;
+      for (; t + 1 < nt; t += 2) {
+        step(t, std::integral_constant<int, 0>(), s0, s1);
+        step(t + 1, std::integral_constant<int, 1>(), s1, s0);
+      }
+      if (t < nt) step(t, std::integral_constant<int, 0>(), s0, s1);
+    } else {
+      for (int t = 0; t < nt; ++t) step(t, t & 1, s0, s1);
     }
     l = pair_sum(l);
   }
@@ -446,27 +573,30 @@ struct PackedKeys {  // of one sequence and one head
 
 // A workgroup's rows and share of the keys.  Many rows: all keys, and the result; few: the keys are divided among `shares` workgroups.
 template <typename T, int D>
-__global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void prompt_kernel(PromptArgs a) {
+__global__ __launch_bounds__(kThreads, D == 64 ? 4 : 2) void prompt_kernel(PromptArgs a) {
   typedef Attend<T, D, 4, true> A;
   typedef typename Kind<T>::V8 V8;
   constexpr int ROWS = 128;
   extern __shared__ __align__(16) char sm[];
   __shared__ int poison;
-  int x = blockIdx.x;
-  const int head = x % a.kv_heads;
-  x /= a.kv_heads;
-  const int share = x % a.shares;
-  x /= a.shares;
-  const int ratio = a.ratio;
+  uint32_t x = blockIdx.x;
+  const int head = x % (uint32_t)a.kv_heads;
+  x /= (uint32_t)a.kv_heads;
+  int share = 0;
+  if (a.shares > 1) {
+    share = x % (uint32_t)a.shares;
+    x /= (uint32_t)a.shares;
+  }
+  const uint32_t ratio = a.ratio;
   int seq, tile, q0, nq;
-  if (!find_tile(a.cu_q, a.seqs, a.total_q, x, [=](int n) { return (int)((n * (int64_t)ratio + ROWS - 1) / ROWS); }, &seq, &q0, &nq, &tile)) return;
+  if (!find_tile(a.cu_q, a.seqs, a.total_q, x, [=](int n) { return (int)((n * ratio + ROWS - 1) / ROWS); }, &seq, &q0, &nq, &tile)) return;
   const int k0 = min(max(a.cu_k[seq], 0), a.total_k), nk = min(max(a.cu_k[seq + 1], k0), a.total_k) - k0;
   const int rows = nq * ratio;
   tile = (rows + ROWS - 1) / ROWS - 1 - tile;  // the tiles with most keys come first
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int first_row = tile * ROWS, last_row = min(first_row + ROWS, rows) - 1;
   const int row = first_row + wave * 32 + (lane & 31), r = min(row, last_row);
-  const int token = r / ratio, h = head * ratio + r % ratio;
+  const int token = (uint32_t)r / ratio, h = head * ratio + (r - token * ratio);
   A w;
   w.sm = sm;
   w.poison = &poison;
@@ -476,10 +606,12 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void prompt_kernel(Promp
   for (int kk = 0; kk < D / 16; ++kk) w.qf[kk] = *reinterpret_cast<const V8*>(q + 16 * kk);
   auto limit = [&](int t) { return a.causal ? min(max(t + 1 + nk - nq, 0), nk) : nk; };
   w.lim = limit(token);
+  w.all_see = __builtin_amdgcn_readlane(w.lim, 0);  // a later row sees as much or more
+  w.any_sees = __builtin_amdgcn_readlane(w.lim, 31);
   PackedKeys<T> src{(const T*)a.k + (int64_t)k0 * a.ks + head * D, (const T*)a.v + (int64_t)k0 * a.vs + head * D, a.ks, a.vs, nk};
   const int each = a.shares == 1 ? nk : max(256, ((nk + a.shares - 1) / a.shares + A::TILE - 1) & -A::TILE);
-  const int end = uniform(limit(last_row / ratio)), first = (int)min((int64_t)share * each, (int64_t)end);
-  w.run_direct(src, first, min(end, first + each), uniform(limit(first_row / ratio)), a.c);
+  const int end = uniform(limit((uint32_t)last_row / ratio)), first = (int)min((int64_t)share * each, (int64_t)end);
+  w.run_direct(src, first, min(end, first + each), uniform(limit((uint32_t)first_row / ratio)), a.c);
   if (row > last_row) return;
   if (a.shares == 1) {
     const float inv = 1.f / w.l;
@@ -558,10 +690,11 @@ __device__ __forceinline__ void attend_rows(const PagedArgs& a, char* sm, int* p
 #pragma unroll
   for (int kk = 0; kk < D / 16; ++kk) w.qf[kk] = *reinterpret_cast<const V8*>(q + 16 * kk);
   w.lim = min(min(max(a.lengths[b], 0), a.width << a.page_log), shared_end);
-  // what every row sees
+  w.all_see = uniform(wave_min(w.lim));
+  w.any_sees = -uniform(wave_min(-w.lim));
+  // what every row of the workgroup sees
   __shared__ int seen[kWaves];
-  const int mine = wave_min(w.lim);
-  if (lane == 0) seen[wave] = mine;
+  if (lane == 0) seen[wave] = w.all_see;
   __syncthreads();
   const int whole = min(min(seen[0], seen[1]), min(seen[2], seen[3]));
   PagedKeys<T, D> src{(const T*)a.k, (const T*)a.v, a.table + (int64_t)src_row * a.width, head, a.kv_heads, a.page_log, a.pages, end};
@@ -792,7 +925,7 @@ extern "C" int hq_prompt_attention(const void* q, const void* k, const void* v, 
   if (misaligned(q, q_stride) || misaligned(k, k_stride) || misaligned(v, v_stride) || ((uintptr_t)out & 15) ||
       (((uintptr_t)cu_q | (uintptr_t)cu_k) & 3))
     return HQ_ERR_MISALIGNED;
-  if (total_q * (heads / kv_heads) > INT_MAX - 128 || total_k > INT_MAX - 128 || k_stride > 1 << 24 || v_stride > 1 << 24)  // 32-bit offsets in a tile
+  if (total_q * (heads / kv_heads) > INT_MAX - 128 || total_k > INT_MAX - 128 || k_stride > 1 << 22 || v_stride > 1 << 22)  // 32-bit offsets in a tile
     return HQ_ERR_TOO_LARGE;
   const HqDevice* dev = nullptr;
   const int rc = hq_current_device(&dev);
