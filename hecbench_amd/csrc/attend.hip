@@ -3,8 +3,11 @@
 // For a query row q: out = sum_j p_j v_j / sum_j p_j, p_j = 2^(c q.k_j - m), c = scale * log2(e), in one pass over the keys with the
 // running maximum m of the row; a larger maximum scales what has been summed so far.
 //
+// Two ways through the keys.  Many rows (Many): a tile of 64 keys in LDS serves 128 rows, 32 a wave.  Few (Few): 16 rows at most, each
+// wave goes through keys of its own, as what bounds it is their way from memory, and the waves' sums come together at the end.
+//
 // Rows: the R = heads / kv_heads query heads of a key / value head and the tokens (or requests) are one list of rows
-// (token, head of the group), so that a tile of keys in LDS serves all of them.  A wave has 32 rows.  The scores are computed
+// (token, head of the group), so that a tile of keys in LDS serves all of them.  The scores are computed
 // transposed, S^T = K Q^T: the matrix core leaves a row's scores in one lane and its partner 32 lanes on, so maximum and sum are
 // sums within a lane and one exchange, and the same registers are, rounded, the operand of O^T = V^T P^T without another move: the
 // order of the keys in that sum is free, and the transposing LDS read fetches V's rows in the order in which S^T left them.
@@ -25,17 +28,20 @@ typedef __attribute__((address_space(3))) char lds_char;
 
 template <typename T>
 struct Kind;
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 template <>
 struct Kind<__bf16> {
   typedef bf16x8 V8;
   static constexpr uint32_t kExp = 0x7f807f80u, kStep = 0x00800080u, kOne = 0x3f803f80u;
   static __device__ __forceinline__ f32x16 mfma(V8 a, V8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+  static __device__ __forceinline__ f32x4 mfma(V8 a, V8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 };
 template <>
 struct Kind<_Float16> {
   typedef f16x8 V8;
   static constexpr uint32_t kExp = 0x7c007c00u, kStep = 0x04000400u, kOne = 0x3c003c00u;
   static __device__ __forceinline__ f32x16 mfma(V8 a, V8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+  static __device__ __forceinline__ f32x4 mfma(V8 a, V8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 };
 
 // The larger of a lane's value and its partner's, 32 lanes on.
@@ -46,6 +52,15 @@ __device__ __forceinline__ float pair_max(float v) {
 __device__ __forceinline__ float pair_sum(float v) {
   const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   return __uint_as_float(s[0]) + __uint_as_float(s[1]);
+}
+// The same over the four lanes of a row of Few, 16 lanes apart.
+__device__ __forceinline__ float quarters_max(float v) {
+  const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return pair_max(fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1])));
+}
+__device__ __forceinline__ float quarters_sum(float v) {
+  const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return pair_sum(__uint_as_float(s[0]) + __uint_as_float(s[1]));
 }
 __device__ __forceinline__ float finite_or_zero(float m) { return m == -INFINITY ? 0.f : m; }
 
@@ -59,69 +74,46 @@ __device__ __forceinline__ const P* uniform(const P* p) {
 
 constexpr int kThreads = 256, kWaves = 4;
 
+
 __device__ __forceinline__ int wave_min(int v) {
 #pragma unroll
   for (int d = 32; d; d >>= 1) v = min(v, __shfl_xor(v, d));
   return v;
 }
 
-// What one workgroup attends: up to 128 rows (RW = 4 waves of them, all of which see every key of a tile) or up to 32 rows (RW = 1,
-// the waves share the tile's keys among them).
-template <typename T, int D, int RW, bool DIRECT = false>
-struct Attend {
-  typedef typename Kind<T>::V8 V8;
-  static constexpr int KW = kWaves / RW;            // waves that divide a tile's keys
-  static constexpr int NB = RW == 4 ? 2 : 1;        // blocks of 32 keys of a wave
-  static constexpr int TILE = 32 * NB * KW;         // keys of a tile
-  static constexpr int CH = D / 8;                  // 16-byte pieces of a row
-  static constexpr int NL = TILE * CH / kThreads;   // pieces that a thread brings
-  static constexpr int STEP = kThreads / CH;        // rows between two of them
-  static constexpr int BUF = 2 * TILE * D * 2;      // a tile's keys and values
-  static constexpr int LDS = (DIRECT ? 2 : 1) * BUF;
+// ---- keys and values in LDS --------------------------------------------------------------------------------------------
+// A row's 16-byte pieces are stored in an order that depends on the row, so that the lanes of a read pass meet different banks (0
+// conflicts counted): the keys' by all bits of the row, which 16 lanes read piece by piece, the values' by the bits of the four or eight
+// rows that transposing reads take together, 64 or 32 bytes of each.
+template <int D>
+__device__ __forceinline__ int k_piece(int row, int ch) { return D == 128 ? ch ^ (row & 15) : ch ^ ((row >> 1) & 7); }
+template <int D>
+__device__ __forceinline__ int v_piece(int row, int ch) {
+  return (D == 128 ? ch ^ ((row & 3) << 2) : ch ^ (((row >> 1) & 1) << 2)) ^ (((row >> 2) & 1) << 1);
+}
 
-  // A row's pieces are stored in an order that depends on the row, so that the lanes of a read pass meet different banks: the keys'
-  // pieces by all bits of the row, which 16 lanes read piece by piece, the values' by the two bits of the four rows that a
-  // transposing read takes together, 64 bytes of each.
-  static __device__ __forceinline__ int k_piece(int row, int ch) { return D == 128 ? ch ^ (row & 15) : ch ^ ((row >> 1) & 7); }
-  static __device__ __forceinline__ int v_piece(int row, int ch) { return D == 128 ? ch ^ ((row & 3) << 2) : ch ^ (((row >> 1) & 1) << 2); }
+// One instruction brings 1 KB from memory into LDS past the registers, the lanes' pieces one behind the other, so it is the lane's
+// address that follows the order of the pieces.  (The compiler does not see that it writes LDS; the waits are explicit.)
+__device__ __forceinline__ void to_lds(uint32_t lds, const void* from, uint32_t off) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(from) : "memory");
+}
+__device__ __forceinline__ void to_lds(uint32_t lds, const void* from) {  // a lane's own address
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(from) : "memory");
+}
+__device__ __forceinline__ uint32_t lds_address(const char* p) { return (uint32_t)(uintptr_t)(lds_char*)p; }
 
-  char* sm;
-  int* poison;  // in LDS: the tile whose values hold something that is not finite
-  V8 qf[D / 16];
-  f32x16 o[D / 32];
-  float m = -INFINITY, l = 0.f;
-  hq_u4v kr[NL], vr[NL];
-  int lim;              // keys below this are seen by the lane's row
-  int all_see, any_sees;  // below the first by all rows of the wave, below the second by one of them
-
-  __device__ __forceinline__ void clear() {
-#pragma unroll
-    for (int d = 0; d < D / 32; ++d)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) o[d][r] = 0.f;
-  }
-
-  template <typename SRC>
-  __device__ __forceinline__ void load(const SRC& src, int base) {
-    const int ch = threadIdx.x % CH, row = threadIdx.x / CH;
-#pragma unroll
-    for (int i = 0; i < NL; ++i) {
-      const T *k, *v;
-      const bool there = src.at(base + row + i * STEP, &k, &v);
-      kr[i] = *reinterpret_cast<const hq_u4v*>(k + ch * 8);
-      vr[i] = *reinterpret_cast<const hq_u4v*>(v + ch * 8);
-      if (!there) kr[i] = vr[i] = hq_u4v{0, 0, 0, 0};
-    }
-  }
-
-  // DIRECT: a tile goes from memory into LDS past the registers, its second buffer is filled while the first is worked on, and one barrier
-  // a tile does.  An instruction brings 1 KB, the lanes' pieces one behind the other, so it is the lane's address that follows the
-  // order of the pieces.
+// The tiles of one sequence's keys, one head, for the four waves of Many.  Rows behind the last one repeat it.
+template <typename T, int D>
+struct PackedTiles {
+  static constexpr int CH = D / 8, NL = 64 * CH / kThreads;  // pieces of a row; instructions of a wave for the keys of a tile
+  const T *k, *v;
+  int64_t ks, vs;
+  int n, first;
   uint32_t koff[NL], voff[NL];
   // (Of a thread number that the compiler cannot see through where it happens inside the loop, once: nothing of it is then kept in
   // registers all along.)
   template <typename F>
-  static __device__ __forceinline__ void direct_offsets(uint32_t (&off)[NL], int stride, int rows, F piece) {
+  static __device__ __forceinline__ void offsets(uint32_t (&off)[NL], int stride, int rows, F piece) {
     int tid = threadIdx.x;
     asm volatile("" : "+v"(tid));
 #pragma unroll
@@ -130,15 +122,108 @@ struct Attend {
       off[i] = __umul24(min(row, rows - 1), 2 * stride) + piece(row, tid % CH) * 16;
     }
   }
-  static __device__ __forceinline__ void direct_load(const T* from, const uint32_t (&off)[NL], char* to) {
+  static __device__ __forceinline__ void load(const T* from, const uint32_t (&off)[NL], char* to) {
     from = uniform(from);
-    const uint32_t lds = uniform((int)((uint32_t)(uintptr_t)(lds_char*)to + (threadIdx.x >> 6) * (NL * 1024)));
+    const uint32_t lds = uniform((int)(lds_address(to) + (threadIdx.x >> 6) * (NL * 1024)));
 #pragma unroll
-    for (int i = 0; i < NL; ++i)
-      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds + i * 1024), "v"(off[i]), "s"(from) : "memory");
+    for (int i = 0; i < NL; ++i) to_lds(lds + i * 1024, from, off[i]);
   }
-  // What store() does on the way, on a tile that is in LDS.
-  static __device__ __forceinline__ void clean(char* values, uint32_t (&bad)[(NL + 3) / 4]) {
+  __device__ __forceinline__ void start(int f) {
+    first = f;
+    offsets(koff, (int)ks, n - first, k_piece<D>);
+    offsets(voff, (int)vs, n - first, v_piece<D>);
+  }
+  __device__ __forceinline__ void advance(int) {}
+  __device__ __forceinline__ void load_k(int t, char* to) {
+    const int base = first + t * 64;
+    if (base + 64 > n) offsets(koff, (int)ks, n - base, k_piece<D>);
+    load(k + base * ks, koff, to);
+  }
+  __device__ __forceinline__ void load_v(int t, char* to) {
+    const int base = first + t * 64;
+    if (base + 64 > n) offsets(voff, (int)vs, n - base, v_piece<D>);
+    load(v + base * vs, voff, to);
+  }
+};
+
+// The pages of one request, one head.  Eight tokens from a multiple of eight on are in one page.
+template <typename T, int D>
+struct Pages {
+  const T *k, *v;
+  const int* table;  // the request's row
+  int head, kv_heads, page_log, pages;
+  __device__ __forceinline__ int id(int key) const {  // -1: no page, to be read as zeros
+    const int p = table[key >> page_log];
+    return (unsigned)p < (unsigned)pages ? p : -1;
+  }
+  __device__ __forceinline__ int64_t at(int page, int key) const {
+    return ((((int64_t)page * kv_heads + head) << page_log) + (key & ((1 << page_log) - 1))) * D;
+  }
+};
+__device__ __forceinline__ void zero_lds(char* to) {  // what one to_lds() would write
+  reinterpret_cast<hq_u4v*>(to)[threadIdx.x & 63] = hq_u4v{0, 0, 0, 0};
+}
+
+// The same tiles of pages.  Rows behind the last one are whatever its page holds.
+template <typename T, int D>
+struct PagedTiles {
+  static constexpr int CH = D / 8, NL = 64 * CH / kThreads, RG = 64 / CH;  // RG: rows of an instruction, all in one page
+  Pages<T, D> p;
+  int n, first;
+  int ids_next, ids_k, ids_v;  // pages of the instructions' rows, one a lane: of the tile to come, of the keys' and of the values' next
+  uint32_t koff[NL], voff[NL];
+  __device__ __forceinline__ int ids(int t) const { return p.id(min(first + t * 64 + (int)(threadIdx.x & (64 / RG - 1)) * RG, n - 1)); }
+  __device__ __forceinline__ void load(const T* pool, int id, int t, const uint32_t (&off)[NL], char* to) {
+    const int wave = uniform((int)(threadIdx.x >> 6));
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      const int j = wave * NL + i, page = __builtin_amdgcn_readlane(id, j);
+      if (page >= 0) to_lds(uniform((int)lds_address(to) + j * 1024), uniform(pool + p.at(page, first + t * 64 + j * RG)), off[i]);
+      else zero_lds(to + j * 1024);
+    }
+  }
+  __device__ __forceinline__ void start(int f) {
+    first = f;
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      const int row = ((threadIdx.x >> 6) * NL + i) * RG + lane / CH;
+      koff[i] = (lane / CH) * D * 2 + k_piece<D>(row, lane % CH) * 16;
+      voff[i] = (lane / CH) * D * 2 + v_piece<D>(row, lane % CH) * 16;
+    }
+    ids_next = ids(0);
+  }
+  // Before the first load of tile t: its pages are there, those of the tile behind it are asked for.
+  __device__ __forceinline__ void advance(int t) {
+    ids_v = ids_k;
+    ids_k = ids_next;
+    ids_next = ids(t + 1);
+  }
+  __device__ __forceinline__ void load_k(int t, char* to) { load(p.k, ids_k, t, koff, to); }
+  __device__ __forceinline__ void load_v(int t, char* to) { load(p.v, D == 128 ? ids_v : ids_k, t, voff, to); }
+};
+
+// ---- many rows -----------------------------------------------------------------------------------------------------------
+// 128 rows of a workgroup, 32 a wave.
+template <typename T, int D>
+struct Many {
+  typedef typename Kind<T>::V8 V8;
+  static constexpr int NB = 2, TILE = 64;           // blocks of 32 keys, keys of a tile
+  static constexpr int CH = D / 8, NL = 64 * CH / kThreads;
+  static constexpr int HALF = TILE * D * 2, LDS = 4 * HALF;  // keys or values of a tile; two of each
+  static constexpr bool K_AHEAD = D == 128;         // see run()
+
+  char* sm;
+  int* poison;  // in LDS: the tile whose values hold something that is not finite
+  V8 qf[D / 16];
+  f32x16 o[D / 32];
+  float m = -INFINITY, l = 0.f;
+  int lim;                // keys below this are seen by the lane's row
+  int all_see, any_sees;  // below the first by all rows of the wave, below the second by one of them
+
+  // In a tile that not every row sees whole, a value that is not finite would reach the rows that do not see it (0 times infinity): it
+  // becomes zero, and the bits returned say which values were.
+  static __device__ __forceinline__ void clean(char* values, uint32_t& bad) {
     hq_u4v* vs = reinterpret_cast<hq_u4v*>(values) + threadIdx.x;
     hq_u4v v[NL];
     uint32_t any = 0;
@@ -148,68 +233,39 @@ struct Attend {
     for (int i = 0; i < NL; ++i)
 #pragma unroll
       for (int w = 0; w < 4; ++w) any |= (v[i][w] & Kind<T>::kExp) + Kind<T>::kStep;
-#pragma unroll
-    for (int i = 0; i < (NL + 3) / 4; ++i) bad[i] = 0;
+    bad = 0;
     if (!(any & 0x80008000u)) return;
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
         const uint32_t e = ((v[i][w] & Kind<T>::kExp) + Kind<T>::kStep) & 0x80008000u;
-        bad[i / 4] |= ((e >> 15 & 1u) | (e >> 30 & 2u)) << (8 * (i % 4) + 2 * w);
+        bad |= ((e >> 15 & 1u) | (e >> 30 & 2u)) << (8 * i + 2 * w);
         v[i][w] &= ~((e >> 15) * 0xffffu);
       }
       vs[i * kThreads] = v[i];
     }
   }
 
-  // Into LDS.  In a tile that not every row sees whole, a value that is not finite would reach the rows that do not see it (0 times
-  // infinity): it is stored as zero, and the bits returned say which values were.
-  __device__ __forceinline__ void store(bool partly, uint32_t (&bad)[(NL + 3) / 4]) {
-    const int ch = threadIdx.x % CH, row0 = threadIdx.x / CH;
-    char* vs = sm + TILE * D * 2;
-#pragma unroll
-    for (int i = 0; i < NL; ++i) {
-      const int row = row0 + i * STEP;
-      *reinterpret_cast<hq_u4v*>(sm + row * D * 2 + k_piece(row, ch) * 16) = kr[i];
-      if (partly) {
-        if (i % 4 == 0) bad[i / 4] = 0;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          const uint32_t e = ((vr[i][w] & Kind<T>::kExp) + Kind<T>::kStep) & 0x80008000u;
-          if (e) {
-            bad[i / 4] |= ((e >> 15 & 1u) | (e >> 30 & 2u)) << (8 * (i % 4) + 2 * w);
-            vr[i][w] &= ~((e >> 15) * 0xffffu);
-          }
-        }
-      }
-      *reinterpret_cast<hq_u4v*>(vs + row * D * 2 + v_piece(row, ch) * 16) = vr[i];
-    }
-  }
   // The same places again, one for each value that was not finite and zero for the others.
-  static __device__ __forceinline__ void store_bad(char* vs, const uint32_t (&bad)[(NL + 3) / 4]) {
-    const int ch = threadIdx.x % CH, row0 = threadIdx.x / CH;
+  static __device__ __forceinline__ void store_bad(char* values, uint32_t bad) {
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
       hq_u4v w;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const uint32_t b = bad[i / 4] >> (8 * (i % 4) + 2 * j);
+        const uint32_t b = bad >> (8 * i + 2 * j);
         w[j] = (b & 1 ? Kind<T>::kOne & 0xffffu : 0u) | (b & 2 ? Kind<T>::kOne & 0xffff0000u : 0u);
       }
-      if (DIRECT) {
-        reinterpret_cast<hq_u4v*>(vs)[threadIdx.x + i * kThreads] = w;
-      } else {
-        const int row = row0 + i * STEP;
-        *reinterpret_cast<hq_u4v*>(vs + row * D * 2 + v_piece(row, ch) * 16) = w;
-      }
+      reinterpret_cast<hq_u4v*>(values)[threadIdx.x + i * kThreads] = w;
     }
   }
 
-  // V^T of 32 elements of the head (block d) and 16 keys (block b, half t) as the matrix core takes it: see the top of the file.
-  static __device__ __forceinline__ V8 v_operand(const char* values, int key0, int b, int t, int d) {
+  // V^T of 32 elements of the head (block d) and 16 keys (block b, half t) as the matrix core takes it: the keys in the order in which
+  // the scores' registers hold them.
+  static __device__ __forceinline__ V8 v_operand(const char* values, int b, int t, int d) {
     const int lane = threadIdx.x & 63;
-    const int row = key0 + 32 * b + 16 * t + 4 * (lane >> 5) + ((lane >> 2) & 3);
+    const int row = 32 * b + 16 * t + 4 * (lane >> 5) + ((lane >> 2) & 3);
     const int ch = 4 * d + 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1);
     lds_char* vs = (lds_char*)values + (lane & 1) * 8;
     typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
@@ -217,13 +273,13 @@ struct Attend {
       s16x4 h[2];
       V8 v;
     } u;
-    u.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(vs + row * D * 2 + v_piece(row, ch) * 16));
-    u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(vs + (row + 8) * D * 2 + v_piece(row + 8, ch) * 16));
+    u.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(vs + row * D * 2 + v_piece<D>(row, ch) * 16));
+    u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(vs + (row + 8) * D * 2 + v_piece<D>(row + 8, ch) * 16));
     return u.v;
   }
 
-  // The wave's part of a tile, step by step.  Scores of its rows and the keys from key0 on:
-  __device__ __forceinline__ void scores(f32x16 (&s)[NB], const char* keys, int key0) const {
+  // The wave's part of a tile, step by step.  Scores of its rows and the tile's keys:
+  __device__ __forceinline__ void scores(f32x16 (&s)[NB], const char* keys) const {
     const int lane = threadIdx.x & 63, half = lane >> 5;
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
@@ -231,8 +287,8 @@ struct Attend {
       for (int r = 0; r < 16; ++r) s[b][r] = 0.f;
 #pragma unroll
       for (int kk = 0; kk < D / 16; ++kk) {
-        const int row = key0 + 32 * b + (lane & 31);
-        const V8 a = *reinterpret_cast<const V8*>(keys + row * D * 2 + k_piece(row, 2 * kk + half) * 16);
+        const int row = 32 * b + (lane & 31);
+        const V8 a = *reinterpret_cast<const V8*>(keys + row * D * 2 + k_piece<D>(row, 2 * kk + half) * 16);
         s[b] = Kind<T>::mfma(a, qf[kk], s[b]);
       }
     }
@@ -287,13 +343,13 @@ struct Attend {
         }
     l += sum[0] + sum[1];
   }
-  __device__ __forceinline__ void values(const V8 (&p)[NB][2], const char* values, int key0) {
+  __device__ __forceinline__ void values(const V8 (&p)[NB][2], const char* values) {
 #pragma unroll
     for (int d = 0; d < D / 32; ++d)
 #pragma unroll
       for (int b = 0; b < NB; ++b)
 #pragma unroll
-        for (int t = 0; t < 2; ++t) o[d] = Kind<T>::mfma(v_operand(values, key0, b, t, d), p[b][t], o[d]);
+        for (int t = 0; t < 2; ++t) o[d] = Kind<T>::mfma(v_operand(values, b, t, d), p[b][t], o[d]);
   }
   // scores() of the next tile and weights() of this one, an instruction of the matrix core and its share of the others in turn: left
   // alone, the compiler moves the reads of all operands to the front and runs out of registers.
@@ -302,7 +358,7 @@ struct Attend {
     constexpr int STEPS = NB * D / 16, EACH = NB * 16 / STEPS, AHEAD = 4;
     auto operand = [&](int j) {
       const int row = 32 * (j / (D / 16)) + (lane & 31);
-      return *reinterpret_cast<const V8*>(keys + row * D * 2 + k_piece(row, 2 * (j % (D / 16)) + half) * 16);
+      return *reinterpret_cast<const V8*>(keys + row * D * 2 + k_piece<D>(row, 2 * (j % (D / 16)) + half) * 16);
     };
     const float ms = finite_or_zero(m);
     float sum[2] = {0.f, 0.f};
@@ -339,7 +395,7 @@ struct Attend {
   // values() of this tile, and the maximum of the next one's scores.
   __device__ __forceinline__ float values_and_top(const V8 (&p)[NB][2], const char* vs, const f32x16 (&n)[NB]) {
     constexpr int STEPS = D / 32 * NB * 2, EACH = NB * 16 / STEPS, AHEAD = 4;
-    auto operand = [&](int j) { return v_operand(vs, 0, j / 2 % NB, j % 2, j / (2 * NB)); };
+    auto operand = [&](int j) { return v_operand(vs, j / 2 % NB, j % 2, j / (2 * NB)); };
     V8 a[AHEAD];
     float top = n[0][0];
 #pragma unroll
@@ -356,7 +412,7 @@ struct Attend {
     return pair_max(top);
   }
   // Rows that see a value that is not finite.
-  __device__ __forceinline__ void spoil(char* values, int key0, int left, const uint32_t (&bad)[(NL + 3) / 4]) {
+  __device__ __forceinline__ void spoil(char* values, int left, uint32_t bad) {
     __syncthreads();
     store_bad(values, bad);
     __syncthreads();
@@ -372,18 +428,15 @@ struct Attend {
           V8 seen;
 #pragma unroll
           for (int i = 0; i < 8; ++i) seen[i] = 32 * b + 16 * t + 8 * (i / 4) + i % 4 < left ? (T)1.f : (T)0.f;
-          n = Kind<T>::mfma(v_operand(values, key0, b, t, d), seen, n);
+          n = Kind<T>::mfma(v_operand(values, b, t, d), seen, n);
         }
 #pragma unroll
       for (int r = 0; r < 16; ++r) o[d][r] = n[r] > 0.f ? NAN : o[d][r];
     }
   }
   __device__ __forceinline__ bool spoiled(int tileno) const { return *(volatile __attribute__((address_space(3))) int*)poison == tileno; }
-  __device__ __forceinline__ void note(const uint32_t (&bad)[(NL + 3) / 4], int tileno) {
-    uint32_t any = 0;
-#pragma unroll
-    for (int i = 0; i < (NL + 3) / 4; ++i) any |= bad[i];
-    if (any) *poison = tileno;
+  __device__ __forceinline__ void note(uint32_t bad, int tileno) {
+    if (bad) *poison = tileno;
   }
 
   // The row's sums as one of several shares; none: the row sees nothing in any of them, which share 0 says by an infinite maximum.
@@ -398,71 +451,34 @@ struct Attend {
     if (half == 0) *reinterpret_cast<float2*>(pm + 2 * at) = float2{none ? INFINITY : m, l};
   }
 
-  // Keys [first, end) of src; whole: keys below it are seen by every row of the workgroup.
+  // Keys [first, end) of src; whole: keys below it are seen by every row of the workgroup.  A tile is on its way from memory while the one
+  // before it is worked on, with one barrier a tile.  Heads of 128: the scores of the next tile are in the matrix core while the vector
+  // unit makes this one's weights of its own, and the next scores' maximum is taken under this tile's product with the values; the
+  // keys so run a tile ahead.  Heads of 64, where the vector unit is the busier of the two and the registers saved are two waves more: one step after
+  // the other (16384 tokens, heads of 128: 2186 us one after the other, 2116 so; 8192 tokens, heads of 64: 359 and 376).
   template <typename SRC>
-  __device__ __forceinline__ void run(const SRC& src, int first, int end, int whole, float c) {
-    clear();
+  __device__ __forceinline__ void run(SRC& src, int first, int end, int whole, float c) {
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[d][r] = 0.f;
     if (first >= end) return;
-    uint32_t bad[(NL + 3) / 4] = {};
-    char* const vs = sm + TILE * D * 2;
-    const int key0 = RW == 4 ? 0 : (threadIdx.x >> 6) * 32 * NB;
-    load(src, first);
-    for (int base = first, tileno = 0; base < end; base += TILE, ++tileno) {
-      const bool partly = base + TILE > whole;
-      __syncthreads();
-      store(partly, bad);
-      if (partly) note(bad, tileno);
-      __syncthreads();
-      if (base + TILE < end) load(src, base + TILE);
-      const int left = lim - base - key0 - 4 * ((threadIdx.x >> 5) & 1);
-      if (base + key0 < any_sees) {
-        f32x16 s[NB];
-        V8 p[NB][2];
-        scores(s, sm, key0);
-        if (base + key0 + 32 * NB > all_see) mask(s, left);
-        raise(top_of(s) * c);
-        weights(p, s, c);
-        values(p, vs, key0);
-      }
-      if (partly && spoiled(tileno)) spoil(vs, key0, left, bad);
-    }
-    l = pair_sum(l);
-  }
-
-  // The same, DIRECT.  Heads of 128: the scores of the next tile are in the matrix core while the vector unit makes this one's weights
-  // of its own, and the next scores' maximum is taken under this tile's product with the values; the keys so run a tile ahead.  Heads
-  // of 64, where the vector unit is the busier of the two and the registers saved are two waves more: one step after the other
-  // (16384 tokens, heads of 128: 2186 us one after the other, 2130 so; 8192 tokens, heads of 64: 359 and 376).
-  template <typename SRC>
-  __device__ __forceinline__ void run_direct(const SRC& src, int first, int end, int whole, float c) {
-    clear();
-    if (first >= end) return;
-    constexpr int HALF = TILE * D * 2, K_AHEAD = D == 128;
-    const int nt = (end - first + TILE - 1) / TILE;
-    direct_offsets(koff, (int)src.ks, src.n - first, [](int row, int ch) { return k_piece(row, ch); });
-    direct_offsets(voff, (int)src.vs, src.n - first, [](int row, int ch) { return v_piece(row, ch); });
-    auto load_k = [&](int t, int slot) {
-      const int base = first + t * TILE;
-      if (base + TILE > src.n) direct_offsets(koff, (int)src.ks, src.n - base, [](int row, int ch) { return k_piece(row, ch); });
-      direct_load(src.k + base * src.ks, koff, sm + slot * HALF);
-    };
-    auto load_v = [&](int t, int slot) {
-      const int base = first + t * TILE;
-      if (base + TILE > src.n) direct_offsets(voff, (int)src.vs, src.n - base, [](int row, int ch) { return v_piece(row, ch); });
-      direct_load(src.v + base * src.vs, voff, sm + (2 + slot) * HALF);
-    };
-    const int half4 = 4 * ((threadIdx.x >> 5) & 1);
+    const int nt = (end - first + TILE - 1) / TILE, half4 = 4 * ((threadIdx.x >> 5) & 1);
     f32x16 s0[NB], s1[NB];
     float top = 0.f;
-    load_k(0, 0);
-    load_v(0, 0);
+    src.start(first);
+    src.advance(0);
+    src.load_k(0, sm);
+    if (!K_AHEAD) src.load_v(0, sm + 2 * HALF);
 #pragma unroll
     for (int kk = 0; kk < D / 16; ++kk) asm volatile("" : "+v"(qf[kk]));  // here, not at every tile: the loads in flight then are the next tile's
     if (K_AHEAD) {
+      src.advance(1);
+      src.load_v(0, sm + 2 * HALF);
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       __syncthreads();
-      if (nt > 1) load_k(1, 1);
-      scores(s0, sm, 0);
+      if (nt > 1) src.load_k(1, sm + HALF);
+      scores(s0, sm);
       if (first + TILE > all_see) mask(s0, lim - first - half4);
       top = top_of(s0);
     }
@@ -472,11 +488,14 @@ struct Attend {
       const int base = first + t * TILE;
       const bool partly = base + TILE > whole;
       char* const vs = sm + (2 + SLOT) * HALF;
-      uint32_t bad[(NL + 3) / 4] = {};
+      uint32_t bad = 0;
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       __syncthreads();
-      if (t + 1 + K_AHEAD < nt) load_k(t + 1 + K_AHEAD, (SLOT + 1 + K_AHEAD) % 2);
-      if (t + 1 < nt) load_v(t + 1, 1 - SLOT);
+      if (t + 1 < nt) {
+        src.advance(t + 1 + K_AHEAD);
+        if (t + 1 + K_AHEAD < nt) src.load_k(t + 1 + K_AHEAD, sm + (SLOT + 1 + K_AHEAD) % 2 * HALF);
+        src.load_v(t + 1, sm + (3 - SLOT) * HALF);
+      }
       if (partly) {
         clean(vs, bad);
         note(bad, t);
@@ -490,16 +509,16 @@ struct Attend {
           if (base + 2 * TILE > all_see) mask(n, lim - base - TILE - half4);
           top = values_and_top(p, vs, n);
         } else {
-          scores(s, sm + SLOT * HALF, 0);
+          scores(s, sm + SLOT * HALF);
           if (base + TILE > all_see) mask(s, lim - base - half4);
           raise(top_of(s) * c);
           weights(p, s, c);
-          values(p, vs, 0);
+          values(p, vs);
         }
       }
-      if (partly && spoiled(t)) spoil(vs, 0, lim - base - half4, bad);
+      if (partly && spoiled(t)) spoil(vs, lim - base - half4, bad);
     };
-    if (K_AHEAD) {
+    if constexpr (K_AHEAD) {
       int t = 0;
       for (; t + 1 < nt; t += 2) {
         step(t, std::integral_constant<int, 0>(), s0, s1);
@@ -510,6 +529,188 @@ struct Attend {
       for (int t = 0; t < nt; ++t) step(t, t & 1, s0, s1);
     }
     l = pair_sum(l);
+  }
+
+  // The row's result.
+  __device__ __forceinline__ void put(T* out, bool none) const {
+    const int half = (threadIdx.x >> 5) & 1;
+    const float inv = 1.f / l;
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        typedef T T4 __attribute__((ext_vector_type(4)));
+        T4 v;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = (T)(none ? 0.f : o[d][4 * g + i] * inv);
+        *reinterpret_cast<T4*>(out + 32 * d + 8 * g + 4 * half) = v;
+      }
+  }
+};
+
+// ---- few rows ------------------------------------------------------------------------------------------------------------
+// Up to 16 rows that all see the same keys.  The workgroup's keys are dealt out to its waves in blocks of 32; a wave's block is on its
+// way into LDS of its own while the wave works on what it has: the keys' half is free, and filled again, once the scores are made, the values'
+// once they are summed, and no wave waits for another.  A row's scores are in four lanes, 16 apart (16x16 tiles: with 32 rows a
+// tile half of the vector unit's work would be for rows that are not there).  Bound by memory.
+template <typename T, int D>
+struct Few {
+  typedef typename Kind<T>::V8 V8;
+  static constexpr int CH = D / 8, RG = 64 / CH, G = 32 / RG;  // pieces of a row; rows of an instruction; instructions of a block's keys
+  static constexpr int HALF = 32 * D * 2, LDS = kWaves * 2 * HALF, STRIDE = D + 4;
+  static_assert(kWaves * 16 * STRIDE * 4 <= LDS, "the waves' sums");
+
+  char* sm;
+  V8 qf[D / 32];
+  f32x4 o[D / 16];
+  float m = -INFINITY, l = 0.f;
+
+  __device__ __forceinline__ void run(const Pages<T, D>& p, int first, int end, float c) {
+    const int lane = threadIdx.x & 63, wave = uniform((int)(threadIdx.x >> 6)), quarter = lane >> 4;
+#pragma unroll
+    for (int d = 0; d < D / 16; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const int blocks = (end - first + 31) / 32;
+    if (wave >= blocks) return;
+    char* const ks = sm + wave * 2 * HALF;
+    char* const vs = ks + HALF;
+    uint32_t koff[G], voff[G];
+#pragma unroll
+    for (int i = 0; i < G; ++i) {
+      const int row = i * RG + lane / CH;
+      koff[i] = (lane / CH) * D * 2 + k_piece<D>(row, lane % CH) * 16;
+      voff[i] = (lane / CH) * D * 2 + v_piece<D>(row, lane % CH) * 16;
+    }
+    // pages of 64 / G blocks, a lane for each instruction of each
+    constexpr int SET = 64 / G;
+    auto ids_of = [&](int set) { return p.id(min(first + (wave + kWaves * (set * SET + lane / G)) * 32 + lane % G * RG, end - 1)); };
+    int ids = ids_of(0), ids_next = 0;
+    // Whether all G instructions were needed: what the waits count.
+    auto load = [&](const T* pool, int block, int set_ids, const uint32_t (&off)[G], char* to, bool values) {
+      const int base = first + block * 32, at = block / kWaves % SET * G;
+      const uint32_t lds = uniform((int)lds_address(to));
+      bool whole = true;
+      if (base + 32 <= end) {
+#pragma unroll
+        for (int i = 0; i < G; ++i) {
+          const int page = __builtin_amdgcn_readlane(set_ids, at + i);
+          if (page >= 0) to_lds(lds + i * 1024, uniform(pool + p.at(page, base + i * RG)), off[i]);
+          else zero_lds(to + i * 1024);
+          whole &= page >= 0;
+        }
+      } else {  // the last block: rows behind the last key repeat it, every lane by an address of its own
+#pragma unroll
+        for (int i = 0; i < G; ++i) {
+          const int row = i * RG + lane / CH, key = min(base + row, end - 1), page = __shfl(set_ids, at + (key - base) / RG);
+          const int ch = values ? v_piece<D>(row, lane % CH) : k_piece<D>(row, lane % CH);
+          if (page >= 0) to_lds(lds + i * 1024, pool + p.at(page, key) + ch * 8);
+          else zero_lds(to + i * 1024);
+          whole &= __ballot(page < 0) == 0;
+        }
+      }
+      return whole;
+    };
+    // Waits for everything but the last load(), if that was a whole one.
+    auto wait_but = [](bool whole) {
+      if (whole) asm volatile("s_waitcnt vmcnt(%0)" ::"i"(G) : "memory");
+      else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    };
+    load(p.k, wave, ids, koff, ks, false);
+    bool whole_k = false, whole_v = load(p.v, wave, ids, voff, vs, true);
+#pragma unroll
+    for (int kk = 0; kk < D / 32; ++kk) asm volatile("" : "+v"(qf[kk]));
+    for (int block = wave; block < blocks; block += kWaves) {
+      const int base = first + block * 32, nth = block / kWaves, next = block + kWaves;
+      const bool more = next < blocks, set_ends = (nth + 1) % SET == 0;
+      if (nth % SET == 0 && block + SET * kWaves < blocks) ids_next = ids_of(nth / SET + 1);
+      wait_but(whole_v);  // the values may still be on their way
+      f32x4 s[2];
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        s[b] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int kk = 0; kk < D / 32; ++kk) {
+          const int row = 16 * b + (lane & 15);
+          s[b] = Kind<T>::mfma(*reinterpret_cast<const V8*>(ks + row * D * 2 + k_piece<D>(row, 4 * kk + quarter) * 16), qf[kk], s[b]);
+        }
+      }
+      float top = -INFINITY;
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          if (base + 32 > end && 16 * b + 4 * quarter + r >= end - base) s[b][r] = -INFINITY;
+          top = fmaxf(top, s[b][r]);
+        }
+      asm volatile("" : "+v"(top)::"memory");  // the keys have been read
+      whole_k = more && load(p.k, next, set_ends ? ids_next : ids, koff, ks, false);
+      top = quarters_max(top) * c;
+      if (__builtin_amdgcn_ballot_w64(top > m + 8.f)) {  // as in Many
+        const float mn = top > m + 8.f ? top : m, f = mn == m ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+        m = mn;
+        l *= f;
+#pragma unroll
+        for (int d = 0; d < D / 16; ++d)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) o[d][r] *= f;
+      }
+      const float ms = finite_or_zero(m);
+      V8 w;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float e = __builtin_amdgcn_exp2f(fmaf(s[i / 4][i % 4], c, -ms));
+        l += e;
+        w[i] = (T)e;  // rounded as in Many
+      }
+      wait_but(whole_k);
+#pragma unroll
+      for (int d = 0; d < D / 16; ++d) {
+        const int row = 4 * quarter + ((lane >> 2) & 3), ch = 2 * d + ((lane >> 1) & 1);
+        lds_char* at = (lds_char*)vs + (lane & 1) * 8;
+        typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+        union {
+          s16x4 h[2];
+          V8 v;
+        } u;
+        u.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at + row * D * 2 + v_piece<D>(row, ch) * 16));
+        u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at + (row + 16) * D * 2 + v_piece<D>(row + 16, ch) * 16));
+        o[d] = Kind<T>::mfma(u.v, w, o[d]);
+      }
+#pragma unroll
+      for (int d = 0; d < D / 16; ++d) asm volatile("" : "+v"(o[d])::"memory");  // the values have been read
+      whole_v = more && load(p.v, next, set_ends ? ids_next : ids, voff, vs, true);
+      if (set_ends) ids = ids_next;
+    }
+    l = quarters_sum(l);
+  }
+
+  // The waves' sums together: a thread's part of a row's, D / 16 elements from it % 16 of row it / 16 on, and the row's maximum and sum.
+  __device__ __forceinline__ void join(float (&sum)[D / 16], float* top, float* total) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, quarter = lane >> 4;
+    __shared__ float tops[kWaves][16], totals[kWaves][16];
+    if (quarter == 0) tops[wave][lane] = m;
+    __syncthreads();  // and nobody reads keys or values any more
+    float mm = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) mm = fmaxf(mm, tops[i][lane & 15]);
+    const float f = __builtin_amdgcn_exp2f(m - finite_or_zero(mm));
+    if (quarter == 0) totals[wave][lane] = l * f;
+    float* sums = reinterpret_cast<float*>(sm);
+#pragma unroll
+    for (int d = 0; d < D / 16; ++d) *reinterpret_cast<f32x4*>(sums + (wave * 16 + (lane & 15)) * STRIDE + 16 * d + 4 * quarter) = o[d] * f;
+    __syncthreads();
+    const int row = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * (D / 16);
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) sum[i] = 0.f;
+    *total = 0.f;
+    mm = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) sum[i] += sums[(w * 16 + row) * STRIDE + d0 + i];
+      *total += totals[w][row];
+      mm = fmaxf(mm, tops[w][row]);
+    }
+    *top = mm;
   }
 };
 
@@ -558,23 +759,10 @@ struct PromptArgs {
   float c;
 };
 
-template <typename T>
-struct PackedKeys {  // of one sequence and one head
-  const T *k, *v;
-  int64_t ks, vs;
-  int n;
-  __device__ __forceinline__ bool at(int key, const T** kp, const T** vp) const {
-    key = min(key, n - 1);
-    *kp = k + key * ks;
-    *vp = v + key * vs;
-    return true;
-  }
-};
-
 // A workgroup's rows and share of the keys.  Many rows: all keys, and the result; few: the keys are divided among `shares` workgroups.
 template <typename T, int D>
 __global__ __launch_bounds__(kThreads, D == 64 ? 4 : 2) void prompt_kernel(PromptArgs a) {
-  typedef Attend<T, D, 4, true> A;
+  typedef Many<T, D> A;
   typedef typename Kind<T>::V8 V8;
   constexpr int ROWS = 128;
   extern __shared__ __align__(16) char sm[];
@@ -608,24 +796,18 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 4 : 2) void prompt_kernel(Promp
   w.lim = limit(token);
   w.all_see = __builtin_amdgcn_readlane(w.lim, 0);  // a later row sees as much or more
   w.any_sees = __builtin_amdgcn_readlane(w.lim, 31);
-  PackedKeys<T> src{(const T*)a.k + (int64_t)k0 * a.ks + head * D, (const T*)a.v + (int64_t)k0 * a.vs + head * D, a.ks, a.vs, nk};
+  PackedTiles<T, D> src;
+  src.k = (const T*)a.k + (int64_t)k0 * a.ks + head * D;
+  src.v = (const T*)a.v + (int64_t)k0 * a.vs + head * D;
+  src.ks = a.ks;
+  src.vs = a.vs;
+  src.n = nk;
   const int each = a.shares == 1 ? nk : max(256, ((nk + a.shares - 1) / a.shares + A::TILE - 1) & -A::TILE);
   const int end = uniform(limit((uint32_t)last_row / ratio)), first = (int)min((int64_t)share * each, (int64_t)end);
-  w.run_direct(src, first, min(end, first + each), uniform(limit((uint32_t)first_row / ratio)), a.c);
+  w.run(src, first, min(end, first + each), uniform(limit((uint32_t)first_row / ratio)), a.c);
   if (row > last_row) return;
   if (a.shares == 1) {
-    const float inv = 1.f / w.l;
-    T* out = (T*)a.out + ((int64_t)(q0 + token) * a.heads + h) * D + 4 * (lane >> 5);
-#pragma unroll
-    for (int d = 0; d < D / 32; ++d)
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        typedef T T4 __attribute__((ext_vector_type(4)));
-        T4 v;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = (T)(w.lim == 0 ? 0.f : w.o[d][4 * g + i] * inv);  // a token that sees no key
-        *reinterpret_cast<T4*>(out + 32 * d + 8 * g) = v;
-      }
+    w.put((T*)a.out + ((int64_t)(q0 + token) * a.heads + h) * D, w.lim == 0);
   } else {
     w.put_share(a.po, a.pm, ((int64_t)(q0 + token) * a.heads + h) * a.shares + share, w.lim == 0);
   }
@@ -636,179 +818,182 @@ struct PagedArgs {
   const void *q, *k, *v;
   void* out;
   const int *table, *lengths, *groups, *shared;
-  float *po, *pm;      // partial sums [batch * heads][slots][D], and {maximum, sum} [batch * heads][slots]
+  float *po, *pm;      // shares of the sums [batch * heads][slots][D], and {maximum, sum} [batch * heads][slots]
+  int* np;             // shares that the common keys are divided into, said by the kernel
   int64_t qs;
   int ngroups, batch, width, pages, page_log, heads, kv_heads, ratio;
-  int np, ns;          // shares that a group's common keys, and a request's own, are divided into
+  int most_np, ns;     // at most; shares of a request's own keys
   int prefix_items;    // workgroups of the common keys
   float c;
 };
 
-template <typename T, int D>
-struct PagedKeys {
-  const T *k, *v;
-  const int* pages_of;  // the row of the table
-  int head, kv_heads, page_log, pages, n;
-  __device__ __forceinline__ bool at(int key, const T** kp, const T** vp) const {
-    key = min(key, n - 1);
-    const int page = pages_of[key >> page_log], p = (unsigned)page < (unsigned)pages ? page : 0;
-    const int64_t off = ((((int64_t)p * kv_heads + head) << page_log) + (key & ((1 << page_log) - 1))) * D;
-    *kp = k + off;
-    *vp = v + off;
-    return p == page;
-  }
-};
-
-// Tokens that the requests of group g have in common: those of the first one's row that the caller says are.
+// Tokens that the requests of group g have in common: those of the first one's row that the caller says are, in whole pages (the
+// others are in the same page too, but every request reads what it has there as its own).
 __device__ __forceinline__ int shared_tokens(const PagedArgs& a, int g) {
   const int first = min(max(a.groups[g], 0), a.batch - 1);
-  return min(min(max(a.shared[g], 0), max(a.lengths[first], 0)), a.width << a.page_log);
+  return min(min(max(a.shared[g], 0), max(a.lengths[first], 0)), a.width << a.page_log) & -(1 << a.page_log);
+}
+// The group of request b, -1 if it is in none.
+__device__ __forceinline__ int group_of(const PagedArgs& a, int b) {
+  for (int g0 = 0; g0 < a.ngroups; g0 += 64) {
+    const int g = g0 + (threadIdx.x & 63);
+    const unsigned long long here = __ballot(g < a.ngroups && b >= a.groups[min(g, a.ngroups)] && b < a.groups[min(g + 1, a.ngroups)]);
+    if (here) return g0 + __ffsll(here) - 1;
+  }
+  return -1;
 }
 
-// Keys of share s of n, as many as make `shares` shares of whole tiles of 128, 256 at least.
-__device__ __forceinline__ void share_of(int n, int shares, int s, int* first, int* end) {
-  int each = (n + shares - 1) / shares;
-  each = max(256, (each + 127) & ~127);
-  *first = min((int64_t)s * each, (int64_t)n);
+// Keys of share s of n, as many as make `shares` shares of whole tiles of 128, `least` at least.
+__device__ __forceinline__ void share_of(int n, int shares, int least, int s, int* first, int* end) {
+  const int each = max(least, ((n + shares - 1) / shares + 127) & ~127);
+  *first = (int)min((int64_t)s * each, (int64_t)n);
   *end = min(*first + each, n);
 }
 
-template <typename T, int D, int RW>
-__device__ __forceinline__ void attend_rows(const PagedArgs& a, char* sm, int* poison, int b0, int nrows, int first_row, int head, int src_row,
-                                            int first, int end, int shared_end, int slot) {
-  typedef Attend<T, D, RW> A;
+template <typename T, int D>
+__device__ __forceinline__ Pages<T, D> pages_of(const PagedArgs& a, int request, int head) {
+  return Pages<T, D>{(const T*)a.k, (const T*)a.v, a.table + (int64_t)request * a.width, head, a.kv_heads, a.page_log, a.pages};
+}
+
+// Up to 16 of the rows (request, head of the group) of requests b0 ..., from first_row on, all of which see the keys.
+template <typename T, int D>
+__device__ __forceinline__ void few_rows(const PagedArgs& a, char* sm, int b0, int nrows, int first_row, int head, int first, int end, int slot) {
   typedef typename Kind<T>::V8 V8;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int slots = a.np + a.ns;
-  const int last_row = min(first_row + 32 * RW, nrows) - 1;
-  const int row = first_row + (RW == 4 ? wave * 32 : 0) + (lane & 31), r = min(row, last_row);
-  const int b = b0 + r / a.ratio, h = head * a.ratio + r % a.ratio;
-  A w;
+  const int lane = threadIdx.x & 63, last_row = min(first_row + 16, nrows) - 1, r = min(first_row + (lane & 15), last_row);
+  const uint32_t ratio = a.ratio;
+  const int b = b0 + (uint32_t)r / ratio, h = head * ratio + (uint32_t)r % ratio;
+  Few<T, D> w;
   w.sm = sm;
-  w.poison = poison;
-  const T* q = (const T*)a.q + (int64_t)b * a.qs + (int64_t)h * D + 8 * (lane >> 5);
+  const T* q = (const T*)a.q + (int64_t)b * a.qs + (int64_t)h * D + 8 * (lane >> 4);
 #pragma unroll
-  for (int kk = 0; kk < D / 16; ++kk) w.qf[kk] = *reinterpret_cast<const V8*>(q + 16 * kk);
-  w.lim = min(min(max(a.lengths[b], 0), a.width << a.page_log), shared_end);
-  w.all_see = uniform(wave_min(w.lim));
-  w.any_sees = -uniform(wave_min(-w.lim));
-  // what every row of the workgroup sees
-  __shared__ int seen[kWaves];
-  if (lane == 0) seen[wave] = w.all_see;
-  __syncthreads();
-  const int whole = min(min(seen[0], seen[1]), min(seen[2], seen[3]));
-  PagedKeys<T, D> src{(const T*)a.k, (const T*)a.v, a.table + (int64_t)src_row * a.width, head, a.kv_heads, a.page_log, a.pages, end};
-  w.run(src, first, end, whole, a.c);
-  const int64_t at = ((int64_t)b * a.heads + h) * slots + slot;
-  if (RW == 1) {  // the four waves' sums come together
-    float* sum = reinterpret_cast<float*>(sm);          // [wave][D][32]
-    __shared__ float top[kWaves][32], total[kWaves][32];
-    __syncthreads();
-    if (lane < 32) top[wave][lane] = w.m;
-    __syncthreads();
-    float m = -INFINITY;
+  for (int kk = 0; kk < D / 32; ++kk) w.qf[kk] = *reinterpret_cast<const V8*>(q + 32 * kk);
+  w.run(pages_of<T, D>(a, b0, head), first, end, a.c);
+  float sum[D / 16], top, total;
+  w.join(sum, &top, &total);
+  const int mine = first_row + (threadIdx.x >> 4), d0 = (threadIdx.x & 15) * (D / 16), slots = a.most_np + a.ns;
+  if (mine > last_row) return;
+  const int64_t at = (int64_t)(b0 + (uint32_t)mine / ratio) * a.heads + head * ratio + (uint32_t)mine % ratio;
+  if (slots == 1) {
+    typedef T TD __attribute__((ext_vector_type(D / 16)));
+    TD v;
 #pragma unroll
-    for (int i = 0; i < kWaves; ++i) m = fmaxf(m, top[i][lane & 31]);
-    const float f = __builtin_amdgcn_exp2f(w.m - finite_or_zero(m));
-    if (lane < 32) total[wave][lane] = w.l * f;
-#pragma unroll
-    for (int d = 0; d < D / 32; ++d)
-#pragma unroll
-      for (int i = 0; i < 16; ++i)
-        sum[(wave * D + 32 * d + 8 * (i / 4) + 4 * (lane >> 5) + i % 4) * 32 + (lane & 31)] = w.o[d][i] * f;
-    __syncthreads();
-    float all = 0.f;
-#pragma unroll
-    for (int i = 0; i < kWaves; ++i) all += total[i][lane & 31];
-    if (row > last_row) return;
-    const int part = threadIdx.x >> 5;  // eight parts of the head
-    if (slots == 1) {
-      T* out = (T*)a.out + ((int64_t)b * a.heads + h) * D;
-      const float inv = 1.f / all;
-      for (int d = part * (D / 8); d < (part + 1) * (D / 8); ++d) {
-        float v = 0.f;
-#pragma unroll
-        for (int i = 0; i < kWaves; ++i) v += sum[(i * D + d) * 32 + (lane & 31)];
-        out[d] = (T)(w.lim <= 0 ? 0.f : v * inv);
-      }
-    } else {
-      for (int d = part * (D / 8); d < (part + 1) * (D / 8); ++d) {
-        float v = 0.f;
-#pragma unroll
-        for (int i = 0; i < kWaves; ++i) v += sum[(i * D + d) * 32 + (lane & 31)];
-        a.po[at * D + d] = v;
-      }
-      if (part == 0) {
-        a.pm[2 * at] = m;
-        a.pm[2 * at + 1] = all;
-      }
-    }
+    for (int i = 0; i < D / 16; ++i) v[i] = (T)(first >= end ? 0.f : sum[i] / total);
+    *reinterpret_cast<TD*>((T*)a.out + at * D + d0) = v;
   } else {
-    if (row <= last_row) w.put_share(a.po, a.pm, at, false);
+#pragma unroll
+    for (int i = 0; i < D / 16; i += 4)
+      *reinterpret_cast<hq_f4v*>(a.po + (at * slots + slot) * D + d0 + i) = hq_f4v{sum[i], sum[i + 1], sum[i + 2], sum[i + 3]};
+    if (d0 == 0) *reinterpret_cast<float2*>(a.pm + 2 * (at * slots + slot)) = float2{top, total};
   }
 }
 
+// Up to 128 of them; a row sees keys up to its request's length.
 template <typename T, int D>
-__global__ __launch_bounds__(kThreads, 2) void paged_kernel(PagedArgs a) {
+__device__ __forceinline__ void many_rows(const PagedArgs& a, char* sm, int* poison, int b0, int nrows, int first_row, int head, int first, int end,
+                                          int slot) {
+  typedef typename Kind<T>::V8 V8;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int last_row = min(first_row + 128, nrows) - 1, row = first_row + wave * 32 + (lane & 31), r = min(row, last_row);
+  const uint32_t ratio = a.ratio;
+  const int b = b0 + (uint32_t)r / ratio, h = head * ratio + (uint32_t)r % ratio;
+  Many<T, D> w;
+  w.sm = sm;
+  w.poison = poison;
+  set_up(poison);
+  const T* q = (const T*)a.q + (int64_t)b * a.qs + (int64_t)h * D + 8 * (lane >> 5);
+#pragma unroll
+  for (int kk = 0; kk < D / 16; ++kk) w.qf[kk] = *reinterpret_cast<const V8*>(q + 16 * kk);
+  w.lim = min(min(max(a.lengths[b], 0), a.width << a.page_log), end);
+  w.all_see = uniform(wave_min(w.lim));
+  w.any_sees = first_row + wave * 32 > last_row ? 0 : -uniform(wave_min(-w.lim));  // a wave without rows works on nothing
+  __shared__ int seen[kWaves];  // what every row of the workgroup sees
+  if (lane == 0) seen[wave] = w.all_see;
+  __syncthreads();
+  const int whole = min(min(seen[0], seen[1]), min(seen[2], seen[3]));
+  PagedTiles<T, D> src;
+  src.p = pages_of<T, D>(a, b0, head);
+  src.n = end;
+  w.run(src, first, end, uniform(whole), a.c);
+  if (row > last_row) return;
+  const int slots = a.most_np + a.ns;
+  const int64_t at = (int64_t)b * a.heads + h;
+  if (slots == 1) w.put((T*)a.out + at * D, w.lim == 0);
+  else w.put_share(a.po, a.pm, at * slots + slot, false);
+}
+
+template <typename T, int D>
+__global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void paged_kernel(PagedArgs a) {
   extern __shared__ __align__(16) char sm[];
   __shared__ int poison;
-  set_up(&poison);
-  int x = blockIdx.x;
-  if (x < a.prefix_items) {
-    const int head = x % a.kv_heads;
-    x /= a.kv_heads;
-    const int share = x % a.np;
+  uint32_t x = blockIdx.x;
+  if ((int)x < a.prefix_items) {
+    // The common keys: as many shares as there are workgroups for the tiles of rows that there are.
+    const int ratio = a.ratio, batch = a.batch;
+    auto tiles = [=](int n) { return (int)(((int64_t)n * ratio + 127) / 128); };
+    int all = 0;
+    for (int g = threadIdx.x & 63; g < a.ngroups; g += 64) {
+      const int b = min(max(a.groups[g], 0), batch);
+      all += tiles(min(max(a.groups[g + 1], b), batch) - b);
+    }
+#pragma unroll
+    for (int d = 32; d; d >>= 1) all += __shfl_xor(all, d);
+    all = uniform(all);
+    const int np = all ? min(max(a.prefix_items / (all * a.kv_heads), 1), a.most_np) : 0;
+    if (x == 0 && threadIdx.x == 0) *a.np = np;
+    if (np == 0) return;
+    const int head = x % (uint32_t)a.kv_heads;
+    x /= (uint32_t)a.kv_heads;
+    const int share = x % (uint32_t)np;
     int g, tile, b0, nb;
-    const int ratio = a.ratio;
-    if (!find_tile(a.groups, a.ngroups, a.batch, x / a.np, [=](int n) { return (int)((n * (int64_t)ratio + 127) / 128); }, &g, &b0, &nb, &tile)) return;
-    const int n = shared_tokens(a, g);
+    if (!find_tile(a.groups, a.ngroups, batch, x / (uint32_t)np, tiles, &g, &b0, &nb, &tile)) return;
+    const int n = uniform(shared_tokens(a, g));
     int first, end;
-    share_of(n, a.np, share, &first, &end);
-    if (nb * ratio <= 32)
-      attend_rows<T, D, 1>(a, sm, &poison, b0, nb * ratio, 0, head, b0, first, end, n, share);
-    else
-      attend_rows<T, D, 4>(a, sm, &poison, b0, nb * ratio, tile * 128, head, b0, first, end, n, share);
+    share_of(n, np, 256, share, &first, &end);
+    const int lane = threadIdx.x & 63;
+    const bool few = nb * ratio <= 16 && !__ballot(lane < nb && a.lengths[b0 + min(lane, nb - 1)] < end);
+    if (few) few_rows<T, D>(a, sm, b0, nb * ratio, 0, head, first, end, share);
+    else many_rows<T, D>(a, sm, &poison, b0, nb * ratio, tile * 128, head, first, end, share);
   } else {
     x -= a.prefix_items;
-    const int head = x % a.kv_heads;
-    x /= a.kv_heads;
-    const int share = x % a.ns, tiles = (a.ratio + 31) / 32;
-    const int tile = x / a.ns % tiles, b = x / a.ns / tiles;
-    int from = 0;
-    for (int g = 0; g < a.ngroups; ++g)
-      if (b >= a.groups[g] && b < a.groups[g + 1]) from = shared_tokens(a, g);
-    const int n = min(max(a.lengths[b], 0), a.width << a.page_log);
-    from = min(from, n);
+    const int head = x % (uint32_t)a.kv_heads;
+    x /= (uint32_t)a.kv_heads;
+    const int share = x % (uint32_t)a.ns;
+    x /= (uint32_t)a.ns;
+    const int tiles = a.ratio <= 16 ? 1 : (a.ratio + 127) / 128, tile = tiles == 1 ? 0 : x % (uint32_t)tiles, b = tiles == 1 ? x : x / (uint32_t)tiles;
+    const int g = group_of(a, b), n = min(max(a.lengths[b], 0), a.width << a.page_log), from = uniform(g < 0 ? 0 : min(shared_tokens(a, g), n));
     int first, end;
-    share_of(n - from, a.ns, share, &first, &end);
-    attend_rows<T, D, 1>(a, sm, &poison, b, a.ratio, tile * 32, head, b, from + first, from + end, INT_MAX, a.np + share);
+    share_of(n - from, a.ns, 128, share, &first, &end);
+    if (a.ratio <= 16) few_rows<T, D>(a, sm, b, a.ratio, 0, head, from + first, from + end, a.most_np + share);
+    else many_rows<T, D>(a, sm, &poison, b, a.ratio, tile * 128, head, from + first, from + end, a.most_np + share);
   }
 }
 
 // The shares of a row together, one wave a row: their maxima and sums a lane each, then the sums of the values, 16 bytes a lane,
-// several shares at a time.  first: shares before it were not written.
+// several shares at a time.  Of the shares, those from `np` to `own` were not written.
 template <typename T, int D>
-__device__ __forceinline__ void join_shares(const float* po, const float* pm, int64_t row, int first, int slots, bool none, T* out) {
+__device__ __forceinline__ void join_shares(const float* po, const float* pm, int64_t row, int np, int own, int slots, bool none, T* out) {
   constexpr int LANES = D / 4, AT_ONCE = 64 / LANES;  // lanes of a share, shares of a load
   const int lane = threadIdx.x & 63, d = (lane % LANES) * 4;
   const float2* ml = reinterpret_cast<const float2*>(pm) + row * slots;
   float m = -INFINITY;
-  for (int s = first + lane; s < slots; s += 64) m = fmaxf(m, ml[s].x);
+  const int gap = own - np, n = slots - gap;
+  auto slot = [=](int s) { return s < np ? s : s + gap; };
+  for (int s = lane; s < n; s += 64) m = fmaxf(m, ml[slot(s)].x);
   m = hq_wave_max(m);
   const float ms = finite_or_zero(m);
   float l = 0.f;
   hq_f4v o = {0.f, 0.f, 0.f, 0.f};
-  for (int s0 = first; s0 < slots; s0 += 64) {
+  for (int s0 = 0; s0 < n; s0 += 64) {
     const int s = s0 + lane;
-    const float2 mine = s < slots ? ml[s] : float2{-INFINITY, 0.f};
+    const float2 mine = s < n ? ml[slot(s)] : float2{-INFINITY, 0.f};
     const float f = __builtin_amdgcn_exp2f(mine.x - ms);
     l += mine.y * f;
-    const int n = min(slots - s0, 64);
+    const int here = min(n - s0, 64);
 #pragma unroll 4
-    for (int i = 0; i < n; i += AT_ONCE) {
+    for (int i = 0; i < here; i += AT_ONCE) {
       const int at = i + lane / LANES;
       const float w = __shfl(f, at & 63);
-      if (at < n && w != 0.f) o += *reinterpret_cast<const hq_f4v*>(po + (row * slots + s0 + at) * D + d) * w;
+      if (at < here && w != 0.f) o += *reinterpret_cast<const hq_f4v*>(po + (row * slots + slot(s0 + at)) * D + d) * w;
     }
   }
   l = hq_wave_sum(l);
@@ -829,11 +1014,8 @@ template <typename T, int D>
 __global__ __launch_bounds__(kThreads) void join_paged_kernel(PagedArgs a) {
   const int64_t row = (int64_t)blockIdx.x * kWaves + (threadIdx.x >> 6);
   if (row >= (int64_t)a.batch * a.heads) return;
-  const int b = row / a.heads;
-  bool grouped = false;
-  for (int g = 0; g < a.ngroups; ++g) grouped |= b >= a.groups[g] && b < a.groups[g + 1];
-  // nobody wrote the common shares of a request without a group
-  join_shares<T, D>(a.po, a.pm, row, grouped ? 0 : a.np, a.np + a.ns, a.lengths[b] <= 0, (T*)a.out);
+  const int b = row / a.heads, np = group_of(a, b) >= 0 ? *a.np : 0;
+  join_shares<T, D>(a.po, a.pm, row, np, a.most_np, a.most_np + a.ns, a.lengths[b] <= 0, (T*)a.out);
 }
 
 template <typename T, int D>
@@ -843,7 +1025,7 @@ __global__ __launch_bounds__(kThreads) void join_prompt_kernel(PromptArgs a) {
   const int token = row / a.heads;
   if (token < a.cu_q[0] || token >= a.cu_q[a.seqs]) return;
   const float2 first = reinterpret_cast<const float2*>(a.pm)[row * a.shares];
-  join_shares<T, D>(a.po, a.pm, row, 0, a.shares, first.x == INFINITY && first.y == 0.f, (T*)a.out);
+  join_shares<T, D>(a.po, a.pm, row, 0, 0, a.shares, first.x == INFINITY && first.y == 0.f, (T*)a.out);
 }
 
 // Scores are compared and masked by -infinity before they are scaled: a scale of zero (all keys alike) becomes one that no score notices.
@@ -867,39 +1049,41 @@ int launch_prompt(PromptArgs a, int cus, hipStream_t stream) {
     a.po = ws.partial;
     a.pm = ws.partial + rows * a.shares * D;
   }
-  const int rc = hq_launch_as_is(prompt_kernel<T, D>, dim3((unsigned)(items * a.shares)), dim3(kThreads), Attend<T, D, 4, true>::LDS, stream, a);
+  const int rc = hq_launch_as_is(prompt_kernel<T, D>, dim3((unsigned)(items * a.shares)), dim3(kThreads), Many<T, D>::LDS, stream, a);
   if (rc != HQ_OK || a.shares == 1) return rc;
   return hq_launch_as_is(join_prompt_kernel<T, D>, dim3((unsigned)((rows + kWaves - 1) / kWaves)), dim3(kThreads), 0, stream, a);
 }
 
+// Half of the workgroups that the device holds at once for the common keys, and the requests' own keys divided until they fill the rest.
 template <typename T, int D>
 int launch_paged(PagedArgs a, int cus, hipStream_t stream) {
-  const int64_t cap = (int64_t)a.width << a.page_log, most = (cap + 255) / 256;
-  const int tiles = (a.ratio + 31) / 32;
-  const int64_t own = (int64_t)a.batch * a.kv_heads * tiles, row_tiles = (int64_t)a.batch * a.ratio / 128 + a.ngroups;
-  auto shares = [&](int64_t items) {
-    const int64_t want = (2 * (int64_t)cus + items - 1) / items;
-    return (int)(want < most ? (want < 1 ? 1 : want) : (most < 1 ? 1 : most));
-  };
-  a.ns = shares(own);
-  a.np = a.ngroups ? shares(row_tiles * a.kv_heads) : 0;
-  const int64_t prefix = a.ngroups ? row_tiles * a.kv_heads * a.np : 0, grid = prefix + own * a.ns;
+  const int64_t cap = (int64_t)a.width << a.page_log, rows = (int64_t)a.batch * a.heads;
+  const int64_t own = (int64_t)a.batch * a.kv_heads * (a.ratio <= 16 ? 1 : (a.ratio + 127) / 128);
+  const int64_t room = a.ngroups ? cus : 2 * cus;
+  a.ns = (int)std::max<int64_t>(1, std::min(room / own, (cap + 127) / 128));
+  a.most_np = 0;
+  int64_t prefix = 0;
+  if (a.ngroups) {
+    const int64_t tiles = (int64_t)a.batch * a.ratio / 128 + a.ngroups;  // at most
+    prefix = std::max<int64_t>(cus, tiles * a.kv_heads);
+    a.most_np = (int)std::max<int64_t>(1, std::min<int64_t>(cus / a.kv_heads, (cap + 255) / 256));
+  }
+  const int64_t grid = prefix + own * a.ns, slots = a.most_np + a.ns;
   if (grid > INT_MAX) return HQ_ERR_TOO_LARGE;
   a.prefix_items = (int)prefix;
-  const int64_t slots = a.np + a.ns, rows = (int64_t)a.batch * a.heads;
   if (slots > 1) {
     HqWorkspace ws;
-    const int rc = hq_get_workspace(stream, (size_t)rows * slots * (D + 2), 0, &ws);
+    const int rc = hq_get_workspace(stream, (size_t)(rows * slots * (D + 2) + 1), 0, &ws);
     if (rc != HQ_OK) return rc;
     a.po = ws.partial;
-    a.pm = ws.partial + rows * slots * D;
+    a.pm = a.po + rows * slots * D;
+    a.np = reinterpret_cast<int*>(a.pm + 2 * rows * slots);
   }
-  constexpr int lds = Attend<T, D, 1>::LDS > Attend<T, D, 4>::LDS ? Attend<T, D, 1>::LDS : Attend<T, D, 4>::LDS;
-  constexpr int sums = kWaves * D * 32 * 4, most_lds = lds > sums ? lds : sums;
-  static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&paged_kernel<T, D>),
-                                                     hipFuncAttributeMaxDynamicSharedMemorySize, most_lds);
+  constexpr int lds = std::max(Many<T, D>::LDS, Few<T, D>::LDS);
+  static const hipError_t attr =
+      hipFuncSetAttribute(reinterpret_cast<const void*>(&paged_kernel<T, D>), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
   if (attr != hipSuccess) return (int)attr;
-  int rc = hq_launch_as_is(paged_kernel<T, D>, dim3((unsigned)grid), dim3(kThreads), most_lds, stream, a);
+  const int rc = hq_launch_as_is(paged_kernel<T, D>, dim3((unsigned)grid), dim3(kThreads), lds, stream, a);
   if (rc != HQ_OK || slots == 1) return rc;
   return hq_launch_as_is(join_paged_kernel<T, D>, dim3((unsigned)((rows + kWaves - 1) / kWaves)), dim3(kThreads), 0, stream, a);
 }
