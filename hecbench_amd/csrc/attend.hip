@@ -819,7 +819,7 @@ struct PagedArgs {
   void* out;
   const int *table, *lengths, *groups, *shared;
   float *po, *pm;      // shares of the sums [batch * heads][slots][D], and {maximum, sum} [batch * heads][slots]
-  int* np;             // shares that the common keys are divided into, said by the kernel
+  int* np;             // said by the kernel: shares that the common keys are divided into, and of each request whether it has any
   int64_t qs;
   int ngroups, batch, width, pages, page_log, heads, kv_heads, ratio;
   int most_np, ns;     // at most; shares of a request's own keys
@@ -827,18 +827,25 @@ struct PagedArgs {
   float c;
 };
 
-// Tokens that the requests of group g have in common: those of the first one's row that the caller says are, in whole pages (the
-// others are in the same page too, but every request reads what it has there as its own).
-__device__ __forceinline__ int shared_tokens(const PagedArgs& a, int g) {
-  const int first = min(max(a.groups[g], 0), a.batch - 1);
-  return min(min(max(a.shared[g], 0), max(a.lengths[first], 0)), a.width << a.page_log) & -(1 << a.page_log);
-}
-// The group of request b, -1 if it is in none.
-__device__ __forceinline__ int group_of(const PagedArgs& a, int b) {
+// The groups of requests, 64 at a time, a lane each: first request, requests, and the tokens that they have in common: those of the first
+// one's row that the caller says are, in whole pages (what is behind is in the same page too, but every request reads what it has
+// there as its own).  The lengths are the only load that waits for another.
+struct Groups {
+  int begin, count, shared;
+  __device__ __forceinline__ Groups(const PagedArgs& a, int g0) {
+    const int g = g0 + (threadIdx.x & 63), at = min(g, a.ngroups - 1);
+    const int b = a.groups[at], e = a.groups[at + 1], s = a.shared[at];
+    begin = min(max(b, 0), a.batch);
+    count = g < a.ngroups ? min(max(e, begin), a.batch) - begin : 0;
+    shared = min(min(max(s, 0), max(a.lengths[min(begin, a.batch - 1)], 0)), a.width << a.page_log) & -(1 << a.page_log);
+  }
+};
+// Common tokens of request b's group; -1: it is in none.
+__device__ __forceinline__ int shared_of(const PagedArgs& a, int b) {
   for (int g0 = 0; g0 < a.ngroups; g0 += 64) {
-    const int g = g0 + (threadIdx.x & 63);
-    const unsigned long long here = __ballot(g < a.ngroups && b >= a.groups[min(g, a.ngroups)] && b < a.groups[min(g + 1, a.ngroups)]);
-    if (here) return g0 + __ffsll(here) - 1;
+    const Groups g(a, g0);
+    const unsigned long long here = __ballot(b >= g.begin && b < g.begin + g.count);
+    if (here) return __builtin_amdgcn_readlane(g.shared, __ffsll(here) - 1);
   }
   return -1;
 }
@@ -928,28 +935,43 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void paged_kernel(PagedA
   uint32_t x = blockIdx.x;
   if ((int)x < a.prefix_items) {
     // The common keys: as many shares as there are workgroups for the tiles of rows that there are.
-    const int ratio = a.ratio, batch = a.batch;
-    auto tiles = [=](int n) { return (int)(((int64_t)n * ratio + 127) / 128); };
-    int all = 0;
-    for (int g = threadIdx.x & 63; g < a.ngroups; g += 64) {
-      const int b = min(max(a.groups[g], 0), batch);
-      all += tiles(min(max(a.groups[g + 1], b), batch) - b);
-    }
+    const int ratio = a.ratio, lane = threadIdx.x & 63;
+    auto tiles = [=](const Groups& g) { return (int)(((int64_t)g.count * ratio + 127) / 128); };
+    auto running = [=](int v) {  // sums over the lanes up to each
 #pragma unroll
-    for (int d = 32; d; d >>= 1) all += __shfl_xor(all, d);
-    all = uniform(all);
+      for (int d = 1; d < 64; d <<= 1) {
+        const int u = __shfl_up(v, d);
+        if (lane >= d) v += u;
+      }
+      return v;
+    };
+    const Groups some(a, 0);
+    int all = __builtin_amdgcn_readlane(running(tiles(some)), 63);
+    for (int g0 = 64; g0 < a.ngroups; g0 += 64) all += __builtin_amdgcn_readlane(running(tiles(Groups(a, g0))), 63);
     const int np = all ? min(max(a.prefix_items / (all * a.kv_heads), 1), a.most_np) : 0;
     if (x == 0 && threadIdx.x == 0) *a.np = np;
     if (np == 0) return;
     const int head = x % (uint32_t)a.kv_heads;
     x /= (uint32_t)a.kv_heads;
     const int share = x % (uint32_t)np;
-    int g, tile, b0, nb;
-    if (!find_tile(a.groups, a.ngroups, batch, x / (uint32_t)np, tiles, &g, &b0, &nb, &tile)) return;
-    const int n = uniform(shared_tokens(a, g));
+    int tile = x / (uint32_t)np;
+    if (tile >= all) return;
+    int b0 = 0, nb = 0, n = 0;
+    for (int g0 = 0; nb == 0; g0 += 64) {
+      const Groups g = g0 ? Groups(a, g0) : some;
+      const int own = tiles(g), sum = running(own), total = __builtin_amdgcn_readlane(sum, 63);
+      if (tile < total) {
+        const int at = __ffsll(__ballot(sum > tile)) - 1;
+        b0 = __builtin_amdgcn_readlane(g.begin, at);
+        nb = __builtin_amdgcn_readlane(g.count, at);
+        n = __builtin_amdgcn_readlane(g.shared, at);
+        tile -= __builtin_amdgcn_readlane(sum - own, at);
+      } else {
+        tile -= total;
+      }
+    }
     int first, end;
     share_of(n, np, 256, share, &first, &end);
-    const int lane = threadIdx.x & 63;
     const bool few = nb * ratio <= 16 && !__ballot(lane < nb && a.lengths[b0 + min(lane, nb - 1)] < end);
     if (few) few_rows<T, D>(a, sm, b0, nb * ratio, 0, head, first, end, share);
     else many_rows<T, D>(a, sm, &poison, b0, nb * ratio, tile * 128, head, first, end, share);
@@ -960,7 +982,8 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void paged_kernel(PagedA
     const int share = x % (uint32_t)a.ns;
     x /= (uint32_t)a.ns;
     const int tiles = a.ratio <= 16 ? 1 : (a.ratio + 127) / 128, tile = tiles == 1 ? 0 : x % (uint32_t)tiles, b = tiles == 1 ? x : x / (uint32_t)tiles;
-    const int g = group_of(a, b), n = min(max(a.lengths[b], 0), a.width << a.page_log), from = uniform(g < 0 ? 0 : min(shared_tokens(a, g), n));
+    const int n = min(max(a.lengths[b], 0), a.width << a.page_log), shared = shared_of(a, b), from = uniform(min(max(shared, 0), n));
+    if (blockIdx.x - a.prefix_items == (uint32_t)b * a.kv_heads * a.ns * tiles && threadIdx.x == 0 && a.np) a.np[1 + b] = shared >= 0;
     int first, end;
     share_of(n - from, a.ns, 128, share, &first, &end);
     if (a.ratio <= 16) few_rows<T, D>(a, sm, b, a.ratio, 0, head, from + first, from + end, a.most_np + share);
@@ -968,32 +991,37 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void paged_kernel(PagedA
   }
 }
 
-// The shares of a row together, one wave a row: their maxima and sums a lane each, then the sums of the values, 16 bytes a lane,
-// several shares at a time.  Of the shares, those from `np` to `own` were not written.
-template <typename T, int D>
+// The shares of a row together, by WAVES waves: their maxima and sums a lane each, then the sums of the values, 16 bytes a lane, several
+// shares at a time; a wave takes every WAVES-th group of them.  Of the shares, those from `np` to `own` were not written.  Bound by two
+// trips to memory, one behind the other.
+template <typename T, int D, int WAVES>
 __device__ __forceinline__ void join_shares(const float* po, const float* pm, int64_t row, int np, int own, int slots, bool none, T* out) {
   constexpr int LANES = D / 4, AT_ONCE = 64 / LANES;  // lanes of a share, shares of a load
-  const int lane = threadIdx.x & 63, d = (lane % LANES) * 4;
+  const int lane = threadIdx.x & 63, d = (lane % LANES) * 4, wave = WAVES == 1 ? 0 : threadIdx.x >> 6;
   const float2* ml = reinterpret_cast<const float2*>(pm) + row * slots;
+  const float2 ahead = ml[min(lane, slots - 1)];  // under way before np is known
+  auto share = [&](int s0) {
+    const int s = s0 + lane;
+    const float2 x = s0 ? ml[min(s, slots - 1)] : ahead;
+    return s < np || (s >= own && s < slots) ? x : float2{-INFINITY, 0.f};
+  };
   float m = -INFINITY;
-  const int gap = own - np, n = slots - gap;
-  auto slot = [=](int s) { return s < np ? s : s + gap; };
-  for (int s = lane; s < n; s += 64) m = fmaxf(m, ml[slot(s)].x);
+  for (int s0 = 0; s0 < slots; s0 += 64) m = fmaxf(m, share(s0).x);
   m = hq_wave_max(m);
   const float ms = finite_or_zero(m);
   float l = 0.f;
   hq_f4v o = {0.f, 0.f, 0.f, 0.f};
-  for (int s0 = 0; s0 < n; s0 += 64) {
-    const int s = s0 + lane;
-    const float2 mine = s < n ? ml[slot(s)] : float2{-INFINITY, 0.f};
+  for (int s0 = 0; s0 < slots; s0 += 64) {
+    const int here = min(slots - s0, 64);
+    const float2 mine = share(s0);
     const float f = __builtin_amdgcn_exp2f(mine.x - ms);
     l += mine.y * f;
-    const int here = min(n - s0, 64);
-#pragma unroll 4
-    for (int i = 0; i < here; i += AT_ONCE) {
+#pragma unroll 8
+    for (int i = wave * AT_ONCE; i < here; i += WAVES * AT_ONCE) {
       const int at = i + lane / LANES;
       const float w = __shfl(f, at & 63);
-      if (at < here && w != 0.f) o += *reinterpret_cast<const hq_f4v*>(po + (row * slots + slot(s0 + at)) * D + d) * w;
+      // a share that no key went into has weight 0, and nothing was written for it
+      if (at < here && w != 0.f) o += *reinterpret_cast<const hq_f4v*>(po + (row * slots + s0 + at) * D + d) * w;
     }
   }
   l = hq_wave_sum(l);
@@ -1001,6 +1029,14 @@ __device__ __forceinline__ void join_shares(const float* po, const float* pm, in
   for (int x = LANES; x < 64; x <<= 1)
 #pragma unroll
     for (int i = 0; i < 4; ++i) o[i] += __shfl_xor(o[i], x);
+  if (WAVES > 1) {
+    __shared__ hq_f4v sums[WAVES][LANES];
+    if (lane < LANES) sums[wave][lane] = o;
+    __syncthreads();
+    if (wave > 0 || lane >= LANES) return;
+#pragma unroll
+    for (int w = 1; w < WAVES; ++w) o += sums[w][lane];
+  }
   if (lane < LANES) {
     typedef T T4 __attribute__((ext_vector_type(4)));
     T4 v;
@@ -1010,22 +1046,30 @@ __device__ __forceinline__ void join_shares(const float* po, const float* pm, in
   }
 }
 
-template <typename T, int D>
+// A row of few shares takes a wave, one of many a workgroup (1024 rows of 128, 33 shares: 9.3 us by waves, 7.0 by workgroups; 4096
+// rows, 9 shares: 7.2 and 10.6).
+constexpr int kSharesOfAWave = 16;
+template <typename T, int D, int WAVES>
 __global__ __launch_bounds__(kThreads) void join_paged_kernel(PagedArgs a) {
-  const int64_t row = (int64_t)blockIdx.x * kWaves + (threadIdx.x >> 6);
+  const int64_t row = WAVES > 1 ? blockIdx.x : (int64_t)blockIdx.x * kWaves + (threadIdx.x >> 6);
   if (row >= (int64_t)a.batch * a.heads) return;
-  const int b = row / a.heads, np = group_of(a, b) >= 0 ? *a.np : 0;
-  join_shares<T, D>(a.po, a.pm, row, np, a.most_np, a.most_np + a.ns, a.lengths[b] <= 0, (T*)a.out);
+  const int b = row / a.heads, np = a.np[1 + b] ? a.np[0] : 0;
+  join_shares<T, D, WAVES>(a.po, a.pm, row, np, a.most_np, a.most_np + a.ns, a.lengths[b] <= 0, (T*)a.out);
 }
 
-template <typename T, int D>
+template <typename T, int D, int WAVES>
 __global__ __launch_bounds__(kThreads) void join_prompt_kernel(PromptArgs a) {
-  const int64_t row = (int64_t)blockIdx.x * kWaves + (threadIdx.x >> 6);
+  const int64_t row = WAVES > 1 ? blockIdx.x : (int64_t)blockIdx.x * kWaves + (threadIdx.x >> 6);
   if (row >= (int64_t)a.total_q * a.heads) return;
   const int token = row / a.heads;
   if (token < a.cu_q[0] || token >= a.cu_q[a.seqs]) return;
   const float2 first = reinterpret_cast<const float2*>(a.pm)[row * a.shares];
-  join_shares<T, D>(a.po, a.pm, row, 0, 0, a.shares, first.x == INFINITY && first.y == 0.f, (T*)a.out);
+  join_shares<T, D, WAVES>(a.po, a.pm, row, 0, 0, a.shares, first.x == INFINITY && first.y == 0.f, (T*)a.out);
+}
+template <typename A>
+int launch_join(void (*by_waves)(A), void (*by_workgroups)(A), int64_t rows, int64_t slots, hipStream_t stream, const A& a) {
+  if (slots <= kSharesOfAWave) return hq_launch_as_is(by_waves, dim3((unsigned)((rows + kWaves - 1) / kWaves)), dim3(kThreads), 0, stream, a);
+  return hq_launch_as_is(by_workgroups, dim3((unsigned)rows), dim3(kThreads), 0, stream, a);
 }
 
 // Scores are compared and masked by -infinity before they are scaled: a scale of zero (all keys alike) becomes one that no score notices.
@@ -1051,7 +1095,7 @@ int launch_prompt(PromptArgs a, int cus, hipStream_t stream) {
   }
   const int rc = hq_launch_as_is(prompt_kernel<T, D>, dim3((unsigned)(items * a.shares)), dim3(kThreads), Many<T, D>::LDS, stream, a);
   if (rc != HQ_OK || a.shares == 1) return rc;
-  return hq_launch_as_is(join_prompt_kernel<T, D>, dim3((unsigned)((rows + kWaves - 1) / kWaves)), dim3(kThreads), 0, stream, a);
+  return launch_join(join_prompt_kernel<T, D, 1>, join_prompt_kernel<T, D, kWaves>, rows, a.shares, stream, a);
 }
 
 // Half of the workgroups that the device holds at once for the common keys, and the requests' own keys divided until they fill the rest.
@@ -1073,7 +1117,7 @@ int launch_paged(PagedArgs a, int cus, hipStream_t stream) {
   a.prefix_items = (int)prefix;
   if (slots > 1) {
     HqWorkspace ws;
-    const int rc = hq_get_workspace(stream, (size_t)(rows * slots * (D + 2) + 1), 0, &ws);
+    const int rc = hq_get_workspace(stream, (size_t)(rows * slots * (D + 2) + 1 + a.batch), 0, &ws);
     if (rc != HQ_OK) return rc;
     a.po = ws.partial;
     a.pm = a.po + rows * slots * D;
@@ -1085,7 +1129,7 @@ int launch_paged(PagedArgs a, int cus, hipStream_t stream) {
   if (attr != hipSuccess) return (int)attr;
   const int rc = hq_launch_as_is(paged_kernel<T, D>, dim3((unsigned)grid), dim3(kThreads), lds, stream, a);
   if (rc != HQ_OK || slots == 1) return rc;
-  return hq_launch_as_is(join_paged_kernel<T, D>, dim3((unsigned)((rows + kWaves - 1) / kWaves)), dim3(kThreads), 0, stream, a);
+  return launch_join(join_paged_kernel<T, D, 1>, join_paged_kernel<T, D, kWaves>, rows, slots, stream, a);
 }
 
 // One of the four kernels by type and head size.
