@@ -89,10 +89,44 @@ __device__ __forceinline__ int block_scan(int v, int* parts, int* total) {
   return before + sum - v;
 }
 
+// Ranks among the marked ones of a stretch of 16 * 256 pages, page i * 256 + thread being marked[i] of its thread: a bit a page, whose
+// sums meet once, so that a stretch costs one trip to memory and two barriers (page by page in steps of 256 threads: 16 of each; 4096
+// pages' counts 16 us, and PLAN in stretches).
+constexpr int kEach = 16, kStretch = kEach * kThreads;
+struct Ranks {
+  unsigned long long bits[kEach];
+  int before[kEach], all;
+  __device__ __forceinline__ Ranks(const bool (&marked)[kEach], int* counts) {  // counts: kEach * 4 words of LDS
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      bits[i] = __ballot(marked[i]);
+      if (lane == 0) counts[i * (kThreads / 64) + wave] = __popcll(bits[i]);
+    }
+    __syncthreads();
+    static_assert(kEach * kThreads / 64 == 64, "a lane each");
+    const int mine = counts[lane];
+    int sum = mine;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int u = __shfl_up(sum, d);
+      if (lane >= d) sum += u;
+    }
+    all = __builtin_amdgcn_readlane(sum, 63);
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) before[i] = __shfl(sum - mine, i * (kThreads / 64) + wave);
+  }
+  __device__ __forceinline__ int of(int i) const {
+    return before[i] + __popcll(bits[i] & ((1ull << (threadIdx.x & 63)) - 1));
+  }
+};
+
+constexpr int kListLds = 4096;  // pages handed out that are listed in LDS; the others are in memory
 // One workgroup a row: what it inherits, and how the pages' counts change by it; the last one to arrive hands out pages.
 __global__ __launch_bounds__(kThreads) void step_kernel(StepArgs a) {
-  extern __shared__ int off[];
-  __shared__ int parts[kThreads / 64], flag;
+  extern __shared__ int lds[];
+  __shared__ int parts[kEach * kThreads / 64], flag;
   const int s = blockIdx.x, tid = threadIdx.x;
   const int cap = a.width * a.page;
   auto length_of = [&](int r) { return min(max(a.lengths[r], 0), cap); };
@@ -142,52 +176,71 @@ __global__ __launch_bounds__(kThreads) void step_kernel(StepArgs a) {
   if (!flag) return;
 
   // where each row's requests begin in the order of all
+  int* const off = lds;
+  int* const source = lds + a.rows;
+  int* const list = source + a.rows;
   int total = 0;
   for (int r0 = 0; r0 < a.rows; r0 += kThreads) {
     const int r = r0 + tid;
+    const int n = r < a.rows ? get(a.need + r) : 0, from = r < a.rows ? get(a.source + r) : 0;
     int all;
-    const int before = block_scan(r < a.rows ? get(a.need + r) : 0, parts, &all);
-    if (r < a.rows) off[r] = total + before;
+    const int before = block_scan(n, parts, &all);
+    if (r < a.rows) {
+      off[r] = total + before;
+      source[r] = from;
+    }
     total += all;
   }
   // free pages, lowest first, to the requests in their order
   int nfree = 0;
-  for (int i0 = 0; i0 < a.pages; i0 += kThreads) {
-    const int i = i0 + tid;
-    int count = 1;
-    if (i < a.pages) {
-      const int d = get(a.change + i);
-      count = a.refs[i] + d;
-      if (d) put(a.change + i, 0);
+  for (int i0 = 0; i0 < a.pages; i0 += kStretch) {
+    int count[kEach], change[kEach];
+    bool free[kEach];
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const int p = min(i0 + i * kThreads + tid, a.pages - 1);
+      count[i] = a.refs[p];
+      change[i] = get(a.change + p);
     }
-    const bool free = count <= 0;
-    int all;
-    const int rank = nfree + block_scan(free, parts, &all);
-    if (i < a.pages) {
-      const bool taken = free && rank < total;
-      a.refs_out[i] = taken ? 1 : count;
-      if (taken) put(a.list + rank, i);
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      count[i] += change[i];
+      free[i] = i0 + i * kThreads + tid < a.pages && count[i] <= 0;
     }
-    nfree += all;
+    const Ranks ranks(free, parts);
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const int p = i0 + i * kThreads + tid, rank = nfree + ranks.of(i);
+      if (p >= a.pages) continue;
+      if (change[i]) put(a.change + p, 0);
+      const bool taken = free[i] && rank < total;
+      a.refs_out[p] = taken ? 1 : count[i];
+      if (taken) {
+        if (rank < kListLds) list[rank] = p;
+        else put(a.list + rank, p);
+      }
+    }
+    nfree += ranks.all;
   }
   if (tid == 0) {
     *a.missing = max(total - nfree, 0);
     put((int*)a.arrived, 0);
     flag = 0;
   }
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  if (total > kListLds) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
+  auto page_of = [&](int rank) { return rank >= nfree ? -1 : rank < kListLds ? list[rank] : get(a.list + rank); };
   for (int r = tid; r < a.rows; r += kThreads) {
-    const int start = start_of(r), source = get(a.source + r), n = get(a.need + r);
-    const int from = source >= 0 ? start / a.page : (start + a.page - 1) / a.page;
+    const int start = start_of(r), first = off[r], n = (r + 1 < a.rows ? off[r + 1] : total) - first;
+    const int from = source[r] >= 0 ? start / a.page : (start + a.page - 1) / a.page;
     int end = end_of(r, start);
-    if (off[r] + n > nfree) end = min(end, (from + max(nfree - off[r], 0)) * a.page);
+    if (first + n > nfree) end = min(end, (from + max(nfree - first, 0)) * a.page);
     a.lengths_out[r] = end;
     a.starts_out[r] = min(start, end);
-    if (source >= 0 && off[r] < nfree) {
+    if (source[r] >= 0 && first < nfree) {
       const int at = atomicAdd(&flag, 1);
-      a.copies[2 * at] = source;
-      a.copies[2 * at + 1] = get(a.list + off[r]);
+      a.copies[2 * at] = source[r];
+      a.copies[2 * at + 1] = page_of(first);
     }
   }
   for (int x = tid; x < total; x += kThreads) {
@@ -197,21 +250,28 @@ __global__ __launch_bounds__(kThreads) void step_kernel(StepArgs a) {
       if (off[mid] <= x) lo = mid;
       else hi = mid - 1;
     }
-    const int start = start_of(lo), from = get(a.source + lo) >= 0 ? start / a.page : (start + a.page - 1) / a.page;
-    a.table_out[(int64_t)lo * a.width + from + x - off[lo]] = x < nfree ? get(a.list + x) : -1;
+    const int start = start_of(lo), from = source[lo] >= 0 ? start / a.page : (start + a.page - 1) / a.page;
+    a.table_out[(int64_t)lo * a.width + from + x - off[lo]] = page_of(x);
   }
   __syncthreads();
   if (tid == 0) *a.ncopies = flag;
 }
 
-// Pages {source, target} of every plane.
+// Pages {source, target} of every plane, eight 16-byte pieces of a thread on their way at a time, stored past the L2.
 __device__ __forceinline__ void copy_pages(hq_u4v* pool, const int* pairs, int n, int planes, int pages, int64_t pieces) {
   for (int64_t x = blockIdx.x; x < (int64_t)n * planes; x += gridDim.x) {
     const int c = x % n;
     const int64_t plane = x / n;
     const hq_u4v* from = pool + (plane * pages + pairs[2 * c]) * pieces;
     hq_u4v* to = pool + (plane * pages + pairs[2 * c + 1]) * pieces;
-    for (int64_t i = threadIdx.x; i < pieces; i += kThreads) to[i] = from[i];
+    for (int64_t i0 = threadIdx.x; i0 < pieces; i0 += 8 * kThreads) {
+      hq_u4v v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = from[min(i0 + i * kThreads, pieces - 1)];
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (i0 + i * kThreads < pieces) hq_store_stream(to + i0 + i * kThreads, v[i]);
+    }
   }
 }
 __global__ __launch_bounds__(kThreads) void step_copy_kernel(StepArgs a) {
@@ -232,26 +292,41 @@ struct CompactArgs {
 
 // The i-th page in use behind the first `live` goes to the i-th hole among them.
 __global__ __launch_bounds__(kThreads) void compact_plan_kernel(CompactArgs a) {
-  __shared__ int parts[kThreads / 64];
+  __shared__ int parts[kEach * kThreads / 64];
+  int n[kEach];
+  auto load = [&](int i0) {
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) n[i] = a.refs[min(i0 + i * kThreads + (int)threadIdx.x, a.pages - 1)];
+  };
   int live = 0;
-  for (int i0 = 0; i0 < a.pages; i0 += kThreads) {
-    int all;
-    block_scan(i0 + (int)threadIdx.x < a.pages && a.refs[i0 + threadIdx.x] > 0, parts, &all);
+  for (int i0 = 0; i0 < a.pages; i0 += kStretch) {
+    load(i0);
+    int mine = 0, all;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) mine += i0 + i * kThreads + (int)threadIdx.x < a.pages && n[i] > 0;
+    block_scan(mine, parts, &all);
     live += all;
   }
   int holes = 0, movers = 0;
-  for (int i0 = 0; i0 < a.pages; i0 += kThreads) {
-    const int i = i0 + threadIdx.x;
-    const int n = i < a.pages ? a.refs[i] : 0;
-    const bool hole = i < live && n <= 0, mover = i >= live && n > 0;
-    int all;
-    int rank = holes + block_scan(hole, parts, &all);
-    if (hole) put(a.pairs + 2 * rank + 1, i);
-    holes += all;
-    rank = movers + block_scan(mover, parts, &all);
-    if (mover) put(a.pairs + 2 * rank, i);
-    movers += all;
-    if (i < a.pages && !hole) a.refs_out[i] = mover ? 0 : n;
+  for (int i0 = 0; i0 < a.pages; i0 += kStretch) {
+    if (a.pages > kStretch) load(i0);  // else they are still there
+    bool hole[kEach], mover[kEach];
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const int p = i0 + i * kThreads + threadIdx.x;
+      hole[i] = p < live && n[i] <= 0;
+      mover[i] = p < a.pages && p >= live && n[i] > 0;
+    }
+    const Ranks to(hole, parts), from(mover, parts);
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const int p = i0 + i * kThreads + threadIdx.x;
+      if (hole[i]) put(a.pairs + 2 * (holes + to.of(i)) + 1, p);
+      if (mover[i]) put(a.pairs + 2 * (movers + from.of(i)), p);
+      if (p < a.pages && !hole[i]) a.refs_out[p] = mover[i] ? 0 : n[i];
+    }
+    holes += to.all;
+    movers += from.all;
   }
   if (threadIdx.x == 0) {
     *a.live = live;
@@ -354,7 +429,10 @@ extern "C" int hq_cache_step(void* pool, int planes, int64_t page_bytes, const i
   a.width = table_width;
   a.pages = num_pages;
   a.page = page_size;
-  rc = hq_launch_as_is(step_kernel, dim3(rows > 1 ? rows : 1), dim3(kThreads), 4 * (size_t)rows, (hipStream_t)stream, a);
+  const size_t lds = 8 * (size_t)rows + 4 * kListLds;
+  static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&step_kernel), hipFuncAttributeMaxDynamicSharedMemorySize, 8 * 16384 + 4 * kListLds);
+  if (attr != hipSuccess) return (int)attr;
+  rc = hq_launch_as_is(step_kernel, dim3(rows > 1 ? rows : 1), dim3(kThreads), lds, (hipStream_t)stream, a);
   if (rc != HQ_OK || rows == 0 || planes == 0 || page_bytes == 0 || num_pages == 0) return rc;
   const int64_t items = (int64_t)rows * planes, grid = 16 * (int64_t)dev->cus;
   return hq_launch_as_is(step_copy_kernel, dim3((unsigned)(items < grid ? items : grid)), dim3(kThreads), 0, (hipStream_t)stream, a);
