@@ -1,4 +1,5 @@
 // The paged key / value cache: tokens into pages, the page tables from one token to the next, live pages to the front.
+#include <algorithm>
 #include <climits>
 
 #include "hq_internal.h"
@@ -96,13 +97,19 @@ constexpr int kEach = 16, kStretch = kEach * kThreads;
 struct Ranks {
   unsigned long long bits[kEach];
   int before[kEach], all;
-  __device__ __forceinline__ Ranks(const bool (&marked)[kEach], int* counts) {  // counts: kEach * 4 words of LDS
+  // counts: kEach * 4 words of LDS; n: pages of the stretch, which ends there
+  __device__ __forceinline__ Ranks(const bool (&marked)[kEach], int n, int* counts) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    __syncthreads();
+    if (wave == 0) counts[lane] = 0;
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
-      bits[i] = __ballot(marked[i]);
-      if (lane == 0) counts[i * (kThreads / 64) + wave] = __popcll(bits[i]);
+      bits[i] = 0;
+      if (i * kThreads < n) {
+        bits[i] = __ballot(marked[i]);
+        if (lane == 0) counts[i * (kThreads / 64) + wave] = __popcll(bits[i]);
+      }
     }
     __syncthreads();
     static_assert(kEach * kThreads / 64 == 64, "a lane each");
@@ -115,7 +122,8 @@ struct Ranks {
     }
     all = __builtin_amdgcn_readlane(sum, 63);
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) before[i] = __shfl(sum - mine, i * (kThreads / 64) + wave);
+    for (int i = 0; i < kEach; ++i)
+      if (i * kThreads < n) before[i] = __shfl(sum - mine, i * (kThreads / 64) + wave);
   }
   __device__ __forceinline__ int of(int i) const {
     return before[i] + __popcll(bits[i] & ((1ull << (threadIdx.x & 63)) - 1));
@@ -199,15 +207,19 @@ __global__ __launch_bounds__(kThreads) void step_kernel(StepArgs a) {
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
       const int p = min(i0 + i * kThreads + tid, a.pages - 1);
-      count[i] = a.refs[p];
-      change[i] = get(a.change + p);
+      count[i] = 0;
+      change[i] = 1;
+      if (i0 + i * kThreads < a.pages) {
+        count[i] = a.refs[p];
+        change[i] = get(a.change + p);
+      }
     }
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
       count[i] += change[i];
       free[i] = i0 + i * kThreads + tid < a.pages && count[i] <= 0;
     }
-    const Ranks ranks(free, parts);
+    const Ranks ranks(free, a.pages - i0, parts);
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
       const int p = i0 + i * kThreads + tid, rank = nfree + ranks.of(i);
@@ -317,7 +329,7 @@ __global__ __launch_bounds__(kThreads) void compact_plan_kernel(CompactArgs a) {
       hole[i] = p < live && n[i] <= 0;
       mover[i] = p < a.pages && p >= live && n[i] > 0;
     }
-    const Ranks to(hole, parts), from(mover, parts);
+    const Ranks to(hole, a.pages - i0, parts), from(mover, a.pages - i0, parts);
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
       const int p = i0 + i * kThreads + threadIdx.x;
@@ -348,6 +360,62 @@ __global__ __launch_bounds__(kThreads) void compact_move_kernel(CompactArgs a) {
     a.table_out[i] = e >= live && e < a.pages && a.refs[e] > 0 ? a.to[e] : e;
   }
   copy_pages(a.pool, a.pairs, *a.nmoves, a.planes, a.pages, a.page_pieces);
+}
+
+// The same in one launch where the counts are one stretch: every workgroup makes the plan for itself, in LDS (300 of 512 pages: 9.6 us in
+// two launches, ONE_C in one).
+__global__ __launch_bounds__(kThreads) void compact_small_kernel(CompactArgs a) {
+  __shared__ int parts[kEach * kThreads / 64];
+  __shared__ int pairs[kStretch];       // half of the pages at most move
+  __shared__ unsigned short to[kStretch];
+  int n[kEach], mine = 0, live;
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) if (i * kThreads < a.pages) n[i] = a.refs[min(i * kThreads + (int)threadIdx.x, a.pages - 1)];
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) if (i * kThreads < a.pages) mine += i * kThreads + (int)threadIdx.x < a.pages && n[i] > 0;
+  block_scan(mine, parts, &live);
+  bool hole[kEach], mover[kEach];
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    const int p = i * kThreads + threadIdx.x;
+    hole[i] = mover[i] = false;
+    if (i * kThreads < a.pages) {
+      hole[i] = p < live && n[i] <= 0;
+      mover[i] = p < a.pages && p >= live && n[i] > 0;
+    }
+  }
+  const Ranks holes(hole, a.pages, parts), movers(mover, a.pages, parts);
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    const int p = i * kThreads + threadIdx.x;
+    if (i * kThreads < a.pages) {
+      if (hole[i]) pairs[2 * holes.of(i) + 1] = p;
+      if (mover[i]) pairs[2 * movers.of(i)] = p;
+    }
+  }
+  __syncthreads();
+  if (blockIdx.x == 0) {
+    if (threadIdx.x == 0) *a.live = live;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+    const int p = i * kThreads + threadIdx.x;
+      if (i * kThreads < a.pages && p < a.pages) a.refs_out[p] = hole[i] ? a.refs[pairs[2 * holes.of(i)]] : mover[i] ? 0 : n[i];
+    }
+  }
+  const int64_t entries = (int64_t)a.rows * a.width;
+  if ((int64_t)blockIdx.x * kThreads < entries) {
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+    const int p = i * kThreads + threadIdx.x;
+      if (i * kThreads < a.pages) to[p] = mover[i] ? pairs[2 * movers.of(i) + 1] : p;
+    }
+    __syncthreads();
+    for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < entries; i += (int64_t)gridDim.x * kThreads) {
+      const int e = a.table[i];
+      a.table_out[i] = (unsigned)e < (unsigned)a.pages ? to[e] : e;
+    }
+  }
+  copy_pages(a.pool, pairs, movers.all, a.planes, a.pages, a.page_pieces);
 }
 
 bool meet(const void* a, int64_t na, const void* b, int64_t nb) {
@@ -457,9 +525,6 @@ extern "C" int hq_cache_compact(void* pool, int planes, int64_t page_bytes, cons
   const HqDevice* dev = nullptr;
   int rc = hq_current_device(&dev);
   if (rc != HQ_OK) return rc;
-  HqWorkspace ws;
-  rc = hq_get_workspace((hipStream_t)stream, (size_t)(2 * (int64_t)num_pages + 1), 0, &ws);
-  if (rc != HQ_OK) return rc;
   CompactArgs a{};
   a.pool = (hq_u4v*)pool;
   a.table = table;
@@ -467,15 +532,24 @@ extern "C" int hq_cache_compact(void* pool, int planes, int64_t page_bytes, cons
   a.table_out = table_out;
   a.refs_out = refs_out;
   a.live = live;
-  a.nmoves = (int*)ws.partial;
-  a.to = a.nmoves + 1;
-  a.pairs = a.to + num_pages;  // half of the pages at most move
   a.page_pieces = page_bytes / 16;
   a.planes = planes;
   a.rows = rows;
   a.width = table_width;
   a.pages = num_pages;
+  // workgroups that can have something to do
+  const int64_t most = std::max({(int64_t)1, (entries + kThreads - 1) / kThreads, page_bytes ? (int64_t)(num_pages / 2) * planes : 0});
+  // (every workgroup makes the plan, so there are no more of them than the pages' bytes are worth)
+  const int64_t each = num_pages * page_bytes * planes > (int64_t)1 << 28 ? 6 : 1;
+  if (num_pages <= kStretch && num_pages > 0)
+    return hq_launch_as_is(compact_small_kernel, dim3((unsigned)std::min<int64_t>(most, each * dev->cus)), dim3(kThreads), 0, (hipStream_t)stream, a);
+  HqWorkspace ws;
+  rc = hq_get_workspace((hipStream_t)stream, (size_t)(2 * (int64_t)num_pages + 1), 0, &ws);
+  if (rc != HQ_OK) return rc;
+  a.nmoves = (int*)ws.partial;
+  a.to = a.nmoves + 1;
+  a.pairs = a.to + num_pages;  // half of the pages at most move
   rc = hq_launch_as_is(compact_plan_kernel, dim3(1), dim3(kThreads), 0, (hipStream_t)stream, a);
   if (rc != HQ_OK || (entries == 0 && (planes == 0 || page_bytes == 0))) return rc;
-  return hq_launch_as_is(compact_move_kernel, dim3(16 * (unsigned)dev->cus), dim3(kThreads), 0, (hipStream_t)stream, a);
+  return hq_launch_as_is(compact_move_kernel, dim3((unsigned)std::min<int64_t>(most, 16 * dev->cus)), dim3(kThreads), 0, (hipStream_t)stream, a);
 }
