@@ -94,25 +94,26 @@ __device__ __forceinline__ int block_scan(int v, int* parts, int* total) {
 // sums meet once, so that a stretch costs one trip to memory and two barriers (page by page in steps of 256 threads: 16 of each; 4096
 // pages' counts 16 us, and PLAN in stretches).
 constexpr int kEach = 16, kStretch = kEach * kThreads;
+template <int THREADS = kThreads, int EACH = kStretch / THREADS>
 struct Ranks {
-  unsigned long long bits[kEach];
-  int before[kEach], all;
-  // counts: kEach * 4 words of LDS; n: pages of the stretch, which ends there
-  __device__ __forceinline__ Ranks(const bool (&marked)[kEach], int n, int* counts) {
+  unsigned long long bits[EACH];
+  int before[EACH], all;
+  // counts: 64 words of LDS; n: pages of the stretch, which ends there
+  __device__ __forceinline__ Ranks(const bool (&marked)[EACH], int n, int* counts) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     __syncthreads();
     if (wave == 0) counts[lane] = 0;
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) {
+    for (int i = 0; i < EACH; ++i) {
       bits[i] = 0;
-      if (i * kThreads < n) {
+      if (i * THREADS < n) {
         bits[i] = __ballot(marked[i]);
-        if (lane == 0) counts[i * (kThreads / 64) + wave] = __popcll(bits[i]);
+        if (lane == 0) counts[i * (THREADS / 64) + wave] = __popcll(bits[i]);
       }
     }
     __syncthreads();
-    static_assert(kEach * kThreads / 64 == 64, "a lane each");
+    static_assert(EACH * THREADS / 64 == 64, "a lane each");
     const int mine = counts[lane];
     int sum = mine;
 #pragma unroll
@@ -122,8 +123,8 @@ struct Ranks {
     }
     all = __builtin_amdgcn_readlane(sum, 63);
 #pragma unroll
-    for (int i = 0; i < kEach; ++i)
-      if (i * kThreads < n) before[i] = __shfl(sum - mine, i * (kThreads / 64) + wave);
+    for (int i = 0; i < EACH; ++i)
+      if (i * THREADS < n) before[i] = __shfl(sum - mine, i * (THREADS / 64) + wave);
   }
   __device__ __forceinline__ int of(int i) const {
     return before[i] + __popcll(bits[i] & ((1ull << (threadIdx.x & 63)) - 1));
@@ -219,7 +220,7 @@ __global__ __launch_bounds__(kThreads) void step_kernel(StepArgs a) {
       count[i] += change[i];
       free[i] = i0 + i * kThreads + tid < a.pages && count[i] <= 0;
     }
-    const Ranks ranks(free, a.pages - i0, parts);
+    const Ranks<> ranks(free, a.pages - i0, parts);
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
       const int p = i0 + i * kThreads + tid, rank = nfree + ranks.of(i);
@@ -270,13 +271,17 @@ __global__ __launch_bounds__(kThreads) void step_kernel(StepArgs a) {
 }
 
 // Pages {source, target} of every plane, eight 16-byte pieces of a thread on their way at a time, stored past the L2.
+// Every 256 threads of a workgroup take a page of their own.
+template <int THREADS = kThreads>
 __device__ __forceinline__ void copy_pages(hq_u4v* pool, const int* pairs, int n, int planes, int pages, int64_t pieces) {
-  for (int64_t x = blockIdx.x; x < (int64_t)n * planes; x += gridDim.x) {
+  constexpr int GROUPS = THREADS / kThreads;
+  const int group = threadIdx.x / kThreads, tid = threadIdx.x % kThreads;
+  for (int64_t x = blockIdx.x * GROUPS + group; x < (int64_t)n * planes; x += gridDim.x * GROUPS) {
     const int c = x % n;
     const int64_t plane = x / n;
     const hq_u4v* from = pool + (plane * pages + pairs[2 * c]) * pieces;
     hq_u4v* to = pool + (plane * pages + pairs[2 * c + 1]) * pieces;
-    for (int64_t i0 = threadIdx.x; i0 < pieces; i0 += 8 * kThreads) {
+    for (int64_t i0 = tid; i0 < pieces; i0 += 8 * kThreads) {
       hq_u4v v[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] = from[min(i0 + i * kThreads, pieces - 1)];
@@ -288,6 +293,123 @@ __device__ __forceinline__ void copy_pages(hq_u4v* pool, const int* pairs, int n
 }
 __global__ __launch_bounds__(kThreads) void step_copy_kernel(StepArgs a) {
   copy_pages(a.pool, a.copies, *a.ncopies, a.planes, a.pages, a.page_pieces);
+}
+
+// Small tables in one launch: every workgroup works out the whole step in LDS, from the tables alone, then writes its part of the rows and
+// of the copies; nobody waits for anybody.  A thread has a row, and up to 16 entries of the table, whose loads are under way together
+// (48 rows of 128 pages: 10.6 us in two launches, ONE_S in one).
+constexpr int kSmallRows = 1024, kSmallEntries = 16 * kSmallRows;
+__global__ __launch_bounds__(kSmallRows) void step_small_kernel(StepArgs a) {
+  constexpr int THREADS = kSmallRows, EACH = kStretch / THREADS, BATCH = 8;
+  __shared__ int parts[64];
+  __shared__ int change[kStretch], length[kSmallRows], first[kSmallRows], off[kSmallRows + 1], pairs[2 * kSmallRows];
+  __shared__ unsigned short list[kStretch];
+  __shared__ unsigned short from[kSmallRows];
+  __shared__ short parent[kSmallRows];
+  const int tid = threadIdx.x, cap = a.width * a.page, r = tid;
+  const bool row = r < a.rows;
+  int p = -1, add = 0, count[EACH];
+  if (row) {
+    p = a.parent[r];
+    add = max(a.add[r], 0);
+    length[r] = min(max(a.lengths[r], 0), cap);
+    if (p < 0 || p >= a.rows) p = -1;
+    parent[r] = (short)p;
+    first[r] = INT_MAX;
+  }
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) {
+    count[i] = i * THREADS + tid < a.pages ? a.refs[i * THREADS + tid] : 1;
+    change[i * THREADS + tid] = 0;
+  }
+  __syncthreads();
+  if (p >= 0) atomicMin(first + p, r);
+  __syncthreads();
+  // what the row inherits, from which entry on it asks for pages, and where its requests begin in the order of all
+  int start = 0, end = 0, source = -1, need = 0, total;
+  if (row) {
+    start = p < 0 ? 0 : length[p];
+    end = (int)min((int64_t)start + add, (int64_t)cap);
+    const int full = start / a.page, used = (start + a.page - 1) / a.page, last = (end + a.page - 1) / a.page;
+    if (used > full && first[p] != r) {
+      const int tail = a.table[(int64_t)p * a.width + full];
+      if ((unsigned)tail < (unsigned)a.pages) source = tail;
+    }
+    from[r] = (unsigned short)(source >= 0 ? full : used);
+    need = max(last, used) - from[r];
+  }
+  const int before = block_scan(need, parts, &total);
+  if (row) off[r] = before;
+  if (tid == 0) off[a.rows] = total;
+  __syncthreads();
+  const int entries = a.rows * a.width;
+  const float by_width = 1.f / a.width;
+  auto row_of = [=](int x) { return (int)((x + 0.5f) * by_width); };  // exact: entries * 2^-22 is far below a half
+  for (int x0 = tid; x0 < entries; x0 += BATCH * THREADS) {
+    int old[BATCH], now[BATCH];
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i) {
+      const int x = x0 + i * THREADS;
+      old[i] = now[i] = -1;
+      if (x0 - tid + i * THREADS >= entries || x >= entries) continue;
+      const int s = row_of(x), j = x - s * a.width;
+      if (parent[s] == s && first[s] == s) continue;  // it goes on as it is
+      if (j < (length[s] + a.page - 1) / a.page) old[i] = a.table[x];
+      if (j < from[s]) now[i] = a.table[(int64_t)parent[s] * a.width + j];
+    }
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i) {
+      if ((unsigned)old[i] < (unsigned)a.pages) atomicSub(change + old[i], 1);
+      if ((unsigned)now[i] < (unsigned)a.pages) atomicAdd(change + now[i], 1);
+    }
+  }
+  __syncthreads();
+  bool free[EACH];
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) {
+    count[i] += change[i * THREADS + tid];
+    free[i] = i * THREADS + tid < a.pages && count[i] <= 0;
+  }
+  const Ranks<THREADS> ranks(free, a.pages, parts);
+  const int nfree = ranks.all;
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) {
+    const int page = i * THREADS + tid;
+    if (page >= a.pages) continue;
+    const bool taken = free[i] && ranks.of(i) < total;
+    if (taken) list[ranks.of(i)] = (unsigned short)page;
+    if (blockIdx.x == 0) a.refs_out[page] = taken ? 1 : count[i];
+  }
+  __syncthreads();
+  // the copies, and the rows' lengths
+  const bool copy = source >= 0 && before < nfree;
+  int copies;
+  const int at = block_scan(copy, parts, &copies);
+  if (copy) {
+    pairs[2 * at] = source;
+    pairs[2 * at + 1] = list[before];
+  }
+  if (blockIdx.x == 0) {
+    if (tid == 0) *a.missing = max(total - nfree, 0);
+    if (row) {
+      if (before + need > nfree) end = min(end, (from[r] + max(nfree - before, 0)) * a.page);
+      a.lengths_out[r] = end;
+      a.starts_out[r] = min(start, end);
+    }
+  }
+  for (int x = blockIdx.x * THREADS + tid; x < entries; x += gridDim.x * THREADS) {
+    const int s = row_of(x), j = x - s * a.width, asked = j - from[s];
+    int e = -1;
+    if (asked < 0) {
+      e = a.table[(int64_t)parent[s] * a.width + j];
+      if ((unsigned)e >= (unsigned)a.pages) e = -1;
+    } else if (off[s] + asked < min(off[s + 1], nfree)) {
+      e = list[off[s] + asked];
+    }
+    a.table_out[x] = e;
+  }
+  __syncthreads();
+  copy_pages<THREADS>(a.pool, pairs, copies, a.planes, a.pages, a.page_pieces);
 }
 
 // ---- live pages to the front ----------------------------------------------------------------------------------------------
@@ -329,7 +451,7 @@ __global__ __launch_bounds__(kThreads) void compact_plan_kernel(CompactArgs a) {
       hole[i] = p < live && n[i] <= 0;
       mover[i] = p < a.pages && p >= live && n[i] > 0;
     }
-    const Ranks to(hole, a.pages - i0, parts), from(mover, a.pages - i0, parts);
+    const Ranks<> to(hole, a.pages - i0, parts), from(mover, a.pages - i0, parts);
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
       const int p = i0 + i * kThreads + threadIdx.x;
@@ -384,7 +506,7 @@ __global__ __launch_bounds__(kThreads) void compact_small_kernel(CompactArgs a) 
       mover[i] = p < a.pages && p >= live && n[i] > 0;
     }
   }
-  const Ranks holes(hole, a.pages, parts), movers(mover, a.pages, parts);
+  const Ranks<> holes(hole, a.pages, parts), movers(mover, a.pages, parts);
 #pragma unroll
   for (int i = 0; i < kEach; ++i) {
     const int p = i * kThreads + threadIdx.x;
@@ -468,10 +590,6 @@ extern "C" int hq_cache_step(void* pool, int planes, int64_t page_bytes, const i
   const HqDevice* dev = nullptr;
   int rc = hq_current_device(&dev);
   if (rc != HQ_OK) return rc;
-  HqWorkspace ws;
-  const int64_t most = entries < num_pages ? entries : num_pages;
-  rc = hq_get_workspace((hipStream_t)stream, (size_t)(4 * (int64_t)rows + 1 + most), (size_t)num_pages + 1, &ws);
-  if (rc != HQ_OK) return rc;
   StepArgs a{};
   a.pool = (hq_u4v*)pool;
   a.table = table;
@@ -484,6 +602,23 @@ extern "C" int hq_cache_step(void* pool, int planes, int64_t page_bytes, const i
   a.refs_out = refs_out;
   a.starts_out = starts_out;
   a.missing = missing;
+  a.page_pieces = page_bytes / 16;
+  a.planes = planes;
+  a.rows = rows;
+  a.width = table_width;
+  a.pages = num_pages;
+  a.page = page_size;
+  if (rows <= kSmallRows && entries <= kSmallEntries && num_pages <= kStretch) {
+    // one workgroup a compute unit, two where there may be a lot to copy
+    const int64_t bytes = (int64_t)rows * planes * page_bytes, each = bytes > (int64_t)1 << 26 ? 2 : 1;
+    const int64_t most = std::max((entries + kSmallRows - 1) / kSmallRows, page_bytes ? ((int64_t)rows * planes + 3) / 4 : 0);
+    return hq_launch_as_is(step_small_kernel, dim3((unsigned)std::max<int64_t>(1, std::min(most, each * dev->cus))), dim3(kSmallRows), 0,
+                           (hipStream_t)stream, a);
+  }
+  HqWorkspace ws;
+  const int64_t most = entries < num_pages ? entries : num_pages;
+  rc = hq_get_workspace((hipStream_t)stream, (size_t)(4 * (int64_t)rows + 1 + most), (size_t)num_pages + 1, &ws);
+  if (rc != HQ_OK) return rc;
   a.need = (int*)ws.partial;
   a.source = a.need + rows;
   a.copies = a.source + rows;
@@ -491,12 +626,6 @@ extern "C" int hq_cache_step(void* pool, int planes, int64_t page_bytes, const i
   a.list = a.ncopies + 1;
   a.arrived = ws.counters;
   a.change = (int*)ws.counters + 1;
-  a.page_pieces = page_bytes / 16;
-  a.planes = planes;
-  a.rows = rows;
-  a.width = table_width;
-  a.pages = num_pages;
-  a.page = page_size;
   const size_t lds = 8 * (size_t)rows + 4 * kListLds;
   static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&step_kernel), hipFuncAttributeMaxDynamicSharedMemorySize, 8 * 16384 + 4 * kListLds);
   if (attr != hipSuccess) return (int)attr;
