@@ -149,15 +149,19 @@ struct PackedTiles {
 // The pages of one request, one head.  Eight tokens from a multiple of eight on are in one page.
 template <typename T, int D>
 struct Pages {
-  const T *k, *v;
-  const int* table;  // the request's row
-  int head, kv_heads, page_log, pages;
+  const char *k, *v;    // this head's rows in page 0
+  const int* table;     // the request's row
+  uint32_t page_bytes;  // of all heads
+  int page_log, pages;
+  __device__ __forceinline__ Pages(const T* k0, const T* v0, const int* row, int head, int kv_heads, int log, int n)
+      : k((const char*)(k0 + ((int64_t)head << log) * D)), v((const char*)(v0 + ((int64_t)head << log) * D)), table(row),
+        page_bytes((uint32_t)kv_heads * (D * 2) << log), page_log(log), pages(n) {}
   __device__ __forceinline__ int id(int key) const {  // -1: no page, to be read as zeros
     const int p = table[key >> page_log];
     return (unsigned)p < (unsigned)pages ? p : -1;
   }
-  __device__ __forceinline__ int64_t at(int page, int key) const {
-    return ((((int64_t)page * kv_heads + head) << page_log) + (key & ((1 << page_log) - 1))) * D;
+  __device__ __forceinline__ uint64_t at(int page, int key) const {
+    return (uint64_t)(uint32_t)page * page_bytes + (uint32_t)(key & ((1 << page_log) - 1)) * (D * 2);
   }
 };
 __device__ __forceinline__ void zero_lds(char* to) {  // what one to_lds() would write
@@ -172,14 +176,16 @@ struct PagedTiles {
   int n, first;
   int ids_next, ids_k, ids_v;  // pages of the instructions' rows, one a lane: of the tile to come, of the keys' and of the values' next
   uint32_t koff[NL], voff[NL];
+  __device__ PagedTiles(const Pages<T, D>& pages, int end) : p(pages), n(end) {}
   __device__ __forceinline__ int ids(int t) const { return p.id(min(first + t * 64 + (int)(threadIdx.x & (64 / RG - 1)) * RG, n - 1)); }
-  __device__ __forceinline__ void load(const T* pool, int id, int t, const uint32_t (&off)[NL], char* to) {
-    const int wave = uniform((int)(threadIdx.x >> 6));
+  __device__ __forceinline__ void load(const char* pool, int id, int t, const uint32_t (&off)[NL], char* to) {
+    const int wave = uniform((int)(threadIdx.x >> 6)), lds = uniform((int)lds_address(to));
+    const unsigned long long none = __ballot(id < 0);
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
       const int j = wave * NL + i, page = __builtin_amdgcn_readlane(id, j);
-      if (page >= 0) to_lds(uniform((int)lds_address(to) + j * 1024), uniform(pool + p.at(page, first + t * 64 + j * RG)), off[i]);
-      else zero_lds(to + j * 1024);
+      if (none && page < 0) zero_lds(to + j * 1024);
+      else to_lds(lds + j * 1024, pool + p.at(page, first + t * 64 + j * RG), off[i]);
     }
   }
   __device__ __forceinline__ void start(int f) {
@@ -585,24 +591,24 @@ struct Few {
     auto ids_of = [&](int set) { return p.id(min(first + (wave + kWaves * (set * SET + lane / G)) * 32 + lane % G * RG, end - 1)); };
     int ids = ids_of(0), ids_next = 0;
     // Whether all G instructions were needed: what the waits count.
-    auto load = [&](const T* pool, int block, int set_ids, const uint32_t (&off)[G], char* to, bool values) {
+    auto load = [&](const char* pool, int block, int set_ids, const uint32_t (&off)[G], char* to, bool values) {
       const int base = first + block * 32, at = block / kWaves % SET * G;
       const uint32_t lds = uniform((int)lds_address(to));
       bool whole = true;
       if (base + 32 <= end) {
+        whole = !(__ballot(set_ids < 0) >> at & ((1ull << G) - 1));
 #pragma unroll
         for (int i = 0; i < G; ++i) {
           const int page = __builtin_amdgcn_readlane(set_ids, at + i);
-          if (page >= 0) to_lds(lds + i * 1024, uniform(pool + p.at(page, base + i * RG)), off[i]);
-          else zero_lds(to + i * 1024);
-          whole &= page >= 0;
+          if (!whole && page < 0) zero_lds(to + i * 1024);
+          else to_lds(lds + i * 1024, pool + p.at(page, base + i * RG), off[i]);
         }
       } else {  // the last block: rows behind the last key repeat it, every lane by an address of its own
 #pragma unroll
         for (int i = 0; i < G; ++i) {
           const int row = i * RG + lane / CH, key = min(base + row, end - 1), page = __shfl(set_ids, at + (key - base) / RG);
           const int ch = values ? v_piece<D>(row, lane % CH) : k_piece<D>(row, lane % CH);
-          if (page >= 0) to_lds(lds + i * 1024, pool + p.at(page, key) + ch * 8);
+          if (page >= 0) to_lds(lds + i * 1024, pool + p.at(page, key) + ch * 16);
           else zero_lds(to + i * 1024);
           whole &= __ballot(page < 0) == 0;
         }
@@ -859,7 +865,7 @@ __device__ __forceinline__ void share_of(int n, int shares, int least, int s, in
 
 template <typename T, int D>
 __device__ __forceinline__ Pages<T, D> pages_of(const PagedArgs& a, int request, int head) {
-  return Pages<T, D>{(const T*)a.k, (const T*)a.v, a.table + (int64_t)request * a.width, head, a.kv_heads, a.page_log, a.pages};
+  return Pages<T, D>((const T*)a.k, (const T*)a.v, a.table + (int64_t)request * a.width, head, a.kv_heads, a.page_log, a.pages);
 }
 
 // Up to 16 of the rows (request, head of the group) of requests b0 ..., from first_row on, all of which see the keys.
@@ -917,9 +923,7 @@ __device__ __forceinline__ void many_rows(const PagedArgs& a, char* sm, int* poi
   if (lane == 0) seen[wave] = w.all_see;
   __syncthreads();
   const int whole = min(min(seen[0], seen[1]), min(seen[2], seen[3]));
-  PagedTiles<T, D> src;
-  src.p = pages_of<T, D>(a, b0, head);
-  src.n = end;
+  PagedTiles<T, D> src(pages_of<T, D>(a, b0, head), end);
   w.run(src, first, end, uniform(whole), a.c);
   if (row > last_row) return;
   const int slots = a.most_np + a.ns;
@@ -1078,11 +1082,12 @@ bool bad_scale(float s) { return !(s >= 0.f) || std::isinf(s); }
 bool misaligned(const void* p, int64_t stride) { return ((uintptr_t)p & 15) || stride % 8; }
 
 // Few rows leave compute units idle, and each of their workgroups with all keys: then the keys are divided, so that there are up to
-// two workgroups a compute unit, each with 256 keys at least.
+// two workgroups a compute unit, each with 256 keys at least; not for 640 keys or less, where that gains less than the second launch
+// costs (500 tokens: 15.1 us, in two shares 19.6).
 template <typename T, int D>
 int launch_prompt(PromptArgs a, int cus, hipStream_t stream) {
   const int64_t items = ((int64_t)a.total_q * a.ratio / 128 + a.seqs) * a.kv_heads;
-  const int64_t want = 2 * (int64_t)cus / items, most = ((int64_t)a.total_k + 255) / 256;
+  const int64_t want = 2 * (int64_t)cus / items, most = a.total_k > 640 ? ((int64_t)a.total_k + 255) / 256 : 1;
   a.shares = (int)std::max<int64_t>(1, std::min(want, most));
   if (items * a.shares > INT_MAX) return HQ_ERR_TOO_LARGE;
   const int64_t rows = (int64_t)a.total_q * a.heads;
