@@ -156,10 +156,9 @@ struct Pages {
   __device__ __forceinline__ Pages(const T* k0, const T* v0, const int* row, int head, int kv_heads, int log, int n)
       : k((const char*)(k0 + ((int64_t)head << log) * D)), v((const char*)(v0 + ((int64_t)head << log) * D)), table(row),
         page_bytes((uint32_t)kv_heads * (D * 2) << log), page_log(log), pages(n) {}
-  __device__ __forceinline__ int id(int key) const {  // -1: no page, to be read as zeros
-    const int p = table[key >> page_log];
-    return (unsigned)p < (unsigned)pages ? p : -1;
-  }
+  // The table's entry, as it is: looking at it where it is loaded would be waiting for it, and for all that is asked for in between.
+  __device__ __forceinline__ int id(int key) const { return table[key >> page_log]; }
+  __device__ __forceinline__ bool none(int id) const { return (unsigned)id >= (unsigned)pages; }  // no page: to be read as zeros
   __device__ __forceinline__ uint64_t at(int page, int key) const {
     return (uint64_t)(uint32_t)page * page_bytes + (uint32_t)(key & ((1 << page_log) - 1)) * (D * 2);
   }
@@ -168,45 +167,70 @@ __device__ __forceinline__ void zero_lds(char* to) {  // what one to_lds() would
   reinterpret_cast<hq_u4v*>(to)[threadIdx.x & 63] = hq_u4v{0, 0, 0, 0};
 }
 
+// Where the rows of a wave's instructions are: a lane works out an instruction's place, which then costs two moves to scalar registers
+// and an addition (worked out by the scalar unit, load after load, 30 instructions each: 0.6 us a tile with nothing under it).
+struct Places {
+  uint32_t lo, hi;           // of a lane's instruction
+  unsigned long long none;   // instructions whose rows are in no page
+  template <typename T, int D>
+  __device__ __forceinline__ void set(const Pages<T, D>& p, int id, int key) {
+    const uint64_t x = p.at(id, key);
+    lo = (uint32_t)x;
+    hi = (uint32_t)(x >> 32);
+    none = __ballot(p.none(id));
+  }
+  __device__ __forceinline__ const char* of(const char* pool, int lane) const {
+    return pool + ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)hi, lane) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)lo, lane));
+  }
+  // Instructions first ... first + N - 1, into `to` and on; off: the lane's offset in the first one, from which the others' differ in what
+  // k_piece() or v_piece() make of the rows between.  Whether all of them were needed.
+  template <int D, bool VALUES, int N>
+  __device__ __forceinline__ bool load(const char* pool, int first, uint32_t off0, char* to) const {
+    auto off = [=](int i) { return off0 ^ (uint32_t)(VALUES ? (D == 128 ? (i & 1) * 32 : 0) : D == 128 ? (i & 3) * 64 : (i & 1) * 64); };
+    const uint32_t lds = uniform((int)lds_address(to));
+    if (!(none >> first & ((1ull << N) - 1))) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) to_lds(lds + i * 1024, of(pool, first + i), off(i));
+      return true;
+    }
+    for (int i = 0; i < N; ++i) {
+      if (none >> (first + i) & 1) zero_lds(to + i * 1024);
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        if (j == i && !(none >> (first + i) & 1)) to_lds(lds + j * 1024, of(pool, first + j), off(j));
+    }
+    return false;
+  }
+};
+
 // The same tiles of pages.  Rows behind the last one are whatever its page holds.
 template <typename T, int D>
 struct PagedTiles {
   static constexpr int CH = D / 8, NL = 64 * CH / kThreads, RG = 64 / CH;  // RG: rows of an instruction, all in one page
   Pages<T, D> p;
   int n, first;
-  int ids_next, ids_k, ids_v;  // pages of the instructions' rows, one a lane: of the tile to come, of the keys' and of the values' next
-  uint32_t koff[NL], voff[NL];
+  int ids;          // pages of the wave's instructions' rows, one a lane, of the tile to come
+  Places next, now; // of the tile whose keys are loaded next, and (heads of 128, whose keys are a tile ahead) of its predecessor
+  uint32_t koff, voff;
   __device__ PagedTiles(const Pages<T, D>& pages, int end) : p(pages), n(end) {}
-  __device__ __forceinline__ int ids(int t) const { return p.id(min(first + t * 64 + (int)(threadIdx.x & (64 / RG - 1)) * RG, n - 1)); }
-  __device__ __forceinline__ void load(const char* pool, int id, int t, const uint32_t (&off)[NL], char* to) {
-    const int wave = uniform((int)(threadIdx.x >> 6)), lds = uniform((int)lds_address(to));
-    const unsigned long long none = __ballot(id < 0);
-#pragma unroll
-    for (int i = 0; i < NL; ++i) {
-      const int j = wave * NL + i, page = __builtin_amdgcn_readlane(id, j);
-      if (none && page < 0) zero_lds(to + j * 1024);
-      else to_lds(lds + j * 1024, pool + p.at(page, first + t * 64 + j * RG), off[i]);
-    }
-  }
+  __device__ __forceinline__ int key(int t) const { return first + t * 64 + (int)((threadIdx.x >> 6) * NL + threadIdx.x % NL) * RG; }
   __device__ __forceinline__ void start(int f) {
     first = f;
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int i = 0; i < NL; ++i) {
-      const int row = ((threadIdx.x >> 6) * NL + i) * RG + lane / CH;
-      koff[i] = (lane / CH) * D * 2 + k_piece<D>(row, lane % CH) * 16;
-      voff[i] = (lane / CH) * D * 2 + v_piece<D>(row, lane % CH) * 16;
-    }
-    ids_next = ids(0);
+    const int lane = threadIdx.x & 63, row = lane / CH;  // of a multiple of 16
+    koff = row * D * 2 + k_piece<D>(row, lane % CH) * 16;
+    voff = row * D * 2 + v_piece<D>(row, lane % CH) * 16;
+    ids = p.id(min(key(0), n - 1));
   }
   // Before the first load of tile t: its pages are there, those of the tile behind it are asked for.
   __device__ __forceinline__ void advance(int t) {
-    ids_v = ids_k;
-    ids_k = ids_next;
-    ids_next = ids(t + 1);
+    now = next;
+    next.set(p, ids, key(t));
+    ids = p.id(min(key(t + 1), n - 1));
   }
-  __device__ __forceinline__ void load_k(int t, char* to) { load(p.k, ids_k, t, koff, to); }
-  __device__ __forceinline__ void load_v(int t, char* to) { load(p.v, D == 128 ? ids_v : ids_k, t, voff, to); }
+  __device__ __forceinline__ void load_k(int, char* to) { next.template load<D, false, NL>(p.k, 0, koff, to + (threadIdx.x >> 6) * (NL * 1024)); }
+  __device__ __forceinline__ void load_v(int, char* to) {
+    (D == 128 ? now : next).template load<D, true, NL>(p.v, 0, voff, to + (threadIdx.x >> 6) * (NL * 1024));
+  }
 };
 
 // ---- many rows -----------------------------------------------------------------------------------------------------------
@@ -579,39 +603,32 @@ struct Few {
     if (wave >= blocks) return;
     char* const ks = sm + wave * 2 * HALF;
     char* const vs = ks + HALF;
-    uint32_t koff[G], voff[G];
-#pragma unroll
-    for (int i = 0; i < G; ++i) {
-      const int row = i * RG + lane / CH;
-      koff[i] = (lane / CH) * D * 2 + k_piece<D>(row, lane % CH) * 16;
-      voff[i] = (lane / CH) * D * 2 + v_piece<D>(row, lane % CH) * 16;
-    }
+    const uint32_t koff = (lane / CH) * D * 2 + k_piece<D>(lane / CH, lane % CH) * 16, voff = (lane / CH) * D * 2 + v_piece<D>(lane / CH, lane % CH) * 16;
     // pages of 64 / G blocks, a lane for each instruction of each
     constexpr int SET = 64 / G;
     auto ids_of = [&](int set) { return p.id(min(first + (wave + kWaves * (set * SET + lane / G)) * 32 + lane % G * RG, end - 1)); };
+    Places here;
+    auto places_of = [&](int set, int id) {
+      Places x;
+      x.set(p, id, first + (wave + kWaves * (set * SET + lane / G)) * 32 + lane % G * RG);
+      return x;
+    };
     int ids = ids_of(0), ids_next = 0;
+    here = places_of(0, ids);
     // Whether all G instructions were needed: what the waits count.
-    auto load = [&](const char* pool, int block, int set_ids, const uint32_t (&off)[G], char* to, bool values) {
+    auto load = [&](const char* pool, int block, const Places& places, int set_ids, char* to, auto values) {
       const int base = first + block * 32, at = block / kWaves % SET * G;
+      if (base + 32 <= end) return places.template load<D, values, G>(pool, at, values ? voff : koff, to);
+      // the last block: rows behind the last key repeat it, every lane by an address of its own
       const uint32_t lds = uniform((int)lds_address(to));
       bool whole = true;
-      if (base + 32 <= end) {
-        whole = !(__ballot(set_ids < 0) >> at & ((1ull << G) - 1));
 #pragma unroll
-        for (int i = 0; i < G; ++i) {
-          const int page = __builtin_amdgcn_readlane(set_ids, at + i);
-          if (!whole && page < 0) zero_lds(to + i * 1024);
-          else to_lds(lds + i * 1024, pool + p.at(page, base + i * RG), off[i]);
-        }
-      } else {  // the last block: rows behind the last key repeat it, every lane by an address of its own
-#pragma unroll
-        for (int i = 0; i < G; ++i) {
-          const int row = i * RG + lane / CH, key = min(base + row, end - 1), page = __shfl(set_ids, at + (key - base) / RG);
-          const int ch = values ? v_piece<D>(row, lane % CH) : k_piece<D>(row, lane % CH);
-          if (page >= 0) to_lds(lds + i * 1024, pool + p.at(page, key) + ch * 16);
-          else zero_lds(to + i * 1024);
-          whole &= __ballot(page < 0) == 0;
-        }
+      for (int i = 0; i < G; ++i) {
+        const int row = i * RG + lane / CH, key = min(base + row, end - 1), page = __shfl(set_ids, at + (key - base) / RG);
+        const int ch = values ? v_piece<D>(row, lane % CH) : k_piece<D>(row, lane % CH);
+        if (!p.none(page)) to_lds(lds + i * 1024, pool + p.at(page, key) + ch * 16);
+        else zero_lds(to + i * 1024);
+        whole &= __ballot(p.none(page)) == 0;
       }
       return whole;
     };
@@ -620,8 +637,8 @@ struct Few {
       if (whole) asm volatile("s_waitcnt vmcnt(%0)" ::"i"(G) : "memory");
       else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     };
-    load(p.k, wave, ids, koff, ks, false);
-    bool whole_k = false, whole_v = load(p.v, wave, ids, voff, vs, true);
+    load(p.k, wave, here, ids, ks, std::false_type());
+    bool whole_k = false, whole_v = load(p.v, wave, here, ids, vs, std::true_type());
 #pragma unroll
     for (int kk = 0; kk < D / 32; ++kk) asm volatile("" : "+v"(qf[kk]));
     for (int block = wave; block < blocks; block += kWaves) {
@@ -648,7 +665,11 @@ struct Few {
           top = fmaxf(top, s[b][r]);
         }
       asm volatile("" : "+v"(top)::"memory");  // the keys have been read
-      whole_k = more && load(p.k, next, set_ends ? ids_next : ids, koff, ks, false);
+      if (set_ends && more) {
+        ids = ids_next;
+        here = places_of(nth / SET + 1, ids);
+      }
+      whole_k = more && load(p.k, next, here, ids, ks, std::false_type());
       top = quarters_max(top) * c;
       if (__builtin_amdgcn_ballot_w64(top > m + 8.f)) {  // as in Many
         const float mn = top > m + 8.f ? top : m, f = mn == m ? 1.f : __builtin_amdgcn_exp2f(m - mn);
@@ -683,8 +704,7 @@ struct Few {
       }
 #pragma unroll
       for (int d = 0; d < D / 16; ++d) asm volatile("" : "+v"(o[d])::"memory");  // the values have been read
-      whole_v = more && load(p.v, next, set_ends ? ids_next : ids, voff, vs, true);
-      if (set_ends) ids = ids_next;
+      whole_v = more && load(p.v, next, here, ids, vs, std::true_type());
     }
     l = quarters_sum(l);
   }
@@ -868,11 +888,11 @@ __device__ __forceinline__ Pages<T, D> pages_of(const PagedArgs& a, int request,
   return Pages<T, D>((const T*)a.k, (const T*)a.v, a.table + (int64_t)request * a.width, head, a.kv_heads, a.page_log, a.pages);
 }
 
-// Up to 16 of the rows (request, head of the group) of requests b0 ..., from first_row on, all of which see the keys.
+// Up to 16 rows (request, head of the group), those of requests b0 ..., all of which see the keys.
 template <typename T, int D>
-__device__ __forceinline__ void few_rows(const PagedArgs& a, char* sm, int b0, int nrows, int first_row, int head, int first, int end, int slot) {
+__device__ __forceinline__ void few_rows(const PagedArgs& a, char* sm, int b0, int nrows, int head, int first, int end, int slot) {
   typedef typename Kind<T>::V8 V8;
-  const int lane = threadIdx.x & 63, last_row = min(first_row + 16, nrows) - 1, r = min(first_row + (lane & 15), last_row);
+  const int lane = threadIdx.x & 63, last_row = nrows - 1, r = min(lane & 15, last_row);
   const uint32_t ratio = a.ratio;
   const int b = b0 + (uint32_t)r / ratio, h = head * ratio + (uint32_t)r % ratio;
   Few<T, D> w;
@@ -883,7 +903,7 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, char* sm, int b0, i
   w.run(pages_of<T, D>(a, b0, head), first, end, a.c);
   float sum[D / 16], top, total;
   w.join(sum, &top, &total);
-  const int mine = first_row + (threadIdx.x >> 4), d0 = (threadIdx.x & 15) * (D / 16), slots = a.most_np + a.ns;
+  const int mine = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * (D / 16), slots = a.most_np + a.ns;
   if (mine > last_row) return;
   const int64_t at = (int64_t)(b0 + (uint32_t)mine / ratio) * a.heads + head * ratio + (uint32_t)mine % ratio;
   if (slots == 1) {
@@ -937,6 +957,8 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void paged_kernel(PagedA
   extern __shared__ __align__(16) char sm[];
   __shared__ int poison;
   uint32_t x = blockIdx.x;
+  int b0 = 0, nb = 1, row0 = 0, head, first, end, slot;
+  bool few = a.ratio <= 16;
   if ((int)x < a.prefix_items) {
     // The common keys: as many shares as there are workgroups for the tiles of rows that there are.
     const int ratio = a.ratio, lane = threadIdx.x & 63;
@@ -955,12 +977,13 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void paged_kernel(PagedA
     const int np = all ? min(max(a.prefix_items / (all * a.kv_heads), 1), a.most_np) : 0;
     if (x == 0 && threadIdx.x == 0) *a.np = np;
     if (np == 0) return;
-    const int head = x % (uint32_t)a.kv_heads;
+    head = x % (uint32_t)a.kv_heads;
     x /= (uint32_t)a.kv_heads;
-    const int share = x % (uint32_t)np;
+    slot = x % (uint32_t)np;
     int tile = x / (uint32_t)np;
     if (tile >= all) return;
-    int b0 = 0, nb = 0, n = 0;
+    int n = 0;
+    nb = 0;
     for (int g0 = 0; nb == 0; g0 += 64) {
       const Groups g = g0 ? Groups(a, g0) : some;
       const int own = tiles(g), sum = running(own), total = __builtin_amdgcn_readlane(sum, 63);
@@ -974,25 +997,27 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void paged_kernel(PagedA
         tile -= total;
       }
     }
-    int first, end;
-    share_of(n, np, 256, share, &first, &end);
-    const bool few = nb * ratio <= 16 && !__ballot(lane < nb && a.lengths[b0 + min(lane, nb - 1)] < end);
-    if (few) few_rows<T, D>(a, sm, b0, nb * ratio, 0, head, first, end, share);
-    else many_rows<T, D>(a, sm, &poison, b0, nb * ratio, tile * 128, head, first, end, share);
+    share_of(n, np, 256, slot, &first, &end);
+    few = nb * ratio <= 16 && !__ballot(lane < nb && a.lengths[b0 + min(lane, nb - 1)] < end);
+    row0 = tile * 128;
   } else {
     x -= a.prefix_items;
-    const int head = x % (uint32_t)a.kv_heads;
+    head = x % (uint32_t)a.kv_heads;
     x /= (uint32_t)a.kv_heads;
     const int share = x % (uint32_t)a.ns;
     x /= (uint32_t)a.ns;
-    const int tiles = a.ratio <= 16 ? 1 : (a.ratio + 127) / 128, tile = tiles == 1 ? 0 : x % (uint32_t)tiles, b = tiles == 1 ? x : x / (uint32_t)tiles;
-    const int n = min(max(a.lengths[b], 0), a.width << a.page_log), shared = shared_of(a, b), from = uniform(min(max(shared, 0), n));
-    if (blockIdx.x - a.prefix_items == (uint32_t)b * a.kv_heads * a.ns * tiles && threadIdx.x == 0 && a.np) a.np[1 + b] = shared >= 0;
-    int first, end;
+    const int tiles = few ? 1 : (a.ratio + 127) / 128, tile = few ? 0 : x % (uint32_t)tiles;
+    b0 = few ? x : x / (uint32_t)tiles;
+    const int n = min(max(a.lengths[b0], 0), a.width << a.page_log), shared = shared_of(a, b0), from = uniform(min(max(shared, 0), n));
+    if (head == 0 && share == 0 && tile == 0 && threadIdx.x == 0 && a.np) a.np[1 + b0] = shared >= 0;
     share_of(n - from, a.ns, 128, share, &first, &end);
-    if (a.ratio <= 16) few_rows<T, D>(a, sm, b, a.ratio, 0, head, from + first, from + end, a.most_np + share);
-    else many_rows<T, D>(a, sm, &poison, b, a.ratio, tile * 128, head, from + first, from + end, a.most_np + share);
+    first += from;
+    end += from;
+    row0 = tile * 128;
+    slot = a.most_np + share;
   }
+  if (few) few_rows<T, D>(a, sm, b0, nb * a.ratio, head, first, end, slot);
+  else many_rows<T, D>(a, sm, &poison, b0, nb * a.ratio, row0, head, first, end, slot);
 }
 
 // The shares of a row together, by WAVES waves: their maxima and sums a lane each, then the sums of the values, 16 bytes a lane, several
