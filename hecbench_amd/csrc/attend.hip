@@ -561,10 +561,10 @@ struct Many {
     l = pair_sum(l);
   }
 
-  // The row's result.
+  // The row's result.  (By way of LDS, so that a store writes whole rows: no faster.)
   __device__ __forceinline__ void put(T* out, bool none) const {
     const int half = (threadIdx.x >> 5) & 1;
-    const float inv = 1.f / l;
+    const float inv = none ? 0.f : 1.f / l;  // and the sums are zero
 #pragma unroll
     for (int d = 0; d < D / 32; ++d)
 #pragma unroll
@@ -572,7 +572,7 @@ struct Many {
         typedef T T4 __attribute__((ext_vector_type(4)));
         T4 v;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = (T)(none ? 0.f : o[d][4 * g + i] * inv);
+        for (int i = 0; i < 4; ++i) v[i] = (T)(o[d][4 * g + i] * inv);
         *reinterpret_cast<T4*>(out + 32 * d + 8 * g + 4 * half) = v;
       }
   }
@@ -745,28 +745,46 @@ __device__ __forceinline__ void set_up(int* poison) {
   if (threadIdx.x == 0) *poison = -1;
 }
 
-// Item x of a list in which entry i, bounds[i] to bounds[i + 1], cut to 0 ... most, has tiles(its length) tiles: the entry, its begin and
-// length, and which of its tiles.  A wave looks at 64 entries at a time.
-template <typename F>
-__device__ __forceinline__ bool find_tile(const int* bounds, int n, int most, int x, F tiles, int* entry, int* begin, int* length, int* which) {
+// A sequence's tokens and keys.
+struct Sequence {
+  int q0, nq, k0, nk, tile;
+};
+// Tile x of a list in which sequence i has tiles(its tokens) tiles: its sequence, and which of its tiles.  A wave looks at 64 sequences at a
+// time, keys' bounds along with tokens', so that one trip to memory does.  Up to kSorted sequences are taken longest first, so that the
+// workgroups that come last are short ones (24 of up to 901 tokens, 32 heads of 64: SORTED); the tiles of a sequence stay together, as
+// they read the same keys.
+constexpr int kSorted = 32;
+template <typename A, typename F>
+__device__ __forceinline__ bool find_tile(const A& a, int x, F tiles, Sequence* s) {
   const int lane = threadIdx.x & 63;
-  for (int i0 = 0; i0 < n; i0 += 64) {
-    const int i = i0 + lane;
-    const int b = i < n ? min(max(bounds[i], 0), most) : 0, len = i < n ? min(max(bounds[i + 1], b), most) - b : 0;
+  for (int i0 = 0; i0 < a.seqs; i0 += 64) {
+    const int i = min(i0 + lane, a.seqs - 1);
+    const int qb = a.cu_q[i], qe = a.cu_q[i + 1], kb = a.cu_k[i], ke = a.cu_k[i + 1];
+    const int b = min(max(qb, 0), a.total_q), len = i0 + lane < a.seqs ? min(max(qe, b), a.total_q) - b : 0;
+    const int k = min(max(kb, 0), a.total_k), keys = min(max(ke, k), a.total_k) - k;
     const int t = tiles(len);
-    int sum = t;
+    int before = 0, total;  // tiles ahead of the lane's sequence
+    if (a.seqs <= kSorted) {
+      for (int j = 0; j < a.seqs; ++j) {
+        const int other = __builtin_amdgcn_readlane(t, j);
+        before += other > t || (other == t && j < lane) ? other : 0;
+      }
+      total = INT_MAX;
+    } else {
+      int sum = t;
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int u = __shfl_up(sum, d);
-      if (lane >= d) sum += u;
+      for (int d = 1; d < 64; d <<= 1) {
+        const int u = __shfl_up(sum, d);
+        if (lane >= d) sum += u;
+      }
+      before = sum - t;
+      total = __builtin_amdgcn_readlane(sum, 63);
     }
-    const int total = __builtin_amdgcn_readlane(sum, 63);
-    if (x < total) {
-      const int at = __ffsll(__ballot(sum > x)) - 1;
-      *entry = i0 + at;
-      *begin = __builtin_amdgcn_readlane(b, at);
-      *length = __builtin_amdgcn_readlane(len, at);
-      *which = x - __builtin_amdgcn_readlane(sum - t, at);
+    const unsigned long long here = __ballot(x >= before && x < before + t);
+    if (here) {
+      const int at = __ffsll(here) - 1;
+      *s = Sequence{__builtin_amdgcn_readlane(b, at), __builtin_amdgcn_readlane(len, at), __builtin_amdgcn_readlane(k, at),
+                    __builtin_amdgcn_readlane(keys, at), x - __builtin_amdgcn_readlane(before, at)};
       return true;
     }
     x -= total;
@@ -802,11 +820,18 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 4 : 2) void prompt_kernel(Promp
     x /= (uint32_t)a.shares;
   }
   const uint32_t ratio = a.ratio;
-  int seq, tile, q0, nq;
-  if (!find_tile(a.cu_q, a.seqs, a.total_q, x, [=](int n) { return (int)((n * ratio + ROWS - 1) / ROWS); }, &seq, &q0, &nq, &tile)) return;
-  const int k0 = min(max(a.cu_k[seq], 0), a.total_k), nk = min(max(a.cu_k[seq + 1], k0), a.total_k) - k0;
-  const int rows = nq * ratio;
-  tile = (rows + ROWS - 1) / ROWS - 1 - tile;  // the tiles with most keys come first
+  __shared__ Sequence found;  // by the first wave: for short sequences the search is a sixth of the vector instructions
+  if (threadIdx.x < 64) {
+    Sequence s = {};
+    if (!find_tile(a, x, [=](int n) { return (int)((n * ratio + ROWS - 1) / ROWS); }, &s)) s.tile = -1;
+    if (threadIdx.x == 0) found = s;
+  }
+  set_up(&poison);
+  __syncthreads();
+  const Sequence s = {uniform(found.q0), uniform(found.nq), uniform(found.k0), uniform(found.nk), uniform(found.tile)};
+  if (s.tile < 0) return;
+  const int q0 = s.q0, nq = s.nq, k0 = s.k0, nk = s.nk, rows = nq * ratio;
+  const int tile = (rows + ROWS - 1) / ROWS - 1 - s.tile;  // the tiles with most keys come first
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int first_row = tile * ROWS, last_row = min(first_row + ROWS, rows) - 1;
   const int row = first_row + wave * 32 + (lane & 31), r = min(row, last_row);
@@ -814,7 +839,6 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 4 : 2) void prompt_kernel(Promp
   A w;
   w.sm = sm;
   w.poison = &poison;
-  set_up(&poison);
   const T* q = (const T*)a.q + (int64_t)(q0 + token) * a.qs + (int64_t)h * D + 8 * (lane >> 5);
 #pragma unroll
   for (int kk = 0; kk < D / 16; ++kk) w.qf[kk] = *reinterpret_cast<const V8*>(q + 16 * kk);
