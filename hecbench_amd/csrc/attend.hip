@@ -561,19 +561,26 @@ struct Many {
     l = pair_sum(l);
   }
 
-  // The row's result.  (By way of LDS, so that a store writes whole rows: no faster.)
+  // The row's result.  A lane and its partner hold every other four elements of their row; two exchanges a pair of fours make them eights,
+  // half the stores (24 sequences of up to 901 tokens, 32 heads of 64: 71.5 -> 70 us; by way of LDS, in whole rows, no faster).
   __device__ __forceinline__ void put(T* out, bool none) const {
-    const int half = (threadIdx.x >> 5) & 1;
     const float inv = none ? 0.f : 1.f / l;  // and the sums are zero
+    typedef T T2 __attribute__((ext_vector_type(2)));
+    hq_u4v* to = reinterpret_cast<hq_u4v*>(out) + ((threadIdx.x >> 5) & 1);
 #pragma unroll
     for (int d = 0; d < D / 32; ++d)
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        typedef T T4 __attribute__((ext_vector_type(4)));
-        T4 v;
+      for (int g = 0; g < 4; g += 2) {
+        hq_u4v v;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = (T)(o[d][4 * g + i] * inv);
-        *reinterpret_cast<T4*>(out + 32 * d + 8 * g + 4 * half) = v;
+        for (int i = 0; i < 2; ++i) {
+          const int r = 4 * g + 2 * i;
+          const auto s = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, T2{(T)(o[d][r] * inv), (T)(o[d][r + 1] * inv)}),
+                                                          __builtin_bit_cast(uint32_t, T2{(T)(o[d][r + 4] * inv), (T)(o[d][r + 5] * inv)}), false, false);
+          v[i] = s[0];
+          v[2 + i] = s[1];
+        }
+        to[4 * d + g] = v;
       }
   }
 };
@@ -750,10 +757,8 @@ struct Sequence {
   int q0, nq, k0, nk, tile;
 };
 // Tile x of a list in which sequence i has tiles(its tokens) tiles: its sequence, and which of its tiles.  A wave looks at 64 sequences at a
-// time, keys' bounds along with tokens', so that one trip to memory does.  Up to kSorted sequences are taken longest first, so that the
-// workgroups that come last are short ones (24 of up to 901 tokens, 32 heads of 64: SORTED); the tiles of a sequence stay together, as
-// they read the same keys.
-constexpr int kSorted = 32;
+// time, keys' bounds along with tokens', so that one trip to memory does.  (Longest sequences first: no faster; nor is a workgroup that
+// goes from tile to tile.)
 template <typename A, typename F>
 __device__ __forceinline__ bool find_tile(const A& a, int x, F tiles, Sequence* s) {
   const int lane = threadIdx.x & 63;
@@ -763,23 +768,13 @@ __device__ __forceinline__ bool find_tile(const A& a, int x, F tiles, Sequence* 
     const int b = min(max(qb, 0), a.total_q), len = i0 + lane < a.seqs ? min(max(qe, b), a.total_q) - b : 0;
     const int k = min(max(kb, 0), a.total_k), keys = min(max(ke, k), a.total_k) - k;
     const int t = tiles(len);
-    int before = 0, total;  // tiles ahead of the lane's sequence
-    if (a.seqs <= kSorted) {
-      for (int j = 0; j < a.seqs; ++j) {
-        const int other = __builtin_amdgcn_readlane(t, j);
-        before += other > t || (other == t && j < lane) ? other : 0;
-      }
-      total = INT_MAX;
-    } else {
-      int sum = t;
+    int sum = t;
 #pragma unroll
-      for (int d = 1; d < 64; d <<= 1) {
-        const int u = __shfl_up(sum, d);
-        if (lane >= d) sum += u;
-      }
-      before = sum - t;
-      total = __builtin_amdgcn_readlane(sum, 63);
+    for (int d = 1; d < 64; d <<= 1) {
+      const int u = __shfl_up(sum, d);
+      if (lane >= d) sum += u;
     }
+    const int before = sum - t, total = __builtin_amdgcn_readlane(sum, 63);
     const unsigned long long here = __ballot(x >= before && x < before + t);
     if (here) {
       const int at = __ffsll(here) - 1;
@@ -820,16 +815,8 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 4 : 2) void prompt_kernel(Promp
     x /= (uint32_t)a.shares;
   }
   const uint32_t ratio = a.ratio;
-  __shared__ Sequence found;  // by the first wave: for short sequences the search is a sixth of the vector instructions
-  if (threadIdx.x < 64) {
-    Sequence s = {};
-    if (!find_tile(a, x, [=](int n) { return (int)((n * ratio + ROWS - 1) / ROWS); }, &s)) s.tile = -1;
-    if (threadIdx.x == 0) found = s;
-  }
-  set_up(&poison);
-  __syncthreads();
-  const Sequence s = {uniform(found.q0), uniform(found.nq), uniform(found.k0), uniform(found.nk), uniform(found.tile)};
-  if (s.tile < 0) return;
+  Sequence s;
+  if (!find_tile(a, x, [=](int n) { return (int)((n * ratio + ROWS - 1) / ROWS); }, &s)) return;
   const int q0 = s.q0, nq = s.nq, k0 = s.k0, nk = s.nk, rows = nq * ratio;
   const int tile = (rows + ROWS - 1) / ROWS - 1 - s.tile;  // the tiles with most keys come first
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -839,6 +826,7 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 4 : 2) void prompt_kernel(Promp
   A w;
   w.sm = sm;
   w.poison = &poison;
+  set_up(&poison);
   const T* q = (const T*)a.q + (int64_t)(q0 + token) * a.qs + (int64_t)h * D + 8 * (lane >> 5);
 #pragma unroll
   for (int kk = 0; kk < D / 16; ++kk) w.qf[kk] = *reinterpret_cast<const V8*>(q + 16 * kk);
@@ -855,7 +843,7 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 4 : 2) void prompt_kernel(Promp
   const int each = a.shares == 1 ? nk : max(256, ((nk + a.shares - 1) / a.shares + A::TILE - 1) & -A::TILE);
   const int end = uniform(limit((uint32_t)last_row / ratio)), first = (int)min((int64_t)share * each, (int64_t)end);
   w.run(src, first, min(end, first + each), uniform(limit((uint32_t)first_row / ratio)), a.c);
-  if (row > last_row) return;
+  if (row > last_row) return;  // and so does the partner
   if (a.shares == 1) {
     w.put((T*)a.out + ((int64_t)(q0 + token) * a.heads + h) * D, w.lim == 0);
   } else {
