@@ -284,3 +284,97 @@ def test_other_stream_and_graph(hq):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(got, hq.paged_attention(*args)) and torch.equal(pgot, hq.prompt_attention(pq, pk, pv, cu))
+
+
+# ---- the ways through the kernels that the sizes above do not take ---------------------------------------------------------------
+def test_prompt_divided_keys_leave_what_is_no_ones(hq):
+    """Few rows and many keys: the shares' sums, rows that see nothing, and tokens of no sequence."""
+    dtype, u = TYPES["bf16"]
+    for heads in ((8, 2), (3, 1)):
+        nq, nk = [40, 0, 3, 70], [2500, 100, 1, 60]  # the last one's first tokens see nothing
+        q, k, v = randn(1, 120, heads[0], 128).to(dtype), randn(2, sum(nk), heads[1], 128).to(dtype), randn(3, sum(nk), heads[1], 128).to(dtype)
+        out = torch.full((120, heads[0], 128), 7.0, dtype=dtype, device="cuda")
+        hq.prompt_attention(q, k, v, i32(bounds(nq)), i32(bounds(nk)), out=out)
+        check_prompt(out[:113], q[:113], k, v, nq, nk, True, 1 / math.sqrt(128), u)
+        assert (out[113:] == 7.0).all()
+        k2, v2 = k.clone(), v.clone()
+        k2[2480:2500], v2[2480:2500] = math.nan, math.inf  # seen by the last 20 of the 40
+        got = hq.prompt_attention(q, k2, v2, i32(bounds(nq)), i32(bounds(nk)))
+        assert torch.equal(got[:20], out[:20]) and torch.equal(got[40:113], out[40:113]) and not torch.isfinite(got[21:40]).any()
+
+
+def test_prompt_rows_far_apart(hq):
+    """Offsets beyond 32 bits: tokens 2 MB apart."""
+    dtype, u = TYPES["f16"]
+    n, D = 2300, 64
+    flat = torch.zeros(n << 20, dtype=dtype, device="cuda")
+    k = flat.as_strided((n, 1, D), (1 << 20, D, 1))
+    v = flat.as_strided((n, 1, D), (1 << 20, D, 1), storage_offset=D)
+    k.copy_(randn(2, n, 1, D))
+    v.copy_(randn(3, n, 1, D))
+    q = randn(1, 5, 2, D).to(dtype)
+    out = hq.prompt_attention(q, k, v, i32([0, 5]), i32([0, n]))
+    check_prompt(out, q, k, v, [5], [n], True, 0.125, u)
+
+
+@pytest.mark.parametrize("kind,D", [("bf16", 128), ("f16", 64)])
+def test_paged_long_rows_in_one_share(hq, kind, D):
+    """So many requests that nobody's keys are divided: a wave's blocks take several sets of page numbers."""
+    dtype, u = TYPES[kind]
+    lengths = [3333 if i == 3 else 2050 if i == 7 else (i * 37) % 70 for i in range(280)]
+    q, k, v, table, lengths = paged_case(1, dtype, lengths, (2, 2), D, 16)
+    check_paged(hq.paged_attention(q, k, v, i32(table), i32(lengths)), q, k, v, table, lengths, 1 / math.sqrt(D), u)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_paged_missing_pages_anywhere(hq, D):
+    """Entries that are no pages in whole blocks, next to the end, in what is shared and in what is not."""
+    dtype, u = TYPES["f16"]
+    lengths, groups, shared = [1000, 1003, 990, 700, 20], [0, 3, 5], [640, 16]
+    for heads in ((4, 2), (24, 1)):
+        q, k, v, table, _ = paged_case(4, dtype, lengths, heads, D, 16, groups, shared)
+        zero = len(k)
+        k0, v0 = torch.cat([k, torch.zeros_like(k[:1])]), torch.cat([v, torch.zeros_like(v[:1])])
+        bad = [row[:] for row in table]
+        for s, places in ((0, (41, 50, 51, 61, 62)), (1, (40, 62)), (2, (61,)), (3, (1, 2, 3, 4, 20, 43)), (4, (1,))):
+            for j in places:
+                bad[s][j] = (-1, zero, 2 ** 31 - 1)[j % 3]
+        for row in bad[:3]:
+            row[5] = row[39] = -1
+        want = [[zero if not 0 <= p < zero else p for p in row] for row in bad]
+        out = hq.paged_attention(q, k, v, i32(bad), i32(lengths), i32(groups), i32(shared))
+        check_paged(out, q, k0, v0, want, lengths, 1 / math.sqrt(D), u)
+
+
+def test_paged_many_groups(hq):
+    """More groups than a wave has lanes, some of them empty, and requests behind the last."""
+    dtype, u = TYPES["bf16"]
+    groups, lengths = [0], []
+    for g in range(75):
+        n = (g * 5) % 3
+        lengths += [48 + (g * 11 + i * 7) % 90 for i in range(n)]
+        groups.append(len(lengths))
+    lengths += [30, 5]
+    shared = [(g * 16) % 64 for g in range(75)]
+    for heads in ((4, 1), (32, 1)):
+        q, k, v, table, _ = paged_case(8, dtype, lengths, heads, 64, 16, groups, shared)
+        out = hq.paged_attention(q, k, v, i32(table), i32(lengths), i32(groups), i32(shared))
+        check_paged(out, q, k, v, table, lengths, 0.125, u)
+
+
+def test_paged_beyond_32_bits(hq):
+    """A cache of more than 4 GB: the last pages, written and read."""
+    dtype, u = TYPES["bf16"]
+    pages, heads, page, D = 2200, 8, 1024, 128
+    k = torch.zeros((pages, heads, page, D), dtype=dtype, device="cuda")
+    v = torch.zeros_like(k)
+    n = 1500
+    table = [[2199, 2100], [3, 2150]]
+    kn, vn = randn(1, 2 * n, heads, D).to(dtype), randn(2, 2 * n, heads, D).to(dtype)
+    hq.cache_write(kn, vn, k, v, i32(table), i32([0, 0]), i32([0, n, 2 * n]))
+    assert torch.equal(k[2100, :, :n - page], kn[page:n].transpose(0, 1)) and torch.equal(v[2150, :, :n - page], vn[n + page:].transpose(0, 1))
+    q = randn(3, 2, 16, D).to(dtype)
+    out = hq.paged_attention(q, k, v, i32(table), i32([n, n]))
+    check_paged(out, q, k, v, table, [n, n], 1 / math.sqrt(D), u)
+    out = hq.paged_attention(q[:1].expand(2, 16, D).contiguous(), k, v, i32([table[1], table[1]]), i32([n, n]), i32([0, 2]), i32([page]))
+    check_paged(out, q[:1].expand(2, 16, D), k, v, [table[1], table[1]], [n, n], 1 / math.sqrt(D), u)

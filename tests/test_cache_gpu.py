@@ -271,3 +271,36 @@ def test_a_search_with_forks_end_to_end(hq):
                 want = torch.softmax(x, 0) @ torch.from_numpy(b[:, h // 2]).double().cuda()
                 assert (out[s, h].double() - want).abs().max() <= 2.0 ** -9 * float(np.abs(b).max())
         parent, add = [int(p) for p in r.integers(0, rows, rows)], [1] * rows
+
+
+def test_step_that_hands_out_thousands_of_pages(hq):
+    """More than a workgroup lists in its own memory, with enough of them and without, in large and in small tables."""
+    for rows, width, pages in ((400, 30, 14000), (400, 30, 9000), (500, 32, 4096), (1024, 16, 4000), (1025, 16, 4000)):
+        page = 4
+        r = np.random.default_rng(rows + pages)
+        table, lengths, refs = random_tables(r, rows, width, page, pages, 1)
+        parent = [-1 if r.random() < 0.7 else int(r.integers(0, rows)) for _ in range(rows)]
+        add = [int(n) for n in r.integers(0, (width + 2) * page, rows)]
+        check_step(hq, 1, page, table, lengths, refs, parent, add, planes=1, elems=8)
+
+
+def test_pages_of_every_size(hq):
+    """Page sizes that are no multiple of what a workgroup copies at a time."""
+    for elems in (8, 2040, 2048, 16392, 70000):
+        r = np.random.default_rng(elems)
+        table, lengths, refs = random_tables(r, 16, 6, 16, 150, 2)
+        check_step(hq, 2, 16, table, lengths, refs, [int(p) for p in r.integers(0, 16, 16)], [1] * 16, planes=3, elems=elems)
+
+
+def test_what_one_step_leaves_the_next_one_finds(hq):
+    """A step of large tables leaves its counts at zero for the next, whatever that one's size; other operators in between."""
+    r = np.random.default_rng(9)
+    big = random_tables(r, 300, 40, 4, 9000, 10)
+    small = random_tables(r, 8, 500, 16, 5000, 2)
+    for i in range(4):
+        for (table, lengths, refs), page in ((big, 4), (small, 16)):
+            n = len(table)
+            check_step(hq, i, page, table, lengths, refs, [int(p) for p in r.integers(-1, n, n)], [3] * n, planes=1, elems=8)
+        x = torch.randn(4096, device="cuda")
+        assert hq.q3_matvec(x, torch.zeros((384, 256), dtype=torch.int32, device="cuda"), torch.ones(256, device="cuda"),
+                            torch.zeros(256, device="cuda")).abs().max() == 0
