@@ -857,6 +857,7 @@ struct PagedArgs {
   void* out;
   const int *table, *lengths, *groups, *shared;
   float *po, *pm;      // shares of the sums [batch * heads][slots][D], and {maximum, sum} [batch * heads][slots]
+  unsigned* arrived;   // not null: nothing is common, and the last of a request's and head's shares to arrive joins them
   int* np;             // said by the kernel: shares that the common keys are divided into, and of each request whether it has any
   int64_t qs;
   int ngroups, batch, width, pages, page_log, heads, kv_heads, ratio;
@@ -900,6 +901,75 @@ __device__ __forceinline__ Pages<T, D> pages_of(const PagedArgs& a, int request,
   return Pages<T, D>((const T*)a.k, (const T*)a.v, a.table + (int64_t)request * a.width, head, a.kv_heads, a.page_log, a.pages);
 }
 
+// The shares of up to 16 rows together, by one workgroup: 16 threads a row, whose loads are of two values
+// each, side by side, and the shares divided among the sets of threads that there are then.  Written by others a moment ago: read past the caches of this XCD.
+template <typename T, int D>
+__device__ __forceinline__ void join_here(const PagedArgs& a, char* sm, int nrows, int64_t row0, bool none) {
+  constexpr int N = D / 16, AT_ONCE = 4;
+  const int log = nrows > 8 ? 4 : nrows > 4 ? 3 : nrows > 2 ? 2 : nrows > 1, sets = 16 >> log;
+  const int set = threadIdx.x >> (4 + log), row = (threadIdx.x >> 4) & ((1 << log) - 1), d0 = (threadIdx.x & 15) * 2, slots = a.ns;
+  const int64_t at = row0 + min(row, nrows - 1);
+  const unsigned long long* const pm = reinterpret_cast<const unsigned long long*>(a.pm) + at * slots;
+  const unsigned long long* const po = reinterpret_cast<const unsigned long long*>(a.po + at * slots * D + d0);
+  float m = -INFINITY, l = 0.f, o[N] = {};
+  for (int s0 = set; s0 < slots; s0 += AT_ONCE * sets) {
+    unsigned long long ml[AT_ONCE], v[AT_ONCE][N / 2];
+#pragma unroll
+    for (int i = 0; i < AT_ONCE; ++i) {
+      const int s = min(s0 + i * sets, slots - 1);
+      ml[i] = __hip_atomic_load(pm + s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+#pragma unroll
+      for (int j = 0; j < N / 2; ++j) v[i][j] = __hip_atomic_load(po + (int64_t)s * (D / 2) + 16 * j, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    float top = m;
+#pragma unroll
+    for (int i = 0; i < AT_ONCE; ++i) top = fmaxf(top, __uint_as_float((uint32_t)ml[i]));
+    const float f = __builtin_amdgcn_exp2f(m - finite_or_zero(top));
+    m = top;
+    l *= f;
+#pragma unroll
+    for (int j = 0; j < N; ++j) o[j] *= f;
+#pragma unroll
+    for (int i = 0; i < AT_ONCE; ++i) {
+      const float w = s0 + i * sets < slots ? __builtin_amdgcn_exp2f(__uint_as_float((uint32_t)ml[i]) - finite_or_zero(m)) : 0.f;
+      if (w != 0.f) {  // not so for a share that no key went into
+        l += w * __uint_as_float((uint32_t)(ml[i] >> 32));
+#pragma unroll
+        for (int j = 0; j < N; ++j) o[j] += w * __uint_as_float((uint32_t)(v[i][j / 2] >> 32 * (j & 1)));
+      }
+    }
+  }
+  if (sets > 1) {
+    float* const sums = reinterpret_cast<float*>(sm) + threadIdx.x;  // N + 2 planes of a float a thread
+    sums[0] = m;
+    sums[kThreads] = l;
+#pragma unroll
+    for (int j = 0; j < N; ++j) sums[(2 + j) * kThreads] = o[j];
+    __syncthreads();
+    if (set) return;
+    const int step = 16 << log;
+    float top = m;
+    for (int s = 1; s < sets; ++s) top = fmaxf(top, sums[s * step]);
+    const float own = __builtin_amdgcn_exp2f(m - finite_or_zero(top));
+    l *= own;
+#pragma unroll
+    for (int j = 0; j < N; ++j) o[j] *= own;
+    for (int s = 1; s < sets; ++s) {
+      const float w = __builtin_amdgcn_exp2f(sums[s * step] - finite_or_zero(top));
+      l += w * sums[s * step + kThreads];
+#pragma unroll
+      for (int j = 0; j < N; ++j) o[j] += w * sums[s * step + (2 + j) * kThreads];
+    }
+  }
+  if (row >= nrows) return;
+  typedef T T2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+  for (int j = 0; j < N; j += 2)
+    *reinterpret_cast<T2*>((T*)a.out + at * D + d0 + 16 * j) = none ? T2{(T)0.f, (T)0.f} : T2{(T)(o[j] / l), (T)(o[j + 1] / l)};
+}
+
+constexpr int kApart = 16;  // counters, a line of 64 bytes each: atomics on one line wait for each other (64 shares: 17.7 us, apart 14.5)
+
 // Up to 16 rows (request, head of the group), those of requests b0 ..., all of which see the keys.
 template <typename T, int D>
 __device__ __forceinline__ void few_rows(const PagedArgs& a, char* sm, int b0, int nrows, int head, int first, int end, int slot) {
@@ -916,20 +986,38 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, char* sm, int b0, i
   float sum[D / 16], top, total;
   w.join(sum, &top, &total);
   const int mine = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * (D / 16), slots = a.most_np + a.ns;
-  if (mine > last_row) return;
+  const bool row = mine <= last_row;
   const int64_t at = (int64_t)(b0 + (uint32_t)mine / ratio) * a.heads + head * ratio + (uint32_t)mine % ratio;
+  typedef T TD __attribute__((ext_vector_type(D / 16)));
   if (slots == 1) {
-    typedef T TD __attribute__((ext_vector_type(D / 16)));
     TD v;
 #pragma unroll
     for (int i = 0; i < D / 16; ++i) v[i] = (T)(first >= end ? 0.f : sum[i] / total);
-    *reinterpret_cast<TD*>((T*)a.out + at * D + d0) = v;
-  } else {
+    if (row) *reinterpret_cast<TD*>((T*)a.out + at * D + d0) = v;
+    return;
+  }
+  float* const po = a.po + at * slots * D + d0;
+  unsigned long long* const pm = reinterpret_cast<unsigned long long*>(a.pm) + at * slots;
+  if (row) {
 #pragma unroll
     for (int i = 0; i < D / 16; i += 4)
-      *reinterpret_cast<hq_f4v*>(a.po + (at * slots + slot) * D + d0 + i) = hq_f4v{sum[i], sum[i + 1], sum[i + 2], sum[i + 3]};
-    if (d0 == 0) *reinterpret_cast<float2*>(a.pm + 2 * (at * slots + slot)) = float2{top, total};
+      hq_store_share(reinterpret_cast<hq_f4v*>(po + (int64_t)slot * D + i), hq_f4v{sum[i], sum[i + 1], sum[i + 2], sum[i + 3]});
+    if (d0 == 0)
+      __hip_atomic_store(pm + slot, (unsigned long long)__float_as_uint(total) << 32 | __float_as_uint(top), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
+  if (!a.arrived) return;
+  // The last share to arrive joins them all, and there is no second launch.  For up to 32 shares: the last one's trips grow with them
+  // (32 / 8 heads of 128; a request of 333 keys in two launches 9.4 us, in one 8.3; 4 of 8192, 16 shares, 22.0 and 20.6; 2 of 8192, 32
+  // shares, 15.9 and 15.8; one, 64 shares, 13.3 and 14.5).
+  __shared__ unsigned before;
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  unsigned* const count = a.arrived + (b0 * a.kv_heads + head) * kApart;
+  if (threadIdx.x == 0) before = __hip_atomic_fetch_add(count, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  __syncthreads();
+  if (before != (unsigned)slots - 1) return;
+  if (threadIdx.x == 0) __hip_atomic_store(count, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  join_here<T, D>(a, sm, nrows, (int64_t)b0 * a.heads + head * ratio, a.lengths[b0] <= 0);
 }
 
 // Up to 128 of them; a row sees keys up to its request's length.
@@ -1145,6 +1233,7 @@ template <typename T, int D>
 int launch_paged(PagedArgs a, int cus, hipStream_t stream) {
   const int64_t cap = (int64_t)a.width << a.page_log, rows = (int64_t)a.batch * a.heads;
   const int64_t own = (int64_t)a.batch * a.kv_heads * (a.ratio <= 16 ? 1 : (a.ratio + 127) / 128);
+  if (a.ngroups >= a.batch) a.ngroups = 0;  // groups of one, as good as: whoever shares nothing is not asked about it
   const int64_t room = a.ngroups ? cus : 2 * cus;
   a.ns = (int)std::max<int64_t>(1, std::min(room / own, (cap + 127) / 128));
   a.most_np = 0;
@@ -1157,10 +1246,12 @@ int launch_paged(PagedArgs a, int cus, hipStream_t stream) {
   const int64_t grid = prefix + own * a.ns, slots = a.most_np + a.ns;
   if (grid > INT_MAX) return HQ_ERR_TOO_LARGE;
   a.prefix_items = (int)prefix;
+  const bool alone = !a.ngroups && a.ratio <= 16 && slots <= 32;
   if (slots > 1) {
     HqWorkspace ws;
-    const int rc = hq_get_workspace(stream, (size_t)(rows * slots * (D + 2) + 1 + a.batch), 0, &ws);
+    const int rc = hq_get_workspace(stream, (size_t)(rows * slots * (D + 2) + 1 + a.batch), alone ? (size_t)own * kApart : 0, &ws);
     if (rc != HQ_OK) return rc;
+    a.arrived = alone ? ws.counters : nullptr;
     a.po = ws.partial;
     a.pm = a.po + rows * slots * D;
     a.np = reinterpret_cast<int*>(a.pm + 2 * rows * slots);
@@ -1170,7 +1261,7 @@ int launch_paged(PagedArgs a, int cus, hipStream_t stream) {
       hipFuncSetAttribute(reinterpret_cast<const void*>(&paged_kernel<T, D>), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
   if (attr != hipSuccess) return (int)attr;
   const int rc = hq_launch_as_is(paged_kernel<T, D>, dim3((unsigned)grid), dim3(kThreads), lds, stream, a);
-  if (rc != HQ_OK || slots == 1) return rc;
+  if (rc != HQ_OK || slots == 1 || alone) return rc;
   return launch_join(join_paged_kernel<T, D, 1>, join_paged_kernel<T, D, kWaves>, rows, slots, stream, a);
 }
 
