@@ -1286,7 +1286,8 @@ extern "C" int hq_prompt_attention(const void* q, const void* k, const void* v, 
   if (misaligned(q, q_stride) || misaligned(k, k_stride) || misaligned(v, v_stride) || ((uintptr_t)out & 15) ||
       (((uintptr_t)cu_q | (uintptr_t)cu_k) & 3))
     return HQ_ERR_MISALIGNED;
-  if (total_q * (heads / kv_heads) > INT_MAX - 128 || total_k > INT_MAX - 128 || k_stride > 1 << 22 || v_stride > 1 << 22)  // 32-bit offsets in a tile
+  if (total_q > INT_MAX || total_q * (heads / kv_heads) > INT_MAX - 128 || total_k > INT_MAX - 128 || k_stride > 1 << 22 ||
+      v_stride > 1 << 22)  // 32-bit offsets in a tile
     return HQ_ERR_TOO_LARGE;
   const HqDevice* dev = nullptr;
   const int rc = hq_current_device(&dev);

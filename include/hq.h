@@ -333,15 +333,16 @@ int hq_mxfp4_qdq(const void* in, void* out, int64_t n_elems, int dtype, void* st
  *   over the sequence's keys; causal != 0: over those with j <= i + (number of keys) - (number of tokens), i and j counted
  *   within the sequence.  A token that sees no key gets zeros.  A key that a token does not see has no effect on it, whatever it
  *   holds; a value that is not finite makes the results of the tokens that see it NaN.  q [total_q][heads][head_dim], rows q_stride
- *   elements apart, k and v [total_k][kv_heads][head_dim] likewise (parts of a fused projection's rows); out contiguous; all 16-byte
- *   aligned, strides multiples of 8.  Tokens of no sequence are not written.
+ *   elements apart, k and v [total_k][kv_heads][head_dim] likewise (parts of a fused projection's rows), k_stride and v_stride up to
+ *   2^22; out contiguous; all 16-byte aligned, strides multiples of 8.  Tokens of no sequence are not written.
  * hq_paged_attention: one query a request.  Token t of request s is token t % page_size of page table[s][t / page_size]
  *   (table [batch][table_width], pages [num_pages][kv_heads][page_size][head_dim], contiguous); request s sees its first lengths[s] tokens.
- *   Requests groups[g] ... groups[g+1]-1 (bounds in ascending order) have their first shared[g] tokens, as far as the first one's length reaches, in the same
- *   pages, which are read once for all of them, from the first one's row; ngroups 0: nothing is shared.  page_size a power of two, 8 ... 1024.  A table entry
- *   that is needed and no page counts as a page of zeros.  Partial sums of divided keys are in the stream's workspace.
+ *   Requests groups[g] ... groups[g+1]-1 (bounds in ascending order) have their first shared[g] tokens, as far as the first one's
+ *   length reaches, in the same pages, which are read once for all of them, from the first one's row (every row of the table lists
+ *   them); ngroups 0: nothing is shared.  page_size a power of two, 8 ... 1024.  A table entry that is needed and no page counts as
+ *   a page of zeros.
  * hq_cache_write: tokens cu[s] ... cu[s+1]-1 of k and v [tokens][kv_heads][head_dim] (strides as above) become tokens starts[s], ... of row s
- *   of the table.  A token whose place is outside its row, or in no page, is left out.
+ *   of the table; any head_dim that is a multiple of 8, any page_size.  A token whose place is outside its row, or in no page, is left out.
  * hq_cache_step: from the tables of one step to the next one's.  Row s inherits row parent[s] (of the old tables; any number outside
  *   0 ... rows-1: nothing) and gets room for add[s] tokens (negative: none) as far as its table_width pages reach.  Whole pages are
  *   shared; a half-filled one stays with the first row that inherits it and is copied, all page_bytes of it in every one of the
@@ -352,7 +353,8 @@ int hq_mxfp4_qdq(const void* in, void* out, int64_t n_elems, int dtype, void* st
  *   are -1.  Outputs share no memory with inputs (HQ_ERR_BAD_SHAPE).  rows <= 16384.
  * hq_cache_compact: n pages are in use (refs > 0); those at n and beyond move, in order, into the free ones below n, in every plane;
  *   table_out and refs_out follow, *live = n.
- * The last two and hq_paged_attention use the stream's workspace: before a stream is captured, run the largest call once.
+ * All but hq_cache_write may use the stream's workspace (partial sums of divided keys, arrival counters, plans of large tables): before
+ * a stream is captured, run the largest call on it once, or reserve.
  */
 int hq_prompt_attention(const void* q, const void* k, const void* v, void* out, int dtype, const int32_t* cu_q, const int32_t* cu_k, int seqs,
                         int64_t total_q, int64_t total_k, int heads, int kv_heads, int head_dim, int64_t q_stride, int64_t k_stride,

@@ -378,3 +378,60 @@ def test_paged_beyond_32_bits(hq):
     check_paged(out, q, k, v, table, [n, n], 1 / math.sqrt(D), u)
     out = hq.paged_attention(q[:1].expand(2, 16, D).contiguous(), k, v, i32([table[1], table[1]]), i32([n, n]), i32([0, 2]), i32([page]))
     check_paged(out, q[:1].expand(2, 16, D), k, v, [table[1], table[1]], [n, n], 1 / math.sqrt(D), u)
+
+
+@pytest.mark.parametrize("kind,D", [("bf16", 128), ("f16", 64)])
+@pytest.mark.parametrize("heads", [(1, 1), (4, 2), (10, 2), (16, 1), (17, 1)])
+def test_paged_shares_joined_here_and_in_a_second_launch(hq, kind, D, heads):
+    """1 to 64 shares a row, full and without a key, each call twice and on counters that the call before left."""
+    dtype, u = TYPES[kind]
+    for n, lengths in enumerate([[300], [1500, 2], [4000], [4100, 0, 129], [9000], [130] * 40, [513] * 9]):
+        q, k, v, table, lengths = paged_case(20 + n, dtype, lengths, heads, D, 16)
+        out = hq.paged_attention(q, k, v, i32(table), i32(lengths))
+        check_paged(out, q, k, v, table, lengths, 1 / math.sqrt(D), u)
+        assert torch.equal(out, hq.paged_attention(q, k, v, i32(table), i32(lengths)))
+
+
+def test_paged_shares_joined_in_a_graph(hq):
+    dtype, u = TYPES["bf16"]
+    q, k, v, table, lengths = paged_case(5, dtype, [2900, 950, 20], (8, 2), 128, 16)
+    args = (q, k, v, i32(table), i32(lengths))
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        hq.paged_attention(*args)
+    s.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=s):
+        got = hq.paged_attention(*args)
+        again = hq.paged_attention(*args)
+    for i in range(4):
+        got.zero_()
+        again.zero_()
+        q.copy_(randn(50 + i, *q.shape))
+        args[4].copy_(i32([2900 - 700 * i, 950 * (i % 2), 20 + i]))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        want = hq.paged_attention(*args)  # NaN where a request is longer than its tokens
+        for x in (got, again):
+            torch.testing.assert_close(x, want, rtol=0, atol=0, equal_nan=True)
+
+
+def test_paged_as_many_groups_as_requests(hq):
+    """Some of them empty, the keys of another common."""
+    dtype, u = TYPES["bf16"]
+    groups, shared = [0, 3, 3, 3], [992, 16, 5]
+    q, k, v, table, lengths = paged_case(31, dtype, [1000, 1100, 999], (8, 2), 128, 16, groups, shared)
+    out = hq.paged_attention(q, k, v, i32(table), i32(lengths), i32(groups), i32(shared))
+    check_paged(out, q, k, v, table, lengths, 1 / math.sqrt(128), u)
+
+
+def test_paged_infinite_scores_in_one_share(hq):
+    """One key of an infinite score among 1000: the row is NaN, whichever share holds it, and the other rows are not touched."""
+    dtype, u = TYPES["bf16"]
+    for at in (0, 200, 999):
+        q, k, v, table, lengths = paged_case(41, dtype, [1000, 1000], (8, 2), 128, 16)
+        k[table[0][at // 16], 1, at % 16] = math.inf
+        q[0, 4:].abs_()
+        out = hq.paged_attention(q, k, v, i32(table), i32(lengths))
+        assert torch.isnan(out[0, 4:]).all() and torch.isfinite(out[0, :4]).all() and torch.isfinite(out[1]).all()

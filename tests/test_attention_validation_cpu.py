@@ -138,3 +138,14 @@ def test_entry_points():
 
     assert compact(live=None) == -1 and compact(pool=None) == -1 and compact(to=1 << 20) == -2 and compact(ro=(3 << 20) + 4) == -2
     assert compact(bytes=8) == -2 and compact(pool=4) == -4
+
+
+def test_entry_points_at_their_limits():
+    """A product of sizes that passes 64 bits, and strides whose offsets within a tile would pass 32."""
+    lib = _lib.load()
+
+    def prompt(tq=4, tk=4, ks=128, vs=128):
+        return lib.hq_prompt_attention(16, 16, 16, 16, 1, 16, 16, 1, tq, tk, 8, 2, 64, 512, ks, vs, 0.1, 1, None)
+
+    assert prompt(tq=2 ** 62) == -6 and prompt(tq=2 ** 29) == -6 and prompt(tk=2 ** 31) == -6
+    assert prompt(ks=2 ** 22 + 8) == -6 and prompt(vs=2 ** 40) == -6

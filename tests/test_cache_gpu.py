@@ -304,3 +304,36 @@ def test_what_one_step_leaves_the_next_one_finds(hq):
         x = torch.randn(4096, device="cuda")
         assert hq.q3_matvec(x, torch.zeros((384, 256), dtype=torch.int32, device="cuda"), torch.ones(256, device="cuda"),
                             torch.zeros(256, device="cuda")).abs().max() == 0
+
+
+def test_large_tables_on_another_stream_and_in_a_graph(hq):
+    """The ways of more than one launch, which keep counters between calls."""
+    r = np.random.default_rng(8)
+    rows, pages = 1100, 7000
+    table, lengths, refs = random_tables(r, rows, 4, 16, pages, 2)
+    args = [i32(table), i32(lengths), i32(refs), i32(r.integers(-1, rows, rows)), i32([1] * rows)]
+    s = torch.cuda.Stream()
+    for call in (lambda p: hq.cache_step(p, 16, *args), lambda p: hq.cache_compact(p, args[0], args[2])):
+        pool = pool_of(4, 1, pages, 16)
+        wpool = pool.clone()
+        want = call(wpool)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(s):
+            mine = pool.clone()
+            got = call(mine)
+        s.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want)) and torch.equal(mine, wpool)
+        graph = torch.cuda.CUDAGraph()
+        static = pool.clone()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph, stream=s):
+            got = call(static)
+        for i in range(3):
+            args[3].copy_(i32(np.random.default_rng(i).integers(-1, rows, rows)))
+            fresh = pool_of(5 + i, 1, pages, 16)
+            static.copy_(fresh)
+            torch.cuda.synchronize()
+            graph.replay()
+            torch.cuda.synchronize()
+            want = call(fresh)
+            assert all(torch.equal(a, b) for a, b in zip(got, want)) and torch.equal(static, fresh)
