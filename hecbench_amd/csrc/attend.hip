@@ -856,12 +856,14 @@ struct PagedArgs {
   const void *q, *k, *v;
   void* out;
   const int *table, *lengths, *groups, *shared;
-  float *po, *pm;      // shares of the sums [batch * heads][slots][D], and {maximum, sum} [batch * heads][slots]
+  float *po, *pm;      // a place for each share of each row: its sums [D]; and its {maximum, sum}
   unsigned* arrived;   // not null: nothing is common, and the last of a request's and head's shares to arrive joins them
-  int* np;             // said by the kernel: shares that the common keys are divided into, and of each request whether it has any
+  int* np;             // said by the kernel: shares that the common keys are divided into, and of each request whether it has any; without
+                       // groups, the first of each request's shares, and how many
   int64_t qs;
   int ngroups, batch, width, pages, page_log, heads, kv_heads, ratio;
-  int most_np, ns;     // at most; shares of a request's own keys
+  int most_np, ns;     // at most; shares of a request's own keys; without groups, 0: by their number
+  int per_row, items;  // places from a row's to the next one's; without groups, shares of all requests, at most
   int prefix_items;    // workgroups of the common keys
   float c;
 };
@@ -896,6 +898,63 @@ __device__ __forceinline__ void share_of(int n, int shares, int least, int s, in
   *end = min(*first + each, n);
 }
 
+// Sums of whole numbers over the wave, and over the lanes up to each.
+struct AddWhole {
+  __device__ __forceinline__ float operator()(float x, float y) const { return __uint_as_float(__float_as_uint(x) + __float_as_uint(y)); }
+};
+__device__ __forceinline__ unsigned wave_sum(unsigned v) { return __float_as_uint(hq_wave(__uint_as_float(v), AddWhole())); }
+__device__ __forceinline__ unsigned running_sum(unsigned v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr:1, 2, 4, 8: within the rows of 16
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast:15 into rows 1 and 3, :31 into rows 2 and 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
+  return v;
+}
+
+// Share x of the requests' keys, all of one size: the smallest multiple of 128 of which there are no more shares than a.items, one a
+// request at least.  Lengths differ, and a share is a workgroup's work (32 requests of up to 4000, two equal shares each: 62.0 us, 57.2
+// so; 16 of up to 1000: 13.0 and 12.4).  Runs of equal length, whoever's the keys are, are better still for such (56.4), but a workgroup that goes on to the next request
+// waits for it (8 of up to 2000: 12.1 us, in runs 13.7).  A request a lane; one request, and more than 64, in a.ns equal shares each.
+constexpr int kUnit = 128;
+struct Share {
+  int b, first, end, before, count;  // request; keys; shares of the requests before it, and of it
+  // false: there is no such share
+  __device__ __forceinline__ bool find(const PagedArgs& a, unsigned x, bool says) {
+    const int lane = threadIdx.x & 63, cap = a.width << a.page_log;
+    if (a.ns) {
+      b = x / (uint32_t)a.ns;
+      before = b * a.ns;
+      count = a.ns;
+      share_of(min(max(a.lengths[b], 0), cap), a.ns, kUnit, x - before, &first, &end);
+      return true;
+    }
+    const int n = min(max(a.lengths[min(lane, a.batch - 1)], 0), cap);
+    const unsigned units = lane < a.batch ? max((unsigned)(n + kUnit - 1) / kUnit, 1u) : 0, items = a.items;
+    unsigned each = 1, own = units, all = wave_sum(units);
+    while (all > items) {  // ends where the longest request is one share
+      each += max(1u, (unsigned)((float)each * (float)(all - items) / (float)items));
+      // as many as hold them all; one too many, and without a key, where the quotient is a whole number but for its rounding
+      own = lane < a.batch ? (unsigned)((float)(units - 1) * (__builtin_amdgcn_rcpf((float)each) * 1.000001f)) + 1 : 0;
+      all = wave_sum(own);
+    }
+    if (x >= all) return false;
+    const unsigned to = running_sum(own);
+    if (says && lane < a.batch) {
+      a.np[2 * lane] = to - own;
+      a.np[2 * lane + 1] = own;
+    }
+    b = __ffsll(__ballot(to > x)) - 1;
+    const int keys = __builtin_amdgcn_readlane(n, b);
+    count = __builtin_amdgcn_readlane(own, b);
+    before = __builtin_amdgcn_readlane(to, b) - count;
+    first = (int)min((int64_t)(x - before) * each * kUnit, (int64_t)keys);
+    end = (int)min((int64_t)(x - before + 1) * each * kUnit, (int64_t)keys);
+    return true;
+  }
+};
+
 template <typename T, int D>
 __device__ __forceinline__ Pages<T, D> pages_of(const PagedArgs& a, int request, int head) {
   return Pages<T, D>((const T*)a.k, (const T*)a.v, a.table + (int64_t)request * a.width, head, a.kv_heads, a.page_log, a.pages);
@@ -904,22 +963,22 @@ __device__ __forceinline__ Pages<T, D> pages_of(const PagedArgs& a, int request,
 // The shares of up to 16 rows together, by one workgroup: 16 threads a row, whose loads are of two values
 // each, side by side, and the shares divided among the sets of threads that there are then.  Written by others a moment ago: read past the caches of this XCD.
 template <typename T, int D>
-__device__ __forceinline__ void join_here(const PagedArgs& a, char* sm, int nrows, int64_t row0, bool none) {
+__device__ __forceinline__ void join_here(const PagedArgs& a, char* sm, int nrows, int64_t row0, int64_t place, int slots, bool none) {
   constexpr int N = D / 16, AT_ONCE = 4;
   const int log = nrows > 8 ? 4 : nrows > 4 ? 3 : nrows > 2 ? 2 : nrows > 1, sets = 16 >> log;
-  const int set = threadIdx.x >> (4 + log), row = (threadIdx.x >> 4) & ((1 << log) - 1), d0 = (threadIdx.x & 15) * 2, slots = a.ns;
+  const int set = threadIdx.x >> (4 + log), row = (threadIdx.x >> 4) & ((1 << log) - 1), d0 = (threadIdx.x & 15) * 2;
   const int64_t at = row0 + min(row, nrows - 1);
-  const unsigned long long* const pm = reinterpret_cast<const unsigned long long*>(a.pm) + at * slots;
-  const unsigned long long* const po = reinterpret_cast<const unsigned long long*>(a.po + at * slots * D + d0);
+  const unsigned long long* const pm = reinterpret_cast<const unsigned long long*>(a.pm) + at + place;
+  const unsigned long long* const po = reinterpret_cast<const unsigned long long*>(a.po + (at + place) * D + d0);
   float m = -INFINITY, l = 0.f, o[N] = {};
   for (int s0 = set; s0 < slots; s0 += AT_ONCE * sets) {
     unsigned long long ml[AT_ONCE], v[AT_ONCE][N / 2];
 #pragma unroll
     for (int i = 0; i < AT_ONCE; ++i) {
       const int s = min(s0 + i * sets, slots - 1);
-      ml[i] = __hip_atomic_load(pm + s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      ml[i] = __hip_atomic_load(pm + (int64_t)s * a.heads, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 #pragma unroll
-      for (int j = 0; j < N / 2; ++j) v[i][j] = __hip_atomic_load(po + (int64_t)s * (D / 2) + 16 * j, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      for (int j = 0; j < N / 2; ++j) v[i][j] = __hip_atomic_load(po + (int64_t)s * a.heads * (D / 2) + 16 * j, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
     float top = m;
 #pragma unroll
@@ -972,7 +1031,8 @@ constexpr int kApart = 16;  // counters, a line of 64 bytes each: atomics on one
 
 // Up to 16 rows (request, head of the group), those of requests b0 ..., all of which see the keys.
 template <typename T, int D>
-__device__ __forceinline__ void few_rows(const PagedArgs& a, char* sm, int b0, int nrows, int head, int first, int end, int slot) {
+__device__ __forceinline__ void few_rows(const PagedArgs& a, char* sm, int b0, int nrows, int head, int first, int end, int64_t slot,
+                                         int shares, int before) {
   typedef typename Kind<T>::V8 V8;
   const int lane = threadIdx.x & 63, last_row = nrows - 1, r = min(lane & 15, last_row);
   const uint32_t ratio = a.ratio;
@@ -985,45 +1045,45 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, char* sm, int b0, i
   w.run(pages_of<T, D>(a, b0, head), first, end, a.c);
   float sum[D / 16], top, total;
   w.join(sum, &top, &total);
-  const int mine = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * (D / 16), slots = a.most_np + a.ns;
+  const int mine = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * (D / 16);
   const bool row = mine <= last_row;
   const int64_t at = (int64_t)(b0 + (uint32_t)mine / ratio) * a.heads + head * ratio + (uint32_t)mine % ratio;
   typedef T TD __attribute__((ext_vector_type(D / 16)));
-  if (slots == 1) {
+  if (shares == 1) {
     TD v;
 #pragma unroll
     for (int i = 0; i < D / 16; ++i) v[i] = (T)(first >= end ? 0.f : sum[i] / total);
     if (row) *reinterpret_cast<TD*>((T*)a.out + at * D + d0) = v;
     return;
   }
-  float* const po = a.po + at * slots * D + d0;
-  unsigned long long* const pm = reinterpret_cast<unsigned long long*>(a.pm) + at * slots;
   if (row) {
+    const int64_t place = at * a.per_row + slot;
 #pragma unroll
     for (int i = 0; i < D / 16; i += 4)
-      hq_store_share(reinterpret_cast<hq_f4v*>(po + (int64_t)slot * D + i), hq_f4v{sum[i], sum[i + 1], sum[i + 2], sum[i + 3]});
+      hq_store_share(reinterpret_cast<hq_f4v*>(a.po + place * D + d0 + i), hq_f4v{sum[i], sum[i + 1], sum[i + 2], sum[i + 3]});
     if (d0 == 0)
-      __hip_atomic_store(pm + slot, (unsigned long long)__float_as_uint(total) << 32 | __float_as_uint(top), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      __hip_atomic_store(reinterpret_cast<unsigned long long*>(a.pm) + place, (unsigned long long)__float_as_uint(total) << 32 | __float_as_uint(top),
+                         __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
   if (!a.arrived) return;
   // The last share to arrive joins them all, and there is no second launch.  For up to 32 shares: the last one's trips grow with them
   // (32 / 8 heads of 128; a request of 333 keys in two launches 9.4 us, in one 8.3; 4 of 8192, 16 shares, 22.0 and 20.6; 2 of 8192, 32
   // shares, 15.9 and 15.8; one, 64 shares, 13.3 and 14.5).
-  __shared__ unsigned before;
+  __shared__ unsigned nth;
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
   unsigned* const count = a.arrived + (b0 * a.kv_heads + head) * kApart;
-  if (threadIdx.x == 0) before = __hip_atomic_fetch_add(count, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  if (threadIdx.x == 0) nth = __hip_atomic_fetch_add(count, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   __syncthreads();
-  if (before != (unsigned)slots - 1) return;
+  if (nth != (unsigned)shares - 1) return;
   if (threadIdx.x == 0) __hip_atomic_store(count, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  join_here<T, D>(a, sm, nrows, (int64_t)b0 * a.heads + head * ratio, a.lengths[b0] <= 0);
+  join_here<T, D>(a, sm, nrows, (int64_t)b0 * a.heads + head * ratio, (int64_t)(before - b0) * a.heads, shares, a.lengths[b0] <= 0);
 }
 
 // Up to 128 of them; a row sees keys up to its request's length.
 template <typename T, int D>
 __device__ __forceinline__ void many_rows(const PagedArgs& a, char* sm, int* poison, int b0, int nrows, int first_row, int head, int first, int end,
-                                          int slot) {
+                                          int64_t slot, int shares) {
   typedef typename Kind<T>::V8 V8;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int last_row = min(first_row + 128, nrows) - 1, row = first_row + wave * 32 + (lane & 31), r = min(row, last_row);
@@ -1046,10 +1106,23 @@ __device__ __forceinline__ void many_rows(const PagedArgs& a, char* sm, int* poi
   PagedTiles<T, D> src(pages_of<T, D>(a, b0, head), end);
   w.run(src, first, end, uniform(whole), a.c);
   if (row > last_row) return;
-  const int slots = a.most_np + a.ns;
   const int64_t at = (int64_t)b * a.heads + h;
-  if (slots == 1) w.put((T*)a.out + at * D, w.lim == 0);
-  else w.put_share(a.po, a.pm, at * slots + slot, false);
+  if (shares == 1) w.put((T*)a.out + at * D, w.lim == 0);
+  else w.put_share(a.po, a.pm, at * a.per_row + slot, false);
+}
+
+// Nothing is common: a share a workgroup.
+template <typename T, int D, bool FEW>
+__global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void paged_alone_kernel(PagedArgs a) {
+  extern __shared__ __align__(16) char sm[];
+  __shared__ int poison;
+  const uint32_t x = blockIdx.x, y = x / (uint32_t)a.kv_heads, item = y % (uint32_t)a.items;
+  const int head = x % (uint32_t)a.kv_heads, row0 = y / (uint32_t)a.items * 128;
+  Share s;
+  if (!s.find(a, item, x == 0 && threadIdx.x < 64 && a.np)) return;
+  const int64_t place = ((int64_t)item - s.b) * a.heads;
+  if (FEW) few_rows<T, D>(a, sm, s.b, a.ratio, head, s.first, s.end, place, s.count, s.before);
+  else many_rows<T, D>(a, sm, &poison, s.b, a.ratio, row0, head, s.first, s.end, place, s.count);
 }
 
 template <typename T, int D>
@@ -1063,17 +1136,9 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void paged_kernel(PagedA
     // The common keys: as many shares as there are workgroups for the tiles of rows that there are.
     const int ratio = a.ratio, lane = threadIdx.x & 63;
     auto tiles = [=](const Groups& g) { return (int)(((int64_t)g.count * ratio + 127) / 128); };
-    auto running = [=](int v) {  // sums over the lanes up to each
-#pragma unroll
-      for (int d = 1; d < 64; d <<= 1) {
-        const int u = __shfl_up(v, d);
-        if (lane >= d) v += u;
-      }
-      return v;
-    };
     const Groups some(a, 0);
-    int all = __builtin_amdgcn_readlane(running(tiles(some)), 63);
-    for (int g0 = 64; g0 < a.ngroups; g0 += 64) all += __builtin_amdgcn_readlane(running(tiles(Groups(a, g0))), 63);
+    int all = __builtin_amdgcn_readlane((int)running_sum(tiles(some)), 63);
+    for (int g0 = 64; g0 < a.ngroups; g0 += 64) all += __builtin_amdgcn_readlane((int)running_sum(tiles(Groups(a, g0))), 63);
     const int np = all ? min(max(a.prefix_items / (all * a.kv_heads), 1), a.most_np) : 0;
     if (x == 0 && threadIdx.x == 0) *a.np = np;
     if (np == 0) return;
@@ -1086,7 +1151,7 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void paged_kernel(PagedA
     nb = 0;
     for (int g0 = 0; nb == 0; g0 += 64) {
       const Groups g = g0 ? Groups(a, g0) : some;
-      const int own = tiles(g), sum = running(own), total = __builtin_amdgcn_readlane(sum, 63);
+      const int own = tiles(g), sum = (int)running_sum(own), total = __builtin_amdgcn_readlane(sum, 63);
       if (tile < total) {
         const int at = __ffsll(__ballot(sum > tile)) - 1;
         b0 = __builtin_amdgcn_readlane(g.begin, at);
@@ -1109,29 +1174,30 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void paged_kernel(PagedA
     const int tiles = few ? 1 : (a.ratio + 127) / 128, tile = few ? 0 : x % (uint32_t)tiles;
     b0 = few ? x : x / (uint32_t)tiles;
     const int n = min(max(a.lengths[b0], 0), a.width << a.page_log), shared = shared_of(a, b0), from = uniform(min(max(shared, 0), n));
-    if (head == 0 && share == 0 && tile == 0 && threadIdx.x == 0 && a.np) a.np[1 + b0] = shared >= 0;
+    if (head == 0 && share == 0 && tile == 0 && threadIdx.x == 0) a.np[1 + b0] = shared >= 0;
     share_of(n - from, a.ns, 128, share, &first, &end);
     first += from;
     end += from;
     row0 = tile * 128;
     slot = a.most_np + share;
   }
-  if (few) few_rows<T, D>(a, sm, b0, nb * a.ratio, head, first, end, slot);
-  else many_rows<T, D>(a, sm, &poison, b0, nb * a.ratio, row0, head, first, end, slot);
+  if (few) few_rows<T, D>(a, sm, b0, nb * a.ratio, head, first, end, slot, 0, 0);
+  else many_rows<T, D>(a, sm, &poison, b0, nb * a.ratio, row0, head, first, end, slot, 0);
 }
 
 // The shares of a row together, by WAVES waves: their maxima and sums a lane each, then the sums of the values, 16 bytes a lane, several
 // shares at a time; a wave takes every WAVES-th group of them.  Of the shares, those from `np` to `own` were not written.  Bound by two
 // trips to memory, one behind the other.
 template <typename T, int D, int WAVES>
-__device__ __forceinline__ void join_shares(const float* po, const float* pm, int64_t row, int np, int own, int slots, bool none, T* out) {
+__device__ __forceinline__ void join_shares(const float* po, const float* pm, int64_t row, int64_t place, int step, int np, int own, int slots, bool none,
+                                            T* out) {
   constexpr int LANES = D / 4, AT_ONCE = 64 / LANES;  // lanes of a share, shares of a load
   const int lane = threadIdx.x & 63, d = (lane % LANES) * 4, wave = WAVES == 1 ? 0 : threadIdx.x >> 6;
-  const float2* ml = reinterpret_cast<const float2*>(pm) + row * slots;
-  const float2 ahead = ml[min(lane, slots - 1)];  // under way before np is known
+  const float2* ml = reinterpret_cast<const float2*>(pm) + place;
+  const float2 ahead = ml[(int64_t)min(lane, slots - 1) * step];  // under way before np is known
   auto share = [&](int s0) {
     const int s = s0 + lane;
-    const float2 x = s0 ? ml[min(s, slots - 1)] : ahead;
+    const float2 x = s0 ? ml[(int64_t)min(s, slots - 1) * step] : ahead;
     return s < np || (s >= own && s < slots) ? x : float2{-INFINITY, 0.f};
   };
   float m = -INFINITY;
@@ -1150,7 +1216,7 @@ __device__ __forceinline__ void join_shares(const float* po, const float* pm, in
       const int at = i + lane / LANES;
       const float w = __shfl(f, at & 63);
       // a share that no key went into has weight 0, and nothing was written for it
-      if (at < here && w != 0.f) o += *reinterpret_cast<const hq_f4v*>(po + (row * slots + s0 + at) * D + d) * w;
+      if (at < here && w != 0.f) o += *reinterpret_cast<const hq_f4v*>(po + (place + (int64_t)(s0 + at) * step) * D + d) * w;
     }
   }
   l = hq_wave_sum(l);
@@ -1182,8 +1248,14 @@ template <typename T, int D, int WAVES>
 __global__ __launch_bounds__(kThreads) void join_paged_kernel(PagedArgs a) {
   const int64_t row = WAVES > 1 ? blockIdx.x : (int64_t)blockIdx.x * kWaves + (threadIdx.x >> 6);
   if (row >= (int64_t)a.batch * a.heads) return;
-  const int b = row / a.heads, np = a.np[1 + b] ? a.np[0] : 0;
-  join_shares<T, D, WAVES>(a.po, a.pm, row, np, a.most_np, a.most_np + a.ns, a.lengths[b] <= 0, (T*)a.out);
+  const int b = row / a.heads, slots = a.most_np + a.ns;
+  if (a.ngroups) {
+    const int np = a.np[1 + b] ? a.np[0] : 0;
+    join_shares<T, D, WAVES>(a.po, a.pm, row, row * slots, 1, np, a.most_np, slots, a.lengths[b] <= 0, (T*)a.out);
+  } else {
+    const int before = a.ns ? b * a.ns : a.np[2 * b], count = a.ns ? a.ns : a.np[2 * b + 1];
+    if (count > 1) join_shares<T, D, WAVES>(a.po, a.pm, row, row + (int64_t)(before - b) * a.heads, a.heads, count, count, count, a.lengths[b] <= 0, (T*)a.out);
+  }
 }
 
 template <typename T, int D, int WAVES>
@@ -1193,7 +1265,7 @@ __global__ __launch_bounds__(kThreads) void join_prompt_kernel(PromptArgs a) {
   const int token = row / a.heads;
   if (token < a.cu_q[0] || token >= a.cu_q[a.seqs]) return;
   const float2 first = reinterpret_cast<const float2*>(a.pm)[row * a.shares];
-  join_shares<T, D, WAVES>(a.po, a.pm, row, 0, 0, a.shares, first.x == INFINITY && first.y == 0.f, (T*)a.out);
+  join_shares<T, D, WAVES>(a.po, a.pm, row, row * a.shares, 1, 0, 0, a.shares, first.x == INFINITY && first.y == 0.f, (T*)a.out);
 }
 template <typename A>
 int launch_join(void (*by_waves)(A), void (*by_workgroups)(A), int64_t rows, int64_t slots, hipStream_t stream, const A& a) {
@@ -1231,37 +1303,45 @@ int launch_prompt(PromptArgs a, int cus, hipStream_t stream) {
 // Half of the workgroups that the device holds at once for the common keys, and the requests' own keys divided until they fill the rest.
 template <typename T, int D>
 int launch_paged(PagedArgs a, int cus, hipStream_t stream) {
-  const int64_t cap = (int64_t)a.width << a.page_log, rows = (int64_t)a.batch * a.heads;
-  const int64_t own = (int64_t)a.batch * a.kv_heads * (a.ratio <= 16 ? 1 : (a.ratio + 127) / 128);
+  const int64_t cap = (int64_t)a.width << a.page_log, rows = (int64_t)a.batch * a.heads, tiles = a.ratio <= 16 ? 1 : (a.ratio + 127) / 128;
+  const int64_t own = (int64_t)a.batch * a.kv_heads * tiles;
   if (a.ngroups >= a.batch) a.ngroups = 0;  // groups of one, as good as: whoever shares nothing is not asked about it
-  const int64_t room = a.ngroups ? cus : 2 * cus;
-  a.ns = (int)std::max<int64_t>(1, std::min(room / own, (cap + 127) / 128));
-  a.most_np = 0;
-  int64_t prefix = 0;
+  int64_t prefix = 0, grid, slots, places;
+  bool alone = false;
   if (a.ngroups) {
-    const int64_t tiles = (int64_t)a.batch * a.ratio / 128 + a.ngroups;  // at most
-    prefix = std::max<int64_t>(cus, tiles * a.kv_heads);
+    const int64_t most_tiles = (int64_t)a.batch * a.ratio / 128 + a.ngroups;
+    prefix = std::max<int64_t>(cus, most_tiles * a.kv_heads);
     a.most_np = (int)std::max<int64_t>(1, std::min<int64_t>(cus / a.kv_heads, (cap + 255) / 256));
+    a.ns = (int)std::max<int64_t>(1, std::min(cus / own, (cap + 127) / 128));
+    grid = prefix + own * a.ns;
+    slots = a.per_row = a.most_np + a.ns;
+    places = rows * slots;
+  } else {
+    a.per_row = 1;
+    const int64_t most = a.batch * std::max<int64_t>(1, (cap + kUnit - 1) / kUnit), room = 2 * (int64_t)cus / (a.kv_heads * tiles);
+    if (a.batch == 1 || a.batch > 64 || a.batch >= room || a.batch == most) a.ns = (int)std::max<int64_t>(1, std::min(room, most) / a.batch);
+    a.items = (int)(a.ns ? (int64_t)a.ns * a.batch : std::min(room, most));
+    grid = (int64_t)a.items * a.kv_heads * tiles;
+    places = a.ns == 1 ? 0 : (int64_t)a.items * a.heads;
+    slots = a.items / a.batch;
+    alone = a.ratio <= 16 && slots <= 32;
   }
-  const int64_t grid = prefix + own * a.ns, slots = a.most_np + a.ns;
   if (grid > INT_MAX) return HQ_ERR_TOO_LARGE;
   a.prefix_items = (int)prefix;
-  const bool alone = !a.ngroups && a.ratio <= 16 && slots <= 32;
-  if (slots > 1) {
+  if (places) {
     HqWorkspace ws;
-    const int rc = hq_get_workspace(stream, (size_t)(rows * slots * (D + 2) + 1 + a.batch), alone ? (size_t)own * kApart : 0, &ws);
+    const int rc = hq_get_workspace(stream, (size_t)(places * (D + 2) + 1 + 2 * (int64_t)a.batch), alone ? (size_t)own * kApart : 0, &ws);
     if (rc != HQ_OK) return rc;
     a.arrived = alone ? ws.counters : nullptr;
     a.po = ws.partial;
-    a.pm = a.po + rows * slots * D;
-    a.np = reinterpret_cast<int*>(a.pm + 2 * rows * slots);
+    a.pm = a.po + places * D;
+    a.np = alone ? nullptr : reinterpret_cast<int*>(a.pm + 2 * places);
   }
+  void (*const kernel)(PagedArgs) = a.ngroups ? paged_kernel<T, D> : tiles == 1 && a.ratio <= 16 ? paged_alone_kernel<T, D, true> : paged_alone_kernel<T, D, false>;
   constexpr int lds = std::max(Many<T, D>::LDS, Few<T, D>::LDS);
-  static const hipError_t attr =
-      hipFuncSetAttribute(reinterpret_cast<const void*>(&paged_kernel<T, D>), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-  if (attr != hipSuccess) return (int)attr;
-  const int rc = hq_launch_as_is(paged_kernel<T, D>, dim3((unsigned)grid), dim3(kThreads), lds, stream, a);
-  if (rc != HQ_OK || slots == 1 || alone) return rc;
+  static_assert(lds <= 65536, "no attribute to set");
+  const int rc = hq_launch_as_is(kernel, dim3((unsigned)grid), dim3(kThreads), lds, stream, a);
+  if (rc != HQ_OK || !places || alone) return rc;
   return launch_join(join_paged_kernel<T, D, 1>, join_paged_kernel<T, D, kWaves>, rows, slots, stream, a);
 }
 
