@@ -1300,7 +1300,9 @@ int launch_prompt(PromptArgs a, int cus, hipStream_t stream) {
   return launch_join(join_prompt_kernel<T, D, 1>, join_prompt_kernel<T, D, kWaves>, rows, a.shares, stream, a);
 }
 
-// Half of the workgroups that the device holds at once for the common keys, and the requests' own keys divided until they fill the rest.
+// Common keys: a workgroup a compute unit for them, two for heads of 64, and the requests' own keys divided until they fill as many (64
+// requests in 4 groups behind 15000 keys, 32 / 8 heads, own up to 500: heads of 128 72.9 us, with two 78.1; of 64 50.0, with two 43.2).
+// Nothing common: two workgroups a compute unit, of shares by length (Share).
 template <typename T, int D>
 int launch_paged(PagedArgs a, int cus, hipStream_t stream) {
   const int64_t cap = (int64_t)a.width << a.page_log, rows = (int64_t)a.batch * a.heads, tiles = a.ratio <= 16 ? 1 : (a.ratio + 127) / 128;
@@ -1310,8 +1312,9 @@ int launch_paged(PagedArgs a, int cus, hipStream_t stream) {
   bool alone = false;
   if (a.ngroups) {
     const int64_t most_tiles = (int64_t)a.batch * a.ratio / 128 + a.ngroups;
-    prefix = std::max<int64_t>(cus, most_tiles * a.kv_heads);
-    a.most_np = (int)std::max<int64_t>(1, std::min<int64_t>(cus / a.kv_heads, (cap + 255) / 256));
+    const int64_t common = D == 64 ? 2 * cus : cus;
+    prefix = std::max<int64_t>(common, most_tiles * a.kv_heads);
+    a.most_np = (int)std::max<int64_t>(1, std::min<int64_t>(common / a.kv_heads, (cap + 255) / 256));
     a.ns = (int)std::max<int64_t>(1, std::min(cus / own, (cap + 127) / 128));
     grid = prefix + own * a.ns;
     slots = a.per_row = a.most_np + a.ns;
