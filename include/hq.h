@@ -354,7 +354,7 @@ int hq_mxfp4_qdq(const void* in, void* out, int64_t n_elems, int dtype, void* st
  * hq_cache_compact: n pages are in use (refs > 0); those at n and beyond move, in order, into the free ones below n, in every plane;
  *   table_out and refs_out follow, *live = n.
  * All but hq_cache_write may use the stream's workspace (partial sums of divided keys, arrival counters, plans of large tables): before
- * a stream is captured, run the largest call on it once, or reserve.
+ * a stream is captured, run the largest call on it once (hq_reserve_workspace counts the products' needs only).
  */
 int hq_prompt_attention(const void* q, const void* k, const void* v, void* out, int dtype, const int32_t* cu_q, const int32_t* cu_k, int seqs,
                         int64_t total_q, int64_t total_k, int heads, int kv_heads, int head_dim, int64_t q_stride, int64_t k_stride,
