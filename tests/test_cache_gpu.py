@@ -337,3 +337,22 @@ def test_large_tables_on_another_stream_and_in_a_graph(hq):
             torch.cuda.synchronize()
             want = call(fresh)
             assert all(torch.equal(a, b) for a, b in zip(got, want)) and torch.equal(static, fresh)
+
+
+@pytest.mark.parametrize("planes,pages,elems", [(4, 1024, 131072), (3, 700, 300008), (64, 4096, 2048)])
+def test_compact_of_large_pools(hq, planes, pages, elems):
+    """Pools of a gibibyte and more take the way of a plan and then copies; pages of no whole pieces of a workgroup, and many that move."""
+    r = np.random.default_rng(pages)
+    refs = [int(n) for n in (r.random(pages) < 0.6) * r.integers(1, 4, pages)]
+    pool = pool_of(1, planes, pages, elems)
+    live = sum(n > 0 for n in refs)
+    holes, movers = [p for p in range(live) if refs[p] <= 0], [p for p in range(live, pages) if refs[p] > 0]
+    to, want_refs, want_pool = dict(zip(movers, holes)), refs[:], pool.clone()
+    for source, target in to.items():
+        want_refs[target], want_refs[source] = refs[source], 0
+    want_pool[:, holes[:len(movers)]] = pool[:, movers]
+    table = r.integers(-2, pages + 2, (5, 11)).tolist()
+    t, n, got = hq.cache_compact(pool, i32(table), i32(refs))
+    assert t.tolist() == [[to.get(p, p) for p in row] for row in table]
+    assert n.tolist() == want_refs and got.tolist() == [live]
+    assert torch.equal(pool, want_pool)
