@@ -1278,16 +1278,27 @@ float exponent_scale(float s) { return s * 1.44269504088896340736f > 1e-30f ? s 
 bool bad_scale(float s) { return !(s >= 0.f) || std::isinf(s); }
 bool misaligned(const void* p, int64_t stride) { return ((uintptr_t)p & 15) || stride % 8; }
 
-// Few rows leave compute units idle, and each of their workgroups with all keys: then the keys are divided, so that there are up to
-// two workgroups a compute unit, each with 256 keys at least; not for 640 keys or less, where that gains less than the second launch
-// costs (500 tokens: 15.1 us, in two shares 19.6).
+// Few rows leave compute units idle, and each of their workgroups with all keys: then the keys are divided, 256 a share at least, and the
+// shares joined by a second launch.  Into how many parts, an estimate says, of sequences of the average length (lengths are device memory),
+// in us: a tile of 64 keys takes a workgroup 1.04 alone (heads of 64: 0.88), a compute unit 0.96 (0.65) where it has more of them, and
+// every share of a row is written and read.  40 tokens behind 2900 keys, 32 / 8 heads of 128: 50.9 us, in 12 shares 16.1; 512 behind
+// 8000 143.8, in four 90.5; 1000 by themselves 24.0, in two 35.9; 17 sequences of up to 248, 12 / 1 heads, 11.7 and 29.1.
 template <typename T, int D>
 int launch_prompt(PromptArgs a, int cus, hipStream_t stream) {
-  const int64_t items = ((int64_t)a.total_q * a.ratio / 128 + a.seqs) * a.kv_heads;
-  const int64_t want = 2 * (int64_t)cus / items, most = a.total_k > 640 ? ((int64_t)a.total_k + 255) / 256 : 1;
-  a.shares = (int)std::max<int64_t>(1, std::min(want, most));
+  const int64_t items = ((int64_t)a.total_q * a.ratio / 128 + a.seqs) * a.kv_heads, rows = (int64_t)a.total_q * a.heads;
+  const float queries = (float)a.total_q / a.seqs, keys = (float)a.total_k / a.seqs;
+  const float unit = (D == 128 ? 0.96f : 0.65f) / cus * std::max(queries * a.ratio / 128, 1.f) * a.seqs * a.kv_heads;
+  const float deepest = keys / 64, mean = (a.causal ? keys - std::min(queries, keys) / 2 : keys) / 64;
+  float best = INFINITY;
+  for (int s = 1; s <= 64 && (s == 1 || (s * items <= 4 * (int64_t)cus && (s - 1) * 256 < keys)); ++s) {
+    const float depth = s == 1 ? deepest : std::max(2 * std::ceil(keys / (128 * s)), 4.f);  // whole 128s
+    const float us = std::max(depth * (D == 128 ? 1.04f : 0.88f), mean * unit) + (s == 1 ? 0.f : 4.f + (float)rows * s * (D + 2) * 8 / 4.2e6f);
+    if (us < best) {
+      best = us;
+      a.shares = s;
+    }
+  }
   if (items * a.shares > INT_MAX) return HQ_ERR_TOO_LARGE;
-  const int64_t rows = (int64_t)a.total_q * a.heads;
   if (a.shares > 1) {
     HqWorkspace ws;
     const int rc = hq_get_workspace(stream, (size_t)(rows * a.shares * (D + 2)), 0, &ws);
