@@ -915,8 +915,9 @@ __device__ __forceinline__ unsigned running_sum(unsigned v) {
 
 // Share x of the requests' keys, all of one size: the smallest multiple of 128 of which there are no more shares than a.items, one a
 // request at least.  Lengths differ, and a share is a workgroup's work (32 requests of up to 4000, two equal shares each: 62.0 us, 57.2
-// so; 16 of up to 1000: 13.0 and 12.4).  Runs of equal length, whoever's the keys are, are better still for such (56.4), but a workgroup that goes on to the next request
-// waits for it (8 of up to 2000: 12.1 us, in runs 13.7).  A request a lane; one request, and more than 64, in a.ns equal shares each.
+// so; 16 of up to 1000: 13.0 and 12.4; but 8 of up to 2000, whose 128s are a few more than the shares, 12.0 and 12.9).  Runs of equal
+// length, whoever's the keys are, are better still for such (56.4), but a workgroup that goes on to the next request waits for it (8 of
+// up to 2000: 13.7).  A request a lane; one request, and more than 64, in a.ns equal shares each.
 constexpr int kUnit = 128;
 struct Share {
   int b, first, end, before, count;  // request; keys; shares of the requests before it, and of it
@@ -960,8 +961,8 @@ __device__ __forceinline__ Pages<T, D> pages_of(const PagedArgs& a, int request,
   return Pages<T, D>((const T*)a.k, (const T*)a.v, a.table + (int64_t)request * a.width, head, a.kv_heads, a.page_log, a.pages);
 }
 
-// The shares of up to 16 rows together, by one workgroup: 16 threads a row, whose loads are of two values
-// each, side by side, and the shares divided among the sets of threads that there are then.  Written by others a moment ago: read past the caches of this XCD.
+// The shares of up to 16 rows together, by one workgroup: 16 threads a row, whose loads are of two values each, side by side, and the
+// shares divided among the sets of threads that there are then.  Written by others a moment ago: read past the caches of this XCD.
 template <typename T, int D>
 __device__ __forceinline__ void join_here(const PagedArgs& a, char* sm, int nrows, int64_t row0, int64_t place, int slots, bool none) {
   constexpr int N = D / 16, AT_ONCE = 4;
