@@ -865,6 +865,7 @@ struct PagedArgs {
   int most_np, ns;     // at most; shares of a request's own keys; without groups, 0: by their number
   int per_row, items;  // places from a row's to the next one's; without groups, shares of all requests, at most
   int prefix_items;    // workgroups of the common keys
+  int likely;          // shares that the common keys are divided into, if groups are alike
   float c;
 };
 
@@ -1187,15 +1188,22 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void paged_kernel(PagedA
 }
 
 // The shares of a row together, by WAVES waves: their maxima and sums a lane each, then the sums of the values, 16 bytes a lane, several
-// shares at a time; a wave takes every WAVES-th group of them.  Of the shares, those from `np` to `own` were not written.  Bound by two
-// trips to memory, one behind the other.
-template <typename T, int D, int WAVES>
-__device__ __forceinline__ void join_shares(const float* po, const float* pm, int64_t row, int64_t place, int step, int np, int own, int slots, bool none,
-                                            T* out) {
-  constexpr int LANES = D / 4, AT_ONCE = 64 / LANES;  // lanes of a share, shares of a load
-  const int lane = threadIdx.x & 63, d = (lane % LANES) * 4, wave = WAVES == 1 ? 0 : threadIdx.x >> 6;
+// shares at a time; a wave takes every WAVES-th group of them.  Of the shares, those from `np` to `own` were not written.  PRE:
+// the first PRE groups, if below `likely` or from `own` on, are asked for before np and the maxima are there: one trip to memory less
+// where rows are few (32 rows of 64 shares 14.6 -> 12.3 us with the whole call, 1280 of 12 15.4 -> 15.0), and only more to read where
+// they are many (2048 rows of 9 shares 72.8 -> 74.3).
+template <typename T, int D, int WAVES, int PRE>
+__device__ __forceinline__ void join_shares(const float* po, const float* pm, int64_t row, int64_t place, int step, int np, int own, int slots, int likely,
+                                            bool none, T* out) {
+  constexpr int LANES = D / 4, AT_ONCE = 64 / LANES, EVERY = WAVES * AT_ONCE;  // lanes of a share, shares of a load
+  const int lane = threadIdx.x & 63, d = (lane % LANES) * 4, wave = WAVES == 1 ? 0 : threadIdx.x >> 6, mine0 = wave * AT_ONCE + lane / LANES;
   const float2* ml = reinterpret_cast<const float2*>(pm) + place;
-  const float2 ahead = ml[(int64_t)min(lane, slots - 1) * step];  // under way before np is known
+  const float2 ahead = ml[(int64_t)min(lane, slots - 1) * step];
+  auto sums = [&](int s) { return *reinterpret_cast<const hq_f4v*>(po + (place + (int64_t)s * step) * D + d); };
+  auto early = [&](int s) { return s < slots && (s < likely || s >= own); };
+  hq_f4v pre[PRE ? PRE : 1];
+#pragma unroll
+  for (int i = 0; i < PRE; ++i) pre[i] = sums(early(mine0 + i * EVERY) ? mine0 + i * EVERY : 0);
   auto share = [&](int s0) {
     const int s = s0 + lane;
     const float2 x = s0 ? ml[(int64_t)min(s, slots - 1) * step] : ahead;
@@ -1209,15 +1217,25 @@ __device__ __forceinline__ void join_shares(const float* po, const float* pm, in
   hq_f4v o = {0.f, 0.f, 0.f, 0.f};
   for (int s0 = 0; s0 < slots; s0 += 64) {
     const int here = min(slots - s0, 64);
-    const float2 mine = share(s0);
-    const float f = __builtin_amdgcn_exp2f(mine.x - ms);
-    l += mine.y * f;
+    const float2 x = share(s0);
+    const float f = __builtin_amdgcn_exp2f(x.x - ms);
+    l += x.y * f;
+    int i0 = 0;
+    if (PRE && s0 == 0) {
+#pragma unroll
+      for (int i = 0; i < PRE; ++i) {
+        const int at = mine0 + i * EVERY;
+        const float w = __shfl(f, at & 63);
+        // a share that no key went into has weight 0, and nothing was written for it
+        if (at < here && w != 0.f) o += (early(at) ? pre[i] : sums(at)) * w;
+      }
+      i0 = PRE * EVERY;
+    }
 #pragma unroll 8
-    for (int i = wave * AT_ONCE; i < here; i += WAVES * AT_ONCE) {
-      const int at = i + lane / LANES;
+    for (int i = i0; i < here; i += EVERY) {
+      const int at = i + mine0;
       const float w = __shfl(f, at & 63);
-      // a share that no key went into has weight 0, and nothing was written for it
-      if (at < here && w != 0.f) o += *reinterpret_cast<const hq_f4v*>(po + (place + (int64_t)(s0 + at) * step) * D + d) * w;
+      if (at < here && w != 0.f) o += sums(s0 + at) * w;
     }
   }
   l = hq_wave_sum(l);
@@ -1226,12 +1244,12 @@ __device__ __forceinline__ void join_shares(const float* po, const float* pm, in
 #pragma unroll
     for (int i = 0; i < 4; ++i) o[i] += __shfl_xor(o[i], x);
   if (WAVES > 1) {
-    __shared__ hq_f4v sums[WAVES][LANES];
-    if (lane < LANES) sums[wave][lane] = o;
+    __shared__ hq_f4v parts[WAVES][LANES];
+    if (lane < LANES) parts[wave][lane] = o;
     __syncthreads();
     if (wave > 0 || lane >= LANES) return;
 #pragma unroll
-    for (int w = 1; w < WAVES; ++w) o += sums[w][lane];
+    for (int w = 1; w < WAVES; ++w) o += parts[w][lane];
   }
   if (lane < LANES) {
     typedef T T4 __attribute__((ext_vector_type(4)));
@@ -1245,33 +1263,38 @@ __device__ __forceinline__ void join_shares(const float* po, const float* pm, in
 // A row of few shares takes a wave, one of many a workgroup (1024 rows of 128, 33 shares: 9.3 us by waves, 7.0 by workgroups; 4096
 // rows, 9 shares: 7.2 and 10.6).
 constexpr int kSharesOfAWave = 16;
-template <typename T, int D, int WAVES>
+template <typename T, int D, int WAVES, int PRE>
 __global__ __launch_bounds__(kThreads) void join_paged_kernel(PagedArgs a) {
   const int64_t row = WAVES > 1 ? blockIdx.x : (int64_t)blockIdx.x * kWaves + (threadIdx.x >> 6);
   if (row >= (int64_t)a.batch * a.heads) return;
   const int b = row / a.heads, slots = a.most_np + a.ns;
   if (a.ngroups) {
     const int np = a.np[1 + b] ? a.np[0] : 0;
-    join_shares<T, D, WAVES>(a.po, a.pm, row, row * slots, 1, np, a.most_np, slots, a.lengths[b] <= 0, (T*)a.out);
+    join_shares<T, D, WAVES, PRE>(a.po, a.pm, row, row * slots, 1, np, a.most_np, slots, a.likely, a.lengths[b] <= 0, (T*)a.out);
   } else {
     const int before = a.ns ? b * a.ns : a.np[2 * b], count = a.ns ? a.ns : a.np[2 * b + 1];
-    if (count > 1) join_shares<T, D, WAVES>(a.po, a.pm, row, row + (int64_t)(before - b) * a.heads, a.heads, count, count, count, a.lengths[b] <= 0, (T*)a.out);
+    if (count > 1) join_shares<T, D, WAVES, PRE>(a.po, a.pm, row, row + (int64_t)(before - b) * a.heads, a.heads, count, count, count, count, a.lengths[b] <= 0, (T*)a.out);
   }
 }
 
-template <typename T, int D, int WAVES>
+template <typename T, int D, int WAVES, int PRE>
 __global__ __launch_bounds__(kThreads) void join_prompt_kernel(PromptArgs a) {
   const int64_t row = WAVES > 1 ? blockIdx.x : (int64_t)blockIdx.x * kWaves + (threadIdx.x >> 6);
   if (row >= (int64_t)a.total_q * a.heads) return;
   const int token = row / a.heads;
   if (token < a.cu_q[0] || token >= a.cu_q[a.seqs]) return;
   const float2 first = reinterpret_cast<const float2*>(a.pm)[row * a.shares];
-  join_shares<T, D, WAVES>(a.po, a.pm, row, row * a.shares, 1, 0, 0, a.shares, first.x == INFINITY && first.y == 0.f, (T*)a.out);
+  join_shares<T, D, WAVES, PRE>(a.po, a.pm, row, row * a.shares, 1, 0, 0, a.shares, 0, first.x == INFINITY && first.y == 0.f, (T*)a.out);
 }
 template <typename A>
-int launch_join(void (*by_waves)(A), void (*by_workgroups)(A), int64_t rows, int64_t slots, hipStream_t stream, const A& a) {
-  if (slots <= kSharesOfAWave) return hq_launch_as_is(by_waves, dim3((unsigned)((rows + kWaves - 1) / kWaves)), dim3(kThreads), 0, stream, a);
-  return hq_launch_as_is(by_workgroups, dim3((unsigned)rows), dim3(kThreads), 0, stream, a);
+struct Joins {  // by waves and by workgroups, and the same with loads ahead
+  void (*waves)(A), (*workgroups)(A), (*waves_ahead)(A), (*workgroups_ahead)(A);
+};
+template <typename A>
+int launch_join(const Joins<A>& by, int64_t rows, int64_t slots, hipStream_t stream, const A& a) {
+  if (slots <= kSharesOfAWave)
+    return hq_launch_as_is(rows < 2048 ? by.waves_ahead : by.waves, dim3((unsigned)((rows + kWaves - 1) / kWaves)), dim3(kThreads), 0, stream, a);
+  return hq_launch_as_is(rows < 2048 ? by.workgroups_ahead : by.workgroups, dim3((unsigned)rows), dim3(kThreads), 0, stream, a);
 }
 
 // Scores are compared and masked by -infinity before they are scaled: a scale of zero (all keys alike) becomes one that no score notices.
@@ -1309,7 +1332,9 @@ int launch_prompt(PromptArgs a, int cus, hipStream_t stream) {
   }
   const int rc = hq_launch_as_is(prompt_kernel<T, D>, dim3((unsigned)(items * a.shares)), dim3(kThreads), Many<T, D>::LDS, stream, a);
   if (rc != HQ_OK || a.shares == 1) return rc;
-  return launch_join(join_prompt_kernel<T, D, 1>, join_prompt_kernel<T, D, kWaves>, rows, a.shares, stream, a);
+  return launch_join(Joins<PromptArgs>{join_prompt_kernel<T, D, 1, 0>, join_prompt_kernel<T, D, kWaves, 0>, join_prompt_kernel<T, D, 1, 8>,
+                                       join_prompt_kernel<T, D, kWaves, 8>},
+                     rows, a.shares, stream, a);
 }
 
 // Common keys: a workgroup a compute unit for them, two for heads of 64, and the requests' own keys divided until they fill as many (64
@@ -1333,8 +1358,8 @@ int launch_paged(PagedArgs a, int cus, hipStream_t stream) {
     places = rows * slots;
     // The kernel uses as many of them as there are workgroups for the tiles, groups alike these; where rows are many, by them is how the
     // shares are joined (9 of 33: 4096 rows 80.7 -> 78.8 us with the whole call, 2048 rows 72.6 -> 73.4).
-    const int64_t used = std::min<int64_t>(a.most_np, prefix / (a.kv_heads * std::max<int64_t>(a.ngroups, (int64_t)a.batch * a.ratio / 128)));
-    joined = (rows >= 4096 ? used : a.most_np) + a.ns;
+    a.likely = (int)std::min<int64_t>(a.most_np, prefix / (a.kv_heads * std::max<int64_t>(a.ngroups, (int64_t)a.batch * a.ratio / 128)));
+    joined = (rows >= 4096 ? a.likely : a.most_np) + a.ns;
   } else {
     a.per_row = 1;
     const int64_t most = a.batch * std::max<int64_t>(1, (cap + kUnit - 1) / kUnit), room = 2 * (int64_t)cus / (a.kv_heads * tiles);
@@ -1361,7 +1386,9 @@ int launch_paged(PagedArgs a, int cus, hipStream_t stream) {
   static_assert(lds <= 65536, "no attribute to set");
   const int rc = hq_launch_as_is(kernel, dim3((unsigned)grid), dim3(kThreads), lds, stream, a);
   if (rc != HQ_OK || !places || alone) return rc;
-  return launch_join(join_paged_kernel<T, D, 1>, join_paged_kernel<T, D, kWaves>, rows, joined, stream, a);
+  return launch_join(Joins<PagedArgs>{join_paged_kernel<T, D, 1, 0>, join_paged_kernel<T, D, kWaves, 0>, join_paged_kernel<T, D, 1, 8>,
+                                      join_paged_kernel<T, D, kWaves, 8>},
+                     rows, joined, stream, a);
 }
 
 // One of the four kernels by type and head size.
