@@ -1069,8 +1069,8 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, char* sm, int b0, i
   }
   if (!a.arrived) return;
   // The last share to arrive joins them all, and there is no second launch.  For up to 32 shares: the last one's trips grow with them
-  // (32 / 8 heads of 128; a request of 333 keys in two launches 9.4 us, in one 8.3; 4 of 8192, 16 shares, 22.0 and 20.6; 2 of 8192, 32
-  // shares, 15.9 and 15.8; one, 64 shares, 13.3 and 14.5).
+  // (32 / 8 heads of 128; a request of 333 keys in two launches 9.7 us, in one 8.2; 4 of 8192, 16 shares, 21.6 and 20.7; 2 of 8192, 32
+  // shares, 15.4 and 15.7; one, 64 shares, 11.9 and 14.5).
   __shared__ unsigned nth;
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
