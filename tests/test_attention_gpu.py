@@ -435,3 +435,25 @@ def test_paged_infinite_scores_in_one_share(hq):
         q[0, 4:].abs_()
         out = hq.paged_attention(q, k, v, i32(table), i32(lengths))
         assert torch.isnan(out[0, 4:]).all() and torch.isfinite(out[0, :4]).all() and torch.isfinite(out[1]).all()
+
+
+@pytest.mark.parametrize("heads,groups", [((64, 8), [0, 16, 32, 48, 64]), ((32, 8), [0, 16, 32, 48, 64]), ((64, 8), [0, 3, 3, 60]), ((32, 8), [0, 64])])
+def test_paged_many_rows_joined(hq, heads, groups):
+    """2048 and 4096 rows: groups alike, of very different sizes, one of all."""
+    dtype, u = TYPES["bf16"]
+    shared = [480, 16, 992, 320][:len(groups) - 1]
+    lengths = [(s * 37) % 400 + 500 for s in range(64)]
+    lengths[5], lengths[63] = 0, 1500
+    q, k, v, table, lengths = paged_case(51, dtype, lengths, heads, 128, 16, groups, shared)
+    out = hq.paged_attention(q, k, v, i32(table), i32(lengths), i32(groups), i32(shared))
+    check_paged(out, q, k, v, table, lengths, 1 / math.sqrt(128), u)
+
+
+@pytest.mark.parametrize("kind,D", [("bf16", 128), ("f16", 64)])
+@pytest.mark.parametrize("queries,keys,heads", [([100], [6100], (32, 8)), ([3, 0, 40], [2000, 900, 2500], (8, 8)), ([600], [600], (2, 2)), ([1], [9000], (4, 4))])
+def test_prompt_divided_keys_joined(hq, kind, D, queries, keys, heads):
+    """Few rows and many, few shares and many, sequences of different lengths whose keys are divided alike."""
+    dtype, u = TYPES[kind]
+    q, k, v = randn(1, sum(queries), heads[0], D).to(dtype), randn(2, sum(keys), heads[1], D).to(dtype), randn(3, sum(keys), heads[1], D).to(dtype)
+    out = hq.prompt_attention(q, k, v, i32(bounds(queries)), i32(bounds(keys)))
+    check_prompt(out, q, k, v, queries, keys, True, 1 / math.sqrt(D), u)
