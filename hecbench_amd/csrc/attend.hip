@@ -12,6 +12,7 @@
 // sums within a lane and one exchange, and the same registers are, rounded, the operand of O^T = V^T P^T without another move: the
 // order of the keys in that sum is free, and the transposing LDS read fetches V's rows in the order in which S^T left them.
 #include <algorithm>
+#include <cfloat>
 #include <climits>
 #include <cmath>
 #include <type_traits>
@@ -63,6 +64,9 @@ __device__ __forceinline__ float quarters_sum(float v) {
   return pair_sum(__uint_as_float(s[0]) + __uint_as_float(s[1]));
 }
 __device__ __forceinline__ float finite_or_zero(float m) { return m == -INFINITY ? 0.f : m; }
+// A share's maximum as those who join the shares read it: -infinity means that the row sees no key of the share, which has no sums then; a
+// row that has that of all its shares gives zeros.  One that sees keys, all of whose scores are -infinity or NaN, says the lowest number.
+__device__ __forceinline__ float share_top(float m, bool sees) { return sees ? fmaxf(m, -FLT_MAX) : -INFINITY; }
 
 // A value that is the same in all lanes, in scalar registers.
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
@@ -469,16 +473,16 @@ struct Many {
     if (bad) *poison = tileno;
   }
 
-  // The row's sums as one of several shares; none: the row sees nothing in any of them, which share 0 says by an infinite maximum.
-  __device__ __forceinline__ void put_share(float* po, float* pm, int64_t at, bool none) const {
+  // The row's sums as one of several shares; sees: one of the share's keys at least.
+  __device__ __forceinline__ void put_share(float* po, float* pm, int64_t at, bool sees) const {
     const int half = (threadIdx.x >> 5) & 1;
-    if (m != -INFINITY)  // a share that no key went into is not read
+    if (sees)
 #pragma unroll
       for (int d = 0; d < D / 32; ++d)
 #pragma unroll
         for (int g = 0; g < 4; ++g)
           *reinterpret_cast<hq_f4v*>(po + at * D + 32 * d + 8 * g + 4 * half) = hq_f4v{o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]};
-    if (half == 0) *reinterpret_cast<float2*>(pm + 2 * at) = float2{none ? INFINITY : m, l};
+    if (half == 0) *reinterpret_cast<float2*>(pm + 2 * at) = float2{share_top(m, sees), l};
   }
 
   // Keys [first, end) of src; whole: keys below it are seen by every row of the workgroup.  A tile is on its way from memory while the one
@@ -847,7 +851,7 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 4 : 2) void prompt_kernel(Promp
   if (a.shares == 1) {
     w.put((T*)a.out + ((int64_t)(q0 + token) * a.heads + h) * D, w.lim == 0);
   } else {
-    w.put_share(a.po, a.pm, ((int64_t)(q0 + token) * a.heads + h) * a.shares + share, w.lim == 0);
+    w.put_share(a.po, a.pm, ((int64_t)(q0 + token) * a.heads + h) * a.shares + share, w.lim > first);
   }
 }
 
@@ -965,7 +969,7 @@ __device__ __forceinline__ Pages<T, D> pages_of(const PagedArgs& a, int request,
 // The shares of up to 16 rows together, by one workgroup: 16 threads a row, whose loads are of two values each, side by side, and the
 // shares divided among the sets of threads that there are then.  Written by others a moment ago: read past the caches of this XCD.
 template <typename T, int D>
-__device__ __forceinline__ void join_here(const PagedArgs& a, char* sm, int nrows, int64_t row0, int64_t place, int slots, bool none) {
+__device__ __forceinline__ void join_here(const PagedArgs& a, char* sm, int nrows, int64_t row0, int64_t place, int slots) {
   constexpr int N = D / 16, AT_ONCE = 4;
   const int log = nrows > 8 ? 4 : nrows > 4 ? 3 : nrows > 2 ? 2 : nrows > 1, sets = 16 >> log;
   const int set = threadIdx.x >> (4 + log), row = (threadIdx.x >> 4) & ((1 << log) - 1), d0 = (threadIdx.x & 15) * 2;
@@ -1012,6 +1016,7 @@ __device__ __forceinline__ void join_here(const PagedArgs& a, char* sm, int nrow
     float top = m;
     for (int s = 1; s < sets; ++s) top = fmaxf(top, sums[s * step]);
     const float own = __builtin_amdgcn_exp2f(m - finite_or_zero(top));
+    m = top;
     l *= own;
 #pragma unroll
     for (int j = 0; j < N; ++j) o[j] *= own;
@@ -1023,6 +1028,7 @@ __device__ __forceinline__ void join_here(const PagedArgs& a, char* sm, int nrow
     }
   }
   if (row >= nrows) return;
+  const bool none = m == -INFINITY;
   typedef T T2 __attribute__((ext_vector_type(2)));
 #pragma unroll
   for (int j = 0; j < N; j += 2)
@@ -1064,7 +1070,7 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, char* sm, int b0, i
     for (int i = 0; i < D / 16; i += 4)
       hq_store_share(reinterpret_cast<hq_f4v*>(a.po + place * D + d0 + i), hq_f4v{sum[i], sum[i + 1], sum[i + 2], sum[i + 3]});
     if (d0 == 0)
-      __hip_atomic_store(reinterpret_cast<unsigned long long*>(a.pm) + place, (unsigned long long)__float_as_uint(total) << 32 | __float_as_uint(top),
+      __hip_atomic_store(reinterpret_cast<unsigned long long*>(a.pm) + place, (unsigned long long)__float_as_uint(total) << 32 | __float_as_uint(share_top(top, first < end)),
                          __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
   if (!a.arrived) return;
@@ -1079,7 +1085,7 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, char* sm, int b0, i
   __syncthreads();
   if (nth != (unsigned)shares - 1) return;
   if (threadIdx.x == 0) __hip_atomic_store(count, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  join_here<T, D>(a, sm, nrows, (int64_t)b0 * a.heads + head * ratio, (int64_t)(before - b0) * a.heads, shares, a.lengths[b0] <= 0);
+  join_here<T, D>(a, sm, nrows, (int64_t)b0 * a.heads + head * ratio, (int64_t)(before - b0) * a.heads, shares);
 }
 
 // Up to 128 of them; a row sees keys up to its request's length.
@@ -1110,7 +1116,7 @@ __device__ __forceinline__ void many_rows(const PagedArgs& a, char* sm, int* poi
   if (row > last_row) return;
   const int64_t at = (int64_t)b * a.heads + h;
   if (shares == 1) w.put((T*)a.out + at * D, w.lim == 0);
-  else w.put_share(a.po, a.pm, at * a.per_row + slot, false);
+  else w.put_share(a.po, a.pm, at * a.per_row + slot, w.lim > first);
 }
 
 // Nothing is common: a share a workgroup.
@@ -1194,7 +1200,7 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void paged_kernel(PagedA
 // they are many (2048 rows of 9 shares 72.8 -> 74.3).
 template <typename T, int D, int WAVES, int PRE>
 __device__ __forceinline__ void join_shares(const float* po, const float* pm, int64_t row, int64_t place, int step, int np, int own, int slots, int likely,
-                                            bool none, T* out) {
+                                            T* out) {
   constexpr int LANES = D / 4, AT_ONCE = 64 / LANES, EVERY = WAVES * AT_ONCE;  // lanes of a share, shares of a load
   const int lane = threadIdx.x & 63, d = (lane % LANES) * 4, wave = WAVES == 1 ? 0 : threadIdx.x >> 6, mine0 = wave * AT_ONCE + lane / LANES;
   const float2* ml = reinterpret_cast<const float2*>(pm) + place;
@@ -1212,6 +1218,7 @@ __device__ __forceinline__ void join_shares(const float* po, const float* pm, in
   float m = -INFINITY;
   for (int s0 = 0; s0 < slots; s0 += 64) m = fmaxf(m, share(s0).x);
   m = hq_wave_max(m);
+  const bool none = m == -INFINITY;
   const float ms = finite_or_zero(m);
   float l = 0.f;
   hq_f4v o = {0.f, 0.f, 0.f, 0.f};
@@ -1270,10 +1277,10 @@ __global__ __launch_bounds__(kThreads) void join_paged_kernel(PagedArgs a) {
   const int b = row / a.heads, slots = a.most_np + a.ns;
   if (a.ngroups) {
     const int np = a.np[1 + b] ? a.np[0] : 0;
-    join_shares<T, D, WAVES, PRE>(a.po, a.pm, row, row * slots, 1, np, a.most_np, slots, a.likely, a.lengths[b] <= 0, (T*)a.out);
+    join_shares<T, D, WAVES, PRE>(a.po, a.pm, row, row * slots, 1, np, a.most_np, slots, a.likely, (T*)a.out);
   } else {
     const int before = a.ns ? b * a.ns : a.np[2 * b], count = a.ns ? a.ns : a.np[2 * b + 1];
-    if (count > 1) join_shares<T, D, WAVES, PRE>(a.po, a.pm, row, row + (int64_t)(before - b) * a.heads, a.heads, count, count, count, count, a.lengths[b] <= 0, (T*)a.out);
+    if (count > 1) join_shares<T, D, WAVES, PRE>(a.po, a.pm, row, row + (int64_t)(before - b) * a.heads, a.heads, count, count, count, count, (T*)a.out);
   }
 }
 
@@ -1283,8 +1290,7 @@ __global__ __launch_bounds__(kThreads) void join_prompt_kernel(PromptArgs a) {
   if (row >= (int64_t)a.total_q * a.heads) return;
   const int token = row / a.heads;
   if (token < a.cu_q[0] || token >= a.cu_q[a.seqs]) return;
-  const float2 first = reinterpret_cast<const float2*>(a.pm)[row * a.shares];
-  join_shares<T, D, WAVES, PRE>(a.po, a.pm, row, row * a.shares, 1, 0, 0, a.shares, 0, first.x == INFINITY && first.y == 0.f, (T*)a.out);
+  join_shares<T, D, WAVES, PRE>(a.po, a.pm, row, row * a.shares, 1, 0, 0, a.shares, 0, (T*)a.out);
 }
 template <typename A>
 struct Joins {  // by waves and by workgroups, and the same with loads ahead
