@@ -996,8 +996,9 @@ __device__ __forceinline__ void join_here(const PagedArgs& a, char* sm, int nrow
     for (int j = 0; j < N; ++j) o[j] *= f;
 #pragma unroll
     for (int i = 0; i < AT_ONCE; ++i) {
-      const float w = s0 + i * sets < slots ? __builtin_amdgcn_exp2f(__uint_as_float((uint32_t)ml[i]) - finite_or_zero(m)) : 0.f;
-      if (w != 0.f) {  // not so for a share that no key went into
+      // A share of weight 0 counts too: what is not finite in it stays so (one without keys holds zeros).
+      const float w = __builtin_amdgcn_exp2f(__uint_as_float((uint32_t)ml[i]) - finite_or_zero(m));
+      if (s0 + i * sets < slots) {
         l += w * __uint_as_float((uint32_t)(ml[i] >> 32));
 #pragma unroll
         for (int j = 0; j < N; ++j) o[j] += w * __uint_as_float((uint32_t)(v[i][j / 2] >> 32 * (j & 1)));
@@ -1225,7 +1226,8 @@ __device__ __forceinline__ void join_shares(const float* po, const float* pm, in
   for (int s0 = 0; s0 < slots; s0 += 64) {
     const int here = min(slots - s0, 64);
     const float2 x = share(s0);
-    const float f = __builtin_amdgcn_exp2f(x.x - ms);
+    // the share's weight; -1: it has no keys, and nothing was written for it (one of weight 0 counts: what is not finite in it stays so)
+    const float f = x.x == -INFINITY ? -1.f : __builtin_amdgcn_exp2f(x.x - ms);
     l += x.y * f;
     int i0 = 0;
     if (PRE && s0 == 0) {
@@ -1233,8 +1235,7 @@ __device__ __forceinline__ void join_shares(const float* po, const float* pm, in
       for (int i = 0; i < PRE; ++i) {
         const int at = mine0 + i * EVERY;
         const float w = __shfl(f, at & 63);
-        // a share that no key went into has weight 0, and nothing was written for it
-        if (at < here && w != 0.f) o += (early(at) ? pre[i] : sums(at)) * w;
+        if (at < here && !(w < 0.f)) o += (early(at) ? pre[i] : sums(at)) * w;
       }
       i0 = PRE * EVERY;
     }
@@ -1242,7 +1243,7 @@ __device__ __forceinline__ void join_shares(const float* po, const float* pm, in
     for (int i = i0; i < here; i += EVERY) {
       const int at = i + mine0;
       const float w = __shfl(f, at & 63);
-      if (at < here && w != 0.f) o += sums(s0 + at) * w;
+      if (at < here && !(w < 0.f)) o += sums(s0 + at) * w;
     }
   }
   l = hq_wave_sum(l);

@@ -23,6 +23,97 @@ def test_paged_tables_of_no_width(hq, heads, D):
         assert (out == 0).all()
 
 
+def alike(seed, n, heads, dtype, D):
+    """A request's keys, of which the first has a score of 200 and all others less than 1 in magnitude: 2^-287 of its weight."""
+    k = randn(seed, n, heads, D) * 0.01
+    k[0], k[:, :, 0] = 0, 0
+    k[0, :, 0] = 100
+    q0 = 2.0 * math.sqrt(D)
+    return k.to(dtype), q0
+
+
+# ---- numbers that are not finite, in one share -----------------------------------------------------------------------------
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("heads,D", [((8, 2), 128), ((1, 1), 64), ((24, 1), 64)])
+@pytest.mark.parametrize("page", [8, 16])
+def test_paged_nan_keys_alone_in_the_last_share(hq, kind, heads, D, page):
+    """The last share holds nothing but keys of NaN: joined in one launch, in two, and without being divided the request is NaN."""
+    dtype, u = TYPES[kind]
+    for lengths, bad in (([129], 1), ([257], 1), ([9000], 40), ([129, 300], 1), ([129] + [200] * 300, 1)):
+        q, k, v, table, lengths = paged_case(7, dtype, lengths, heads, D, page)
+        for t in range(lengths[0] - bad, lengths[0]):
+            k[table[0][t // page], :, t % page] = math.nan
+        out = hq.paged_attention(q, k, v, i32(table), i32(lengths))
+        assert torch.isnan(out[0]).all()
+        check_paged(out[1:], q[1:], k, v, table[1:], lengths[1:], 1 / math.sqrt(D), u)
+
+
+@pytest.mark.parametrize("heads,D", [((8, 2), 128), ((24, 1), 64)])
+def test_paged_nan_keys_behind_what_is_common(hq, heads, D):
+    """One request's own key is NaN: it is, and the others of its group are not."""
+    dtype, u = TYPES["bf16"]
+    q, k, v, table, lengths = paged_case(9, dtype, [513, 600, 520], heads, D, 16, [0, 3], [512])
+    k[table[0][32], :, 0] = math.nan
+    out = hq.paged_attention(q, k, v, i32(table), i32(lengths), i32([0, 3]), i32([512]))
+    assert torch.isnan(out[0]).all()
+    check_paged(out[1:], q[1:], k, v, table[1:], lengths[1:], 1 / math.sqrt(D), u)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("D", [64, 128])
+def test_prompt_nan_keys_fill_shares(hq, kind, D):
+    dtype, u = TYPES[kind]
+    nq, nk = [3, 5], [2500, 900]
+    q, k, v = randn(1, 8, 8, D).to(dtype), randn(2, 3400, 2, D).to(dtype), randn(3, 3400, 2, D).to(dtype)
+    k[1700:2490, 1] = math.nan
+    out = hq.prompt_attention(q, k, v, i32(bounds(nq)), i32(bounds(nk)))
+    assert torch.isnan(out[:3, 4:]).all()
+    check_prompt(out[:3, :4], q[:3, :4], k[:2500, :1], v[:2500, :1], [3], [2500], True, 1 / math.sqrt(D), u)
+    check_prompt(out[3:], q[3:], k[2500:], v[2500:], [5], [900], True, 1 / math.sqrt(D), u)
+
+
+@pytest.mark.parametrize("what", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("heads,D", [((8, 2), 128), ((1, 1), 64), ((24, 1), 64)])
+def test_paged_values_without_weight(hq, what, heads, D):
+    """A value that is not finite makes its element NaN, however small its weight and whichever share holds it, and no other."""
+    for kind in ("bf16", "f16"):
+        dtype, u = TYPES[kind]
+        for lengths, groups in (([100], None), ([129], None), ([257], None), ([9000], None), ([129] + [200] * 300, None), ([700, 600], ([0, 2], [512]))):
+            q, k, v, table, lengths = paged_case(11, dtype, lengths, heads, D, 16, *(groups or ()))
+            rows, q0 = alike(3, lengths[0], heads[1], dtype, D)
+            q[0, :, 0] = q0
+            for t in range(lengths[0]):
+                k[table[0][t // 16], :, t % 16] = rows[t]
+            args = (i32(table), i32(lengths)) + (tuple(i32(g) for g in groups) if groups else ())
+            want = hq.paged_attention(q, k, v, *args)
+            check_paged(want[:1], q[:1], k, v, table[:1], lengths[:1], 1 / math.sqrt(D), u)
+            v[table[0][(lengths[0] - 1) // 16], 0, (lengths[0] - 1) % 16, 5] = what
+            got = hq.paged_attention(q, k, v, *args)
+            r = heads[0] // heads[1]
+            assert torch.isnan(got[0, :r, 5]).all()
+            got[0, :r, 5] = want[0, :r, 5]
+            assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("what", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("D", [64, 128])
+def test_prompt_values_without_weight(hq, what, D):
+    for kind in ("bf16", "f16"):
+        dtype, u = TYPES[kind]
+        for nq, nk in ((3, 2500), (40, 2900), (500, 500)):
+            q, v = randn(1, nq, 8, D).to(dtype), randn(3, nk, 2, D).to(dtype)
+            k, q0 = alike(2, nk, 2, dtype, D)
+            q[:, :, 0] = q0
+            cu = i32([0, nq]), i32([0, nk])
+            want = hq.prompt_attention(q, k, v, *cu)
+            check_prompt(want, q, k, v, [nq], [nk], True, 1 / math.sqrt(D), u)
+            v[nk - 2, 1, 5] = what  # seen by the last two tokens
+            got = hq.prompt_attention(q, k, v, *cu)
+            assert torch.isnan(got[-2:, 4:, 5]).all()
+            got[-2:, 4:, 5] = want[-2:, 4:, 5]
+            assert torch.equal(got, want)
+
+
 def test_keys_of_minus_infinity_in_one_share_and_in_all(hq):
     """Keys whose score is -inf have no weight, also where a share holds nothing else; where all have it the softmax is NaN."""
     dtype, u = TYPES["bf16"]
