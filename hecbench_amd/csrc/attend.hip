@@ -64,6 +64,9 @@ __device__ __forceinline__ float quarters_sum(float v) {
   return pair_sum(__uint_as_float(s[0]) + __uint_as_float(s[1]));
 }
 __device__ __forceinline__ float finite_or_zero(float m) { return m == -INFINITY ? 0.f : m; }
+// A result of a sum o of values and what it is to be scaled by.  A sum that is not finite gives NaN: whether an infinite value comes out
+// of a sum as an infinity depends on whether its weight, or that of its share, has become 0 (the tiles that not all rows see mark NaN).
+__device__ __forceinline__ float result(float o, float scaled) { return fmaf(o, 0.f, scaled); }
 // A share's maximum as those who join the shares read it: -infinity means that the row sees no key of the share, which has no sums then; a
 // row that has that of all its shares gives zeros.  One that sees keys, all of whose scores are -infinity or NaN, says the lowest number.
 __device__ __forceinline__ float share_top(float m, bool sees) { return sees ? fmaxf(m, -FLT_MAX) : -INFINITY; }
@@ -569,6 +572,7 @@ struct Many {
   // half the stores (24 sequences of up to 901 tokens, 32 heads of 64: 71.5 -> 70 us; by way of LDS, in whole rows, no faster).
   __device__ __forceinline__ void put(T* out, bool none) const {
     const float inv = none ? 0.f : 1.f / l;  // and the sums are zero
+    auto of = [=](float x) { return result(x, x * inv); };
     typedef T T2 __attribute__((ext_vector_type(2)));
     hq_u4v* to = reinterpret_cast<hq_u4v*>(out) + ((threadIdx.x >> 5) & 1);
 #pragma unroll
@@ -579,8 +583,8 @@ struct Many {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const int r = 4 * g + 2 * i;
-          const auto s = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, T2{(T)(o[d][r] * inv), (T)(o[d][r + 1] * inv)}),
-                                                          __builtin_bit_cast(uint32_t, T2{(T)(o[d][r + 4] * inv), (T)(o[d][r + 5] * inv)}), false, false);
+          const auto s = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, T2{(T)of(o[d][r]), (T)of(o[d][r + 1])}),
+                                                          __builtin_bit_cast(uint32_t, T2{(T)of(o[d][r + 4]), (T)of(o[d][r + 5])}), false, false);
           v[i] = s[0];
           v[2 + i] = s[1];
         }
@@ -1033,7 +1037,7 @@ __device__ __forceinline__ void join_here(const PagedArgs& a, char* sm, int nrow
   typedef T T2 __attribute__((ext_vector_type(2)));
 #pragma unroll
   for (int j = 0; j < N; j += 2)
-    *reinterpret_cast<T2*>((T*)a.out + at * D + d0 + 16 * j) = none ? T2{(T)0.f, (T)0.f} : T2{(T)(o[j] / l), (T)(o[j + 1] / l)};
+    *reinterpret_cast<T2*>((T*)a.out + at * D + d0 + 16 * j) = none ? T2{(T)0.f, (T)0.f} : T2{(T)result(o[j], o[j] / l), (T)result(o[j + 1], o[j + 1] / l)};
 }
 
 constexpr int kApart = 16;  // counters, a line of 64 bytes each: atomics on one line wait for each other (64 shares: 17.7 us, apart 14.5)
@@ -1061,7 +1065,7 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, char* sm, int b0, i
   if (shares == 1) {
     TD v;
 #pragma unroll
-    for (int i = 0; i < D / 16; ++i) v[i] = (T)(first >= end ? 0.f : sum[i] / total);
+    for (int i = 0; i < D / 16; ++i) v[i] = (T)(first >= end ? 0.f : result(sum[i], sum[i] / total));
     if (row) *reinterpret_cast<TD*>((T*)a.out + at * D + d0) = v;
     return;
   }
@@ -1263,7 +1267,7 @@ __device__ __forceinline__ void join_shares(const float* po, const float* pm, in
     typedef T T4 __attribute__((ext_vector_type(4)));
     T4 v;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = (T)(none ? 0.f : o[i] / l);
+    for (int i = 0; i < 4; ++i) v[i] = (T)(none ? 0.f : result(o[i], o[i] / l));
     *reinterpret_cast<T4*>(out + row * D + d) = v;
   }
 }

@@ -332,9 +332,11 @@ int hq_mxfp4_qdq(const void* in, void* out, int64_t n_elems, int dtype, void* st
  *     out[t][h] = sum_j softmax_j(scale * q[t][h] . k[j][h/R]) * v[j][h/R]
  *   over the sequence's keys; causal != 0: over those with j <= i + (number of keys) - (number of tokens), i and j counted
  *   within the sequence.  A token that sees no key gets zeros.  A key that a token does not see has no effect on it, whatever it
- *   holds; a value that is not finite makes the results of the tokens that see it NaN.  q [total_q][heads][head_dim], rows q_stride
- *   elements apart, k and v [total_k][kv_heads][head_dim] likewise (parts of a fused projection's rows), k_stride and v_stride up to
- *   2^22; out contiguous; all 16-byte aligned, strides multiples of 8.  Tokens of no sequence are not written.
+ *   holds; a value that is not finite makes its element of the results of all tokens that see it NaN, however small its weight (infinities
+ *   too; the same in hq_paged_attention).  bf16 values beyond 2^88 may overflow the fp32 sums, whose weights are up to 2^8.
+ *   q [total_q][heads][head_dim], rows q_stride elements apart, k and v [total_k][kv_heads][head_dim] likewise (parts of a fused
+ *   projection's rows), k_stride and v_stride up to 2^22; out contiguous; all 16-byte aligned, strides multiples of 8.  Tokens of no
+ *   sequence are not written.
  * hq_paged_attention: one query a request.  Token t of request s is token t % page_size of page table[s][t / page_size]
  *   (table [batch][table_width], pages [num_pages][kv_heads][page_size][head_dim], contiguous); request s sees its first lengths[s] tokens.
  *   Requests groups[g] ... groups[g+1]-1 (bounds in ascending order) have their first shared[g] tokens, as far as the first one's

@@ -114,6 +114,36 @@ def test_prompt_values_without_weight(hq, what, D):
             assert torch.equal(got, want)
 
 
+@pytest.mark.parametrize("what", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("D", [64, 128])
+def test_values_that_are_not_finite_are_nan_in_every_tile(hq, what, D):
+    """Tiles that all rows see and tiles that some see, keys divided and not, a prompt's and a cache's: one answer."""
+    for kind in ("bf16", "f16"):
+        dtype, _ = TYPES[kind]
+        for nq, nk, heads in ((300, 300, (8, 2)), (5, 2000, (8, 2)), (1000, 1000, (32, 32))):
+            q, k, v = randn(1, nq, heads[0], D).to(dtype), randn(2, nk, heads[1], D).to(dtype), randn(3, nk, heads[1], D).to(dtype)
+            want = hq.prompt_attention(q, k, v, i32([0, nq]), i32([0, nk]))
+            for at in (3, nk - 200, nk - 1):
+                v2 = v.clone()
+                v2[at, 1, 5] = what
+                got = hq.prompt_attention(q, k, v2, i32([0, nq]), i32([0, nk]))
+                r, first = heads[0] // heads[1], max(at - (nk - nq), 0)
+                assert torch.isnan(got[first:, r:2 * r, 5]).all()
+                got[first:, r:2 * r, 5] = want[first:, r:2 * r, 5]
+                assert torch.equal(got, want)
+        for heads in ((8, 2), (48, 2)):
+            for lengths, groups in (([60], None), ([2000, 100], None), ([900] * 20, ([0, 20], [512])), ([600, 560], ([0, 2], [512]))):
+                q, k, v, table, lengths = paged_case(13, dtype, lengths, heads, D, 16, *(groups or ()))
+                args = (i32(table), i32(lengths)) + (tuple(i32(g) for g in groups) if groups else ())
+                want = hq.paged_attention(q, k, v, *args)
+                v[table[0][1], 1, 3, 5] = what
+                got = hq.paged_attention(q, k, v, *args)
+                r, who = heads[0] // heads[1], slice(None) if groups else slice(0, 1)
+                assert torch.isnan(got[who, r:, 5]).all()
+                got[who, r:, 5] = want[who, r:, 5]
+                assert torch.equal(got, want)
+
+
 def test_keys_of_minus_infinity_in_one_share_and_in_all(hq):
     """Keys whose score is -inf have no weight, also where a share holds nothing else; where all have it the softmax is NaN."""
     dtype, u = TYPES["bf16"]
