@@ -1118,8 +1118,12 @@ __device__ __forceinline__ void many_rows(const PagedArgs& a, char* sm, int* poi
   const int whole = min(min(seen[0], seen[1]), min(seen[2], seen[3]));
   PagedTiles<T, D> src(pages_of<T, D>(a, b0, head), end);
   w.run(src, first, end, uniform(whole), a.c);
-  if (row > last_row) return;
-  const int64_t at = (int64_t)b * a.heads + h;
+  // the row, worked out once more: in the loop there is no register to spare
+  int tid = threadIdx.x;
+  asm volatile("" : "+v"(tid));
+  const int mine = first_row + (tid >> 6) * 32 + (tid & 31);
+  if (mine > last_row) return;
+  const int64_t at = (int64_t)(b0 + (uint32_t)mine / ratio) * a.heads + head * ratio + (uint32_t)mine % ratio;
   if (shares == 1) w.put((T*)a.out + at * D, w.lim == 0);
   else w.put_share(a.po, a.pm, at * a.per_row + slot, w.lim > first);
 }
