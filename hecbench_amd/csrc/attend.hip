@@ -27,6 +27,11 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) char lds_char;
 
+// The weights on their way into the product with the values, in 16 bits: 2^(c s - m), where m is not the row's maximum itself but kLift octaves
+// below it, and stays until the maximum is kMost octaves above.  bf16 has no need of a lift; fp16, whose normal numbers end at 2^-14, has its
+// weights where its range ends.  Each is rounded, to the nearest, by 2^-11 (bf16: 2^-8) of itself at most, as much as the result's own rounding;
+// fp16's below 2^-25 of the row's largest by 2^-36 of that largest at most (with the largest at 1 a key of 2^-18.5 was 0.6 % off, and
+// one of 2^-25 gone).
 template <typename T>
 struct Kind;
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -34,6 +39,7 @@ template <>
 struct Kind<__bf16> {
   typedef bf16x8 V8;
   static constexpr uint32_t kExp = 0x7f807f80u, kStep = 0x00800080u, kOne = 0x3f803f80u;
+  static constexpr float kLift = 0.f, kMost = 8.f;
   static __device__ __forceinline__ f32x16 mfma(V8 a, V8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
   static __device__ __forceinline__ f32x4 mfma(V8 a, V8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 };
@@ -41,6 +47,7 @@ template <>
 struct Kind<_Float16> {
   typedef f16x8 V8;
   static constexpr uint32_t kExp = 0x7c007c00u, kStep = 0x04000400u, kOne = 0x3c003c00u;
+  static constexpr float kLift = 11.f, kMost = 15.f;
   static __device__ __forceinline__ f32x16 mfma(V8 a, V8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
   static __device__ __forceinline__ f32x4 mfma(V8 a, V8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 };
@@ -64,6 +71,14 @@ __device__ __forceinline__ float quarters_sum(float v) {
   return pair_sum(__uint_as_float(s[0]) + __uint_as_float(s[1]));
 }
 __device__ __forceinline__ float finite_or_zero(float m) { return m == -INFINITY ? 0.f : m; }
+// m of a row whose maximum is `top` now (differences: beyond 2^24 numbers are further apart than the lift).
+template <typename T>
+__device__ __forceinline__ bool outgrown(float top, float m) { return top - m > Kind<T>::kMost; }
+template <typename T>
+__device__ __forceinline__ float lifted(float top) {
+  const float m = top - Kind<T>::kLift;
+  return outgrown<T>(top, m) ? top : m;
+}
 // A result of a sum o of values and what it is to be scaled by.  A sum that is not finite gives NaN: whether an infinite value comes out
 // of a sum as an infinity depends on whether its weight, or that of its share, has become 0 (the tiles that not all rows see mark NaN).
 __device__ __forceinline__ float result(float o, float scaled) { return fmaf(o, 0.f, scaled); }
@@ -352,11 +367,11 @@ struct Many {
       for (int r = 0; r < 16; ++r) top = fmaxf(top, s[b][r]);
     return pair_max(top);
   }
-  // A maximum that has grown by less than 2^8 stays: the weights may then be up to 2^8, which neither fp32 sums nor the 16-bit
-  // weights mind, and the sums need no scaling.  The scaling of 64 registers a tile was a fifth of the vector instructions.
+  // m stays where the maximum has grown by some octaves only: neither fp32 sums nor the 16-bit weights mind larger weights, and the sums
+  // need no scaling.  The scaling of 64 registers a tile was a fifth of the vector instructions.
   __device__ __forceinline__ void raise(float top) {
-    if (!__builtin_amdgcn_ballot_w64(top > m + 8.f)) return;
-    const float mn = top > m + 8.f ? top : m;  // each row by its own scores: its bits do not depend on its neighbours
+    if (!__builtin_amdgcn_ballot_w64(outgrown<T>(top, m))) return;
+    const float mn = outgrown<T>(top, m) ? lifted<T>(top) : m;  // each row by its own scores: its bits do not depend on its neighbours
     const float f = mn == m ? 1.f : __builtin_amdgcn_exp2f(m - mn);
     m = mn;
     l *= f;
@@ -376,7 +391,7 @@ struct Many {
         for (int i = 0; i < 8; ++i) {
           const float e = __builtin_amdgcn_exp2f(fmaf(s[b][8 * t + i], c, -ms));
           sum[i & 1] += e;
-          p[b][t][i] = (T)e;  // 2^-9 (bf16) or 2^-12 of a weight at most, to the nearest: as much as the result's own rounding
+          p[b][t][i] = (T)e;
         }
     l += sum[0] + sum[1];
   }
@@ -686,8 +701,8 @@ struct Few {
       }
       whole_k = more && load(p.k, next, here, ids, ks, std::false_type());
       top = quarters_max(top) * c;
-      if (__builtin_amdgcn_ballot_w64(top > m + 8.f)) {  // as in Many
-        const float mn = top > m + 8.f ? top : m, f = mn == m ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+      if (__builtin_amdgcn_ballot_w64(outgrown<T>(top, m))) {  // as in Many
+        const float mn = outgrown<T>(top, m) ? lifted<T>(top) : m, f = mn == m ? 1.f : __builtin_amdgcn_exp2f(m - mn);
         m = mn;
         l *= f;
 #pragma unroll
@@ -701,7 +716,7 @@ struct Few {
       for (int i = 0; i < 8; ++i) {
         const float e = __builtin_amdgcn_exp2f(fmaf(s[i / 4][i % 4], c, -ms));
         l += e;
-        w[i] = (T)e;  // rounded as in Many
+        w[i] = (T)e;
       }
       wait_but(whole_k);
 #pragma unroll

@@ -166,3 +166,67 @@ def test_keys_of_minus_infinity_in_one_share_and_in_all(hq):
         out = hq.paged_attention(q, k, v, i32(table), i32(lengths))
         r = heads[0] // 2
         assert torch.isnan(out[0, r:]).all() and torch.isfinite(out[0, :r]).all() and torch.isfinite(out[1]).all()
+
+
+# ---- weights far below the largest -----------------------------------------------------------------------------------------
+GAPS = [12.3, 18.5, 24.4, 26.2]
+
+
+def sink(gap, n, heads, dtype, D):
+    """n keys, of which the first has a score `gap` octaves above the others' and a value of zero; the others' values are about 1.  q0: of
+    the query's first element, with the usual scale."""
+    k = torch.zeros((n, heads, D), device="cuda")
+    k[0, :, 0] = gap * math.log(2) / 4
+    v = 1 + 0.01 * randn(5, n, heads, D)
+    v[0] = 0
+    return k.to(dtype), v.to(dtype), 4 * math.sqrt(D)
+
+
+def close_to_sink(out, q, k, v, kind):
+    """The bound of every element, as for all results, and the rounding of weights that are below fp16's normal numbers: fp16 weights are
+    scaled so that the row's largest is 2^11 at least, and of those below 2^-14 each is off by 2^-25 at most, so that a sum is by 2^-36 of
+    the sum of |v| at most (the largest weight, and so the sum of the weights, taken as 1)."""
+    u = TYPES[kind][1]
+    s = (q @ k.T) / math.sqrt(q.shape[1])
+    p = torch.softmax(s, 1)
+    big = float(((q.abs() @ k.abs().T) / math.sqrt(q.shape[1])).amax())
+    want, a = p @ v, p @ v.abs()
+    err = (out.double() - want).abs()
+    bound = 1.02 * (u * want.abs() + (u + 2.0 ** -13 + 2.0 ** -15 * big) * a) + 2.0 ** -24
+    if kind == "f16":
+        bound = bound + 2.0 ** -36 * v.abs().sum(0)
+    worst = (err - bound).max().item()
+    assert worst <= 0, (worst, err.max().item(), want.abs().max().item())
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("gap", GAPS)
+def test_prompt_small_weights(hq, kind, D, gap):
+    dtype = TYPES[kind][0]
+    for nq, nk, heads in ((300, 1000, (16, 2)), (2, 100, (2, 2)), (3, 2000, (2, 2))):
+        k, v, q0 = sink(gap, nk, heads[1], dtype, D)
+        q = torch.zeros((nq, heads[0], D), dtype=dtype, device="cuda")
+        q[:, :, 0] = q0
+        out = hq.prompt_attention(q, k, v, i32([0, nq]), i32([0, nk]), causal=False)
+        for h in (0, heads[0] - 1):
+            at = h // (heads[0] // heads[1])
+            close_to_sink(out[:, h], q[:, h].double(), k[:, at].double(), v[:, at].double(), kind)
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("heads,D", [((8, 2), 128), ((4, 4), 64), ((24, 1), 128), ((40, 2), 64)])
+@pytest.mark.parametrize("gap", GAPS)
+def test_paged_small_weights(hq, kind, heads, D, gap):
+    dtype = TYPES[kind][0]
+    for lengths in ([100, 40], [1001, 128], [1001] + [20] * 300):
+        q, k, v, table, lengths = paged_case(17, dtype, lengths, heads, D, 16)
+        ks, vs, q0 = sink(gap, lengths[0], heads[1], dtype, D)
+        q[0] = 0
+        q[0, :, 0] = q0
+        for t in range(lengths[0]):
+            k[table[0][t // 16], :, t % 16], v[table[0][t // 16], :, t % 16] = ks[t], vs[t]
+        out = hq.paged_attention(q, k, v, i32(table), i32(lengths))
+        for h in range(heads[0]):
+            at = h // (heads[0] // heads[1])
+            close_to_sink(out[0, h:h + 1], q[0, h:h + 1].double(), ks[:, at].double(), vs[:, at].double(), kind)
