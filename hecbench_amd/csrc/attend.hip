@@ -79,6 +79,22 @@ __device__ __forceinline__ float lifted(float top) {
   const float m = top - Kind<T>::kLift;
   return outgrown<T>(top, m) ? top : m;
 }
+// Whether m is so far from 0 that c s rounded, as a maximum is, and c s in an exponent, where it is not, may differ by octaves.
+__device__ __forceinline__ bool far(float m) { return fabsf(finite_or_zero(m)) > 0x1p20f; }
+// Scores become the exponents of their weights, of a row far from 0 (the product rounded) or not, whose bits are then those that they would
+// be without.  Kept behind its branch, one register after the other: in front of it, where the compiler moves it, it costs 17 registers too
+// many (24 sequences of up to 901 tokens, 32 heads of 64: 74.6 -> 95.7 us).
+template <typename S>
+__device__ __forceinline__ void exponents(S& s, int n, float c, float m) {
+  float before = far(m) ? c : 1.f, then = far(m) ? 1.f : c, ms = finite_or_zero(m);
+  asm volatile("" : "+v"(before), "+v"(then), "+v"(ms));
+#pragma unroll
+  for (int i = 0; i < n; ++i) {
+    float x = fmaf(s[i] * before, then, -ms);
+    asm volatile("" : "+v"(x));
+    s[i] = x;
+  }
+}
 // A result of a sum o of values and what it is to be scaled by.  A sum that is not finite gives NaN: whether an infinite value comes out
 // of a sum as an infinity depends on whether its weight, or that of its share, has become 0 (the tiles that not all rows see mark NaN).
 __device__ __forceinline__ float result(float o, float scaled) { return fmaf(o, 0.f, scaled); }
@@ -270,6 +286,7 @@ struct Many {
   V8 qf[D / 16];
   f32x16 o[D / 32];
   float m = -INFINITY, l = 0.f;
+  bool slow = false;      // there is a row in the wave whose m is far from 0
   int lim;                // keys below this are seen by the lane's row
   int all_see, any_sees;  // below the first by all rows of the wave, below the second by one of them
 
@@ -367,21 +384,30 @@ struct Many {
       for (int r = 0; r < 16; ++r) top = fmaxf(top, s[b][r]);
     return pair_max(top);
   }
+  // Before a tile's weights, its largest scores known.  Whether the scores are exponents now: in a wave with a row far from 0.
+  __device__ __forceinline__ bool raise(f32x16 (&s)[NB], float top, float c) {
+    scale_sums(top * c);
+    if (__builtin_expect(slow, 0))
+#pragma unroll
+      for (int b = 0; b < NB; ++b) exponents(s[b], 16, c, m);
+    return slow;
+  }
   // m stays where the maximum has grown by some octaves only: neither fp32 sums nor the 16-bit weights mind larger weights, and the sums
   // need no scaling.  The scaling of 64 registers a tile was a fifth of the vector instructions.
-  __device__ __forceinline__ void raise(float top) {
+  __device__ __forceinline__ void scale_sums(float top) {
     if (!__builtin_amdgcn_ballot_w64(outgrown<T>(top, m))) return;
     const float mn = outgrown<T>(top, m) ? lifted<T>(top) : m;  // each row by its own scores: its bits do not depend on its neighbours
     const float f = mn == m ? 1.f : __builtin_amdgcn_exp2f(m - mn);
     m = mn;
+    slow = __builtin_amdgcn_ballot_w64(far(m)) != 0;
     l *= f;
 #pragma unroll
     for (int d = 0; d < D / 32; ++d)
 #pragma unroll
       for (int r = 0; r < 16; ++r) o[d][r] *= f;
   }
-  __device__ __forceinline__ void weights(V8 (&p)[NB][2], const f32x16 (&s)[NB], float c) {
-    const float ms = finite_or_zero(m);
+  // The weights 2^(c s - ms).
+  __device__ __forceinline__ void weights(V8 (&p)[NB][2], const f32x16 (&s)[NB], float c, float ms) {
     float sum[2] = {0.f, 0.f};
 #pragma unroll
     for (int b = 0; b < NB; ++b)
@@ -405,14 +431,13 @@ struct Many {
   }
   // scores() of the next tile and weights() of this one, an instruction of the matrix core and its share of the others in turn: left
   // alone, the compiler moves the reads of all operands to the front and runs out of registers.
-  __device__ __forceinline__ void scores_and_weights(f32x16 (&n)[NB], const char* keys, V8 (&p)[NB][2], const f32x16 (&s)[NB], float c) {
+  __device__ __forceinline__ void scores_and_weights(f32x16 (&n)[NB], const char* keys, V8 (&p)[NB][2], const f32x16 (&s)[NB], float c, float ms) {
     const int lane = threadIdx.x & 63, half = lane >> 5;
     constexpr int STEPS = NB * D / 16, EACH = NB * 16 / STEPS, AHEAD = 4;
     auto operand = [&](int j) {
       const int row = 32 * (j / (D / 16)) + (lane & 31);
       return *reinterpret_cast<const V8*>(keys + row * D * 2 + k_piece<D>(row, 2 * (j % (D / 16)) + half) * 16);
     };
-    const float ms = finite_or_zero(m);
     float sum[2] = {0.f, 0.f};
     V8 a[AHEAD];
     hq_u4v w[NB][2];
@@ -556,15 +581,15 @@ struct Many {
       if (base < any_sees) {
         V8 p[NB][2];
         if (K_AHEAD) {
-          raise(top * c);
-          scores_and_weights(n, sm + (1 - SLOT) * HALF, p, s, c);
+          const bool done = raise(s, top, c);
+          scores_and_weights(n, sm + (1 - SLOT) * HALF, p, s, done ? 1.f : c, done ? 0.f : finite_or_zero(m));
           if (base + 2 * TILE > all_see) mask(n, lim - base - TILE - half4);
           top = values_and_top(p, vs, n);
         } else {
           scores(s, sm + SLOT * HALF);
           if (base + TILE > all_see) mask(s, lim - base - half4);
-          raise(top_of(s) * c);
-          weights(p, s, c);
+          const bool done = raise(s, top_of(s), c);
+          weights(p, s, done ? 1.f : c, done ? 0.f : finite_or_zero(m));
           values(p, vs);
         }
       }
@@ -624,6 +649,7 @@ struct Few {
   V8 qf[D / 32];
   f32x4 o[D / 16];
   float m = -INFINITY, l = 0.f;
+  bool slow = false;  // as in Many
 
   __device__ __forceinline__ void run(const Pages<T, D>& p, int first, int end, float c) {
     const int lane = threadIdx.x & 63, wave = uniform((int)(threadIdx.x >> 6)), quarter = lane >> 4;
@@ -704,17 +730,21 @@ struct Few {
       if (__builtin_amdgcn_ballot_w64(outgrown<T>(top, m))) {  // as in Many
         const float mn = outgrown<T>(top, m) ? lifted<T>(top) : m, f = mn == m ? 1.f : __builtin_amdgcn_exp2f(m - mn);
         m = mn;
+        slow = __builtin_amdgcn_ballot_w64(far(m)) != 0;
         l *= f;
 #pragma unroll
         for (int d = 0; d < D / 16; ++d)
 #pragma unroll
           for (int r = 0; r < 4; ++r) o[d][r] *= f;
       }
-      const float ms = finite_or_zero(m);
+      if (slow)
+#pragma unroll
+        for (int b = 0; b < 2; ++b) exponents(s[b], 4, c, m);
+      const float cs = slow ? 1.f : c, ms = slow ? 0.f : finite_or_zero(m);
       V8 w;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float e = __builtin_amdgcn_exp2f(fmaf(s[i / 4][i % 4], c, -ms));
+        const float e = __builtin_amdgcn_exp2f(fmaf(s[i / 4][i % 4], cs, -ms));
         l += e;
         w[i] = (T)e;
       }

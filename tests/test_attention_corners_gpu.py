@@ -230,3 +230,17 @@ def test_paged_small_weights(hq, kind, heads, D, gap):
         for h in range(heads[0]):
             at = h // (heads[0] // heads[1])
             close_to_sink(out[0, h:h + 1], q[0, h:h + 1].double(), ks[:, at].double(), vs[:, at].double(), kind)
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("D", [64, 128])
+def test_scores_of_every_magnitude(hq, kind, D):
+    """Scores up to 2^40, where fp32 numbers are far further apart than an octave: results stay among the values."""
+    dtype, u = TYPES[kind]
+    q, k, v = randn(1, 300, 8, D).to(dtype), randn(2, 700, 2, D).to(dtype), randn(3, 700, 2, D).to(dtype)
+    pq, pk, pv, table, lengths = paged_case(23, dtype, [700, 100], (8, 2), D, 16)
+    for octaves in range(16, 40):
+        out = hq.prompt_attention(q, k, v, i32([0, 300]), i32([0, 700]), scale=2.0 ** octaves)
+        assert torch.isfinite(out).all() and out.abs().max() <= v.abs().max() * (1 + 2 * u)
+        out = hq.paged_attention(pq, pk, pv, i32(table), i32(lengths), scale=2.0 ** octaves)
+        assert torch.isfinite(out).all() and out.abs().max() <= torch.nan_to_num(pv).abs().max() * (1 + 2 * u)
