@@ -1358,7 +1358,7 @@ int launch_join(const Joins<A>& by, int64_t rows, int64_t slots, hipStream_t str
 }
 
 // Scores are compared and masked by -infinity before they are scaled: a scale of zero (all keys alike) becomes one that no score notices.
-float exponent_scale(float s) { return s * 1.44269504088896340736f > 1e-30f ? s * 1.44269504088896340736f : 1e-30f; }
+float exponent_scale(float s) { return std::max(s * 1.44269504088896340736f, FLT_TRUE_MIN); }
 bool bad_scale(float s) { return !(s >= 0.f) || std::isinf(s); }
 bool misaligned(const void* p, int64_t stride) { return ((uintptr_t)p & 15) || stride % 8; }
 

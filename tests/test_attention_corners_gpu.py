@@ -244,3 +244,12 @@ def test_scores_of_every_magnitude(hq, kind, D):
         assert torch.isfinite(out).all() and out.abs().max() <= v.abs().max() * (1 + 2 * u)
         out = hq.paged_attention(pq, pk, pv, i32(table), i32(lengths), scale=2.0 ** octaves)
         assert torch.isfinite(out).all() and out.abs().max() <= torch.nan_to_num(pv).abs().max() * (1 + 2 * u)
+
+
+def test_scale_of_zero_and_scores_beyond_all_bounds(hq):
+    """A scale of zero makes all keys alike, whatever their products with the query."""
+    dtype, u = TYPES["bf16"]
+    q, k, v = (randn(1, 4, 4, 64) * 2.0 ** 50).to(dtype), (randn(2, 200, 2, 64) * 2.0 ** 50).to(dtype), randn(3, 200, 2, 64).to(dtype)
+    out = hq.prompt_attention(q, k, v, i32([0, 4]), i32([0, 200]), causal=False, scale=0.0)
+    for h in range(4):
+        close(out[:, h], v[:, h // 2].double().mean(0).expand(4, 64), v[:, h // 2].double().abs().mean(0), 0.0, u)
