@@ -1493,7 +1493,7 @@ extern "C" int hq_paged_attention(const void* q, const void* k_pages, const void
   if (dtype != HQ_DTYPE_F16 && dtype != HQ_DTYPE_BF16) return HQ_ERR_BAD_ENUM;
   if (bad_scale(scale)) return HQ_ERR_BAD_SHAPE;
   if (batch == 0) return HQ_OK;
-  if (!q || !out || !lengths || (table_width && (!table || num_pages == 0 || !k_pages || !v_pages)) || (ngroups && (!groups || !shared)))
+  if (!q || !out || !lengths || (table_width && !table) || (table_width && num_pages && (!k_pages || !v_pages)) || (ngroups && (!groups || !shared)))
     return HQ_ERR_NULL_POINTER;
   if (q_stride < (int64_t)heads * head_dim) return HQ_ERR_BAD_SHAPE;
   if (misaligned(q, q_stride) || (((uintptr_t)k_pages | (uintptr_t)v_pages | (uintptr_t)out) & 15) ||

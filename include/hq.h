@@ -341,8 +341,8 @@ int hq_mxfp4_qdq(const void* in, void* out, int64_t n_elems, int dtype, void* st
  *   (table [batch][table_width], pages [num_pages][kv_heads][page_size][head_dim], contiguous); request s sees its first lengths[s] tokens.
  *   Requests groups[g] ... groups[g+1]-1 (bounds in ascending order) have their first shared[g] tokens, as far as the first one's
  *   length reaches, in the same pages, which are read once for all of them, from the first one's row (every row of the table lists
- *   them); ngroups 0: nothing is shared.  page_size a power of two, 8 ... 1024.  A table entry that is needed and no page counts as
- *   a page of zeros.
+ *   them); ngroups 0: nothing is shared, and as many groups as requests or more are taken as none.  page_size a power of two, 8 ... 1024.
+ *   A table entry that is needed and no page counts as a page of zeros (num_pages 0: all of them).
  * hq_cache_write: tokens cu[s] ... cu[s+1]-1 of k and v [tokens][kv_heads][head_dim] (strides as above) become tokens starts[s], ... of row s
  *   of the table; any head_dim that is a multiple of 8, any page_size.  A token whose place is outside its row, or in no page, is left out.
  * hq_cache_step: from the tables of one step to the next one's.  Row s inherits row parent[s] (of the old tables; any number outside

@@ -253,3 +253,14 @@ def test_scale_of_zero_and_scores_beyond_all_bounds(hq):
     out = hq.prompt_attention(q, k, v, i32([0, 4]), i32([0, 200]), causal=False, scale=0.0)
     for h in range(4):
         close(out[:, h], v[:, h // 2].double().mean(0).expand(4, 64), v[:, h // 2].double().abs().mean(0), 0.0, u)
+
+
+def test_paged_pools_of_no_pages(hq):
+    """Every entry that is needed counts as a page of zeros."""
+    pages = torch.zeros((0, 2, 16, 128), dtype=torch.float16, device="cuda")
+    q = randn(1, 3, 8, 128).half()
+    table = i32([[0, 1, 2], [-1, -1, -1], [5, 0, 0]])
+    for groups in ((), (i32([0, 3]), i32([16]))):
+        out = torch.full_like(q, 7.0)
+        hq.paged_attention(q, pages, pages, table, i32([40, 1, 0]), *groups, out=out)
+        assert (out == 0).all()

@@ -1,0 +1,22 @@
+"""Sizes that attention and the cache refuse because what they are multiplied into would not fit, and page sizes that one operator of the
+cache takes and another does not: the C entry points' own checks, before any HIP call."""
+import os
+import re
+
+from hecbench_amd import _lib
+
+MOST = 2 ** 31 - 1
+CSRC = os.path.join(os.path.dirname(os.path.abspath(_lib.__file__)), "csrc")
+
+
+def paged(**kw):
+    a = dict(q=16, k=16, v=16, out=16, dtype=2, table=16, lengths=16, groups=None, shared=None, ngroups=0, batch=1, width=4, pages=9, page=16, heads=8,
+             kv=2, d=128, qs=1024, scale=0.1, stream=None)
+    a.update(kw)
+    return _lib.load().hq_paged_attention(*a.values())
+
+
+def test_pools_of_no_pages_are_taken():
+    """No refusal for want of pages: the next one in the order of the checks comes."""
+    assert paged(pages=0, k=None, v=None, q=24) == -4
+    assert paged(pages=9, k=None, q=24) == -1 and paged(pages=0, table=None) == -1
