@@ -1382,10 +1382,12 @@ int launch_prompt(PromptArgs a, int cus, hipStream_t stream) {
       a.shares = s;
     }
   }
+  const size_t floats = rows * a.shares * (D + 2);
+  if (a.shares > 1 && hq_workspace_out_of_reach(stream, floats, 0)) a.shares = 1;  // longer, and no error
   if (items * a.shares > INT_MAX) return HQ_ERR_TOO_LARGE;
   if (a.shares > 1) {
     HqWorkspace ws;
-    const int rc = hq_get_workspace(stream, (size_t)(rows * a.shares * (D + 2)), 0, &ws);
+    const int rc = hq_get_workspace(stream, floats, 0, &ws);
     if (rc != HQ_OK) return rc;
     a.po = ws.partial;
     a.pm = ws.partial + rows * a.shares * D;
@@ -1405,36 +1407,48 @@ int launch_paged(PagedArgs a, int cus, hipStream_t stream) {
   const int64_t cap = (int64_t)a.width << a.page_log, rows = (int64_t)a.batch * a.heads, tiles = a.ratio <= 16 ? 1 : (a.ratio + 127) / 128;
   const int64_t own = (int64_t)a.batch * a.kv_heads * tiles;
   if (a.ngroups >= a.batch) a.ngroups = 0;  // groups of one, as good as: whoever shares nothing is not asked about it
-  int64_t prefix = 0, grid, slots, places, joined;
-  bool alone = false;
-  if (a.ngroups) {
-    const int64_t most_tiles = (int64_t)a.batch * a.ratio / 128 + a.ngroups;
-    const int64_t common = D == 64 ? 2 * cus : cus;
-    prefix = std::max<int64_t>(common, most_tiles * a.kv_heads);
-    a.most_np = (int)std::max<int64_t>(1, std::min<int64_t>(common / a.kv_heads, (cap + 255) / 256));
-    a.ns = (int)std::max<int64_t>(1, std::min(cus / own, (cap + 127) / 128));
-    grid = prefix + own * a.ns;
-    slots = a.per_row = a.most_np + a.ns;
-    places = rows * slots;
-    // The kernel uses as many of them as there are workgroups for the tiles, groups alike these; where rows are many, by them is how the
-    // shares are joined (9 of 33: 4096 rows 80.7 -> 78.8 us with the whole call, 2048 rows 72.6 -> 73.4).
-    a.likely = (int)std::min<int64_t>(a.most_np, prefix / (a.kv_heads * std::max<int64_t>(a.ngroups, (int64_t)a.batch * a.ratio / 128)));
-    joined = (rows >= 4096 ? a.likely : a.most_np) + a.ns;
-  } else {
-    a.per_row = 1;
-    const int64_t most = a.batch * std::max<int64_t>(1, (cap + kUnit - 1) / kUnit), room = 2 * (int64_t)cus / (a.kv_heads * tiles);
-    if (a.batch == 1 || a.batch > 64 || a.batch >= room || a.batch == most) a.ns = (int)std::max<int64_t>(1, std::min(room, most) / a.batch);
-    a.items = (int)(a.ns ? (int64_t)a.ns * a.batch : std::min(room, most));
-    grid = (int64_t)a.items * a.kv_heads * tiles;
-    places = a.ns == 1 ? 0 : (int64_t)a.items * a.heads;
-    slots = joined = a.items / a.batch;
-    alone = a.ratio <= 16 && slots <= 32;
+  int64_t prefix, grid, slots, places, joined;
+  size_t floats, counters;
+  bool alone, divide = true;
+  for (;;) {
+    prefix = 0;
+    alone = false;
+    if (a.ngroups) {
+      const int64_t most_tiles = (int64_t)a.batch * a.ratio / 128 + a.ngroups;
+      const int64_t common = D == 64 ? 2 * cus : cus;
+      prefix = std::max<int64_t>(common, most_tiles * a.kv_heads);
+      a.most_np = (int)std::max<int64_t>(1, std::min<int64_t>(common / a.kv_heads, (cap + 255) / 256));
+      a.ns = (int)std::max<int64_t>(1, std::min(cus / own, (cap + 127) / 128));
+      grid = prefix + own * a.ns;
+      slots = a.per_row = a.most_np + a.ns;
+      places = rows * slots;
+      // The kernel uses as many of them as there are workgroups for the tiles, groups alike these; where rows are many, by them is how the
+      // shares are joined (9 of 33: 4096 rows 80.7 -> 78.8 us with the whole call, 2048 rows 72.6 -> 73.4).
+      a.likely = (int)std::min<int64_t>(a.most_np, prefix / (a.kv_heads * std::max<int64_t>(a.ngroups, (int64_t)a.batch * a.ratio / 128)));
+      joined = (rows >= 4096 ? a.likely : a.most_np) + a.ns;
+    } else {
+      a.per_row = 1;
+      const int64_t most = a.batch * std::max<int64_t>(1, (cap + kUnit - 1) / kUnit), room = divide ? 2 * (int64_t)cus / (a.kv_heads * tiles) : 1;
+      a.ns = 0;
+      if (a.batch == 1 || a.batch > 64 || a.batch >= room || a.batch == most) a.ns = (int)std::max<int64_t>(1, std::min(room, most) / a.batch);
+      a.items = (int)(a.ns ? (int64_t)a.ns * a.batch : std::min(room, most));
+      grid = (int64_t)a.items * a.kv_heads * tiles;
+      places = a.ns == 1 ? 0 : (int64_t)a.items * a.heads;
+      slots = joined = a.items / a.batch;
+      alone = a.ratio <= 16 && slots <= 32;
+    }
+    floats = places * (D + 2) + 1 + 2 * (int64_t)a.batch;
+    counters = alone ? own * kApart : 0;
+    // While the stream is captured and has no room for shares: every request by itself, then in one share.  Longer, and no error.
+    if (!places || !hq_workspace_out_of_reach(stream, floats, counters)) break;
+    if (!a.ngroups) divide = false;
+    a.ngroups = 0;
   }
   if (grid > INT_MAX) return HQ_ERR_TOO_LARGE;
   a.prefix_items = (int)prefix;
   if (places) {
     HqWorkspace ws;
-    const int rc = hq_get_workspace(stream, (size_t)(places * (D + 2) + 1 + 2 * (int64_t)a.batch), alone ? (size_t)own * kApart : 0, &ws);
+    const int rc = hq_get_workspace(stream, floats, counters, &ws);
     if (rc != HQ_OK) return rc;
     a.arrived = alone ? ws.counters : nullptr;
     a.po = ws.partial;

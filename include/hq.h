@@ -355,8 +355,11 @@ int hq_mxfp4_qdq(const void* in, void* out, int64_t n_elems, int dtype, void* st
  *   are -1.  Outputs share no memory with inputs (HQ_ERR_BAD_SHAPE).  rows <= 16384.
  * hq_cache_compact: n pages are in use (refs > 0); those at n and beyond move, in order, into the free ones below n, in every plane;
  *   table_out and refs_out follow, *live = n.
- * All but hq_cache_write may use the stream's workspace (partial sums of divided keys, arrival counters, plans of large tables): before
- * a stream is captured, run the largest call on it once (hq_reserve_workspace counts the products' needs only).
+ * All but hq_cache_write may use the stream's workspace, of whose need hq_reserve_workspace knows nothing.  Attention keeps the partial sums of
+ * divided keys there, of few rows rather than of many: 64 requests need nothing where one of 9000 keys does.  A call that is captured on a
+ * stream without room for them does not divide the keys: right, and slow where rows are few.  So run every call that is going to be captured
+ * once on the stream before, of its own sizes.  hq_cache_step and hq_cache_compact keep the plans of tables beyond 4096 pages (1024 rows, 16384
+ * entries; pools of 1 GiB) there, more for larger ones, and captured without them they are an error: run the largest once before.
  */
 int hq_prompt_attention(const void* q, const void* k, const void* v, void* out, int dtype, const int32_t* cu_q, const int32_t* cu_k, int seqs,
                         int64_t total_q, int64_t total_k, int heads, int kv_heads, int head_dim, int64_t q_stride, int64_t k_stride,

@@ -264,3 +264,40 @@ def test_paged_pools_of_no_pages(hq):
         out = torch.full_like(q, 7.0)
         hq.paged_attention(q, pages, pages, table, i32([40, 1, 0]), *groups, out=out)
         assert (out == 0).all()
+
+
+# ---- no room for shares -----------------------------------------------------------------------------------------------------
+def captured(call, stream):
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        out = call()
+    return graph, out
+
+
+def test_captured_on_a_stream_that_has_no_workspace(hq):
+    """A call that would divide the keys does without, where the stream is being captured and nothing has been allocated for it."""
+    dtype, u = TYPES["bf16"]
+    pq, pk, pv = randn(1, 40, 32, 128).to(dtype), randn(2, 2940, 8, 128).to(dtype), randn(3, 2940, 8, 128).to(dtype)
+    cu = i32([0, 40]), i32([0, 2940])
+    torch.cuda.synchronize()
+    graph, out = captured(lambda: hq.prompt_attention(pq, pk, pv, *cu), torch.cuda.Stream())
+    for i in range(3):
+        out.zero_()
+        pq.copy_(randn(20 + i, *pq.shape))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        check_prompt(out, pq, pk, pv, [40], [2940], True, 1 / math.sqrt(128), u)
+    for lengths, groups in (([2000], None), ([9000, 17, 400], None), ([900, 1000, 950], ([0, 3], [896]))):
+        for heads in ((8, 2), (24, 1)):
+            q, k, v, table, _ = paged_case(19, dtype, lengths, heads, 128, 16, *(groups or ()))
+            args = (q, k, v, i32(table), i32(lengths)) + (tuple(i32(g) for g in groups) if groups else ())
+            torch.cuda.synchronize()
+            graph, out = captured(lambda: hq.paged_attention(*args), torch.cuda.Stream())
+            for i in range(3):
+                out.zero_()
+                q.copy_(randn(30 + i, *q.shape))
+                torch.cuda.synchronize()
+                graph.replay()
+                torch.cuda.synchronize()
+                check_paged(out, q, k, v, table, lengths, 1 / math.sqrt(128), u)
