@@ -132,12 +132,15 @@ __device__ __forceinline__ int v_piece(int row, int ch) {
 
 // One instruction brings 1 KB from memory into LDS past the registers, the lanes' pieces one behind the other, so it is the lane's
 // address that follows the order of the pieces.  (The compiler does not see that it writes LDS; the waits are explicit.)
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"  // that m0 is the compiler's own is why it is listed
 __device__ __forceinline__ void to_lds(uint32_t lds, const void* from, uint32_t off) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(from) : "memory");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(from) : "memory", "m0");
 }
 __device__ __forceinline__ void to_lds(uint32_t lds, const void* from) {  // a lane's own address
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(from) : "memory");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(from) : "memory", "m0");
 }
+#pragma clang diagnostic pop
 __device__ __forceinline__ uint32_t lds_address(const char* p) { return (uint32_t)(uintptr_t)(lds_char*)p; }
 
 // The tiles of one sequence's keys, one head, for the four waves of Many.  Rows behind the last one repeat it.

@@ -20,3 +20,12 @@ def test_pools_of_no_pages_are_taken():
     """No refusal for want of pages: the next one in the order of the checks comes."""
     assert paged(pages=0, k=None, v=None, q=24) == -4
     assert paged(pages=9, k=None, q=24) == -1 and paged(pages=0, table=None) == -1
+
+
+def test_assembly_that_writes_m0_says_so():
+    for name in sorted(os.listdir(CSRC)):
+        if name.endswith((".hip", ".h")):
+            text = open(os.path.join(CSRC, name)).read()
+            for asm in re.findall(r"asm volatile\((.*?)\);", text, re.S):
+                if "s_mov_b32 m0" in asm:
+                    assert '"m0"' in asm.rsplit(":", 1)[1], (name, asm)
