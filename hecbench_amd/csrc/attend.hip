@@ -1516,7 +1516,9 @@ extern "C" int hq_paged_attention(const void* q, const void* k_pages, const void
   if (misaligned(q, q_stride) || (((uintptr_t)k_pages | (uintptr_t)v_pages | (uintptr_t)out) & 15) ||
       (((uintptr_t)table | (uintptr_t)lengths | (uintptr_t)groups | (uintptr_t)shared) & 3))
     return HQ_ERR_MISALIGNED;
-  if ((int64_t)table_width * page_size > INT_MAX - 256 || (int64_t)batch * heads > INT_MAX / 64) return HQ_ERR_TOO_LARGE;
+  if ((int64_t)table_width * page_size > INT_MAX - 256 || (int64_t)batch * heads > INT_MAX / 64 ||
+      (int64_t)kv_heads * head_dim * 2 * page_size > UINT32_MAX)  // bytes of a page
+    return HQ_ERR_TOO_LARGE;
   const HqDevice* dev = nullptr;
   const int rc = hq_current_device(&dev);
   if (rc != HQ_OK) return rc;

@@ -16,6 +16,12 @@ def paged(**kw):
     return _lib.load().hq_paged_attention(*a.values())
 
 
+def test_pages_of_four_gibibytes():
+    """Bytes of a page, all heads: kv_heads * head_dim * 2 * page_size in 32 bits."""
+    assert paged(page=1024, kv=16384, heads=16384, qs=16384 * 128) == -6
+    assert paged(page=1024, kv=32768, heads=32768, d=64, qs=32768 * 64) == -6
+
+
 def test_pools_of_no_pages_are_taken():
     """No refusal for want of pages: the next one in the order of the checks comes."""
     assert paged(pages=0, k=None, v=None, q=24) == -4
