@@ -1363,6 +1363,9 @@ int launch_join(const Joins<A>& by, int64_t rows, int64_t slots, hipStream_t str
 // Scores are compared and masked by -infinity before they are scaled: a scale of zero (all keys alike) becomes one that no score notices.
 float exponent_scale(float s) { return std::max(s * 1.44269504088896340736f, FLT_TRUE_MIN); }
 bool bad_scale(float s) { return !(s >= 0.f) || std::isinf(s); }
+// Keys of a row are numbered in 32 bits, as are the ends of loads and shares behind the last one: up to 512 shares rounded up to 128 keys, page
+// numbers up to 2048 keys ahead.
+constexpr int kMostKeys = INT_MAX - (1 << 17);
 bool misaligned(const void* p, int64_t stride) { return ((uintptr_t)p & 15) || stride % 8; }
 
 // Few rows leave compute units idle, and each of their workgroups with all keys: then the keys are divided, 256 a share at least, and the
@@ -1489,7 +1492,7 @@ extern "C" int hq_prompt_attention(const void* q, const void* k, const void* v, 
   if (misaligned(q, q_stride) || misaligned(k, k_stride) || misaligned(v, v_stride) || ((uintptr_t)out & 15) ||
       (((uintptr_t)cu_q | (uintptr_t)cu_k) & 3))
     return HQ_ERR_MISALIGNED;
-  if (total_q > INT_MAX || total_q * (heads / kv_heads) > INT_MAX - 128 || total_k > INT_MAX - 128 || k_stride > 1 << 22 ||
+  if (total_q > INT_MAX || total_q * (heads / kv_heads) > INT_MAX - 128 || total_k > kMostKeys || k_stride > 1 << 22 ||
       v_stride > 1 << 22)  // 32-bit offsets in a tile
     return HQ_ERR_TOO_LARGE;
   const HqDevice* dev = nullptr;
@@ -1516,7 +1519,7 @@ extern "C" int hq_paged_attention(const void* q, const void* k_pages, const void
   if (misaligned(q, q_stride) || (((uintptr_t)k_pages | (uintptr_t)v_pages | (uintptr_t)out) & 15) ||
       (((uintptr_t)table | (uintptr_t)lengths | (uintptr_t)groups | (uintptr_t)shared) & 3))
     return HQ_ERR_MISALIGNED;
-  if ((int64_t)table_width * page_size > INT_MAX - 256 || (int64_t)batch * heads > INT_MAX / 64 ||
+  if ((int64_t)table_width * page_size > kMostKeys || (int64_t)batch * heads > INT_MAX / 64 ||
       (int64_t)kv_heads * head_dim * 2 * page_size > UINT32_MAX)  // bytes of a page
     return HQ_ERR_TOO_LARGE;
   const HqDevice* dev = nullptr;

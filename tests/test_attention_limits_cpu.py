@@ -22,6 +22,18 @@ def test_pages_of_four_gibibytes():
     assert paged(page=1024, kv=32768, heads=32768, d=64, qs=32768 * 64) == -6
 
 
+def test_tables_within_a_workgroup_of_two_to_the_31():
+    """Keys are numbered in 32 bits, and a kernel's loads and shares go some way beyond the last."""
+    assert paged(page=1024, width=2 ** 21 - 1) == -6
+    assert paged(page=8, width=(MOST - 300) // 8) == -6
+
+
+def test_prompts_within_a_workgroup_of_two_to_the_31():
+    def prompt(tk):
+        return _lib.load().hq_prompt_attention(16, 16, 16, 16, 1, 16, 16, 1, 4, tk, 8, 2, 64, 512, 128, 128, 0.1, 1, None)
+    assert prompt(MOST - 200) == -6
+
+
 def test_pools_of_no_pages_are_taken():
     """No refusal for want of pages: the next one in the order of the checks comes."""
     assert paged(pages=0, k=None, v=None, q=24) == -4
