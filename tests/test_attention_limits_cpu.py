@@ -16,6 +16,13 @@ def paged(**kw):
     return _lib.load().hq_paged_attention(*a.values())
 
 
+def step(**kw):
+    a = dict(pool=16, planes=2, bytes=32, table=1 << 44, lengths=2 << 44, refs=3 << 44, parent=4 << 44, add=5 << 44, to=6 << 44, lo=7 << 44,
+             ro=8 << 44, so=9 << 44, missing=10 << 44, rows=3, width=4, pages=9, page=16, stream=None)
+    a.update(kw)
+    return _lib.load().hq_cache_step(*a.values())
+
+
 def test_pages_of_four_gibibytes():
     """Bytes of a page, all heads: kv_heads * head_dim * 2 * page_size in 32 bits."""
     assert paged(page=1024, kv=16384, heads=16384, qs=16384 * 128) == -6
@@ -32,6 +39,12 @@ def test_prompts_within_a_workgroup_of_two_to_the_31():
     def prompt(tk):
         return _lib.load().hq_prompt_attention(16, 16, 16, 16, 1, 16, 16, 1, 4, tk, 8, 2, 64, 512, 128, 128, 0.1, 1, None)
     assert prompt(MOST - 200) == -6
+
+
+def test_steps_of_too_many_pages_and_of_pages_too_large():
+    """Pages are numbered in 32 bits by loops that go a stretch beyond the last; a length is rounded up to whole pages in 32 bits."""
+    assert step(pages=MOST) == -6 and step(pages=MOST - 4095) == -6
+    assert step(width=1, page=MOST - 1024) == -6 and step(width=2, page=2 ** 30 - 600) == -6
 
 
 def test_pools_of_no_pages_are_taken():
