@@ -609,7 +609,7 @@ extern "C" int hq_cache_step(void* pool, int planes, int64_t page_bytes, const i
     return HQ_ERR_MISALIGNED;
   const int64_t entries = (int64_t)rows * table_width;
   // lengths rounded up to whole pages, entries and pages stay in 32 bits, as do the stretches in which pages are gone through
-  if (rows > 16384 || ((int64_t)table_width + 1) * page_size > INT_MAX - 1024 || entries > INT_MAX || num_pages > INT_MAX / 4) return HQ_ERR_TOO_LARGE;
+  if (rows > 16384 || ((int64_t)table_width + 1) * page_size > INT_MAX - 1024 || entries > INT_MAX - 1024 || num_pages > INT_MAX / 4) return HQ_ERR_TOO_LARGE;
   const void* ins[] = {table, lengths, refs, parent, add};
   const int64_t nin[] = {4 * entries, 4 * (int64_t)rows, 4 * (int64_t)num_pages, 4 * (int64_t)rows, 4 * (int64_t)rows};
   const void* outs[] = {table_out, lengths_out, refs_out, starts_out, missing};

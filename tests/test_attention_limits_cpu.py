@@ -47,6 +47,11 @@ def test_steps_of_too_many_pages_and_of_pages_too_large():
     assert step(width=1, page=MOST - 1024) == -6 and step(width=2, page=2 ** 30 - 600) == -6
 
 
+def test_steps_of_too_many_entries():
+    """What is handed out is numbered in 32 bits by loops that go a workgroup beyond the last."""
+    assert step(rows=2, width=2 ** 30 - 1, page=1) == -6 and step(rows=16384, width=2 ** 17, page=1) == -6
+
+
 def test_pools_of_no_pages_are_taken():
     """No refusal for want of pages: the next one in the order of the checks comes."""
     assert paged(pages=0, k=None, v=None, q=24) == -4
