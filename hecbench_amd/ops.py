@@ -153,13 +153,13 @@ def paged_attention(q, k_pages, v_pages, table, lengths, groups=None, shared=Non
     """Attention of one token per request over a paged cache: q [requests][heads][64 or 128] over the first lengths[s] tokens of
     row s, token t being token t % page of page table[s][t // page] in k_pages and v_pages [pages][kv_heads][page][head size].
     groups (int32 [n + 1]) and shared (int32 [n]): the first shared[g] tokens of the requests groups[g] .. groups[g + 1] - 1 are in the
-    same pages, as cache_step leaves them, and are read once for all of them."""
+    same pages, as cache_step leaves them, and are read once for all of them.  Tokens of a page: a power of two, 8 ... 1024."""
     return _native.paged_attention(q, k_pages, v_pages, table, lengths, groups, shared, scale, out)
 
 
 def cache_write(k, v, k_pages, v_pages, table, starts, cu):
     """Tokens cu[s] .. cu[s + 1] - 1 of k and v [tokens][kv_heads][head size] become tokens starts[s] and on of row s of the table;
-    a token without a page is left out."""
+    a token without a page is left out.  Tokens of a page: a power of two, 1 ... 1024."""
     _native.cache_write(k, v, k_pages, v_pages, table, starts, cu)
 
 
@@ -168,7 +168,8 @@ def cache_step(pool, page_size, table, lengths, refs, parent, add, out=None):
     tokens more.  Whole pages are shared, a half-filled one is copied in every plane of pool [planes][pages][...] for each row but the
     first that goes on from it, new pages are the free ones (refs[p] <= 0), lowest first, to the rows in order.
     Returns (table, lengths, refs, starts, missing): starts are the lengths before the new tokens, missing (int32 [1]) the pages that
-    there were not - a row ends where its pages end.  out: five tensors for them that share nothing with the arguments."""
+    there were not - a row ends where its pages end.  out: five tensors for them that share nothing with the arguments.
+    page_size: any, but a cache that is to be written and attended to has a power of two, 8 ... 1024."""
     return _native.cache_step(pool, page_size, table, lengths, refs, parent, add, out)
 
 

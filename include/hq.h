@@ -344,7 +344,7 @@ int hq_mxfp4_qdq(const void* in, void* out, int64_t n_elems, int dtype, void* st
  *   them); ngroups 0: nothing is shared, and as many groups as requests or more are taken as none.  page_size a power of two, 8 ... 1024.
  *   A table entry that is needed and no page counts as a page of zeros (num_pages 0: all of them).
  * hq_cache_write: tokens cu[s] ... cu[s+1]-1 of k and v [tokens][kv_heads][head_dim] (strides as above) become tokens starts[s], ... of row s
- *   of the table; any head_dim that is a multiple of 8, any page_size.  A token whose place is outside its row, or in no page, is left out.
+ *   of the table; any head_dim that is a multiple of 8, page_size a power of two, 1 ... 1024.  A token whose place is outside its row, or in no page, is left out.
  * hq_cache_step: from the tables of one step to the next one's.  Row s inherits row parent[s] (of the old tables; any number outside
  *   0 ... rows-1: nothing) and gets room for add[s] tokens (negative: none) as far as its table_width pages reach.  Whole pages are
  *   shared; a half-filled one stays with the first row that inherits it and is copied, all page_bytes of it in every one of the
@@ -352,7 +352,8 @@ int hq_mxfp4_qdq(const void* in, void* out, int64_t n_elems, int dtype, void* st
  *   caller counts there); a page with refs <= 0 after the old rows have gone and the new ones come is free, and the pages that are asked for, row by row
  *   and front to back, are the free ones, lowest first.  Where there are no more, the entry is -1, the row ends before it and
  *   *missing counts it.  lengths_out: the new lengths, starts_out: the inherited part of them; entries behind a row's last page
- *   are -1.  Outputs share no memory with inputs (HQ_ERR_BAD_SHAPE).  rows <= 16384.
+ *   are -1.  Outputs share no memory with inputs (HQ_ERR_BAD_SHAPE).  rows <= 16384.  Any page_size: one that is no power of two from 8 to
+ *   1024 makes tables of a cache that the operators above do not take.
  * hq_cache_compact: n pages are in use (refs > 0); those at n and beyond move, in order, into the free ones below n, in every plane;
  *   table_out and refs_out follow, *live = n.
  * All but hq_cache_write may use the stream's workspace, of whose need hq_reserve_workspace knows nothing.  Attention keeps the partial sums of

@@ -16,6 +16,13 @@ def paged(**kw):
     return _lib.load().hq_paged_attention(*a.values())
 
 
+def write(**kw):
+    a = dict(k=16, v=16, kp=16, vp=16, dtype=1, table=16, starts=16, cu=16, rows=2, tokens=3, width=4, pages=9, page=16, kv=2, d=64, ks=128, vs=128,
+             stream=None)
+    a.update(kw)
+    return _lib.load().hq_cache_write(*a.values())
+
+
 def step(**kw):
     a = dict(pool=16, planes=2, bytes=32, table=1 << 44, lengths=2 << 44, refs=3 << 44, parent=4 << 44, add=5 << 44, to=6 << 44, lo=7 << 44,
              ro=8 << 44, so=9 << 44, missing=10 << 44, rows=3, width=4, pages=9, page=16, stream=None)
@@ -50,6 +57,12 @@ def test_steps_of_too_many_pages_and_of_pages_too_large():
 def test_steps_of_too_many_entries():
     """What is handed out is numbered in 32 bits by loops that go a workgroup beyond the last."""
     assert step(rows=2, width=2 ** 30 - 1, page=1) == -6 and step(rows=16384, width=2 ** 17, page=1) == -6
+
+
+def test_page_sizes_that_are_not_written():
+    """Powers of two up to 1024, as attention takes them from 8 on."""
+    assert write(page=24) == -2 and write(page=2048) == -2 and write(page=3) == -2
+    assert paged(page=24) == -2 and paged(page=2048) == -2
 
 
 def test_pools_of_no_pages_are_taken():
