@@ -713,5 +713,5 @@ extern "C" int hq_cache_compact(void* pool, int planes, int64_t page_bytes, cons
   a.pairs = a.to + num_pages;  // half of the pages at most move
   rc = hq_launch_as_is(compact_plan_kernel, dim3(1), dim3(kThreads), 0, (hipStream_t)stream, a);
   if (rc != HQ_OK || (entries == 0 && (planes == 0 || page_bytes == 0))) return rc;
-  return hq_launch_as_is(compact_move_kernel, dim3((unsigned)std::min<int64_t>(most * ((page_bytes / 16 + kThreads - 1) / kThreads), 32768)), dim3(kThreads), 0, (hipStream_t)stream, a);
+  return hq_launch_as_is(compact_move_kernel, dim3((unsigned)std::min<int64_t>(most * std::max<int64_t>(1, (page_bytes / 16 + kThreads - 1) / kThreads), 32768)), dim3(kThreads), 0, (hipStream_t)stream, a);
 }
