@@ -1019,9 +1019,10 @@ __device__ __forceinline__ Pages<T, D> pages_of(const PagedArgs& a, int request,
 }
 
 // The shares of up to 16 rows together, by one workgroup: 16 threads a row, whose loads are of two values each, side by side, and the
-// shares divided among the sets of threads that there are then.  Written by others a moment ago: read past the caches of this XCD.
+// shares, `step` places apart, divided among the sets of threads that there are then.  Written by others a moment ago: read past the caches
+// of this XCD.  all: the rows' results; else the sums go to the place of the first of the shares, which has been read by then.
 template <typename T, int D>
-__device__ __forceinline__ void join_here(const PagedArgs& a, char* sm, int nrows, int64_t row0, int64_t place, int slots) {
+__device__ __forceinline__ void join_here(const PagedArgs& a, char* sm, int nrows, int64_t row0, int64_t place, int64_t step, int slots, bool all) {
   constexpr int N = D / 16, AT_ONCE = 4;
   const int log = nrows > 8 ? 4 : nrows > 4 ? 3 : nrows > 2 ? 2 : nrows > 1, sets = 16 >> log;
   const int set = threadIdx.x >> (4 + log), row = (threadIdx.x >> 4) & ((1 << log) - 1), d0 = (threadIdx.x & 15) * 2;
@@ -1034,9 +1035,9 @@ __device__ __forceinline__ void join_here(const PagedArgs& a, char* sm, int nrow
 #pragma unroll
     for (int i = 0; i < AT_ONCE; ++i) {
       const int s = min(s0 + i * sets, slots - 1);
-      ml[i] = __hip_atomic_load(pm + (int64_t)s * a.heads, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      ml[i] = __hip_atomic_load(pm + s * step, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 #pragma unroll
-      for (int j = 0; j < N / 2; ++j) v[i][j] = __hip_atomic_load(po + (int64_t)s * a.heads * (D / 2) + 16 * j, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      for (int j = 0; j < N / 2; ++j) v[i][j] = __hip_atomic_load(po + s * step * (D / 2) + 16 * j, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
     float top = m;
 #pragma unroll
@@ -1065,22 +1066,32 @@ __device__ __forceinline__ void join_here(const PagedArgs& a, char* sm, int nrow
     for (int j = 0; j < N; ++j) sums[(2 + j) * kThreads] = o[j];
     __syncthreads();
     if (set) return;
-    const int step = 16 << log;
+    const int apart = 16 << log;
     float top = m;
-    for (int s = 1; s < sets; ++s) top = fmaxf(top, sums[s * step]);
+    for (int s = 1; s < sets; ++s) top = fmaxf(top, sums[s * apart]);
     const float own = __builtin_amdgcn_exp2f(m - finite_or_zero(top));
     m = top;
     l *= own;
 #pragma unroll
     for (int j = 0; j < N; ++j) o[j] *= own;
     for (int s = 1; s < sets; ++s) {
-      const float w = __builtin_amdgcn_exp2f(sums[s * step] - finite_or_zero(top));
-      l += w * sums[s * step + kThreads];
+      const float w = __builtin_amdgcn_exp2f(sums[s * apart] - finite_or_zero(top));
+      l += w * sums[s * apart + kThreads];
 #pragma unroll
-      for (int j = 0; j < N; ++j) o[j] += w * sums[s * step + (2 + j) * kThreads];
+      for (int j = 0; j < N; ++j) o[j] += w * sums[s * apart + (2 + j) * kThreads];
     }
   }
   if (row >= nrows) return;
+  if (!all) {
+    auto put = [](const unsigned long long* to, float x, float y) {
+      __hip_atomic_store(const_cast<unsigned long long*>(to), (unsigned long long)__float_as_uint(y) << 32 | __float_as_uint(x), __ATOMIC_RELAXED,
+                         __HIP_MEMORY_SCOPE_AGENT);
+    };
+#pragma unroll
+    for (int j = 0; j < N / 2; ++j) put(po + 16 * j, o[2 * j], o[2 * j + 1]);
+    if (d0 == 0) put(pm, m, l);
+    return;
+  }
   const bool none = m == -INFINITY;
   typedef T T2 __attribute__((ext_vector_type(2)));
 #pragma unroll
@@ -1088,12 +1099,13 @@ __device__ __forceinline__ void join_here(const PagedArgs& a, char* sm, int nrow
     *reinterpret_cast<T2*>((T*)a.out + at * D + d0 + 16 * j) = none ? T2{(T)0.f, (T)0.f} : T2{(T)result(o[j], o[j] / l), (T)result(o[j + 1], o[j + 1] / l)};
 }
 
+constexpr int kJoin = 32, kTeam = 16;  // shares that are joined at once, of that many and of more
 constexpr int kApart = 16;  // counters, a line of 64 bytes each: atomics on one line wait for each other (64 shares: 17.7 us, apart 14.5)
 
 // Up to 16 rows (request, head of the group), those of requests b0 ..., all of which see the keys.
 template <typename T, int D>
 __device__ __forceinline__ void few_rows(const PagedArgs& a, char* sm, int b0, int nrows, int head, int first, int end, int64_t slot,
-                                         int shares, int before) {
+                                         int shares, int before, int item) {
   typedef typename Kind<T>::V8 V8;
   const int lane = threadIdx.x & 63, last_row = nrows - 1, r = min(lane & 15, last_row);
   const uint32_t ratio = a.ratio;
@@ -1127,18 +1139,27 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, char* sm, int b0, i
                          __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
   if (!a.arrived) return;
-  // The last share to arrive joins them all, and there is no second launch.  For up to 32 shares: the last one's trips grow with them
-  // (32 / 8 heads of 128; a request of 333 keys in two launches 9.7 us, in one 8.2; 4 of 8192, 16 shares, 21.6 and 20.7; 2 of 8192, 32
-  // shares, 15.4 and 15.7; one, 64 shares, 11.9 and 14.5).
+  // The last share to arrive joins them all, and there is no second launch.  (32 / 8 heads of 128; a request of 333 keys in two launches 9.7 us,
+  // in one 8.2; 4 of 8192, 16 shares, 21.6 and 20.7; 2 of 8192, 32 shares, 15.4 and 15.7; one, 64 shares, 11.9 and 14.5.)  The trips of the last
+  // one grow with the shares, of which a long request among short ones has many: beyond 32, every 16 are joined first, by the last of them.
   __shared__ unsigned nth;
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  __syncthreads();
-  unsigned* const count = a.arrived + (b0 * a.kv_heads + head) * kApart;
-  if (threadIdx.x == 0) nth = __hip_atomic_fetch_add(count, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  __syncthreads();
-  if (nth != (unsigned)shares - 1) return;
-  if (threadIdx.x == 0) __hip_atomic_store(count, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  join_here<T, D>(a, sm, nrows, (int64_t)b0 * a.heads + head * ratio, (int64_t)(before - b0) * a.heads, shares);
+  int n = shares, unit = 1, index = item - before;  // what there is to be joined, shares of each, and which of them this is
+  for (;;) {
+    const bool all = n <= kJoin;
+    const int team = all ? 0 : index / kTeam, members = all ? n : min(kTeam, n - team * kTeam), first_share = before + team * kTeam * unit;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    unsigned* const count = a.arrived + (int64_t)((all ? a.items + b0 : first_share) * a.kv_heads + head) * kApart;
+    if (threadIdx.x == 0) nth = __hip_atomic_fetch_add(count, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    if (nth != (unsigned)members - 1) return;
+    if (threadIdx.x == 0) __hip_atomic_store(count, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    join_here<T, D>(a, sm, nrows, (int64_t)b0 * a.heads + head * ratio, (int64_t)(first_share - b0) * a.heads, (int64_t)unit * a.heads, members, all);
+    if (all) return;
+    index = team;
+    n = (n + kTeam - 1) / kTeam;
+    unit *= kTeam;
+  }
 }
 
 // Up to 128 of them; a row sees keys up to its request's length.
@@ -1186,7 +1207,7 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void paged_alone_kernel(
   Share s;
   if (!s.find(a, item, x == 0 && threadIdx.x < 64 && a.np)) return;
   const int64_t place = ((int64_t)item - s.b) * a.heads;
-  if (FEW) few_rows<T, D>(a, sm, s.b, a.ratio, head, s.first, s.end, place, s.count, s.before);
+  if (FEW) few_rows<T, D>(a, sm, s.b, a.ratio, head, s.first, s.end, place, s.count, s.before, item);
   else many_rows<T, D>(a, sm, &poison, s.b, a.ratio, row0, head, s.first, s.end, place, s.count);
 }
 
@@ -1246,7 +1267,7 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void paged_kernel(PagedA
     row0 = tile * 128;
     slot = a.most_np + share;
   }
-  if (few) few_rows<T, D>(a, sm, b0, nb * a.ratio, head, first, end, slot, 0, 0);
+  if (few) few_rows<T, D>(a, sm, b0, nb * a.ratio, head, first, end, slot, 0, 0, 0);
   else many_rows<T, D>(a, sm, &poison, b0, nb * a.ratio, row0, head, first, end, slot, 0);
 }
 
@@ -1444,7 +1465,7 @@ int launch_paged(PagedArgs a, int cus, hipStream_t stream) {
       alone = a.ratio <= 16 && slots <= 32;
     }
     floats = places * (D + 2) + 1 + 2 * (int64_t)a.batch;
-    counters = alone ? own * kApart : 0;
+    counters = alone ? (a.items + (int64_t)a.batch) * a.kv_heads * kApart : 0;  // a place for every share's team, and one for the request
     // While the stream is captured and has no room for shares: every request by itself, then in one share.  Longer, and no error.
     if (!places || !hq_workspace_out_of_reach(stream, floats, counters)) break;
     if (!a.ngroups) divide = false;

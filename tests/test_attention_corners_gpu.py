@@ -266,6 +266,25 @@ def test_paged_pools_of_no_pages(hq):
         assert (out == 0).all()
 
 
+@pytest.mark.parametrize("kind,D", [("bf16", 128), ("f16", 64)])
+@pytest.mark.parametrize("heads", [(12, 1), (1, 1), (16, 2), (3, 1), (24, 1)])
+def test_paged_one_long_request_among_short_ones(hq, kind, D, heads):
+    """Hundreds of shares of one request where the others have one: joined in several steps, on counters that the call before left."""
+    dtype, u = TYPES[kind]
+    for n, lengths in enumerate(([20000] + [1] * 16, [0, 3, 30000] + [130] * 17, [100, 4300, 0, 5000] + [7] * 8, [40000] + [50] * 40)):
+        q, k, v, table, lengths = paged_case(60 + n, dtype, lengths, heads, D, 16)
+        args = (q, k, v, i32(table), i32(lengths))
+        out = hq.paged_attention(*args)
+        check_paged(out, q, k, v, table, lengths, 1 / math.sqrt(D), u)
+        assert torch.equal(out, hq.paged_attention(*args))
+        bad = 0 if lengths[0] > 1000 else 2 if n == 1 else 3
+        k[table[bad][-3], :, 5] = math.nan
+        again = hq.paged_attention(*args)
+        assert torch.isnan(again[bad]).all()
+        again[bad] = out[bad]
+        assert torch.equal(again, out)
+
+
 # ---- no room for shares -----------------------------------------------------------------------------------------------------
 def captured(call, stream):
     graph = torch.cuda.CUDAGraph()
