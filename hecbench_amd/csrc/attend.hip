@@ -1235,7 +1235,7 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void paged_kernel(PagedA
     if (tile >= all) return;
     int n = 0;
     nb = 0;
-    for (int g0 = 0; nb == 0; g0 += 64) {
+    for (int g0 = 0; nb == 0 && g0 < a.ngroups; g0 += 64) {
       const Groups g = g0 ? Groups(a, g0) : some;
       const int own = tiles(g), sum = (int)running_sum(own), total = __builtin_amdgcn_readlane(sum, 63);
       if (tile < total) {
@@ -1248,6 +1248,7 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void paged_kernel(PagedA
         tile -= total;
       }
     }
+    if (nb == 0) return;  // only where bounds that do not ascend make more tiles than 32 bits count
     share_of(n, np, 256, slot, &first, &end);
     few = nb * ratio <= 16 && !__ballot(lane < nb && a.lengths[b0 + min(lane, nb - 1)] < end);
     row0 = tile * 128;

@@ -266,6 +266,17 @@ def test_paged_pools_of_no_pages(hq):
         assert (out == 0).all()
 
 
+def test_paged_bounds_of_groups_that_do_not_ascend(hq):
+    """Whatever they are, the call ends, and requests in no group are what they are without groups."""
+    dtype, u = TYPES["bf16"]
+    q, k, v, table, lengths = paged_case(70, dtype, [300 + 7 * i for i in range(90)], (8, 2), 128, 16)
+    for groups in ([0, 80, 3, 80, -5, 70], [80, 0, 10 ** 9, 5, -2 ** 31, 60], [40, 40, 39, 38, 37, 36]):
+        out = hq.paged_attention(q, k, v, i32(table), i32(lengths), i32(groups), i32([64, 0, 16, 2 ** 31 - 1, -1]))
+        inside = [any(max(min(a, 90), 0) <= s < max(min(b, 90), min(a, 90), 0) for a, b in zip(groups, groups[1:])) for s in range(90)]
+        free = [s for s in range(90) if not inside[s]]
+        check_paged(out[free], q[free], k, v, [table[s] for s in free], [lengths[s] for s in free], 1 / math.sqrt(128), u)
+
+
 @pytest.mark.parametrize("kind,D", [("bf16", 128), ("f16", 64)])
 @pytest.mark.parametrize("heads", [(12, 1), (1, 1), (16, 2), (3, 1), (24, 1)])
 def test_paged_one_long_request_among_short_ones(hq, kind, D, heads):
