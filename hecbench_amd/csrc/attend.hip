@@ -1103,7 +1103,7 @@ constexpr int kJoin = 32, kTeam = 16;  // shares that are joined at once, of tha
 constexpr int kApart = 16;  // counters, a line of 64 bytes each: atomics on one line wait for each other (64 shares: 17.7 us, apart 14.5)
 
 // Up to 16 rows (request, head of the group), those of requests b0 ..., all of which see the keys.
-template <typename T, int D>
+template <typename T, int D, bool JOINS>
 __device__ __forceinline__ void few_rows(const PagedArgs& a, char* sm, int b0, int nrows, int head, int first, int end, int64_t slot,
                                          int shares, int before, int item) {
   typedef typename Kind<T>::V8 V8;
@@ -1138,7 +1138,7 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, char* sm, int b0, i
       __hip_atomic_store(reinterpret_cast<unsigned long long*>(a.pm) + place, (unsigned long long)__float_as_uint(total) << 32 | __float_as_uint(share_top(top, first < end)),
                          __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
-  if (!a.arrived) return;
+  if (!JOINS || !a.arrived) return;
   // The last share to arrive joins them all, and there is no second launch.  (32 / 8 heads of 128; a request of 333 keys in two launches 9.7 us,
   // in one 8.2; 4 of 8192, 16 shares, 21.6 and 20.7; 2 of 8192, 32 shares, 15.4 and 15.7; one, 64 shares, 11.9 and 14.5.)  The trips of the last
   // one grow with the shares, of which a long request among short ones has many: beyond 32, every 16 are joined first, by the last of them.
@@ -1207,7 +1207,7 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void paged_alone_kernel(
   Share s;
   if (!s.find(a, item, x == 0 && threadIdx.x < 64 && a.np)) return;
   const int64_t place = ((int64_t)item - s.b) * a.heads;
-  if (FEW) few_rows<T, D>(a, sm, s.b, a.ratio, head, s.first, s.end, place, s.count, s.before, item);
+  if (FEW) few_rows<T, D, true>(a, sm, s.b, a.ratio, head, s.first, s.end, place, s.count, s.before, item);
   else many_rows<T, D>(a, sm, &poison, s.b, a.ratio, row0, head, s.first, s.end, place, s.count);
 }
 
@@ -1268,7 +1268,7 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void paged_kernel(PagedA
     row0 = tile * 128;
     slot = a.most_np + share;
   }
-  if (few) few_rows<T, D>(a, sm, b0, nb * a.ratio, head, first, end, slot, 0, 0, 0);
+  if (few) few_rows<T, D, false>(a, sm, b0, nb * a.ratio, head, first, end, slot, 0, 0, 0);
   else many_rows<T, D>(a, sm, &poison, b0, nb * a.ratio, row0, head, first, end, slot, 0);
 }
 
