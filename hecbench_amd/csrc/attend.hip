@@ -1,7 +1,7 @@
 // Attention: over whole prompts packed one behind the other, and of one query a request over a paged cache.
 //
-// For a query row q: out = sum_j p_j v_j / sum_j p_j, p_j = 2^(c q.k_j - m), c = scale * log2(e), in one pass over the keys with the
-// running maximum m of the row; a larger maximum scales what has been summed so far.
+// For a query row q: out = sum_j p_j v_j / sum_j p_j, p_j = 2^(c q.k_j - m), c = scale * log2(e), in one pass over the keys with an m that
+// follows the row's maximum; a larger one scales what has been summed so far.
 //
 // Two ways through the keys.  Many rows (Many): a tile of 64 keys in LDS serves 128 rows, 32 a wave.  Few (Few): 16 rows at most, each
 // wave goes through keys of its own, as what bounds it is their way from memory, and the waves' sums come together at the end.
@@ -1139,9 +1139,10 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, char* sm, int b0, i
                          __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
   if (!JOINS || !a.arrived) return;
-  // The last share to arrive joins them all, and there is no second launch.  (32 / 8 heads of 128; a request of 333 keys in two launches 9.7 us,
-  // in one 8.2; 4 of 8192, 16 shares, 21.6 and 20.7; 2 of 8192, 32 shares, 15.4 and 15.7; one, 64 shares, 11.9 and 14.5.)  The trips of the last
-  // one grow with the shares, of which a long request among short ones has many: beyond 32, every 16 are joined first, by the last of them.
+  // The last share to arrive joins them all, and there is no second launch.  (32 / 8 heads of 128; a request of 333 keys in two launches 9.8 us,
+  // in one 8.0; 4 of 8192, 16 shares, 29.6 and 28.7; 2 of 8192, 32 shares, 16.4 and 16.8; one, 64 shares at once, 11.9 and 14.5.)  The trips of the
+  // last one grow with the shares, of which a long request among short ones has many: beyond 32, every 16 are joined first, by the last of them
+  // (12 / 1 heads, one of 60000 among 16 of a token, 469 shares: 86.6 us at once, 22.1).
   __shared__ unsigned nth;
   int n = shares, unit = 1, index = item - before;  // what there is to be joined, shares of each, and which of them this is
   for (;;) {
