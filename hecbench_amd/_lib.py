@@ -58,6 +58,10 @@ _SIGNATURES = {
                            + [_c.c_int64, _c.c_float, _c.c_void_p]),
     "hq_cache_write": (_c.c_int, [_c.c_void_p] * 4 + [_c.c_int] + [_c.c_void_p] * 3 + [_c.c_int, _c.c_int64] + [_c.c_int] * 5
                        + [_c.c_int64] * 2 + [_c.c_void_p]),
+    "hq_norm_rotate": (_c.c_int, [_c.c_void_p] * 4 + [_c.c_int] + [_c.c_void_p] * 4 + [_c.c_int64] + [_c.c_int] * 5 + [_c.c_int64] * 4
+                       + [_c.c_float, _c.c_int, _c.c_void_p]),
+    "hq_cache_write_rotated": (_c.c_int, [_c.c_void_p] * 6 + [_c.c_int] + [_c.c_void_p] * 6 + [_c.c_int, _c.c_int64] + [_c.c_int] * 8
+                               + [_c.c_int64] * 4 + [_c.c_float, _c.c_int, _c.c_void_p]),
     "hq_cache_step": (_c.c_int, [_c.c_void_p, _c.c_int, _c.c_int64] + [_c.c_void_p] * 10 + [_c.c_int] * 4 + [_c.c_void_p]),
     "hq_cache_compact": (_c.c_int, [_c.c_void_p, _c.c_int, _c.c_int64] + [_c.c_void_p] * 5 + [_c.c_int] * 3 + [_c.c_void_p]),
     "hq_probe_stream": (_c.c_int, [_c.c_int, _c.c_void_p, _c.c_void_p, _c.c_int64, _c.c_void_p]),

@@ -521,6 +521,101 @@ PyObject* cache_write(PyObject* const* a) {  // k, v, k_pages, v_pages, table, s
   Py_RETURN_NONE;
 }
 
+// The rows that take what the argument `like` becomes: the caller's (its own object is returned), or new ones one behind the other.
+struct RowsOut {
+  PyObject* given;
+  at::Tensor t;
+  int64_t stride;
+  RowsOut(PyObject* o, const char* name, const Rows& like)
+      : given(o == Py_None ? nullptr : o), stride(like.heads * like.size) {
+    if (!given) return;
+    const Rows r = rows_of(o, name, dt(like.t->scalar_type()));
+    if (r.tokens != like.tokens || r.heads != like.heads || r.size != like.size) value_error(std::string(name) + " must have the shape of its argument");
+    t = *r.t;
+    stride = r.stride;
+  }
+  const at::Tensor* checked() const { return given ? &t : nullptr; }
+  void make(const Rows& like) {
+    if (!given) t = fresh({like.tokens, like.heads, like.size}, like.t->scalar_type(), *like.t);
+  }
+  PyObject* release() {
+    if (given) { Py_INCREF(given); return given; }
+    return THPVariable_Wrap(std::move(t));
+  }
+};
+// cos_sin [positions][rotated elements]
+struct Angles {
+  const at::Tensor* t;
+  int positions = 0, rotary = 0;
+  explicit Angles(PyObject* o, int64_t head_size) : t(tensor(o, "cos_sin", kF32, -1, true)) {
+    if (!t) return;
+    if (t->dim() != 2) value_error("cos_sin must be [positions][rotated elements]");
+    positions = size_of(t->size(0));
+    if (t->size(1) > head_size) value_error("cos_sin must not hold more elements than a head");
+    rotary = (int)t->size(1);
+  }
+};
+
+PyObject* norm_rotate(PyObject* const* a) {  // q, k, cos_sin, positions, q_weight, k_weight, eps, interleaved, q_out, k_out
+  const Rows q = rows_of(a[0], "q", kF16 | kBF16), k = rows_of(a[1], "k", kF16 | kBF16);
+  same_type(*q.t, *k.t, "k");
+  if (k.tokens != q.tokens || k.size != q.size) value_error("k must be [tokens of q][heads][head size of q]");
+  const Angles angles(a[2], q.size);
+  const at::Tensor* positions = tensor(a[3], "positions", kI32, q.tokens, !angles.rotary);
+  const at::Tensor* qw = tensor(a[4], "q_weight", dt(q.t->scalar_type()), q.size, true);
+  const at::Tensor* kw = tensor(a[5], "k_weight", dt(q.t->scalar_type()), q.size, true);
+  const float eps = real(a[6]);
+  const int interleaved = PyObject_IsTrue(a[7]);
+  if (interleaved < 0) throw python_error();
+  RowsOut qo(a[8], "out[0]", q), ko(a[9], "out[1]", k);
+  same_device(q.t, k.t, angles.t, positions, qw, kw, qo.checked(), ko.checked());
+  qo.make(q);
+  ko.make(k);
+  const int hq = size_of(q.heads), hk = size_of(k.heads), d = size_of(q.size);
+  void* st = stream();
+  call("hq_norm_rotate", [&] {
+    return hq_norm_rotate(ptr(q.t), ptr(k.t), qo.t.data_ptr(), ko.t.data_ptr(), act_dtype(*q.t), ptr(qw), ptr(kw), in<float>(angles.t),
+                          in<int32_t>(positions), q.tokens, hq, hk, d, angles.rotary, angles.positions, q.stride, k.stride, qo.stride, ko.stride, eps,
+                          interleaved, st);
+  });
+  THPObjectPtr x(qo.release()), y(ko.release());
+  return PyTuple_Pack(2, x.get(), y.get());
+}
+
+PyObject* cache_write_rotated(PyObject* const* a) {  // q, k, v, k_pages, v_pages, table, starts, cu, cos_sin, q_weight, k_weight, eps, interleaved, out
+  const Rows q = rows_of(a[0], "q", kF16 | kBF16), k = rows_of(a[1], "k", kF16 | kBF16), v = rows_of(a[2], "v", kF16 | kBF16);
+  same_type(*q.t, *k.t, "k");
+  same_type(*q.t, *v.t, "v");
+  if (k.tokens != q.tokens || k.size != q.size) value_error("k must be [tokens of q][heads][head size of q]");
+  if (v.tokens != k.tokens || v.heads != k.heads || v.size != k.size) value_error("v must have the shape of k");
+  const at::Tensor* kp = tensor(a[3], "k_pages", dt(k.t->scalar_type()));
+  if (kp->dim() != 4 || kp->size(1) != k.heads || kp->size(3) != k.size) value_error("k_pages must be [pages][heads of k][tokens of a page][head size of k]");
+  const at::Tensor* vp = tensor(a[4], "v_pages", dt(k.t->scalar_type()), kp->numel());
+  if (vp->sizes() != kp->sizes()) value_error("v_pages must have the shape of k_pages");
+  const at::Tensor* table = tensor(a[5], "table", kI32);
+  if (table->dim() != 2) value_error("table must be [requests][pages of a request]");
+  const at::Tensor* starts = tensor(a[6], "starts", kI32, table->size(0));
+  const at::Tensor* cu = tensor(a[7], "cu", kI32, table->size(0) + 1);
+  const Angles angles(a[8], q.size);
+  const at::Tensor* qw = tensor(a[9], "q_weight", dt(q.t->scalar_type()), q.size, true);
+  const at::Tensor* kw = tensor(a[10], "k_weight", dt(q.t->scalar_type()), q.size, true);
+  const float eps = real(a[11]);
+  const int interleaved = PyObject_IsTrue(a[12]);
+  if (interleaved < 0) throw python_error();
+  RowsOut qo(a[13], "out", q);
+  same_device(q.t, k.t, v.t, kp, vp, table, starts, cu, angles.t, qw, kw, qo.checked());
+  qo.make(q);
+  const int rows = size_of(table->size(0)), width = size_of(table->size(1)), pages = size_of(kp->size(0)), page = size_of(kp->size(2)),
+            hq = size_of(q.heads), hk = size_of(k.heads), d = size_of(q.size);
+  void* st = stream();
+  call("hq_cache_write_rotated", [&] {
+    return hq_cache_write_rotated(ptr(q.t), ptr(k.t), ptr(v.t), qo.t.data_ptr(), kp->data_ptr(), vp->data_ptr(), act_dtype(*q.t), ptr(qw), ptr(kw),
+                                  in<float>(angles.t), in<int32_t>(table), in<int32_t>(starts), in<int32_t>(cu), rows, q.tokens, width, pages, page, hq,
+                                  hk, d, angles.rotary, angles.positions, q.stride, k.stride, v.stride, qo.stride, eps, interleaved, st);
+  });
+  return qo.release();
+}
+
 // The pool [planes][pages][...]: bytes of a page.
 int64_t page_bytes_of(const at::Tensor& pool, int64_t pages) {
   if (pool.dim() < 3 || pool.size(1) != pages) value_error("pool must be [planes][pages][...], with a count in refs for every page");
@@ -625,6 +720,8 @@ PyMethodDef kMethods[] = {
     HQ_METHOD("prompt_attention", prompt_attention, 8),
     HQ_METHOD("paged_attention", paged_attention, 9),
     HQ_METHOD("cache_write", cache_write, 7),
+    HQ_METHOD("norm_rotate", norm_rotate, 10),
+    HQ_METHOD("cache_write_rotated", cache_write_rotated, 14),
     HQ_METHOD("cache_step", cache_step, 8),
     HQ_METHOD("cache_compact", cache_compact, 4),
     {nullptr, nullptr, 0, nullptr}};

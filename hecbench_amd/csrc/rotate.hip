@@ -1,0 +1,340 @@
+// Heads of queries and keys normed and rotated by their tokens' positions, to where the caller says or, the keys, into the pages of the
+// cache, with the values.
+//
+// A head x of D elements: y = x * rsqrt(mean(x^2) + eps) * weight, and every pair (a, b) of the first `rotary` elements of y becomes
+// (a c - b s, b c + a s), c and s the cosine and sine of the pair's angle at the token's position.  One pass in fp32, one rounding.
+//
+// A lane holds two pieces of eight elements of a head, those that are rotated against each other, so that nothing but the sum of
+// the squares goes from lane to lane: D / 16 lanes a head, 64 * 16 / D heads at a time in a wave, a wave a token, whose cosines and
+// sines it reads once for all of them.  Bound by the copy; short calls by the launch and the loads that wait for another (positions, then
+// the table's row; in the cache's form bounds and starts, then the table's row and the page).
+#include <climits>
+#include <cmath>
+
+#include "hq_internal.h"
+
+namespace {
+
+constexpr int kThreads = 256, kWaves = kThreads / 64;
+
+struct RotateArgs {
+  const hq_u4v *q, *k, *v;
+  hq_u4v *qo, *ko, *vo;  // of the cache's form: ko and vo its pages
+  const hq_u4v *qw, *kw; // null: no norm
+  const hq_f4v* cs;      // [positions][rotary]: cosines, sines
+  const int *positions;  // of the plain form
+  const int *table, *starts, *cu;
+  int64_t qs, ks, vs, qos, kos;  // 16-byte pieces from one token to the next
+  int tokens, heads, kv_heads, all, rotary, known;  // all: heads of queries, keys and, in the cache's form, values; known: positions
+  int rows, width, pages, page_log, interleaved;
+  float eps;
+};
+
+template <typename T>
+__device__ __forceinline__ void wide(float (&x)[8], hq_u4v v) {
+  typedef T T8 __attribute__((ext_vector_type(8)));
+  const T8 t = __builtin_bit_cast(T8, v);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = (float)t[i];
+}
+template <typename T>
+__device__ __forceinline__ hq_u4v narrow(const float (&x)[8]) {
+  typedef T T8 __attribute__((ext_vector_type(8)));
+  T8 t;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) t[i] = (T)x[i];
+  return __builtin_bit_cast(hq_u4v, t);
+}
+// Sum over the lanes of a head.
+template <int LANES>
+__device__ __forceinline__ float head_sum(float v) {
+  v = hq_quad(v, HqAdd());
+  return LANES == 8 ? v + hq_dpp<0x141>(v) : v;  // row_half_mirror
+}
+
+// The first i with bounds[i + 1] > t, n if there is none: a wave halves the range sixty-four-fold a step.
+__device__ __forceinline__ int find_row(const int* bounds, int n, int t) {
+  const int lane = threadIdx.x & 63;
+  int lo = 0;
+  while (n > 0) {
+    const int step = (n + 63) >> 6;
+    const int at = lo + min((lane + 1) * step, n);
+    const int below = __popcll(__ballot(bounds[at] <= t));
+    if (below == 64) return lo + n;
+    lo += below * step;
+    n = min(step, n - below * step) - 1;
+  }
+  return lo;
+}
+
+// STEPS sets of heads of a token a wave.
+template <typename T, int D, bool CACHE, int STEPS>
+__global__ __launch_bounds__(kThreads) void rotate_kernel(RotateArgs a, int parts) {
+  constexpr int LANES = D / 16, HEADS = 64 / LANES, CH = D / 8;
+  const unsigned wave = blockIdx.x * kWaves + (threadIdx.x >> 6);
+  const int t = __builtin_amdgcn_readfirstlane(wave / (unsigned)parts), part = __builtin_amdgcn_readfirstlane(wave % (unsigned)parts);
+  if (t >= a.tokens) return;
+  const int lane = threadIdx.x & 63, l = lane % LANES, np = a.rotary / 16;
+  const int pa = l < np ? l : 2 * l, pb = l < np ? l + np : 2 * l + 1;
+  const int first = part * (HEADS * STEPS) + lane / LANES;
+  hq_u4v xa[STEPS], xb[STEPS];
+#pragma unroll
+  for (int i = 0; i < STEPS; ++i) {
+    const int h = min(first + i * HEADS, a.all - 1);
+    const hq_u4v* const from = h < a.heads                  ? a.q + t * a.qs + h * CH
+                               : h < a.heads + a.kv_heads ? a.k + t * a.ks + (h - a.heads) * CH
+                                                          : a.v + t * a.vs + (h - a.heads - a.kv_heads) * CH;
+    xa[i] = from[pa];
+    xb[i] = from[pb];
+  }
+  hq_u4v wqa = {}, wqb = {}, wka = {}, wkb = {};
+  if (a.qw) {
+    wqa = a.qw[pa];
+    wqb = a.qw[pb];
+  }
+  if (a.kw) {
+    wka = a.kw[pa];
+    wkb = a.kw[pb];
+  }
+  int row = 0;
+  int64_t place;
+  if (CACHE) {
+    row = find_row(a.cu, a.rows, t);
+    if (row >= a.rows || t < a.cu[row]) return;
+    place = (int64_t)a.starts[row] + (t - a.cu[row]);
+  } else {
+    place = a.rotary ? a.positions[t] : 0;
+  }
+  float cs[8], sn[8];  // of the lane's pairs
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    cs[i] = 1.f;
+    sn[i] = 0.f;
+  }
+  if (l < np) {
+    const int at = (int)min(max(place, (int64_t)0), (int64_t)a.known - 1);
+    const hq_f4v* const c = a.cs + (int64_t)at * (a.rotary / 4);
+    const int i0 = a.interleaved ? l : 2 * l, i1 = a.interleaved ? l + np : 2 * l + 1, sines = a.rotary / 8;
+    const hq_f4v c0 = c[i0], c1 = c[i1], s0 = c[sines + i0], s1 = c[sines + i1];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      cs[i] = c0[i];
+      cs[4 + i] = c1[i];
+      sn[i] = s0[i];
+      sn[4 + i] = s1[i];
+    }
+  }
+  bool there = true;
+  int64_t to_page = 0;  // pieces of the token's row of head 0 in its page
+  if (CACHE) {
+    there = place >= 0 && place < (int64_t)a.width << a.page_log;
+    const int page = there ? a.table[(int64_t)row * a.width + (place >> a.page_log)] : -1;
+    there = (unsigned)page < (unsigned)a.pages;
+    to_page = ((((int64_t)page * a.kv_heads) << a.page_log) + (place & ((1 << a.page_log) - 1))) * CH;
+  }
+#pragma unroll
+  for (int i = 0; i < STEPS; ++i) {
+    const int h = first + i * HEADS;
+    const bool query = h < a.heads, key = !query && h < a.heads + a.kv_heads;
+    hq_u4v ya = xa[i], yb = xb[i];
+    if (query || key) {
+      float u[8], v[8];
+      wide<T>(u, xa[i]);
+      wide<T>(v, xb[i]);
+      float ss = 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) ss = fmaf(u[j], u[j], fmaf(v[j], v[j], ss));
+      ss = head_sum<LANES>(ss);
+      if (query ? a.qw != nullptr : a.kw != nullptr) {
+        float r = rsqrtf(fmaf(ss, 1.f / D, a.eps)), pre = 1.f;
+        if (__builtin_expect(!(ss < INFINITY), 0)) {  // bf16 holds numbers whose squares fp32 does not
+          pre = 0x1p-70f;
+          ss = 0.f;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) ss = fmaf(u[j] * pre, u[j] * pre, fmaf(v[j] * pre, v[j] * pre, ss));
+          r = rsqrtf(fmaf(head_sum<LANES>(ss), 1.f / D, a.eps * pre * pre));
+        }
+        float wu[8], wv[8];
+        wide<T>(wu, query ? wqa : wka);
+        wide<T>(wv, query ? wqb : wkb);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          u[j] = u[j] * pre * r * wu[j];
+          v[j] = v[j] * pre * r * wv[j];
+        }
+      }
+      if (a.interleaved) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float u0 = u[2 * j], v0 = v[2 * j];
+          u[2 * j] = u0 * cs[j] - u[2 * j + 1] * sn[j];
+          u[2 * j + 1] = u[2 * j + 1] * cs[j] + u0 * sn[j];
+          v[2 * j] = v0 * cs[4 + j] - v[2 * j + 1] * sn[4 + j];
+          v[2 * j + 1] = v[2 * j + 1] * cs[4 + j] + v0 * sn[4 + j];
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float u0 = u[j];
+          u[j] = u0 * cs[j] - v[j] * sn[j];
+          v[j] = v[j] * cs[j] + u0 * sn[j];
+        }
+      }
+      ya = narrow<T>(u);
+      yb = narrow<T>(v);
+    }
+    hq_u4v* to;
+    if (query) to = a.qo + t * a.qos + h * CH;
+    else if (CACHE) to = (key ? a.ko : a.vo) + to_page + ((int64_t)(h - a.heads - (key ? 0 : a.kv_heads)) << a.page_log) * CH;
+    else to = a.ko + t * a.kos + (h - a.heads) * CH;
+    if (h < a.all && (query || there)) {
+      to[pa] = ya;
+      to[pb] = yb;
+    }
+  }
+}
+
+template <typename T, int D, bool CACHE>
+int launch_rotate(const RotateArgs& a, hipStream_t stream) {
+  constexpr int HEADS = 64 * 16 / D, STEPS = 2;
+  const int64_t parts = (a.all + HEADS * STEPS - 1) / (HEADS * STEPS), blocks = (a.tokens * parts + kWaves - 1) / kWaves;
+  if (blocks > INT_MAX / kWaves) return HQ_ERR_TOO_LARGE;
+  return hq_launch_as_is(rotate_kernel<T, D, CACHE, STEPS>, dim3((unsigned)blocks), dim3(kThreads), 0, stream, a, (int)parts);
+}
+#define HQ_BY_TYPE(cache)                                                                                                        \
+  (dtype == HQ_DTYPE_F16 ? (head_dim == 64 ? launch_rotate<_Float16, 64, cache>(a, s) : launch_rotate<_Float16, 128, cache>(a, s)) \
+                         : (head_dim == 64 ? launch_rotate<__bf16, 64, cache>(a, s) : launch_rotate<__bf16, 128, cache>(a, s)))
+
+// Rows of `bytes` bytes each, `stride` bytes apart.  Two of them meet nowhere, or (same) are the same rows.
+struct Region {
+  const void* p;
+  int64_t bytes, stride;
+};
+bool apart(const Region& x, const Region& y, int64_t tokens, bool same) {
+  const uintptr_t a = (uintptr_t)x.p, b = (uintptr_t)y.p;
+  if (same && a == b && (x.stride == y.stride || tokens == 1) && x.bytes == y.bytes) return true;
+  const uint64_t ax = (uint64_t)(tokens - 1) * x.stride + x.bytes, by = (uint64_t)(tokens - 1) * y.stride + y.bytes;
+  if (a + ax <= b || b + by <= a) return true;
+  if (x.stride != y.stride) return false;  // (one inside the other's gaps, by chance: refused)
+  // columns of one wide row: where y's first begins behind one of x's
+  const uint64_t d = (b >= a ? b - a : (uint64_t)x.stride - (a - b) % (uint64_t)x.stride) % (uint64_t)x.stride;
+  return d >= (uint64_t)x.bytes && d + (uint64_t)y.bytes <= (uint64_t)x.stride;
+}
+
+int check(int dtype, int head_dim, int rotary, int num_positions, const float* cos_sin, int64_t tokens, int heads, int kv_heads, float eps) {
+  if (tokens < 0 || heads < 1 || kv_heads < 1 || num_positions < 0 || rotary < 0 || rotary % 16 || rotary > head_dim) return HQ_ERR_BAD_SHAPE;
+  if (head_dim != 64 && head_dim != 128) return HQ_ERR_BAD_SHAPE;
+  if (dtype != HQ_DTYPE_F16 && dtype != HQ_DTYPE_BF16) return HQ_ERR_BAD_ENUM;
+  if (!(eps >= 0x1p-126f) || std::isinf(eps)) return HQ_ERR_BAD_SHAPE;
+  if (rotary && num_positions == 0 && tokens) return HQ_ERR_BAD_SHAPE;
+  if (rotary && tokens && !cos_sin) return HQ_ERR_NULL_POINTER;
+  if (tokens > INT_MAX || heads > 1 << 16 || kv_heads > 1 << 16) return HQ_ERR_TOO_LARGE;
+  return HQ_OK;
+}
+bool odd(const void* p, int64_t stride) { return ((uintptr_t)p & 15) || stride % 8; }
+
+}  // namespace
+
+extern "C" int hq_norm_rotate(const void* q, const void* k, void* q_out, void* k_out, int dtype, const void* q_weight, const void* k_weight,
+                              const float* cos_sin, const int32_t* positions, int64_t tokens, int heads, int kv_heads, int head_dim, int rotary,
+                              int num_positions, int64_t q_stride, int64_t k_stride, int64_t q_out_stride, int64_t k_out_stride, float eps,
+                              int interleaved, void* stream) {
+  const int rc = check(dtype, head_dim, rotary, num_positions, cos_sin, tokens, heads, kv_heads, eps);
+  if (rc != HQ_OK) return rc;
+  if (tokens == 0) return HQ_OK;
+  if (!q || !k || !q_out || !k_out || (rotary && !positions)) return HQ_ERR_NULL_POINTER;
+  const int64_t qn = (int64_t)heads * head_dim, kn = (int64_t)kv_heads * head_dim;
+  if (q_stride < qn || q_out_stride < qn || k_stride < kn || k_out_stride < kn) return HQ_ERR_BAD_SHAPE;
+  if (odd(q, q_stride) || odd(k, k_stride) || odd(q_out, q_out_stride) || odd(k_out, k_out_stride) || odd(q_weight, 0) || odd(k_weight, 0) ||
+      odd(cos_sin, 0) || ((uintptr_t)positions & 3))
+    return HQ_ERR_MISALIGNED;
+  constexpr int64_t kMost = (int64_t)1 << 31;  // elements: bytes of all rows in 63 bits
+  if (q_stride > kMost || k_stride > kMost || q_out_stride > kMost || k_out_stride > kMost) return HQ_ERR_TOO_LARGE;
+  const Region qi{q, 2 * qn, 2 * q_stride}, ki{k, 2 * kn, 2 * k_stride}, qo{q_out, 2 * qn, 2 * q_out_stride}, ko{k_out, 2 * kn, 2 * k_out_stride};
+  if (!apart(qo, qi, tokens, true) || !apart(ko, ki, tokens, true) || !apart(qo, ki, tokens, false) || !apart(ko, qi, tokens, false) ||
+      !apart(qo, ko, tokens, false))
+    return HQ_ERR_BAD_SHAPE;
+  const HqDevice* dev = nullptr;
+  const int dc = hq_current_device(&dev);
+  if (dc != HQ_OK) return dc;
+  RotateArgs a{};
+  a.q = (const hq_u4v*)q;
+  a.k = (const hq_u4v*)k;
+  a.qo = (hq_u4v*)q_out;
+  a.ko = (hq_u4v*)k_out;
+  a.qw = (const hq_u4v*)q_weight;
+  a.kw = (const hq_u4v*)k_weight;
+  a.cs = (const hq_f4v*)cos_sin;
+  a.positions = positions;
+  a.qs = q_stride / 8;
+  a.ks = k_stride / 8;
+  a.qos = q_out_stride / 8;
+  a.kos = k_out_stride / 8;
+  a.tokens = (int)tokens;
+  a.heads = heads;
+  a.kv_heads = kv_heads;
+  a.all = heads + kv_heads;
+  a.rotary = rotary;
+  a.known = num_positions;
+  a.interleaved = interleaved != 0;
+  a.eps = eps;
+  const hipStream_t s = (hipStream_t)stream;
+  return HQ_BY_TYPE(false);
+}
+
+extern "C" int hq_cache_write_rotated(const void* q, const void* k, const void* v, void* q_out, void* k_pages, void* v_pages, int dtype,
+                                      const void* q_weight, const void* k_weight, const float* cos_sin, const int32_t* table,
+                                      const int32_t* starts, const int32_t* cu, int rows, int64_t tokens, int table_width, int num_pages,
+                                      int page_size, int heads, int kv_heads, int head_dim, int rotary, int num_positions, int64_t q_stride,
+                                      int64_t k_stride, int64_t v_stride, int64_t q_out_stride, float eps, int interleaved, void* stream) {
+  const int rc = check(dtype, head_dim, rotary, num_positions, cos_sin, tokens, heads, kv_heads, eps);
+  if (rc != HQ_OK) return rc;
+  if (rows < 0 || table_width < 0 || num_pages < 0) return HQ_ERR_BAD_SHAPE;
+  if (page_size < 1 || page_size > 1024 || (page_size & (page_size - 1))) return HQ_ERR_BAD_SHAPE;
+  if (tokens == 0 || rows == 0) return HQ_OK;
+  if (!q || !k || !v || !q_out || !starts || !cu || (table_width && !table) || (table_width && num_pages && (!k_pages || !v_pages)))
+    return HQ_ERR_NULL_POINTER;
+  const int64_t qn = (int64_t)heads * head_dim, kn = (int64_t)kv_heads * head_dim;
+  if (q_stride < qn || q_out_stride < qn || k_stride < kn || v_stride < kn) return HQ_ERR_BAD_SHAPE;
+  if (odd(q, q_stride) || odd(k, k_stride) || odd(v, v_stride) || odd(q_out, q_out_stride) || odd(k_pages, 0) || odd(v_pages, 0) || odd(q_weight, 0) ||
+      odd(k_weight, 0) || odd(cos_sin, 0) || (((uintptr_t)table | (uintptr_t)starts | (uintptr_t)cu) & 3))
+    return HQ_ERR_MISALIGNED;
+  constexpr int64_t kMost = (int64_t)1 << 31;
+  if (q_stride > kMost || k_stride > kMost || v_stride > kMost || q_out_stride > kMost) return HQ_ERR_TOO_LARGE;
+  const Region qi{q, 2 * qn, 2 * q_stride}, ki{k, 2 * kn, 2 * k_stride}, vi{v, 2 * kn, 2 * v_stride}, qo{q_out, 2 * qn, 2 * q_out_stride};
+  if (!apart(qo, qi, tokens, true) || !apart(qo, ki, tokens, false) || !apart(qo, vi, tokens, false)) return HQ_ERR_BAD_SHAPE;
+  const HqDevice* dev = nullptr;
+  const int dc = hq_current_device(&dev);
+  if (dc != HQ_OK) return dc;
+  RotateArgs a{};
+  a.q = (const hq_u4v*)q;
+  a.k = (const hq_u4v*)k;
+  a.v = (const hq_u4v*)v;
+  a.qo = (hq_u4v*)q_out;
+  a.ko = (hq_u4v*)k_pages;
+  a.vo = (hq_u4v*)v_pages;
+  a.qw = (const hq_u4v*)q_weight;
+  a.kw = (const hq_u4v*)k_weight;
+  a.cs = (const hq_f4v*)cos_sin;
+  a.table = table;
+  a.starts = starts;
+  a.cu = cu;
+  a.qs = q_stride / 8;
+  a.ks = k_stride / 8;
+  a.vs = v_stride / 8;
+  a.qos = q_out_stride / 8;
+  a.tokens = (int)tokens;
+  a.heads = heads;
+  a.kv_heads = kv_heads;
+  a.all = heads + 2 * kv_heads;
+  a.rotary = rotary;
+  a.known = num_positions;
+  a.rows = rows;
+  a.width = table_width;
+  a.pages = num_pages;
+  a.page_log = __builtin_ctz(page_size);
+  a.interleaved = interleaved != 0;
+  a.eps = eps;
+  const hipStream_t s = (hipStream_t)stream;
+  return HQ_BY_TYPE(true);
+}

@@ -177,3 +177,31 @@ def cache_compact(pool, table, refs, out=None):
     """Moves the pages in use (refs[p] > 0) behind the first n, n the number of pages in use, into the free ones among those, in order,
     in every plane of the pool.  Returns (table, refs, n as int32 [1])."""
     return _native.cache_compact(pool, table, refs, out)
+
+
+def rotary_table(positions, rotary, base=10000.0, device="cuda"):
+    """Cosines and sines of a head's angles at positions 0 ... positions - 1, as norm_rotate takes them: fp32 [positions][rotary], the
+    cosines of position * base ** (-2 i / rotary), i < rotary / 2, and then their sines.  Angles in 64 bits: in 32, those of far positions
+    are off by thousandths."""
+    half = rotary // 2
+    angle = torch.arange(positions, dtype=torch.float64)[:, None] * float(base) ** (-torch.arange(half, dtype=torch.float64) / half)
+    return torch.cat([angle.cos(), angle.sin()], 1).float().to(device)
+
+
+def norm_rotate(q, k, cos_sin, positions, q_weight=None, k_weight=None, eps=1e-6, interleaved=False, out=None):
+    """Heads of queries and keys normed and rotated: each of q [tokens][heads][64 or 128] and k [tokens][kv_heads][head size], fp16 or bf16,
+    becomes x * rsqrt(mean(x^2) + eps) * weight (weight [head size] of their type; None: is not normed), and then its first cos_sin.size(1)
+    elements (a multiple of 16) are rotated by row positions[t] of cos_sin, cosines and then sines of the angles (rotary_table; a position
+    that is not in the table is cut to it): element i against element i + half of them, or, interleaved, 2 i against 2 i + 1.  cos_sin
+    None: no rotation.  fp32, one rounding.  q and k may be parts of a fused projection's rows.  Returns (q, k), new tensors or
+    out's two, which may be parts of rows as well, q and k themselves among them."""
+    q_out, k_out = (None, None) if out is None else out
+    return _native.norm_rotate(q, k, cos_sin, positions, q_weight, k_weight, eps, interleaved, q_out, k_out)
+
+
+def cache_write_rotated(q, k, v, k_pages, v_pages, table, starts, cu, cos_sin, q_weight=None, k_weight=None, eps=1e-6, interleaved=False,
+                        out=None):
+    """norm_rotate and cache_write in one: tokens cu[s] ... cu[s + 1] - 1 become tokens starts[s] and on of row s of the table, which is
+    their position too; the keys, normed and rotated, and the values go into the pages, as cache_write would take them.  Returns the
+    queries, normed and rotated (out: parts of rows, q itself among them); those of tokens of no row are left unwritten."""
+    return _native.cache_write_rotated(q, k, v, k_pages, v_pages, table, starts, cu, cos_sin, q_weight, k_weight, eps, interleaved, out)

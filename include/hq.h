@@ -378,6 +378,31 @@ int hq_cache_compact(void* pool, int planes, int64_t page_bytes, const int32_t* 
                      int32_t* refs_out, int32_t* live, int rows, int table_width, int num_pages, void* stream);
 
 /*
+ * Between a layer's projection and its attention.  fp16 or bf16, fp32 inside, one rounding; head_dim 64 or 128.  No counterpart in the
+ * reference.
+ *
+ * hq_norm_rotate: each head x of q [tokens][heads][head_dim] and k [tokens][kv_heads][head_dim] becomes
+ *     y = x * rsqrt(mean(x^2) + eps) * weight        (weight [head_dim] of the data's type; NULL: y = x)
+ *   and every pair (a, b) of the first `rotary` elements of y
+ *     (a * c - b * s, b * c + a * s)                 c = cos_sin[p][i], s = cos_sin[p][rotary / 2 + i], p = positions[t]
+ *   pair i being elements i and i + rotary / 2, or (interleaved != 0) 2 i and 2 i + 1.  rotary a multiple of 16, at most head_dim, 0: none;
+ *   cos_sin fp32 [num_positions][rotary]; a position outside it is cut to it; eps finite, 2^-126 at least.  Rows of q, k and the results are
+ *   their strides (elements, multiples of 8) apart; q_out and k_out may be q and k themselves, or other columns of the same rows, and
+ *   share no memory with the inputs otherwise (HQ_ERR_BAD_SHAPE).  All data 16-byte aligned.
+ * hq_cache_write_rotated: the same for tokens cu[s] ... cu[s+1]-1, at positions starts[s] ... : keys and values go to those tokens of row s
+ *   of the table, as hq_cache_write takes them, the queries to q_out (also those whose keys have no place).  Tokens of no row are not written.
+ */
+int hq_norm_rotate(const void* q, const void* k, void* q_out, void* k_out, int dtype, const void* q_weight, const void* k_weight,
+                   const float* cos_sin, const int32_t* positions, int64_t tokens, int heads, int kv_heads, int head_dim, int rotary,
+                   int num_positions, int64_t q_stride, int64_t k_stride, int64_t q_out_stride, int64_t k_out_stride, float eps, int interleaved,
+                   void* stream);
+int hq_cache_write_rotated(const void* q, const void* k, const void* v, void* q_out, void* k_pages, void* v_pages, int dtype,
+                           const void* q_weight, const void* k_weight, const float* cos_sin, const int32_t* table, const int32_t* starts,
+                           const int32_t* cu, int rows, int64_t tokens, int table_width, int num_pages, int page_size, int heads, int kv_heads,
+                           int head_dim, int rotary, int num_positions, int64_t q_stride, int64_t k_stride, int64_t v_stride,
+                           int64_t q_out_stride, float eps, int interleaved, void* stream);
+
+/*
  * Memory-system probes for the benchmark report (no counterpart in the reference): the rate this device
  * delivers to the simplest kernels, measured next to the library kernels instead of quoted from a data sheet.
  *   hq_probe_stream(mode, src, dst, bytes, stream): mode 0 reads `bytes` bytes of src and writes nothing
