@@ -15,7 +15,7 @@ from .ops import (
     static_scaled_int8_quant, dynamic_scaled_int8_quant,
     gemv_fp16, gemv_int8, gemv_int4, mxfp4_qdq,
     prompt_attention, paged_attention, cache_write, cache_step, cache_compact,
-    rotary_table, norm_rotate, cache_write_rotated,
+    chunk_attention, rotary_table, norm_rotate, cache_write_rotated,
 )
 
 __all__ = [
@@ -26,5 +26,5 @@ __all__ = [
     "static_scaled_int8_quant", "dynamic_scaled_int8_quant",
     "gemv_fp16", "gemv_int8", "gemv_int4", "mxfp4_qdq",
     "prompt_attention", "paged_attention", "cache_write", "cache_step", "cache_compact",
-    "rotary_table", "norm_rotate", "cache_write_rotated",
+    "chunk_attention", "rotary_table", "norm_rotate", "cache_write_rotated",
 ]

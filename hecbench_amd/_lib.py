@@ -54,8 +54,12 @@ _SIGNATURES = {
     "hq_mxfp4_qdq": (_c.c_int, [_c.c_void_p, _c.c_void_p, _c.c_int64, _c.c_int, _c.c_void_p]),
     "hq_prompt_attention": (_c.c_int, [_c.c_void_p] * 4 + [_c.c_int] + [_c.c_void_p] * 2 + [_c.c_int] + [_c.c_int64] * 2 + [_c.c_int] * 3
                             + [_c.c_int64] * 3 + [_c.c_float, _c.c_int, _c.c_void_p]),
+    "hq_prompt_attention_window": (_c.c_int, [_c.c_void_p] * 4 + [_c.c_int] + [_c.c_void_p] * 2 + [_c.c_int] + [_c.c_int64] * 2 + [_c.c_int] * 3
+                                   + [_c.c_int64] * 3 + [_c.c_float, _c.c_int, _c.c_int, _c.c_void_p]),
     "hq_paged_attention": (_c.c_int, [_c.c_void_p] * 4 + [_c.c_int] + [_c.c_void_p] * 4 + [_c.c_int] * 8
                            + [_c.c_int64, _c.c_float, _c.c_void_p]),
+    "hq_chunk_attention": (_c.c_int, [_c.c_void_p] * 4 + [_c.c_int] + [_c.c_void_p] * 3 + [_c.c_int, _c.c_int64] + [_c.c_int] * 6
+                           + [_c.c_int64, _c.c_float, _c.c_int, _c.c_int, _c.c_void_p]),
     "hq_cache_write": (_c.c_int, [_c.c_void_p] * 4 + [_c.c_int] + [_c.c_void_p] * 3 + [_c.c_int, _c.c_int64] + [_c.c_int] * 5
                        + [_c.c_int64] * 2 + [_c.c_void_p]),
     "hq_norm_rotate": (_c.c_int, [_c.c_void_p] * 4 + [_c.c_int] + [_c.c_void_p] * 4 + [_c.c_int64] + [_c.c_int] * 5 + [_c.c_int64] * 4

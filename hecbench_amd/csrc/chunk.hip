@@ -1,0 +1,376 @@
+// Attention of the next tokens of every request - one, a few, a chunk of a prompt - over the paged cache, through a sliding window and a
+// few first tokens that stay visible, or without.
+//
+// A request's rows are its new tokens, each with the heads of a key / value head's group; token i of n, of a request that has `length`
+// tokens with them, is at place length - n + i and sees the keys up to its own (window: see Skip in attend.h).  Up to 16 rows go the way of
+// few rows, bound by the keys' way from memory, the others in tiles of 128 the way of many.  The keys of a tile are divided where
+// there are fewer tiles than the device has room for: the shares of few rows meet in the launch, as the last of them joins them, those of
+// many in a second one.
+#include "attend.h"
+
+namespace {
+
+struct ChunkArgs {
+  const void *q, *k, *v;
+  void* out;
+  const int *table, *lengths, *cu_q;
+  float *po, *pm;     // a place for each row of a share: its sums [D]; and its {maximum, sum}
+  unsigned* arrived;  // counters of the shares of few rows
+  int* said;          // of each request, by the kernel: its first share, and the shares of each of its tiles
+  int64_t qs;
+  int batch, total_q, width, pages, page_log, heads, kv_heads, ratio;
+  int items;          // shares of all tiles, at most
+  int ns;             // more than 64 requests: shares of every tile; else 0: as many as there is room for
+  int place_rows;     // rows of a place
+  int many_divided;   // whether tiles of many rows may be divided
+  int window, sinks;
+  float c;
+};
+
+constexpr int kFew = 16, kUnit = 128, kRows = 128;
+
+// A request: its new tokens and the tokens it has with them.
+struct Request {
+  int q0, nq, length;
+  __device__ __forceinline__ void get(const ChunkArgs& a, int i) {
+    const int qb = a.cu_q[i], qe = a.cu_q[i + 1], n = a.lengths[i];
+    q0 = min(max(qb, 0), a.total_q);
+    nq = min(max(qe, q0), a.total_q) - q0;
+    length = min(max(n, 0), a.width << a.page_log);
+  }
+  __device__ __forceinline__ int tiles(int ratio) const {  // nq * ratio is below 2^31 - 128
+    const int rows = nq * ratio;
+    return rows <= kFew ? rows > 0 : (rows + kRows - 1) / kRows;
+  }
+  __device__ __forceinline__ int place(int token) const { return token - nq + length; }
+};
+
+// A share of a tile's keys.
+struct Item {
+  int b, tile, share, count, before;  // request, tile of it (the last, which sees most, first), which of how many shares; items of the requests before
+  int each;                           // keys of a share; 0: divided evenly
+  Request r;
+
+  template <bool WINDOW>
+  __device__ __forceinline__ bool find(const ChunkArgs& a, int x, bool says) {
+    const int lane = threadIdx.x & 63;
+    if (a.ns) {
+      // Many requests: request i has tiles_from(i) ... , as many as its rows may take at most; which one has x, 64 bounds at a time.
+      auto tiles_from = [&](int i) { return (int)((int64_t)min(max(a.cu_q[i], 0), a.total_q) * a.ratio / kRows) + i; };
+      const int slot = x / a.ns;
+      share = x - slot * a.ns;
+      int lo = 0, n = a.batch;
+      while (n > 1) {
+        const int step = (n + 63) >> 6;
+        const bool below = lane * step < n && tiles_from(lo + lane * step) <= slot;
+        const int at = max(63 - (int)__clzll(__ballot(below) | 1), 0) * step;
+        lo += at;
+        n = min(step, n - at);
+      }
+      b = lo;
+      r.get(a, b);
+      tile = slot - tiles_from(b);
+      count = r.nq * a.ratio <= kFew ? a.ns : 1;
+      each = 0;
+      before = tiles_from(b) * a.ns;
+      return tile >= 0 && tile < r.tiles(a.ratio) && share < count;
+    }
+    Request mine;
+    mine.get(a, min(lane, a.batch - 1));
+    if (lane >= a.batch) mine.nq = 0;
+    const int tiles = mine.tiles(a.ratio), rows = mine.nq * a.ratio;
+    int keys = mine.length;
+    if (WINDOW) keys = (int)min((int64_t)keys, (int64_t)min(a.sinks, keys) + a.window + 14 + (rows <= kFew ? mine.nq : kRows / a.ratio + 2));
+    // The smallest multiple of kUnit of which there are no more shares than a.items: ends where every tile is one share.
+    const bool divisible = a.arrived && (rows <= kFew || a.many_divided);
+    const unsigned units = divisible ? max((unsigned)(keys + kUnit - 1) / kUnit, 1u) : 1, items = a.items, least = wave_sum(tiles);
+    auto shares = [&](unsigned per) { return min((units - 1) / per + 1, 64 * items); };  // sums stay in 32 bits: tiles are divided where they are few
+    unsigned per = 1, own = shares(per), all = wave_sum(tiles * own);
+    while (all > items && all > least) {
+      per += max(1u, (unsigned)((float)per * (float)(all - items) / (float)items));
+      own = shares(per);
+      all = wave_sum(tiles * own);
+    }
+    if ((unsigned)x >= all) return false;
+    const unsigned to = running_sum(tiles * own);
+    if (says && lane < a.batch) {
+      a.said[2 * lane] = to - tiles * own;
+      a.said[2 * lane + 1] = own;
+    }
+    b = __ffsll(__ballot((int)to > x)) - 1;
+    r = Request{__builtin_amdgcn_readlane(mine.q0, b), __builtin_amdgcn_readlane(mine.nq, b), __builtin_amdgcn_readlane(mine.length, b)};
+    count = __builtin_amdgcn_readlane(own, b);
+    before = __builtin_amdgcn_readlane(to, b) - __builtin_amdgcn_readlane(tiles, b) * count;
+    tile = (x - before) / count;
+    share = x - before - tile * count;
+    each = per * kUnit;
+    return true;
+  }
+  // Keys of the share, of the n that the tile goes through.
+  __device__ __forceinline__ void keys(int n, int* first, int* end) const {
+    const int size = each ? each : ((n + count - 1) / count + kUnit - 1) & -kUnit;
+    *first = count == 1 ? 0 : (int)min((int64_t)share * size, (int64_t)n);
+    *end = count == 1 ? n : (int)min((int64_t)(share + 1) * size, (int64_t)n);
+  }
+};
+
+// What rows of a tile see, keys that it leaves out not counted.
+struct Sight {
+  const ChunkArgs& a;
+  const Request& r;
+  Skip skip;
+  bool window;
+  __device__ __forceinline__ Sight(const ChunkArgs& args, const Request& request, bool w, int first_token, int last_token) : a(args), r(request), window(w) {
+    if (window) skip = skip_of(r.place(first_token), r.place(last_token), a.window, a.sinks);
+  }
+  __device__ __forceinline__ int limit(int token) const { return max(r.place(token) + 1, 0) - skip.gap; }
+  __device__ __forceinline__ int low(int token) const { return window ? window_of(r.place(token), a.window) - skip.gap : 0; }
+  // of the keys first ... end - 1, of which there are some, one at least
+  __device__ __forceinline__ bool any(int token, int first, int end) const {
+    return first < end && limit(token) > first && (!window || low(token) < end || a.sinks > first);
+  }
+};
+
+template <typename T, int D>
+__device__ __forceinline__ Pages<T, D> pages_of(const ChunkArgs& a, int request, int head) {
+  return Pages<T, D>((const T*)a.k, (const T*)a.v, a.table + (int64_t)request * a.width, head, a.kv_heads, a.page_log, a.pages);
+}
+
+template <typename T, int D, bool WINDOW>
+__device__ __forceinline__ void few_rows(const ChunkArgs& a, char* sm, const Item& item, int x, int head) {
+  typedef typename Kind<T>::V8 V8;
+  const Request& r = item.r;
+  const int lane = threadIdx.x & 63, nrows = r.nq * a.ratio;
+  const uint32_t ratio = a.ratio;
+  const Sight sight(a, r, WINDOW, 0, r.nq - 1);
+  int first, end;
+  item.keys(uniform(sight.limit(r.nq - 1)), &first, &end);
+  const int mine = min(lane & 15, nrows - 1), token = (uint32_t)mine / ratio, h = head * ratio + (uint32_t)mine % ratio;
+  Few<T, D, true> w;
+  w.sm = sm;
+  w.skip = sight.skip;
+  w.lim = min(sight.limit(token), end);
+  w.lo = sight.low(token);
+  w.sinks = WINDOW ? a.sinks : 0;
+  w.all_see = uniform(min(sight.limit(0), end));
+  w.lo_most = uniform(sight.low(r.nq - 1));
+  const T* q = (const T*)a.q + (int64_t)(r.q0 + token) * a.qs + (int64_t)h * D + 8 * (lane >> 4);
+#pragma unroll
+  for (int kk = 0; kk < D / 32; ++kk) w.qf[kk] = *reinterpret_cast<const V8*>(q + 32 * kk);
+  w.run(pages_of<T, D>(a, item.b, head), first, end, a.c);
+  float sum[D / 16], top, total;
+  w.join(sum, &top, &total);
+  const int row = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * (D / 16);
+  auto out_row = [=](int i) { return (int64_t)(r.q0 + (uint32_t)i / ratio) * a.heads + head * ratio + (uint32_t)i % ratio; };
+  const bool sees = sight.any((uint32_t)min(row, nrows - 1) / ratio, first, end);
+  if (item.count == 1) {
+    typedef T TD __attribute__((ext_vector_type(D / 16)));
+    TD v;
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) v[i] = (T)(sees ? result(sum[i], sum[i] / total) : 0.f);
+    if (row < nrows) *reinterpret_cast<TD*>((T*)a.out + out_row(row) * D + d0) = v;
+    return;
+  }
+  if (row < nrows) {
+    const int64_t place = ((int64_t)x * a.kv_heads + head) * a.place_rows + row;
+#pragma unroll
+    for (int i = 0; i < D / 16; i += 4)
+      hq_store_share(reinterpret_cast<hq_f4v*>(a.po + place * D + d0 + i), hq_f4v{sum[i], sum[i + 1], sum[i + 2], sum[i + 3]});
+    if (d0 == 0)
+      __hip_atomic_store(reinterpret_cast<unsigned long long*>(a.pm) + place, (unsigned long long)__float_as_uint(total) << 32 | __float_as_uint(share_top(top, sees)),
+                         __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  // The last share to arrive joins them; of more than 32, every 16 are joined first, by the last of them.
+  __shared__ unsigned nth;
+  int n = item.count, unit = 1, index = item.share;
+  const int share0 = item.before + item.tile * item.count;
+  for (;;) {
+    const bool all = n <= kJoin;
+    const int team = all ? 0 : index / kTeam, members = all ? n : min(kTeam, n - team * kTeam), first_share = share0 + team * kTeam * unit;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    unsigned* const count = a.arrived + (int64_t)((all ? a.items + share0 : first_share) * a.kv_heads + head) * kApart;
+    if (threadIdx.x == 0) nth = __hip_atomic_fetch_add(count, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    if (nth != (unsigned)members - 1) return;
+    if (threadIdx.x == 0) __hip_atomic_store(count, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    join_here<T, D>(a, sm, nrows, 0, ((int64_t)first_share * a.kv_heads + head) * a.place_rows, (int64_t)unit * a.kv_heads * a.place_rows, members, all,
+                    out_row);
+    if (all) return;
+    index = team;
+    n = (n + kTeam - 1) / kTeam;
+    unit *= kTeam;
+  }
+}
+
+template <typename T, int D, bool WINDOW>
+__device__ __forceinline__ void many_rows(const ChunkArgs& a, char* sm, int* poison, const Item& item, int x, int head) {
+  typedef typename Kind<T>::V8 V8;
+  const Request& r = item.r;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, rows = r.nq * a.ratio;
+  const uint32_t ratio = a.ratio;
+  const int first_row = ((rows + kRows - 1) / kRows - 1 - item.tile) * kRows, last_row = min(first_row + kRows, rows) - 1;
+  const int first_token = (uint32_t)first_row / ratio, last_token = (uint32_t)last_row / ratio;
+  const Sight sight(a, r, WINDOW, first_token, last_token);
+  int first, end;
+  item.keys(uniform(sight.limit(last_token)), &first, &end);
+  const int row = first_row + wave * 32 + (lane & 31), mine = min(row, last_row);
+  const int token = (uint32_t)mine / ratio, h = head * ratio + (uint32_t)mine % ratio;
+  Many<T, D, WINDOW> w;
+  w.sm = sm;
+  w.poison = poison;
+  set_up(poison);
+  const T* q = (const T*)a.q + (int64_t)(r.q0 + token) * a.qs + (int64_t)h * D + 8 * (lane >> 5);
+#pragma unroll
+  for (int kk = 0; kk < D / 16; ++kk) w.qf[kk] = *reinterpret_cast<const V8*>(q + 16 * kk);
+  w.lim = min(sight.limit(token), end);
+  w.all_see = __builtin_amdgcn_readlane(w.lim, 0);  // a later row sees as much or more
+  w.any_sees = first_row + wave * 32 > last_row ? 0 : __builtin_amdgcn_readlane(w.lim, 31);  // a wave without rows works on nothing
+  if (WINDOW) {
+    w.lo = sight.low(token);
+    w.sinks = a.sinks;
+    w.lo_most = __builtin_amdgcn_readlane(w.lo, 31);
+  }
+  PagedTiles<T, D, WINDOW> src(pages_of<T, D>(a, item.b, head), end);
+  src.skip = sight.skip;
+  w.run(src, first, end, uniform(min(sight.limit(first_token), end)), a.c, uniform(sight.low(last_token)));
+  // the row, worked out once more: in the loop there is no register to spare
+  int tid = threadIdx.x;
+  asm volatile("" : "+v"(tid));
+  const int again = first_row + (tid >> 6) * 32 + (tid & 31);
+  if (again > last_row) return;
+  const int t = (uint32_t)again / ratio;
+  const bool sees = sight.any(t, first, end);
+  if (item.count == 1) w.put((T*)a.out + ((int64_t)(r.q0 + t) * a.heads + head * ratio + (uint32_t)again % ratio) * D, !sees);
+  else w.put_share(a.po, a.pm, ((int64_t)x * a.kv_heads + head) * a.place_rows + again - first_row, sees);
+}
+
+template <typename T, int D, bool WINDOW>
+__global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void chunk_kernel(ChunkArgs a) {
+  extern __shared__ __align__(16) char sm[];
+  __shared__ int poison;
+  const uint32_t x = blockIdx.x / (uint32_t)a.kv_heads, head = blockIdx.x - x * (uint32_t)a.kv_heads;
+  Item item;
+  if (!item.find<WINDOW>(a, x, blockIdx.x == 0 && threadIdx.x < 64 && a.said)) return;
+  if (item.r.nq * a.ratio <= kFew) few_rows<T, D, WINDOW>(a, sm, item, x, head);
+  else many_rows<T, D, WINDOW>(a, sm, &poison, item, x, head);
+}
+
+// The shares of rows of many: a row a wave, or a workgroup.
+template <typename T, int D, int WAVES, int PRE>
+__global__ __launch_bounds__(kThreads) void join_chunk_kernel(ChunkArgs a) {
+  const int64_t row = WAVES > 1 ? blockIdx.x : (int64_t)blockIdx.x * kWaves + (threadIdx.x >> 6);
+  if (row >= (int64_t)a.total_q * a.heads) return;
+  const int lane = threadIdx.x & 63, token = uniform((int)(row / a.heads)), h = uniform((int)(row - (int64_t)token * a.heads)), head = h / a.ratio;
+  // its request: the last one that begins at or before it and ends behind it
+  const int i = min(lane, a.batch - 1), qb = a.cu_q[i], qe = a.cu_q[i + 1];
+  const unsigned long long here = __ballot(lane < a.batch && qb <= token && token < qe);
+  if (!here) return;
+  const int b = __ffsll(here) - 1;
+  Request r;
+  r.get(a, b);
+  const int count = uniform(a.said[2 * b + 1]), rows = r.nq * a.ratio;
+  if (rows <= kFew || count <= 1) return;
+  const int mine = (token - r.q0) * a.ratio + (h - head * a.ratio), tile = (rows + kRows - 1) / kRows - 1 - mine / kRows;
+  const int64_t share0 = uniform(a.said[2 * b]) + (int64_t)tile * count;
+  if (share0 < 0 || share0 + count > a.items) return;  // bounds that do not ascend
+  join_shares<T, D, WAVES, PRE>(a.po, a.pm, row, (share0 * a.kv_heads + head) * a.place_rows + mine % kRows, a.kv_heads * a.place_rows, count, count, count,
+                                count, (T*)a.out);
+}
+
+template <typename T, int D, bool WINDOW>
+int launch_chunk(ChunkArgs a, int cus, hipStream_t stream) {
+  const int64_t cap = (int64_t)a.width << a.page_log, rows = (int64_t)a.total_q * a.ratio;
+  const int64_t tiles = rows / kRows + std::min(a.batch, a.total_q);  // at most
+  const int64_t room = std::max<int64_t>(2 * (int64_t)cus / a.kv_heads, 1), units = std::max<int64_t>((cap + kUnit - 1) / kUnit, 1);
+  a.place_rows = (int)std::min<int64_t>(kRows, (rows + 15) & ~15);
+  int64_t items, slots = a.batch > 64 ? rows / kRows + a.batch : tiles;
+  size_t floats = 0, counters = 0;
+  bool divide = tiles < room && units > 1;
+  for (;;) {
+    a.many_divided = divide && (a.total_q > a.batch || a.ratio > kFew);
+    a.ns = 0;
+    if (a.batch > 64) a.ns = (int)(divide ? std::max<int64_t>(1, std::min(room / slots, units)) : 1);
+    items = a.ns ? slots * a.ns : divide ? std::min(room, tiles * units) : tiles;
+    if (a.batch > 64 && a.ns == 1) divide = false;
+    if (a.batch > 64) a.many_divided = 0;
+    if (!divide) break;
+    floats = items * a.kv_heads * a.place_rows * (D + 2) + 2 * (int64_t)a.batch;
+    counters = 2 * items * a.kv_heads * kApart;
+    // While the stream is captured and has no room for shares: undivided.  Longer, and no error.
+    if (!hq_workspace_out_of_reach(stream, floats, counters)) break;
+    divide = false;
+  }
+  if (items * a.kv_heads > INT_MAX) return HQ_ERR_TOO_LARGE;
+  a.items = (int)items;
+  if (divide) {
+    HqWorkspace ws;
+    const int rc = hq_get_workspace(stream, floats, counters, &ws);
+    if (rc != HQ_OK) return rc;
+    const int64_t places = items * a.kv_heads * a.place_rows;
+    a.arrived = ws.counters;
+    a.po = ws.partial;
+    a.pm = a.po + places * D;
+    if (a.many_divided) a.said = reinterpret_cast<int*>(a.pm + 2 * places);
+  }
+  constexpr int lds = std::max(Many<T, D>::LDS, Few<T, D>::LDS);
+  static_assert(lds <= 65536, "no attribute to set");
+  const int rc = hq_launch_as_is(chunk_kernel<T, D, WINDOW>, dim3((unsigned)(items * a.kv_heads)), dim3(kThreads), lds, stream, a);
+  if (rc != HQ_OK || !a.many_divided) return rc;
+  return launch_join(Joins<ChunkArgs>{join_chunk_kernel<T, D, 1, 0>, join_chunk_kernel<T, D, kWaves, 0>, join_chunk_kernel<T, D, 1, 8>,
+                                      join_chunk_kernel<T, D, kWaves, 8>},
+                     (int64_t)a.total_q * a.heads, std::min(units, items), stream, a);
+}
+#define HQ_BY_TYPE(fn, window, ...)                                                                                     \
+  (dtype == HQ_DTYPE_F16 ? (head_dim == 64 ? fn<_Float16, 64, window>(__VA_ARGS__) : fn<_Float16, 128, window>(__VA_ARGS__)) \
+                         : (head_dim == 64 ? fn<__bf16, 64, window>(__VA_ARGS__) : fn<__bf16, 128, window>(__VA_ARGS__)))
+
+}  // namespace
+
+extern "C" int hq_chunk_attention(const void* q, const void* k_pages, const void* v_pages, void* out, int dtype, const int32_t* table,
+                                  const int32_t* lengths, const int32_t* cu_q, int batch, int64_t total_q, int table_width, int num_pages,
+                                  int page_size, int heads, int kv_heads, int head_dim, int64_t q_stride, float scale, int window, int sinks,
+                                  void* stream) {
+  if (batch < 0 || total_q < 0 || table_width < 0 || num_pages < 0 || window < 0 || sinks < 0 || heads < 1 || kv_heads < 1 || heads % kv_heads)
+    return HQ_ERR_BAD_SHAPE;
+  if (page_size < 8 || page_size > 1024 || (page_size & (page_size - 1))) return HQ_ERR_BAD_SHAPE;
+  if (head_dim != 64 && head_dim != 128) return HQ_ERR_BAD_SHAPE;
+  if (dtype != HQ_DTYPE_F16 && dtype != HQ_DTYPE_BF16) return HQ_ERR_BAD_ENUM;
+  if (bad_scale(scale)) return HQ_ERR_BAD_SHAPE;
+  if (batch == 0 || total_q == 0) return HQ_OK;
+  if (!q || !out || !lengths || !cu_q || (table_width && !table) || (table_width && num_pages && (!k_pages || !v_pages))) return HQ_ERR_NULL_POINTER;
+  if (q_stride < (int64_t)heads * head_dim) return HQ_ERR_BAD_SHAPE;
+  if (misaligned(q, q_stride) || (((uintptr_t)k_pages | (uintptr_t)v_pages | (uintptr_t)out) & 15) ||
+      (((uintptr_t)table | (uintptr_t)lengths | (uintptr_t)cu_q) & 3))
+    return HQ_ERR_MISALIGNED;
+  const int ratio = heads / kv_heads;
+  if ((int64_t)table_width * page_size > kMostKeys || total_q > INT_MAX || total_q * ratio > INT_MAX - kRows || total_q * ratio / kRows + batch > INT_MAX / 2 ||
+      (int64_t)kv_heads * head_dim * 2 * page_size > UINT32_MAX)  // bytes of a page
+    return HQ_ERR_TOO_LARGE;
+  const HqDevice* dev = nullptr;
+  const int rc = hq_current_device(&dev);
+  if (rc != HQ_OK) return rc;
+  ChunkArgs a{};
+  a.q = q;
+  a.k = k_pages;
+  a.v = v_pages;
+  a.out = out;
+  a.table = table;
+  a.lengths = lengths;
+  a.cu_q = cu_q;
+  a.qs = q_stride;
+  a.batch = batch;
+  a.total_q = (int)total_q;
+  a.width = table_width;
+  a.pages = num_pages;
+  a.page_log = __builtin_ctz(page_size);
+  a.heads = heads;
+  a.kv_heads = kv_heads;
+  a.ratio = ratio;
+  a.window = window;
+  a.sinks = sinks;
+  a.c = exponent_scale(scale);
+  const hipStream_t s = (hipStream_t)stream;
+  if (window && window < (int64_t)table_width * page_size) return HQ_BY_TYPE(launch_chunk, true, a, dev->cus, s);
+  return HQ_BY_TYPE(launch_chunk, false, a, dev->cus, s);
+}

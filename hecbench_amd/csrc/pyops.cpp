@@ -447,7 +447,22 @@ void same_type(const at::Tensor& like, const at::Tensor& t, const char* name) {
   if (t.scalar_type() != like.scalar_type()) value_error(std::string(name) + " must have the type of the others");
 }
 
-PyObject* prompt_attention(PyObject* const* a) {  // q, k, v, cu_q, cu_k, causal, scale, out
+// window (None: 0, everything is seen) and sinks, which go with it.
+struct Window {
+  int keys = 0, sinks = 0;
+  Window(PyObject* w, PyObject* s) {
+    sinks = bound(s);
+    if (sinks < 0) value_error("sinks must not be negative");
+    if (w == Py_None) {
+      if (sinks) value_error("sinks go with a window");
+      return;
+    }
+    keys = bound(w);
+    if (keys < 1) value_error("window must be a key at least");
+  }
+};
+
+PyObject* prompt_attention(PyObject* const* a) {  // q, k, v, cu_q, cu_k, causal, scale, out, window, sinks
   const Rows q = rows_of(a[0], "q", kF16 | kBF16), k = rows_of(a[1], "k", kF16 | kBF16), v = rows_of(a[2], "v", kF16 | kBF16);
   same_type(*q.t, *k.t, "k");
   same_type(*q.t, *v.t, "v");
@@ -460,11 +475,16 @@ PyObject* prompt_attention(PyObject* const* a) {  // q, k, v, cu_q, cu_k, causal
   if (causal < 0) throw python_error();
   const float scale = scale_of(a[6], q.size);
   const at::Tensor* o = tensor(a[7], "out", dt(q.t->scalar_type()), q.tokens * q.heads * q.size, true);
+  const Window window(a[8], a[9]);
+  if (window.keys && !causal) value_error("a window goes with causal attention");
   same_device(q.t, k.t, v.t, cu_q, cu_k, o);
   Result r(a[7], o, *q.t, {q.tokens, q.heads, q.size}, q.t->scalar_type());
   const int hq = size_of(q.heads), hk = size_of(k.heads), d = size_of(q.size), seqs = size_of(cu_q->numel() - 1);
   void* st = stream();
-  call("hq_prompt_attention", [&] {
+  call(window.keys ? "hq_prompt_attention_window" : "hq_prompt_attention", [&] {
+    if (window.keys)
+      return hq_prompt_attention_window(ptr(q.t), ptr(k.t), ptr(v.t), r.t.data_ptr(), act_dtype(*q.t), in<int32_t>(cu_q), in<int32_t>(cu_k), seqs,
+                                        q.tokens, k.tokens, hq, hk, d, q.stride, k.stride, v.stride, scale, window.keys, window.sinks, st);
     return hq_prompt_attention(ptr(q.t), ptr(k.t), ptr(v.t), r.t.data_ptr(), act_dtype(*q.t), in<int32_t>(cu_q), in<int32_t>(cu_k), seqs, q.tokens,
                                k.tokens, hq, hk, d, q.stride, k.stride, v.stride, scale, causal, st);
   });
@@ -494,6 +514,31 @@ PyObject* paged_attention(PyObject* const* a) {  // q, k_pages, v_pages, table, 
   call("hq_paged_attention", [&] {
     return hq_paged_attention(ptr(q.t), ptr(k), ptr(v), r.t.data_ptr(), act_dtype(*q.t), in<int32_t>(table), in<int32_t>(lengths), in<int32_t>(groups),
                               in<int32_t>(shared), ng, batch, width, pages, page, hq, hk, d, q.stride, scale, st);
+  });
+  return r.release();
+}
+
+PyObject* chunk_attention(PyObject* const* a) {  // q, k_pages, v_pages, table, lengths, cu_q, window, sinks, scale, out
+  const Rows q = rows_of(a[0], "q", kF16 | kBF16);
+  const at::Tensor* k = tensor(a[1], "k_pages", dt(q.t->scalar_type()));
+  if (k->dim() != 4 || k->size(3) != q.size) value_error("k_pages must be [pages][heads][tokens of a page][head size of q]");
+  const at::Tensor* v = tensor(a[2], "v_pages", dt(q.t->scalar_type()), k->numel());
+  if (v->sizes() != k->sizes()) value_error("v_pages must have the shape of k_pages");
+  const at::Tensor* table = tensor(a[3], "table", kI32);
+  if (table->dim() != 2) value_error("table must be [requests][pages of a request]");
+  const at::Tensor* lengths = tensor(a[4], "lengths", kI32, table->size(0));
+  const at::Tensor* cu = tensor(a[5], "cu_q", kI32, table->size(0) + 1);
+  const Window window(a[6], a[7]);
+  const float scale = scale_of(a[8], q.size);
+  const at::Tensor* o = tensor(a[9], "out", dt(q.t->scalar_type()), q.tokens * q.heads * q.size, true);
+  same_device(q.t, k, v, table, lengths, cu, o);
+  Result r(a[9], o, *q.t, {q.tokens, q.heads, q.size}, q.t->scalar_type());
+  const int batch = size_of(table->size(0)), width = size_of(table->size(1)), pages = size_of(k->size(0)), page = size_of(k->size(2)),
+            hq = size_of(q.heads), hk = size_of(k->size(1)), d = size_of(q.size);
+  void* st = stream();
+  call("hq_chunk_attention", [&] {
+    return hq_chunk_attention(ptr(q.t), ptr(k), ptr(v), r.t.data_ptr(), act_dtype(*q.t), in<int32_t>(table), in<int32_t>(lengths), in<int32_t>(cu), batch,
+                              q.tokens, width, pages, page, hq, hk, d, q.stride, scale, window.keys, window.sinks, st);
   });
   return r.release();
 }
@@ -717,8 +762,9 @@ PyMethodDef kMethods[] = {
     HQ_METHOD("gemv_int8", gemv_int<false>, 5),
     HQ_METHOD("gemv_int4", gemv_int<true>, 5),
     HQ_METHOD("mxfp4_qdq", mxfp4_qdq, 2),
-    HQ_METHOD("prompt_attention", prompt_attention, 8),
+    HQ_METHOD("prompt_attention", prompt_attention, 10),
     HQ_METHOD("paged_attention", paged_attention, 9),
+    HQ_METHOD("chunk_attention", chunk_attention, 10),
     HQ_METHOD("cache_write", cache_write, 7),
     HQ_METHOD("norm_rotate", norm_rotate, 10),
     HQ_METHOD("cache_write_rotated", cache_write_rotated, 14),

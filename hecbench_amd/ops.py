@@ -140,13 +140,14 @@ def mxfp4_qdq(x, out=None):
     return _native.mxfp4_qdq(x, out)
 
 
-def prompt_attention(q, k, v, cu_q, cu_k=None, causal=True, scale=None, out=None):
+def prompt_attention(q, k, v, cu_q, cu_k=None, causal=True, scale=None, out=None, window=None, sinks=0):
     """Attention over packed sequences: tokens cu_q[i] .. cu_q[i + 1] - 1 of q [tokens][heads][64 or 128] are sequence i's and see
     its keys cu_k[i] .. cu_k[i + 1] - 1 (cu_k: cu_q's) of k and v [keys][kv_heads][head size]; fp16 or bf16, int32 bounds.
     causal: the last token sees all keys, each one before it a key less; a token that sees none gets zeros.  scale: 1 / sqrt of the
-    head size.  q, k and v may be parts of a fused projection's rows.  Returns [tokens][heads][head size]; tokens of no sequence
+    head size.  q, k and v may be parts of a fused projection's rows.  window, causal only: a token sees no more than the last `window`
+    of its keys, its own among them, and the first `sinks` keys of its sequence.  Returns [tokens][heads][head size]; tokens of no sequence
     are left unwritten."""
-    return _native.prompt_attention(q, k, v, cu_q, cu_k, causal, scale, out)
+    return _native.prompt_attention(q, k, v, cu_q, cu_k, causal, scale, out, window, sinks)
 
 
 def paged_attention(q, k_pages, v_pages, table, lengths, groups=None, shared=None, scale=None, out=None):
@@ -155,6 +156,16 @@ def paged_attention(q, k_pages, v_pages, table, lengths, groups=None, shared=Non
     groups (int32 [n + 1]) and shared (int32 [n]): the first shared[g] tokens of the requests groups[g] .. groups[g + 1] - 1 are in the
     same pages, as cache_step leaves them, and are read once for all of them.  Tokens of a page: a power of two, 8 ... 1024."""
     return _native.paged_attention(q, k_pages, v_pages, table, lengths, groups, shared, scale, out)
+
+
+def chunk_attention(q, k_pages, v_pages, table, lengths, cu_q, window=None, sinks=0, scale=None, out=None):
+    """Attention of any number of new tokens per request - one, drafted ones, a chunk of a prompt - over a paged cache that holds their keys and
+    values already: tokens cu_q[s] ... cu_q[s + 1] - 1 of q [tokens][heads][64 or 128] are the last of the first lengths[s] tokens of row s,
+    token t being token t % page of page table[s][t // page] in k_pages and v_pages [pages][kv_heads][page][head size], and each sees the
+    tokens up to itself.  window: no more than the last `window` of them, itself among them, and the first `sinks` tokens of its request;
+    pages that no token sees are not read, and need not be there.  Returns [tokens][heads][head size]; a token that sees nothing gets
+    zeros, tokens of no request are left unwritten.  Tokens of a page: a power of two, 8 ... 1024."""
+    return _native.chunk_attention(q, k_pages, v_pages, table, lengths, cu_q, window, sinks, scale, out)
 
 
 def cache_write(k, v, k_pages, v_pages, table, starts, cu):

@@ -337,12 +337,18 @@ int hq_mxfp4_qdq(const void* in, void* out, int64_t n_elems, int dtype, void* st
  *   q [total_q][heads][head_dim], rows q_stride elements apart, k and v [total_k][kv_heads][head_dim] likewise (parts of a fused
  *   projection's rows), k_stride and v_stride up to 2^22; out contiguous; all 16-byte aligned, strides multiples of 8.  Tokens of no
  *   sequence are not written.
+ * hq_prompt_attention_window: causal, and key j is seen by the token whose own key is the p-th of its sequence (p as above the largest j that it
+ *   sees) only if j > p - window or j < sinks.  window 1 at least, sinks 0 at least.  Keys that no token sees are not read.
  * hq_paged_attention: one query a request.  Token t of request s is token t % page_size of page table[s][t / page_size]
  *   (table [batch][table_width], pages [num_pages][kv_heads][page_size][head_dim], contiguous); request s sees its first lengths[s] tokens.
  *   Requests groups[g] ... groups[g+1]-1 (bounds in ascending order) have their first shared[g] tokens, as far as the first one's
  *   length reaches, in the same pages, which are read once for all of them, from the first one's row (every row of the table lists
  *   them); ngroups 0: nothing is shared, and as many groups as requests or more are taken as none.  page_size a power of two, 8 ... 1024.
  *   A table entry that is needed and no page counts as a page of zeros (num_pages 0: all of them).
+ * hq_chunk_attention: any number of queries a request, the last of its tokens: tokens cu_q[s] ... cu_q[s+1]-1 of q [total_q][heads][head_dim] are tokens
+ *   lengths[s] - n ... lengths[s]-1 of row s of the table [batch][table_width] (n of them; q, pages and table entries as above), and see the
+ *   tokens up to their own; window > 0: of those, the last `window` and the first `sinks` of the request; tokens and pages that nobody sees
+ *   are not read.  A token before the request's first sees nothing and gets zeros; tokens of no request are not written.
  * hq_cache_write: tokens cu[s] ... cu[s+1]-1 of k and v [tokens][kv_heads][head_dim] (strides as above) become tokens starts[s], ... of row s
  *   of the table; any head_dim that is a multiple of 8, page_size a power of two, 1 ... 1024.  A token whose place is outside its row, or in no page, is left out.
  * hq_cache_step: from the tables of one step to the next one's.  Row s inherits row parent[s] (of the old tables; any number outside
@@ -365,9 +371,15 @@ int hq_mxfp4_qdq(const void* in, void* out, int64_t n_elems, int dtype, void* st
 int hq_prompt_attention(const void* q, const void* k, const void* v, void* out, int dtype, const int32_t* cu_q, const int32_t* cu_k, int seqs,
                         int64_t total_q, int64_t total_k, int heads, int kv_heads, int head_dim, int64_t q_stride, int64_t k_stride,
                         int64_t v_stride, float scale, int causal, void* stream);
+int hq_prompt_attention_window(const void* q, const void* k, const void* v, void* out, int dtype, const int32_t* cu_q, const int32_t* cu_k,
+                               int seqs, int64_t total_q, int64_t total_k, int heads, int kv_heads, int head_dim, int64_t q_stride, int64_t k_stride,
+                               int64_t v_stride, float scale, int window, int sinks, void* stream);
 int hq_paged_attention(const void* q, const void* k_pages, const void* v_pages, void* out, int dtype, const int32_t* table, const int32_t* lengths,
                        const int32_t* groups, const int32_t* shared, int ngroups, int batch, int table_width, int num_pages, int page_size,
                        int heads, int kv_heads, int head_dim, int64_t q_stride, float scale, void* stream);
+int hq_chunk_attention(const void* q, const void* k_pages, const void* v_pages, void* out, int dtype, const int32_t* table, const int32_t* lengths,
+                       const int32_t* cu_q, int batch, int64_t total_q, int table_width, int num_pages, int page_size, int heads, int kv_heads,
+                       int head_dim, int64_t q_stride, float scale, int window, int sinks, void* stream);
 int hq_cache_write(const void* k, const void* v, void* k_pages, void* v_pages, int dtype, const int32_t* table, const int32_t* starts,
                    const int32_t* cu, int rows, int64_t tokens, int table_width, int num_pages, int page_size, int kv_heads, int head_dim,
                    int64_t k_stride, int64_t v_stride, void* stream);
