@@ -3,9 +3,8 @@
 //
 // A request's rows are its new tokens, each with the heads of a key / value head's group; token i of n, of a request that has `length`
 // tokens with them, is at place length - n + i and sees the keys up to its own (window: see Skip in attend.h).  Up to 16 rows go the way of
-// few rows, bound by the keys' way from memory, the others in tiles of 128 the way of many.  The keys of a tile are divided where
-// there are fewer tiles than the device has room for: the shares of few rows meet in the launch, as the last of them joins them, those of
-// many in a second one.
+// few rows, bound by the keys' way from memory, the others in tiles of 128 the way of many.  The keys of a tile are divided where there
+// are fewer tiles than the device has room for, and the shares meet in the launch.
 #include "attend.h"
 
 namespace {
@@ -14,15 +13,15 @@ struct ChunkArgs {
   const void *q, *k, *v;
   void* out;
   const int *table, *lengths, *cu_q;
-  float *po, *pm;     // a place for each row of a share: its sums [D]; and its {maximum, sum}
-  unsigned* arrived;  // counters of the shares of few rows
-  int* said;          // of each request, by the kernel: its first share, and the shares of each of its tiles
+  // Places of shares, 16 rows each of few, 128 each of many, the former first: a row's sums [D]; and its {maximum, sum}
+  float *po, *pm;
+  unsigned* arrived;  // counters of the shares of few rows; null: nothing is divided
+  int* said;          // not null: tiles of many rows may be divided; of each request, by the kernel: its first share, and the shares of a tile
   int64_t qs;
   int batch, total_q, width, pages, page_log, heads, kv_heads, ratio;
-  int items;          // shares of all tiles, at most
+  int few, many;      // shares of tiles of few and of many rows, at most
   int ns;             // more than 64 requests: shares of every tile; else 0: as many as there is room for
-  int place_rows;     // rows of a place
-  int many_divided;   // whether tiles of many rows may be divided
+  int cus, room;      // compute units; shares for two workgroups each
   int window, sinks;
   float c;
 };
@@ -47,11 +46,12 @@ struct Request {
 
 // A share of a tile's keys.
 struct Item {
-  int b, tile, share, count, before;  // request, tile of it (the last, which sees most, first), which of how many shares; items of the requests before
-  int each;                           // keys of a share; 0: divided evenly
+  int b, tile, share, count, first;  // request, tile of it (the last, which sees most, first), which of how many shares, and the number of the first
+  int each;                          // keys of a share; 0: divided evenly
   Request r;
 
-  template <bool WINDOW>
+  // Item x of the call.  Those of many rows come first: they are the longest, and one to a compute unit where there are no more.
+  template <int D, bool WINDOW>
   __device__ __forceinline__ bool find(const ChunkArgs& a, int x, bool says) {
     const int lane = threadIdx.x & 63;
     if (a.ns) {
@@ -72,7 +72,7 @@ struct Item {
       tile = slot - tiles_from(b);
       count = r.nq * a.ratio <= kFew ? a.ns : 1;
       each = 0;
-      before = tiles_from(b) * a.ns;
+      first = slot * a.ns;
       return tile >= 0 && tile < r.tiles(a.ratio) && share < count;
     }
     Request mine;
@@ -81,36 +81,57 @@ struct Item {
     const int tiles = mine.tiles(a.ratio), rows = mine.nq * a.ratio;
     int keys = mine.length;
     if (WINDOW) keys = (int)min((int64_t)keys, (int64_t)min(a.sinks, keys) + a.window + 14 + (rows <= kFew ? mine.nq : kRows / a.ratio + 2));
-    // The smallest multiple of kUnit of which there are no more shares than a.items: ends where every tile is one share.
-    const bool divisible = a.arrived && (rows <= kFew || a.many_divided);
-    const unsigned units = divisible ? max((unsigned)(keys + kUnit - 1) / kUnit, 1u) : 1, items = a.items, least = wave_sum(tiles);
-    auto shares = [&](unsigned per) { return min((units - 1) / per + 1, 64 * items); };  // sums stay in 32 bits: tiles are divided where they are few
-    unsigned per = 1, own = shares(per), all = wave_sum(tiles * own);
-    while (all > items && all > least) {
-      per += max(1u, (unsigned)((float)per * (float)(all - items) / (float)items));
-      own = shares(per);
-      all = wave_sum(tiles * own);
+    const unsigned units = max((unsigned)(keys + kUnit - 1) / kUnit, 1u), few = rows <= kFew ? tiles : 0, many = tiles - few;
+    const unsigned all_many = wave_sum(many);
+    // Tiles of many rows are divided where three shares each, or more, find room, two workgroups a compute unit; where they do not, what
+    // the shares' sums cost, which are written, read and joined, is more than it brings (behind 3500 keys, 32 / 8 heads of 128: 640 tokens 63 us
+    // in three shares, 78 undivided; 768 in two 74 and 78, 896 78 and 78, 1024 82 and 78).  A few of them by themselves are as fast with half as
+    // many shares (128 tokens 26.2 us, with all 28.2; 384 52.8 and 46.0).
+    const unsigned groups = all_many * a.kv_heads, all_few = wave_sum(few);
+    const bool many_too = a.said && 3 * groups <= 2u * a.cus;
+    const unsigned left = many_too ? a.room : max(a.room - (int)min(all_many, (unsigned)a.room), (a.room + 1) / 2);
+    const unsigned room = many_too && !all_few && 8 * groups <= (unsigned)a.cus ? (left + 1) / 2 : left, of = many_too ? tiles : few;
+    // The keys of a share: the smallest multiple of kUnit (two of them for many rows) of which there are no more shares than there is room for, or
+    // what makes one share of every tile.  (Sums stay in 32 bits.)
+    unsigned per = many_too && all_many ? 2 : 1, own = 1;
+    if (a.arrived) {
+      const unsigned least = wave_sum(of);
+      for (;;) {
+        own = min((units - 1) / per + 1, 64 * room);
+        const unsigned all = wave_sum(of * own);
+        if (all <= room || all <= least) break;
+        per += max(1u, (unsigned)((float)per * (float)(all - room) / (float)room));
+      }
     }
-    if ((unsigned)x >= all) return false;
-    const unsigned to = running_sum(tiles * own);
+    const unsigned own_many = many_too ? own : 1, all = wave_sum(many * own_many);
     if (says && lane < a.batch) {
-      a.said[2 * lane] = to - tiles * own;
-      a.said[2 * lane + 1] = own;
+      a.said[2 * lane] = running_sum(many * own_many) - many * own_many;
+      a.said[2 * lane + 1] = own_many;
     }
+    const bool is_many = x < (int)all;
+    if (!is_many) {
+      x -= all;
+      if ((unsigned)x >= wave_sum(few * own)) return false;
+    } else {
+      own = own_many;
+    }
+    const unsigned mine_of = (is_many ? many : few) * own;
+    const unsigned to = running_sum(mine_of);
     b = __ffsll(__ballot((int)to > x)) - 1;
     r = Request{__builtin_amdgcn_readlane(mine.q0, b), __builtin_amdgcn_readlane(mine.nq, b), __builtin_amdgcn_readlane(mine.length, b)};
     count = __builtin_amdgcn_readlane(own, b);
-    before = __builtin_amdgcn_readlane(to, b) - __builtin_amdgcn_readlane(tiles, b) * count;
+    const int before = __builtin_amdgcn_readlane(to, b) - __builtin_amdgcn_readlane(mine_of, b);
     tile = (x - before) / count;
     share = x - before - tile * count;
+    first = before + tile * count;
     each = per * kUnit;
     return true;
   }
   // Keys of the share, of the n that the tile goes through.
-  __device__ __forceinline__ void keys(int n, int* first, int* end) const {
+  __device__ __forceinline__ void keys(int n, int* from, int* to) const {
     const int size = each ? each : ((n + count - 1) / count + kUnit - 1) & -kUnit;
-    *first = count == 1 ? 0 : (int)min((int64_t)share * size, (int64_t)n);
-    *end = count == 1 ? n : (int)min((int64_t)(share + 1) * size, (int64_t)n);
+    *from = count == 1 ? 0 : (int)min((int64_t)share * size, (int64_t)n);
+    *to = count == 1 ? n : (int)min((int64_t)(share + 1) * size, (int64_t)n);
   }
 };
 
@@ -137,7 +158,7 @@ __device__ __forceinline__ Pages<T, D> pages_of(const ChunkArgs& a, int request,
 }
 
 template <typename T, int D, bool WINDOW>
-__device__ __forceinline__ void few_rows(const ChunkArgs& a, char* sm, const Item& item, int x, int head) {
+__device__ __forceinline__ void few_rows(const ChunkArgs& a, char* sm, const Item& item, int head) {
   typedef typename Kind<T>::V8 V8;
   const Request& r = item.r;
   const int lane = threadIdx.x & 63, nrows = r.nq * a.ratio;
@@ -162,40 +183,39 @@ __device__ __forceinline__ void few_rows(const ChunkArgs& a, char* sm, const Ite
   w.join(sum, &top, &total);
   const int row = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * (D / 16);
   auto out_row = [=](int i) { return (int64_t)(r.q0 + (uint32_t)i / ratio) * a.heads + head * ratio + (uint32_t)i % ratio; };
+  auto place_of = [=](int share) { return ((int64_t)share * a.kv_heads + head) * kFew; };
   const bool sees = sight.any((uint32_t)min(row, nrows - 1) / ratio, first, end);
   if (item.count == 1) {
     typedef T TD __attribute__((ext_vector_type(D / 16)));
     TD v;
 #pragma unroll
-    for (int i = 0; i < D / 16; ++i) v[i] = (T)(sees ? result(sum[i], sum[i] / total) : 0.f);
+    for (int j = 0; j < D / 16; ++j) v[j] = (T)(sees ? result(sum[j], sum[j] / total) : 0.f);
     if (row < nrows) *reinterpret_cast<TD*>((T*)a.out + out_row(row) * D + d0) = v;
     return;
   }
   if (row < nrows) {
-    const int64_t place = ((int64_t)x * a.kv_heads + head) * a.place_rows + row;
+    const int64_t place = place_of(item.first + item.share) + row;
 #pragma unroll
-    for (int i = 0; i < D / 16; i += 4)
-      hq_store_share(reinterpret_cast<hq_f4v*>(a.po + place * D + d0 + i), hq_f4v{sum[i], sum[i + 1], sum[i + 2], sum[i + 3]});
+    for (int j = 0; j < D / 16; j += 4)
+      hq_store_share(reinterpret_cast<hq_f4v*>(a.po + place * D + d0 + j), hq_f4v{sum[j], sum[j + 1], sum[j + 2], sum[j + 3]});
     if (d0 == 0)
-      __hip_atomic_store(reinterpret_cast<unsigned long long*>(a.pm) + place, (unsigned long long)__float_as_uint(total) << 32 | __float_as_uint(share_top(top, sees)),
-                         __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      __hip_atomic_store(reinterpret_cast<unsigned long long*>(a.pm) + place,
+                         (unsigned long long)__float_as_uint(total) << 32 | __float_as_uint(share_top(top, sees)), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
   // The last share to arrive joins them; of more than 32, every 16 are joined first, by the last of them.
   __shared__ unsigned nth;
   int n = item.count, unit = 1, index = item.share;
-  const int share0 = item.before + item.tile * item.count;
   for (;;) {
     const bool all = n <= kJoin;
-    const int team = all ? 0 : index / kTeam, members = all ? n : min(kTeam, n - team * kTeam), first_share = share0 + team * kTeam * unit;
+    const int team = all ? 0 : index / kTeam, members = all ? n : min(kTeam, n - team * kTeam), first_share = item.first + team * kTeam * unit;
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
-    unsigned* const count = a.arrived + (int64_t)((all ? a.items + share0 : first_share) * a.kv_heads + head) * kApart;
+    unsigned* const count = a.arrived + (int64_t)((all ? a.few + item.first : first_share) * a.kv_heads + head) * kApart;
     if (threadIdx.x == 0) nth = __hip_atomic_fetch_add(count, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     __syncthreads();
     if (nth != (unsigned)members - 1) return;
     if (threadIdx.x == 0) __hip_atomic_store(count, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    join_here<T, D>(a, sm, nrows, 0, ((int64_t)first_share * a.kv_heads + head) * a.place_rows, (int64_t)unit * a.kv_heads * a.place_rows, members, all,
-                    out_row);
+    join_here<T, D>(a, sm, nrows, 0, place_of(first_share), (int64_t)unit * a.kv_heads * kFew, members, all, out_row);
     if (all) return;
     index = team;
     n = (n + kTeam - 1) / kTeam;
@@ -203,8 +223,11 @@ __device__ __forceinline__ void few_rows(const ChunkArgs& a, char* sm, const Ite
   }
 }
 
+__device__ __forceinline__ int64_t many_place(const ChunkArgs& a, int share, int head) {
+  return (int64_t)a.few * a.kv_heads * kFew + ((int64_t)share * a.kv_heads + head) * kRows;
+}
 template <typename T, int D, bool WINDOW>
-__device__ __forceinline__ void many_rows(const ChunkArgs& a, char* sm, int* poison, const Item& item, int x, int head) {
+__device__ __forceinline__ void many_rows(const ChunkArgs& a, char* sm, int* poison, const Item& item, int head) {
   typedef typename Kind<T>::V8 V8;
   const Request& r = item.r;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, rows = r.nq * a.ratio;
@@ -242,7 +265,7 @@ __device__ __forceinline__ void many_rows(const ChunkArgs& a, char* sm, int* poi
   const int t = (uint32_t)again / ratio;
   const bool sees = sight.any(t, first, end);
   if (item.count == 1) w.put((T*)a.out + ((int64_t)(r.q0 + t) * a.heads + head * ratio + (uint32_t)again % ratio) * D, !sees);
-  else w.put_share(a.po, a.pm, ((int64_t)x * a.kv_heads + head) * a.place_rows + again - first_row, sees);
+  else w.put_share(a.po, a.pm, many_place(a, item.first + item.share, head) + again - first_row, sees);
 }
 
 template <typename T, int D, bool WINDOW>
@@ -251,75 +274,95 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void chunk_kernel(ChunkA
   __shared__ int poison;
   const uint32_t x = blockIdx.x / (uint32_t)a.kv_heads, head = blockIdx.x - x * (uint32_t)a.kv_heads;
   Item item;
-  if (!item.find<WINDOW>(a, x, blockIdx.x == 0 && threadIdx.x < 64 && a.said)) return;
-  if (item.r.nq * a.ratio <= kFew) few_rows<T, D, WINDOW>(a, sm, item, x, head);
-  else many_rows<T, D, WINDOW>(a, sm, &poison, item, x, head);
+  if (!item.find<D, WINDOW>(a, x, blockIdx.x == 0 && threadIdx.x < 64 && a.said)) return;
+  if (item.r.nq * a.ratio <= kFew) few_rows<T, D, WINDOW>(a, sm, item, head);
+  else many_rows<T, D, WINDOW>(a, sm, &poison, item, head);
 }
 
-// The shares of rows of many: a row a wave, or a workgroup.
+// The shares of rows of many together, a row a wave (WAVES 1) or a workgroup, from row to row: where nothing was divided, which the host does
+// not know, it is the fewer workgroups that matter.
 template <typename T, int D, int WAVES, int PRE>
 __global__ __launch_bounds__(kThreads) void join_chunk_kernel(ChunkArgs a) {
-  const int64_t row = WAVES > 1 ? blockIdx.x : (int64_t)blockIdx.x * kWaves + (threadIdx.x >> 6);
-  if (row >= (int64_t)a.total_q * a.heads) return;
-  const int lane = threadIdx.x & 63, token = uniform((int)(row / a.heads)), h = uniform((int)(row - (int64_t)token * a.heads)), head = h / a.ratio;
-  // its request: the last one that begins at or before it and ends behind it
-  const int i = min(lane, a.batch - 1), qb = a.cu_q[i], qe = a.cu_q[i + 1];
-  const unsigned long long here = __ballot(lane < a.batch && qb <= token && token < qe);
-  if (!here) return;
-  const int b = __ffsll(here) - 1;
-  Request r;
-  r.get(a, b);
-  const int count = uniform(a.said[2 * b + 1]), rows = r.nq * a.ratio;
-  if (rows <= kFew || count <= 1) return;
-  const int mine = (token - r.q0) * a.ratio + (h - head * a.ratio), tile = (rows + kRows - 1) / kRows - 1 - mine / kRows;
-  const int64_t share0 = uniform(a.said[2 * b]) + (int64_t)tile * count;
-  if (share0 < 0 || share0 + count > a.items) return;  // bounds that do not ascend
-  join_shares<T, D, WAVES, PRE>(a.po, a.pm, row, (share0 * a.kv_heads + head) * a.place_rows + mine % kRows, a.kv_heads * a.place_rows, count, count, count,
-                                count, (T*)a.out);
+  const int lane = threadIdx.x & 63;
+  const int i = min(lane, a.batch - 1), qb = a.cu_q[i], qe = a.cu_q[i + 1], before = a.said[2 * i], count = a.said[2 * i + 1];
+  if (!__ballot(lane < a.batch && count > 1)) return;
+  const int64_t rows = (int64_t)a.total_q * a.heads, step = WAVES > 1 ? gridDim.x : (int64_t)gridDim.x * kWaves;
+  for (int64_t row = WAVES > 1 ? blockIdx.x : (int64_t)blockIdx.x * kWaves + (threadIdx.x >> 6); row < rows; row += step) {
+    const int token = uniform((int)(row / a.heads)), h = uniform((int)(row - (int64_t)token * a.heads)), head = h / a.ratio;
+    const unsigned long long here = __ballot(lane < a.batch && qb <= token && token < qe);
+    if (!here) continue;
+    const int b = __ffsll(here) - 1, n = __builtin_amdgcn_readlane(count, b);
+    Request r;
+    r.get(a, b);
+    const int of = r.nq * a.ratio;
+    if (of <= kFew || n <= 1) continue;
+    const int mine = (token - r.q0) * a.ratio + (h - head * a.ratio), tile = (of + kRows - 1) / kRows - 1 - mine / kRows;
+    const int64_t first = __builtin_amdgcn_readlane(before, b) + (int64_t)tile * n;
+    if (first < 0 || first + n > a.many) continue;  // bounds that do not ascend
+    if (WAVES > 1) __syncthreads();  // the row before has been put together
+    join_shares<T, D, WAVES, PRE>(a.po, a.pm, row, many_place(a, (int)first, head) + mine % kRows, a.kv_heads * kRows, n, n, n, n, (T*)a.out);
+  }
 }
 
 template <typename T, int D, bool WINDOW>
 int launch_chunk(ChunkArgs a, int cus, hipStream_t stream) {
-  const int64_t cap = (int64_t)a.width << a.page_log, rows = (int64_t)a.total_q * a.ratio;
-  const int64_t tiles = rows / kRows + std::min(a.batch, a.total_q);  // at most
-  const int64_t room = std::max<int64_t>(2 * (int64_t)cus / a.kv_heads, 1), units = std::max<int64_t>((cap + kUnit - 1) / kUnit, 1);
-  a.place_rows = (int)std::min<int64_t>(kRows, (rows + 15) & ~15);
-  int64_t items, slots = a.batch > 64 ? rows / kRows + a.batch : tiles;
+  const int64_t cap = (int64_t)a.width << a.page_log, rows = (int64_t)a.total_q * a.ratio, requests = std::min(a.batch, a.total_q);
+  const int64_t units = std::max<int64_t>((cap + kUnit - 1) / kUnit, 1), room = std::max<int64_t>(2 * (int64_t)cus / a.kv_heads, 1);
+  // Tiles of many rows, at most, each of whose requests has more than kFew of them; and how many there are if all but a token a request are
+  // theirs.
+  const int64_t tiles = rows / kRows + std::min(requests, rows / (kFew + 1)), slots = rows / kRows + a.batch;
+  const int64_t likely = (rows - requests * a.ratio + kRows - 1) / kRows;
+  a.cus = cus;
+  a.room = (int)room;
+  bool divide = units > 1, many_divided;
   size_t floats = 0, counters = 0;
-  bool divide = tiles < room && units > 1;
+  int64_t few, many, places;
   for (;;) {
-    a.many_divided = divide && (a.total_q > a.batch || a.ratio > kFew);
     a.ns = 0;
-    if (a.batch > 64) a.ns = (int)(divide ? std::max<int64_t>(1, std::min(room / slots, units)) : 1);
-    items = a.ns ? slots * a.ns : divide ? std::min(room, tiles * units) : tiles;
-    if (a.batch > 64 && a.ns == 1) divide = false;
-    if (a.batch > 64) a.many_divided = 0;
+    many_divided = false;
+    if (a.batch > 64) {
+      a.ns = (int)(divide ? std::max<int64_t>(1, std::min(room / slots, units)) : 1);
+      divide = a.ns > 1;
+      few = slots * a.ns;
+      many = 0;
+    } else {
+      few = divide ? std::min(std::max(room, requests), requests * units) : requests;
+      many = tiles;
+      if (divide && likely && tiles && tiles < 2 * room) {  // more tiles than that fill the device
+        many = std::max(tiles, std::min(room, tiles * units));
+        many_divided = true;
+      }
+    }
     if (!divide) break;
-    floats = items * a.kv_heads * a.place_rows * (D + 2) + 2 * (int64_t)a.batch;
-    counters = 2 * items * a.kv_heads * kApart;
+    places = (few * kFew + (many_divided ? many * kRows : 0)) * a.kv_heads;
+    floats = places * (D + 2) + 2 * a.batch;
+    counters = 2 * few * a.kv_heads * kApart;
     // While the stream is captured and has no room for shares: undivided.  Longer, and no error.
     if (!hq_workspace_out_of_reach(stream, floats, counters)) break;
     divide = false;
   }
-  if (items * a.kv_heads > INT_MAX) return HQ_ERR_TOO_LARGE;
-  a.items = (int)items;
+  // Divided, tiles of both kinds share the room; else the few have what the many leave.
+  const int64_t grid = a.ns ? few : std::min(few + many, tiles + std::max(room, requests));
+  if (grid * a.kv_heads > INT_MAX) return HQ_ERR_TOO_LARGE;
+  a.few = (int)few;
+  a.many = (int)many;
   if (divide) {
     HqWorkspace ws;
     const int rc = hq_get_workspace(stream, floats, counters, &ws);
     if (rc != HQ_OK) return rc;
-    const int64_t places = items * a.kv_heads * a.place_rows;
     a.arrived = ws.counters;
     a.po = ws.partial;
     a.pm = a.po + places * D;
-    if (a.many_divided) a.said = reinterpret_cast<int*>(a.pm + 2 * places);
+    if (many_divided) a.said = reinterpret_cast<int*>(a.pm + 2 * places);
   }
   constexpr int lds = std::max(Many<T, D>::LDS, Few<T, D>::LDS);
   static_assert(lds <= 65536, "no attribute to set");
-  const int rc = hq_launch_as_is(chunk_kernel<T, D, WINDOW>, dim3((unsigned)(items * a.kv_heads)), dim3(kThreads), lds, stream, a);
-  if (rc != HQ_OK || !a.many_divided) return rc;
-  return launch_join(Joins<ChunkArgs>{join_chunk_kernel<T, D, 1, 0>, join_chunk_kernel<T, D, kWaves, 0>, join_chunk_kernel<T, D, 1, 8>,
-                                      join_chunk_kernel<T, D, kWaves, 8>},
-                     (int64_t)a.total_q * a.heads, std::min(units, items), stream, a);
+  const int rc = hq_launch_as_is(chunk_kernel<T, D, WINDOW>, dim3((unsigned)(grid * a.kv_heads)), dim3(kThreads), lds, stream, a);
+  if (rc != HQ_OK || !a.said) return rc;
+  const int64_t all = std::min((int64_t)a.total_q * a.heads, likely * kRows * a.kv_heads);
+  if (std::min(room / likely, units / 2) <= 2 * kSharesOfAWave)
+    return hq_launch_as_is(join_chunk_kernel<T, D, 1, 0>, dim3((unsigned)((all + kWaves - 1) / kWaves)), dim3(kThreads), 0, stream, a);
+  return hq_launch_as_is(join_chunk_kernel<T, D, kWaves, 8>, dim3((unsigned)all), dim3(kThreads), 0, stream, a);
 }
 #define HQ_BY_TYPE(fn, window, ...)                                                                                     \
   (dtype == HQ_DTYPE_F16 ? (head_dim == 64 ? fn<_Float16, 64, window>(__VA_ARGS__) : fn<_Float16, 128, window>(__VA_ARGS__)) \
