@@ -793,7 +793,8 @@ struct Few {
     // Whether all G instructions were needed: what the waits count.
     auto load = [&](const char* pool, int block, const Places& places, int set_ids, char* to, auto values) {
       const int base = first + block * 32, at = block / kWaves % SET * G;
-      if (base + 32 <= end) return places.template load<D, values, G>(pool, at, values ? voff : koff, to);
+      // (MASKED: rows behind the last one are whatever their page holds, unseen)
+      if (MASKED || base + 32 <= end) return places.template load<D, values, G>(pool, at, values ? voff : koff, to);
       // the last block: rows behind the last key repeat it, every lane by an address of its own
       const uint32_t lds = uniform((int)lds_address(to));
       bool whole = true;

@@ -81,39 +81,36 @@ struct Item {
     const int tiles = mine.tiles(a.ratio), rows = mine.nq * a.ratio;
     int keys = mine.length;
     if (WINDOW) keys = (int)min((int64_t)keys, (int64_t)min(a.sinks, keys) + a.window + 14 + (rows <= kFew ? mine.nq : kRows / a.ratio + 2));
-    const unsigned units = max((unsigned)(keys + kUnit - 1) / kUnit, 1u), few = rows <= kFew ? tiles : 0, many = tiles - few;
-    const unsigned all_many = wave_sum(many);
-    // Tiles of many rows are divided where three shares each, or more, find room, two workgroups a compute unit; where they do not, what
+    const unsigned few = rows <= kFew ? tiles : 0, many = tiles - few;
+    // (Few rows with up to 384 keys are not divided: 147 of them take a workgroup 7.3 us, two 8.9.)
+    const unsigned units = few && keys <= 3 * kUnit ? 1 : max((unsigned)(keys + kUnit - 1) / kUnit, 1u);
+    // Tiles of more than 64 rows are divided where three shares each, or more, find room, two workgroups a compute unit; where they do not, what
     // the shares' sums cost, which are written, read and joined, is more than it brings (behind 3500 keys, 32 / 8 heads of 128: 640 tokens 63 us
     // in three shares, 78 undivided; 768 in two 74 and 78, 896 78 and 78, 1024 82 and 78).  A few of them by themselves are as fast with half as
-    // many shares (128 tokens 26.2 us, with all 28.2; 384 52.8 and 46.0).
-    const unsigned groups = all_many * a.kv_heads, all_few = wave_sum(few);
-    const bool many_too = a.said && 3 * groups <= 2u * a.cus;
-    const unsigned left = many_too ? a.room : max(a.room - (int)min(all_many, (unsigned)a.room), (a.room + 1) / 2);
-    const unsigned room = many_too && !all_few && 8 * groups <= (unsigned)a.cus ? (left + 1) / 2 : left, of = many_too ? tiles : few;
+    // many shares (128 tokens 26.2 us, with all 28.2; 384 52.8 and 46.0).  Fewer rows, bound by memory, are divided in any case.
+    const unsigned all_many = wave_sum(many), heavy = rows > 64 ? tiles : 0, all_heavy = wave_sum(heavy), groups = all_heavy * a.kv_heads;
+    const bool heavy_too = a.said && 3 * groups <= 2u * a.cus, divisible = a.arrived && (rows <= kFew || (a.said && (rows <= 64 || heavy_too)));
+    const unsigned of = divisible ? tiles : 0, all_of = wave_sum(of), rest = min(wave_sum(tiles) - all_of, (unsigned)a.room);
+    const bool half = heavy_too && all_of == all_heavy && 8 * groups <= (unsigned)a.cus;
+    const unsigned room = half ? (a.room + 1) / 2 : max(a.room - rest, (a.room + 1u) / 2);
     // The keys of a share: the smallest multiple of kUnit (two of them for many rows) of which there are no more shares than there is room for, or
     // what makes one share of every tile.  (Sums stay in 32 bits.)
-    unsigned per = many_too && all_many ? 2 : 1, own = 1;
-    if (a.arrived) {
-      const unsigned least = wave_sum(of);
-      for (;;) {
-        own = min((units - 1) / per + 1, 64 * room);
-        const unsigned all = wave_sum(of * own);
-        if (all <= room || all <= least) break;
-        per += max(1u, (unsigned)((float)per * (float)(all - room) / (float)room));
-      }
+    unsigned per = all_many ? 2 : 1, own = 1;
+    for (;;) {
+      own = divisible ? min((units - 1) / per + 1, 64 * room) : 1;
+      const unsigned all = wave_sum(of * own);
+      if (all <= room || all <= all_of) break;
+      per += max(1u, (unsigned)((float)per * (float)(all - room) / (float)room));
     }
-    const unsigned own_many = many_too ? own : 1, all = wave_sum(many * own_many);
+    const unsigned all = wave_sum(many * own);
     if (says && lane < a.batch) {
-      a.said[2 * lane] = running_sum(many * own_many) - many * own_many;
-      a.said[2 * lane + 1] = own_many;
+      a.said[2 * lane] = running_sum(many * own) - many * own;
+      a.said[2 * lane + 1] = own;
     }
     const bool is_many = x < (int)all;
     if (!is_many) {
       x -= all;
       if ((unsigned)x >= wave_sum(few * own)) return false;
-    } else {
-      own = own_many;
     }
     const unsigned mine_of = (is_many ? many : few) * own;
     const unsigned to = running_sum(mine_of);
@@ -329,7 +326,7 @@ int launch_chunk(ChunkArgs a, int cus, hipStream_t stream) {
       few = divide ? std::min(std::max(room, requests), requests * units) : requests;
       many = tiles;
       if (divide && likely && tiles && tiles < 2 * room) {  // more tiles than that fill the device
-        many = std::max(tiles, std::min(room, tiles * units));
+        many = tiles + std::min(room, tiles * units);  // some as they are, beside shares that fill the room
         many_divided = true;
       }
     }
@@ -342,7 +339,7 @@ int launch_chunk(ChunkArgs a, int cus, hipStream_t stream) {
     divide = false;
   }
   // Divided, tiles of both kinds share the room; else the few have what the many leave.
-  const int64_t grid = a.ns ? few : std::min(few + many, tiles + std::max(room, requests));
+  const int64_t grid = a.ns ? few : many_divided ? tiles + std::max(room, requests) : tiles + few;
   if (grid * a.kv_heads > INT_MAX) return HQ_ERR_TOO_LARGE;
   a.few = (int)few;
   a.many = (int)many;
