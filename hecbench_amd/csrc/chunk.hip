@@ -340,7 +340,7 @@ int launch_chunk(ChunkArgs a, int cus, hipStream_t stream) {
   }
   // Divided, tiles of both kinds share the room; else the few have what the many leave.
   const int64_t grid = a.ns ? few : many_divided ? tiles + std::max(room, requests) : tiles + few;
-  if (grid * a.kv_heads > INT_MAX) return HQ_ERR_TOO_LARGE;
+  if (grid * a.kv_heads > UINT32_MAX / kThreads) return HQ_ERR_TOO_LARGE;  // threads are numbered in 32 bits
   a.few = (int)few;
   a.many = (int)many;
   if (divide) {

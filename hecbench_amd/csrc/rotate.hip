@@ -5,9 +5,11 @@
 // (a c - b s, b c + a s), c and s the cosine and sine of the pair's angle at the token's position.  One pass in fp32, one rounding.
 //
 // A lane holds two pieces of eight elements of a head, those that are rotated against each other, so that nothing but the sum of
-// the squares goes from lane to lane: D / 16 lanes a head, 64 * 16 / D heads at a time in a wave, a wave a token, whose cosines and
-// sines it reads once for all of them.  Bound by the copy; short calls by the launch and the loads that wait for another (positions, then
-// the table's row; in the cache's form bounds and starts, then the table's row and the page).
+// the squares goes from lane to lane: D / 16 lanes a head, 64 * 16 / D heads of a token a wave, which are queries, keys or values (of several
+// sets of heads one after the other, whose cosines and sines would be read once: 62.0 us with two, 64.3 with three where 60.9 here), in the
+// order of memory (a token's sets in workgroups far from each other: 78 us).  Bound by the copy: 16384 tokens of 32 / 8 heads of 128 57.8 us,
+// 5.9 TB/s of data, where a plain copy of 512 MB reaches 6.5; short calls by the launch and the loads that wait for another (positions, then
+// the table's row; in the cache's form bounds and starts, then the table's row and the page): one token 4.4 us.
 #include <climits>
 #include <cmath>
 
@@ -25,9 +27,11 @@ struct RotateArgs {
   const int *positions;  // of the plain form
   const int *table, *starts, *cu;
   int64_t qs, ks, vs, qos, kos;  // 16-byte pieces from one token to the next
-  int tokens, heads, kv_heads, all, rotary, known;  // all: heads of queries, keys and, in the cache's form, values; known: positions
+  int tokens, heads, kv_heads, rotary, known;  // known: positions of cs
   int rows, width, pages, page_log, interleaved;
   float eps;
+  int q_sets, k_sets;          // sets of heads
+  unsigned sets, reciprocal;   // of a token, all; 2^32 / sets, rounded up
 };
 
 template <typename T>
@@ -67,34 +71,25 @@ __device__ __forceinline__ int find_row(const int* bounds, int n, int t) {
   return lo;
 }
 
-// STEPS sets of heads of a token a wave.
-template <typename T, int D, bool CACHE, int STEPS>
-__global__ __launch_bounds__(kThreads) void rotate_kernel(RotateArgs a, int parts) {
+// A wave takes a set of a token's heads: of queries, of keys, or of values.
+template <typename T, int D, bool CACHE>
+__global__ __launch_bounds__(kThreads) void rotate_kernel(RotateArgs a) {
   constexpr int LANES = D / 16, HEADS = 64 / LANES, CH = D / 8;
-  const unsigned wave = blockIdx.x * kWaves + (threadIdx.x >> 6);
-  const int t = __builtin_amdgcn_readfirstlane(wave / (unsigned)parts), part = __builtin_amdgcn_readfirstlane(wave % (unsigned)parts);
+  const unsigned wave = __builtin_amdgcn_readfirstlane(blockIdx.x * kWaves + (threadIdx.x >> 6));
+  unsigned token = a.sets == 1 ? wave : __umulhi(wave, a.reciprocal);  // or one more
+  if (token * a.sets > wave) --token;
+  const int t = token, set = wave - token * a.sets;
   if (t >= a.tokens) return;
   const int lane = threadIdx.x & 63, l = lane % LANES, np = a.rotary / 16;
   const int pa = l < np ? l : 2 * l, pb = l < np ? l + np : 2 * l + 1;
-  const int first = part * (HEADS * STEPS) + lane / LANES;
-  hq_u4v xa[STEPS], xb[STEPS];
-#pragma unroll
-  for (int i = 0; i < STEPS; ++i) {
-    const int h = min(first + i * HEADS, a.all - 1);
-    const hq_u4v* const from = h < a.heads                  ? a.q + t * a.qs + h * CH
-                               : h < a.heads + a.kv_heads ? a.k + t * a.ks + (h - a.heads) * CH
-                                                          : a.v + t * a.vs + (h - a.heads - a.kv_heads) * CH;
-    xa[i] = from[pa];
-    xb[i] = from[pb];
-  }
-  hq_u4v wqa = {}, wqb = {}, wka = {}, wkb = {};
-  if (a.qw) {
-    wqa = a.qw[pa];
-    wqb = a.qw[pb];
-  }
-  if (a.kw) {
-    wka = a.kw[pa];
-    wkb = a.kw[pb];
+  const bool query = set < a.q_sets, key = !query && (!CACHE || set < a.q_sets + a.k_sets);
+  const int heads = query ? a.heads : a.kv_heads, h = (set - (query ? 0 : key ? a.q_sets : a.q_sets + a.k_sets)) * HEADS + lane / LANES;
+  const hq_u4v* const from = (query ? a.q + t * a.qs : key ? a.k + t * a.ks : a.v + t * a.vs) + min(h, heads - 1) * CH;
+  const hq_u4v* const weight = query ? a.qw : key ? a.kw : nullptr;
+  hq_u4v xa = from[pa], xb = from[pb], wa = {}, wb = {};
+  if (weight) {
+    wa = weight[pa];
+    wb = weight[pb];
   }
   int row = 0;
   int64_t place;
@@ -111,7 +106,7 @@ __global__ __launch_bounds__(kThreads) void rotate_kernel(RotateArgs a, int part
     cs[i] = 1.f;
     sn[i] = 0.f;
   }
-  if (l < np) {
+  if (l < np && (query || key)) {
     const int at = (int)min(max(place, (int64_t)0), (int64_t)a.known - 1);
     const hq_f4v* const c = a.cs + (int64_t)at * (a.rotary / 4);
     const int i0 = a.interleaved ? l : 2 * l, i1 = a.interleaved ? l + np : 2 * l + 1, sines = a.rotary / 8;
@@ -124,82 +119,88 @@ __global__ __launch_bounds__(kThreads) void rotate_kernel(RotateArgs a, int part
       sn[4 + i] = s1[i];
     }
   }
-  bool there = true;
-  int64_t to_page = 0;  // pieces of the token's row of head 0 in its page
-  if (CACHE) {
-    there = place >= 0 && place < (int64_t)a.width << a.page_log;
-    const int page = there ? a.table[(int64_t)row * a.width + (place >> a.page_log)] : -1;
-    there = (unsigned)page < (unsigned)a.pages;
-    to_page = ((((int64_t)page * a.kv_heads) << a.page_log) + (place & ((1 << a.page_log) - 1))) * CH;
+  hq_u4v* to;
+  bool there = h < heads;
+  if (query) {
+    to = a.qo + t * a.qos + h * CH;
+  } else if (CACHE) {
+    const bool within = place >= 0 && place < (int64_t)a.width << a.page_log;
+    const int page = within ? a.table[(int64_t)row * a.width + (place >> a.page_log)] : -1;
+    there = there && (unsigned)page < (unsigned)a.pages;
+    to = (key ? a.ko : a.vo) + ((((int64_t)page * a.kv_heads + h) << a.page_log) + (place & ((1 << a.page_log) - 1))) * CH;
+  } else {
+    to = a.ko + t * a.kos + h * CH;
   }
-#pragma unroll
-  for (int i = 0; i < STEPS; ++i) {
-    const int h = first + i * HEADS;
-    const bool query = h < a.heads, key = !query && h < a.heads + a.kv_heads;
-    hq_u4v ya = xa[i], yb = xb[i];
-    if (query || key) {
-      float u[8], v[8];
-      wide<T>(u, xa[i]);
-      wide<T>(v, xb[i]);
+  if (query || key) {
+    float u[8], v[8];
+    wide<T>(u, xa);
+    wide<T>(v, xb);
+    if (weight) {
       float ss = 0.f;
 #pragma unroll
       for (int j = 0; j < 8; ++j) ss = fmaf(u[j], u[j], fmaf(v[j], v[j], ss));
       ss = head_sum<LANES>(ss);
-      if (query ? a.qw != nullptr : a.kw != nullptr) {
-        float r = rsqrtf(fmaf(ss, 1.f / D, a.eps)), pre = 1.f;
-        if (__builtin_expect(!(ss < INFINITY), 0)) {  // bf16 holds numbers whose squares fp32 does not
-          pre = 0x1p-70f;
-          ss = 0.f;
-#pragma unroll
-          for (int j = 0; j < 8; ++j) ss = fmaf(u[j] * pre, u[j] * pre, fmaf(v[j] * pre, v[j] * pre, ss));
-          r = rsqrtf(fmaf(head_sum<LANES>(ss), 1.f / D, a.eps * pre * pre));
-        }
-        float wu[8], wv[8];
-        wide<T>(wu, query ? wqa : wka);
-        wide<T>(wv, query ? wqb : wkb);
+      float r = rsqrtf(fmaf(ss, 1.f / D, a.eps));
+      if (__builtin_expect(!(ss < INFINITY), 0)) {  // bf16 holds numbers whose squares fp32 does not
+        constexpr float down = 0x1p-70f;
+        ss = 0.f;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          u[j] = u[j] * pre * r * wu[j];
-          v[j] = v[j] * pre * r * wv[j];
+          u[j] *= down;
+          v[j] *= down;
+          ss = fmaf(u[j], u[j], fmaf(v[j], v[j], ss));
         }
+        r = rsqrtf(fmaf(head_sum<LANES>(ss), 1.f / D, a.eps * down * down));
       }
-      if (a.interleaved) {
+      float wu[8], wv[8];
+      wide<T>(wu, wa);
+      wide<T>(wv, wb);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float u0 = u[2 * j], v0 = v[2 * j];
-          u[2 * j] = u0 * cs[j] - u[2 * j + 1] * sn[j];
-          u[2 * j + 1] = u[2 * j + 1] * cs[j] + u0 * sn[j];
-          v[2 * j] = v0 * cs[4 + j] - v[2 * j + 1] * sn[4 + j];
-          v[2 * j + 1] = v[2 * j + 1] * cs[4 + j] + v0 * sn[4 + j];
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float u0 = u[j];
-          u[j] = u0 * cs[j] - v[j] * sn[j];
-          v[j] = v[j] * cs[j] + u0 * sn[j];
-        }
+      for (int j = 0; j < 8; ++j) {
+        u[j] *= r * wu[j];
+        v[j] *= r * wv[j];
       }
-      ya = narrow<T>(u);
-      yb = narrow<T>(v);
     }
-    hq_u4v* to;
-    if (query) to = a.qo + t * a.qos + h * CH;
-    else if (CACHE) to = (key ? a.ko : a.vo) + to_page + ((int64_t)(h - a.heads - (key ? 0 : a.kv_heads)) << a.page_log) * CH;
-    else to = a.ko + t * a.kos + (h - a.heads) * CH;
-    if (h < a.all && (query || there)) {
-      to[pa] = ya;
-      to[pb] = yb;
+    if (a.interleaved) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float u0 = u[2 * j], v0 = v[2 * j];
+        u[2 * j] = u0 * cs[j] - u[2 * j + 1] * sn[j];
+        u[2 * j + 1] = u[2 * j + 1] * cs[j] + u0 * sn[j];
+        v[2 * j] = v0 * cs[4 + j] - v[2 * j + 1] * sn[4 + j];
+        v[2 * j + 1] = v[2 * j + 1] * cs[4 + j] + v0 * sn[4 + j];
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float u0 = u[j];
+        u[j] = u0 * cs[j] - v[j] * sn[j];
+        v[j] = v[j] * cs[j] + u0 * sn[j];
+      }
     }
+    xa = narrow<T>(u);
+    xb = narrow<T>(v);
+  }
+  if (!there) return;
+  if (D == 128) {  // whole lines, past the L2 (16384 tokens 60.9 -> 57.8 us); of heads of 64 they are halves, which the L2 puts together (33.5; past it 95)
+    hq_store_stream(to + pa, xa);
+    hq_store_stream(to + pb, xb);
+  } else {
+    to[pa] = xa;
+    to[pb] = xb;
   }
 }
 
 template <typename T, int D, bool CACHE>
-int launch_rotate(const RotateArgs& a, hipStream_t stream) {
-  constexpr int HEADS = 64 * 16 / D, STEPS = 2;
-  const int64_t parts = (a.all + HEADS * STEPS - 1) / (HEADS * STEPS), blocks = (a.tokens * parts + kWaves - 1) / kWaves;
-  if (blocks > INT_MAX / kWaves) return HQ_ERR_TOO_LARGE;
-  return hq_launch_as_is(rotate_kernel<T, D, CACHE, STEPS>, dim3((unsigned)blocks), dim3(kThreads), 0, stream, a, (int)parts);
+int launch_rotate(RotateArgs a, hipStream_t stream) {
+  constexpr int HEADS = 64 * 16 / D;
+  a.q_sets = (a.heads + HEADS - 1) / HEADS;
+  a.k_sets = (a.kv_heads + HEADS - 1) / HEADS;
+  a.sets = a.q_sets + (CACHE ? 2 : 1) * a.k_sets;
+  a.reciprocal = (unsigned)(((1ull << 32) + a.sets - 1) / a.sets);
+  const uint64_t blocks = ((uint64_t)a.tokens * a.sets + kWaves - 1) / kWaves;
+  if (blocks > UINT32_MAX / kThreads) return HQ_ERR_TOO_LARGE;  // threads are numbered in 32 bits
+  return hq_launch_as_is(rotate_kernel<T, D, CACHE>, dim3((unsigned)blocks), dim3(kThreads), 0, stream, a);
 }
 #define HQ_BY_TYPE(cache)                                                                                                        \
   (dtype == HQ_DTYPE_F16 ? (head_dim == 64 ? launch_rotate<_Float16, 64, cache>(a, s) : launch_rotate<_Float16, 128, cache>(a, s)) \
@@ -273,7 +274,6 @@ extern "C" int hq_norm_rotate(const void* q, const void* k, void* q_out, void* k
   a.tokens = (int)tokens;
   a.heads = heads;
   a.kv_heads = kv_heads;
-  a.all = heads + kv_heads;
   a.rotary = rotary;
   a.known = num_positions;
   a.interleaved = interleaved != 0;
@@ -326,7 +326,6 @@ extern "C" int hq_cache_write_rotated(const void* q, const void* k, const void* 
   a.tokens = (int)tokens;
   a.heads = heads;
   a.kv_heads = kv_heads;
-  a.all = heads + 2 * kv_heads;
   a.rotary = rotary;
   a.known = num_positions;
   a.rows = rows;
