@@ -202,6 +202,12 @@ struct PackedTiles {
     offsets(voff, (int)vs, n - first, v_piece<D>);
   }
   __device__ __forceinline__ void advance(int) {}
+  // Keys of the first two tiles, if there are two, and values of the first one, all at once.
+  __device__ __forceinline__ void begin(char* k0, char* k1, char* v0, bool two) {
+    load_k(0, k0);
+    load_v(0, v0);
+    if (two) load_k(1, k1);
+  }
   // A tile on both sides of what is left out: every lane by an address of its own.
   template <typename F>
   __device__ __forceinline__ void load_across(const T* from, int64_t stride, int base, char* to, F piece) const {
@@ -304,6 +310,17 @@ struct PagedTiles {
     koff = row * D * 2 + k_piece<D>(row, lane % CH) * 16;
     voff = row * D * 2 + v_piece<D>(row, lane % CH) * 16;
     ids = p.id(place(min(key(0), n - 1)));
+    if (D == 128) {  // the first two tiles' pages by one trip to memory
+      const int then = p.id(place(min(key(1), n - 1)));
+      now.set(p, ids, place(key(0)));
+      next.set(p, then, place(key(1)));
+      ids = p.id(place(min(key(2), n - 1)));
+    }
+  }
+  __device__ __forceinline__ void begin(char* k0, char* k1, char* v0, bool two) const {
+    now.template load<D, false, NL>(p.k, 0, koff, k0 + (threadIdx.x >> 6) * (NL * 1024));
+    load_v(0, v0);
+    if (two) load_k(1, k1);
   }
   // Before the first load of tile t: its pages are there, those of the tile behind it are asked for.
   __device__ __forceinline__ void advance(int t) {
@@ -311,8 +328,8 @@ struct PagedTiles {
     next.set(p, ids, place(key(t)));
     ids = p.id(place(min(key(t + 1), n - 1)));
   }
-  __device__ __forceinline__ void load_k(int, char* to) { next.template load<D, false, NL>(p.k, 0, koff, to + (threadIdx.x >> 6) * (NL * 1024)); }
-  __device__ __forceinline__ void load_v(int, char* to) {
+  __device__ __forceinline__ void load_k(int, char* to) const { next.template load<D, false, NL>(p.k, 0, koff, to + (threadIdx.x >> 6) * (NL * 1024)); }
+  __device__ __forceinline__ void load_v(int, char* to) const {
     (D == 128 ? now : next).template load<D, true, NL>(p.v, 0, voff, to + (threadIdx.x >> 6) * (NL * 1024));
   }
 };
@@ -603,17 +620,18 @@ struct Many {
     f32x16 s0[NB], s1[NB];
     float top = 0.f;
     src.start(first);
-    src.advance(0);
-    src.load_k(0, sm);
-    if (!K_AHEAD) src.load_v(0, sm + 2 * HALF);
+    if (K_AHEAD) {
+      src.begin(sm, sm + HALF, sm + 2 * HALF, nt > 1);
+    } else {
+      src.advance(0);
+      src.load_k(0, sm);
+      src.load_v(0, sm + 2 * HALF);
+    }
 #pragma unroll
     for (int kk = 0; kk < D / 16; ++kk) asm volatile("" : "+v"(qf[kk]));  // here, not at every tile: the loads in flight then are the next tile's
     if (K_AHEAD) {
-      src.advance(1);
-      src.load_v(0, sm + 2 * HALF);
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       __syncthreads();
-      if (nt > 1) src.load_k(1, sm + HALF);
       scores(s0, sm);
       if (partial(first)) mask(s0, first + half4);
       top = top_of(s0);
