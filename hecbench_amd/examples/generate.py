@@ -1,11 +1,12 @@
 """A decoder of 3-bit weights that serves several requests at once: prompts taken in together, every request forked into samples
 behind its prompt, tokens generated for all of them over one paged key / value cache, samples dropped, the cache compacted.
 
-    python -m hecbench_amd.examples.generate [--layers N] [--prompts N] [--samples N] [--tokens N]
+    python -m hecbench_amd.examples.generate [--layers N] [--prompts N] [--samples N] [--tokens N] [--piece N] [--window N] [--sinks N]
 
 The weights are random and nothing is sampled: a token's embedding is what the last layer gave, so what is shown is how the operators
 go together.  Every projection is hq.q3_gemm; what a step does to the cache is hq.cache_step (tables, forks, pages) once for all
-layers, and in each layer hq.cache_write and hq.prompt_attention or hq.paged_attention.
+layers.  In each layer, whole prompts go through hq.norm_rotate, hq.cache_write and hq.prompt_attention; the next tokens, or pieces of
+prompts, through hq.cache_write_rotated and hq.paged_attention or, pieces and windows, hq.chunk_attention.
 """
 import argparse
 import time
@@ -37,12 +38,19 @@ def norm(x):
 
 
 class Decoder:
-    def __init__(self, layers=4, heads=32, kv_heads=8, head_dim=128, hidden=4096, wide=11008, seed=0):
+    """rotary: base of the positions' angles (None: no positions, and no norm of queries and keys), for up to `longest` tokens.  window: a token
+    sees that many tokens up to itself (None: all of them) and the first `sinks`."""
+
+    def __init__(self, layers=4, heads=32, kv_heads=8, head_dim=128, hidden=4096, wide=11008, seed=0, rotary=None, longest=8192, window=None, sinks=0):
+        self.window, self.sinks = window, sinks
         gen = torch.Generator(device="cuda").manual_seed(seed)
         self.heads, self.kv_heads, self.head_dim, self.hidden = heads, kv_heads, head_dim, hidden
         rows = (heads + 2 * kv_heads) * head_dim
         self.layers = [(Linear(hidden, rows, gen), Linear(heads * head_dim, hidden, gen), Linear(hidden, wide, gen), Linear(wide, hidden, gen))
                        for _ in range(layers)]
+        self.angles = None if rotary is None else hq.rotary_table(longest, head_dim, rotary)
+        self.head_norms = [[(1 + 0.1 * torch.randn(head_dim, generator=gen, device="cuda")).half() for _ in range(2)]
+                           for _ in range(layers if rotary is not None else 0)]
 
     def forward(self, x, attend):
         """x [tokens][hidden]; attend(layer, q, k, v) attends and keeps what it must."""
@@ -58,7 +66,7 @@ class Cache:
     """The pages of all layers, and the tables of the requests that are under way."""
 
     def __init__(self, model, rows, pages, page=16, width=64):
-        self.page, self.rows = page, rows
+        self.page, self.rows, self.model = page, rows, model
         self.pool = torch.zeros((2 * len(model.layers), pages, model.kv_heads, page, model.head_dim), dtype=torch.float16, device="cuda")
         self.table = torch.full((rows, width), -1, dtype=torch.int32, device="cuda")
         self.lengths = torch.zeros(rows, dtype=torch.int32, device="cuda")
@@ -74,8 +82,19 @@ class Cache:
         self.table, self.refs, live = hq.cache_compact(self.pool, self.table, self.refs)
         return live
 
-    def write(self, layer, k, v, cu):
-        hq.cache_write(k, v, self.pool[2 * layer], self.pool[2 * layer + 1], self.table, self.starts, cu)
+    def pages(self, layer):
+        return self.pool[2 * layer], self.pool[2 * layer + 1]
+
+    def write(self, layer, q, k, v, cu):
+        """Keys and values of the step's tokens; the queries, which go by the same positions."""
+        if self.model.angles is None:
+            hq.cache_write(k, v, *self.pages(layer), self.table, self.starts, cu)
+            return q
+        return hq.cache_write_rotated(q, k, v, *self.pages(layer), self.table, self.starts, cu, self.model.angles, *self.model.head_norms[layer])
+
+    def attend(self, layer, q, cu):
+        """Of the step's tokens, any number a row, to what is in the cache."""
+        return hq.chunk_attention(q, *self.pages(layer), self.table, self.lengths, cu, window=self.model.window, sinks=self.model.sinks)
 
 
 def i32(values):
@@ -99,9 +118,13 @@ class Server:
         self.same = torch.arange(rows, dtype=torch.int32, device="cuda")
         self.one = torch.ones(rows, dtype=torch.int32, device="cuda")
 
-    def take_in(self):
-        """All prompts in one pass, each into the first row of its samples; then the fork.  The prompts' last outputs, a row a sample."""
+    def take_in(self, piece=None):
+        """All prompts in one pass, or `piece` tokens of each at a time, into the first row of its samples; then the fork.  The prompts' last
+        outputs, a row a sample."""
         n, s, c = len(self.lengths), self.samples, self.cache
+        self.fork = i32([i // s * s for i in range(n * s)])  # every sample goes on from its prompt's row
+        if piece:
+            return self.take_in_pieces(piece)
         add, bounds, at = [0] * (n * s), [0], 0
         for i, length in enumerate(self.lengths):
             add[i * s] = length
@@ -111,13 +134,34 @@ class Server:
         cu, packed = i32(bounds), i32([0] + [b for b in bounds[1::s]])
 
         def attend(layer, q, k, v):
-            c.write(layer, k, v, cu)
-            return hq.prompt_attention(q, k, v, packed)
+            if self.model.angles is not None:  # attention and the cache both take the keys
+                q, k = hq.norm_rotate(q, k, self.model.angles, positions, *self.model.head_norms[layer])
+            hq.cache_write(k, v, *c.pages(layer), c.table, c.starts, cu)
+            return hq.prompt_attention(q, k, v, packed, window=self.model.window, sinks=self.model.sinks)
 
+        positions = torch.cat([torch.arange(length, dtype=torch.int32, device="cuda") for length in self.lengths])
         x = self.model.forward(self.prompts, attend)
         last = x[packed[1:].long() - 1]
-        self.fork = i32([i // s * s for i in range(n * s)])  # every sample goes on from its prompt's row
         return last.repeat_interleave(s, 0)
+
+    def take_in_pieces(self, piece):
+        n, s, c = len(self.lengths), self.samples, self.cache
+        last = [None] * n
+        begins = [sum(self.lengths[:i]) for i in range(n)]
+        for done in range(0, max(self.lengths), piece):
+            new = [max(0, min(piece, length - done)) for length in self.lengths]
+            add, bounds = [0] * (n * s), [0]
+            for i, m in enumerate(new):
+                add[i * s] = m
+                bounds += [bounds[-1] + m] * s
+            cu = i32(bounds)
+            c.step(self.same if done else torch.full((n * s,), -1, dtype=torch.int32, device="cuda"), i32(add))
+            x = self.model.forward(torch.cat([self.prompts[b + done:b + done + m] for b, m in zip(begins, new)]),
+                                   lambda layer, q, k, v: c.attend(layer, c.write(layer, q, k, v, cu), cu))
+            for i, m in enumerate(new):
+                if m and done + m == self.lengths[i]:
+                    last[i] = x[bounds[(i + 1) * s] - 1]
+        return torch.stack(last).repeat_interleave(s, 0)
 
     def token(self, x, parent, add=None):
         """The next token of every row: x [rows][hidden] in, its output back."""
@@ -125,15 +169,17 @@ class Server:
         c.step(parent, self.one if add is None else add)
 
         def attend(layer, q, k, v):
-            c.write(layer, k, v, self.one_each)
-            return hq.paged_attention(q, c.pool[2 * layer], c.pool[2 * layer + 1], c.table, c.lengths, self.groups, self.shared)
+            q = c.write(layer, q, k, v, self.one_each)
+            if self.model.window is not None:
+                return c.attend(layer, q, self.one_each)
+            return hq.paged_attention(q, *c.pages(layer), c.table, c.lengths, self.groups, self.shared)
 
         return self.model.forward(x, attend)
 
-    def run(self, tokens, compact_every=16, spread=0.02):
+    def run(self, tokens, compact_every=16, spread=0.02, piece=None):
         """Generates; the samples of a prompt are told apart by a little noise on their first embedding.  All inputs, [step][row][hidden]."""
         gen = torch.Generator(device="cuda").manual_seed(1)
-        x = self.take_in()
+        x = self.take_in(piece)
         x = x + (torch.randn(x.shape, generator=gen, device="cuda") * spread).half()
         inputs = []
         for i in range(tokens):
@@ -150,16 +196,19 @@ def main():
     ap.add_argument("--prompts", type=int, default=4)
     ap.add_argument("--samples", type=int, default=8)
     ap.add_argument("--tokens", type=int, default=32)
+    ap.add_argument("--piece", type=int, help="take prompts in by so many tokens each at a time")
+    ap.add_argument("--window", type=int, help="tokens that a token sees, itself among them (default: all)")
+    ap.add_argument("--sinks", type=int, default=0, help="first tokens that stay visible behind the window")
     a = ap.parse_args()
     hq.init()
-    model = Decoder(a.layers)
+    model = Decoder(a.layers, rotary=10000.0, window=a.window, sinks=a.sinks)
     gen = torch.Generator(device="cuda").manual_seed(2)
     prompts = [torch.randn((200 + 173 * i, model.hidden), generator=gen, device="cuda").half() for i in range(a.prompts)]
-    Server(model, prompts, a.samples, 2).run(2)  # the first calls size the stream's workspace
+    Server(model, prompts, a.samples, 2).run(2, piece=a.piece)  # the first calls size the stream's workspace
     server = Server(model, prompts, a.samples, a.tokens)
     torch.cuda.synchronize()
     t = time.perf_counter()
-    x = server.take_in()
+    x = server.take_in(a.piece)
     torch.cuda.synchronize()
     t1 = time.perf_counter()
     for i in range(a.tokens):
