@@ -325,7 +325,8 @@ int launch_chunk(ChunkArgs a, int cus, hipStream_t stream) {
     } else {
       few = divide ? std::min(std::max(room, requests), requests * units) : requests;
       many = tiles;
-      if (divide && likely && tiles && tiles < 2 * room) {  // more tiles than that fill the device
+      // (Where the likely ones are too many to be divided, nothing asks for room for their shares and a launch that joins them.)
+      if (divide && tiles && tiles < 2 * room && likely && 3 * likely * a.kv_heads <= 2 * cus) {  // more tiles than that fill the device
         many = tiles + std::min(room, tiles * units);  // some as they are, beside shares that fill the room
         many_divided = true;
       }
