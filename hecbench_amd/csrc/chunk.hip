@@ -90,9 +90,9 @@ struct Item {
     // many shares (128 tokens 26.2 us, with all 28.2; 384 52.8 and 46.0).  Fewer rows, bound by memory, are divided in any case.
     const unsigned all_many = wave_sum(many), heavy = rows > 64 ? tiles : 0, all_heavy = wave_sum(heavy), groups = all_heavy * a.kv_heads;
     const bool heavy_too = a.said && 3 * groups <= 2u * a.cus, divisible = a.arrived && (rows <= kFew || (a.said && (rows <= 64 || heavy_too)));
-    const unsigned of = divisible ? tiles : 0, all_of = wave_sum(of), rest = min(wave_sum(tiles) - all_of, (unsigned)a.room);
+    const unsigned of = divisible ? tiles : 0, all_of = wave_sum(of);
     const bool half = heavy_too && all_of == all_heavy && 8 * groups <= (unsigned)a.cus;
-    const unsigned room = half ? (a.room + 1) / 2 : max(a.room - rest, (a.room + 1u) / 2);
+    const unsigned room = half ? (a.room + 1) / 2 : a.room;
     // The keys of a share: the smallest multiple of kUnit (two of them for many rows) of which there are no more shares than there is room for, or
     // what makes one share of every tile.  (Sums stay in 32 bits.)
     unsigned per = all_many ? 2 : 1, own = 1;
@@ -339,7 +339,7 @@ int launch_chunk(ChunkArgs a, int cus, hipStream_t stream) {
     if (!hq_workspace_out_of_reach(stream, floats, counters)) break;
     divide = false;
   }
-  // Divided, tiles of both kinds share the room; else the few have what the many leave.
+  // What is divided shares the room, beside what is not.
   const int64_t grid = a.ns ? few : many_divided ? tiles + std::max(room, requests) : tiles + few;
   if (grid * a.kv_heads > UINT32_MAX / kThreads) return HQ_ERR_TOO_LARGE;  // threads are numbered in 32 bits
   a.few = (int)few;
