@@ -47,7 +47,7 @@ extern "C" {
 /* element types of the activation vector / matrix */
 #define HQ_DTYPE_F32 0
 #define HQ_DTYPE_F16 1
-#define HQ_DTYPE_BF16 2 /* accepted by the activation quantisers, hq_mxfp4_qdq, attention and its cache only */
+#define HQ_DTYPE_BF16 2 /* accepted by the activation quantisers, hq_mxfp4_qdq, attention, its cache and the rotations only */
 
 /* flags */
 #define HQ_FLAG_ACCUMULATE 1u /* y += result (reference wrapper semantics) */
@@ -338,7 +338,7 @@ int hq_mxfp4_qdq(const void* in, void* out, int64_t n_elems, int dtype, void* st
  *   projection's rows), k_stride and v_stride up to 2^22; out contiguous; all 16-byte aligned, strides multiples of 8.  Tokens of no
  *   sequence are not written.
  * hq_prompt_attention_window: causal, and key j is seen by the token whose own key is the p-th of its sequence (p as above the largest j that it
- *   sees) only if j > p - window or j < sinks.  window 1 at least, sinks 0 at least.  Keys that no token sees are not read.
+ *   sees) only if j > p - window or j < sinks.  window 1 at least, sinks 0 at least.
  * hq_paged_attention: one query a request.  Token t of request s is token t % page_size of page table[s][t / page_size]
  *   (table [batch][table_width], pages [num_pages][kv_heads][page_size][head_dim], contiguous); request s sees its first lengths[s] tokens.
  *   Requests groups[g] ... groups[g+1]-1 (bounds in ascending order) have their first shared[g] tokens, as far as the first one's
@@ -347,8 +347,9 @@ int hq_mxfp4_qdq(const void* in, void* out, int64_t n_elems, int dtype, void* st
  *   A table entry that is needed and no page counts as a page of zeros (num_pages 0: all of them).
  * hq_chunk_attention: any number of queries a request, the last of its tokens: tokens cu_q[s] ... cu_q[s+1]-1 of q [total_q][heads][head_dim] are tokens
  *   lengths[s] - n ... lengths[s]-1 of row s of the table [batch][table_width] (n of them; q, pages and table entries as above), and see the
- *   tokens up to their own; window > 0: of those, the last `window` and the first `sinks` of the request; tokens and pages that nobody sees
- *   are not read.  A token before the request's first sees nothing and gets zeros; tokens of no request are not written.
+ *   tokens up to their own; window > 0: of those, the last `window` and the first `sinks` of the request (window 0: all).  Bounds in ascending
+ *   order.  Pages that hold nothing that a token sees are not read: their entries may be anything.  A token before the request's first sees
+ *   nothing and gets zeros; tokens of no request are not written.
  * hq_cache_write: tokens cu[s] ... cu[s+1]-1 of k and v [tokens][kv_heads][head_dim] (strides as above) become tokens starts[s], ... of row s
  *   of the table; any head_dim that is a multiple of 8, page_size a power of two, 1 ... 1024.  A token whose place is outside its row, or in no page, is left out.
  * hq_cache_step: from the tables of one step to the next one's.  Row s inherits row parent[s] (of the old tables; any number outside
@@ -403,6 +404,7 @@ int hq_cache_compact(void* pool, int planes, int64_t page_bytes, const int32_t* 
  *   share no memory with the inputs otherwise (HQ_ERR_BAD_SHAPE).  All data 16-byte aligned.
  * hq_cache_write_rotated: the same for tokens cu[s] ... cu[s+1]-1, at positions starts[s] ... : keys and values go to those tokens of row s
  *   of the table, as hq_cache_write takes them, the queries to q_out (also those whose keys have no place).  Tokens of no row are not written.
+ * Neither uses a workspace.
  */
 int hq_norm_rotate(const void* q, const void* k, void* q_out, void* k_out, int dtype, const void* q_weight, const void* k_weight,
                    const float* cos_sin, const int32_t* positions, int64_t tokens, int heads, int kv_heads, int head_dim, int rotary,
