@@ -157,8 +157,8 @@ __global__ __launch_bounds__(kThreads) void rotate_kernel(RotateArgs a) {
       wide<T>(wv, wb);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        u[j] *= r * wu[j];
-        v[j] *= r * wv[j];
+        u[j] = u[j] * r * wu[j];  // in this order: u r is sqrt(D) at most, r w has no bound
+        v[j] = v[j] * r * wv[j];
       }
     }
     if (a.interleaved) {

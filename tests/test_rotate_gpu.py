@@ -166,6 +166,18 @@ def test_numbers_at_the_ends(hq):
     assert torch.isnan(got[0, 0]).nonzero().view(-1).tolist() == [3, 35] and torch.isfinite(got[1:]).all()
 
 
+def test_far_weights(hq):
+    """Heads of zeros, and of numbers near the ends, beside weights that make 1 / rms times weight larger or smaller than fp32 holds."""
+    dtype, u = TYPES["bf16"]
+    p = i32([0] * 3)
+    for x, w, eps in ((0.0, 2.0 ** 80, 2.0 ** -126), (2.0 ** 60, 2.0 ** -85, 1e-6), (2.0 ** -60, 2.0 ** 70, 2.0 ** -126)):
+        q = (x * (0.5 + randn(2, 3, 2, 64).abs())).to(dtype)
+        weight = (w * (0.5 + randn(3, 64).abs())).to(dtype)
+        got, _ = hq.norm_rotate(q, q[:, :1], None, p, weight, None, eps)
+        want, size = formula(q, weight, None, p, eps, False)
+        assert torch.isfinite(got).all() and ((got.double() - want).abs() <= u * want.abs() + 2.0 ** -18 * size).all()
+
+
 def test_nothing(hq):
     table = hq.rotary_table(4, 64)
     q, k = torch.zeros((0, 4, 64), dtype=torch.float16, device="cuda"), torch.zeros((0, 2, 64), dtype=torch.float16, device="cuda")
