@@ -31,11 +31,13 @@ constexpr int kFew = 16, kUnit = 128, kRows = 128;
 // A request: its new tokens and the tokens it has with them.
 struct Request {
   int q0, nq, length;
-  __device__ __forceinline__ void get(const ChunkArgs& a, int i) {
+  // false: its bounds do not ascend.
+  __device__ __forceinline__ bool get(const ChunkArgs& a, int i) {
     const int qb = a.cu_q[i], qe = a.cu_q[i + 1], n = a.lengths[i];
     q0 = min(max(qb, 0), a.total_q);
     nq = min(max(qe, q0), a.total_q) - q0;
     length = min(max(n, 0), a.width << a.page_log);
+    return qb <= qe;
   }
   __device__ __forceinline__ int tiles(int ratio) const {  // nq * ratio is below 2^31 - 128
     const int rows = nq * ratio;
@@ -76,7 +78,9 @@ struct Item {
       return tile >= 0 && tile < r.tiles(a.ratio) && share < count;
     }
     Request mine;
-    mine.get(a, min(lane, a.batch - 1));
+    // Bounds that do not ascend may hold a token many times, more tiles than the host counted on: nothing is divided then, so that no share
+    // lies behind the room for them, and no counter waits for one that the grid has no workgroup for.
+    const bool ascend = !__ballot(!mine.get(a, min(lane, a.batch - 1)));
     if (lane >= a.batch) mine.nq = 0;
     const int tiles = mine.tiles(a.ratio), rows = mine.nq * a.ratio;
     int keys = mine.length;
@@ -89,7 +93,7 @@ struct Item {
     // in three shares, 78 undivided; 768 in two 74 and 78, 896 78 and 78, 1024 82 and 78).  A few of them by themselves are as fast with half as
     // many shares (128 tokens 26.2 us, with all 28.2; 384 52.8 and 46.0).  Fewer rows, bound by memory, are divided in any case.
     const unsigned all_many = wave_sum(many), heavy = rows > 64 ? tiles : 0, all_heavy = wave_sum(heavy), groups = all_heavy * a.kv_heads;
-    const bool heavy_too = a.said && 3 * groups <= 2u * a.cus, divisible = a.arrived && (rows <= kFew || (a.said && (rows <= 64 || heavy_too)));
+    const bool heavy_too = a.said && 3 * groups <= 2u * a.cus, divisible = ascend && a.arrived && (rows <= kFew || (a.said && (rows <= 64 || heavy_too)));
     const unsigned of = divisible ? tiles : 0, all_of = wave_sum(of);
     const bool half = heavy_too && all_of == all_heavy && 8 * groups <= (unsigned)a.cus;
     const unsigned room = half ? (a.room + 1) / 2 : a.room;

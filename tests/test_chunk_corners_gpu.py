@@ -164,3 +164,23 @@ def test_two_graphs_of_a_stream_in_turn(hq):
         stream.synchronize()
         for out, (args, cache, new) in ((graphs[i % 2][1], calls[i % 2]), (eager, calls[1 - i % 2])):
             check_chunk(args[0], out, cache, new, None, 0, None, u)
+
+
+@pytest.mark.parametrize("heads,kv,batch", [(4, 1, 64), (8, 2, 64), (32, 8, 20), (16, 1, 63), (8, 2, 90)])
+def test_bounds_that_do_not_ascend(hq, heads, kv, batch):
+    """Whatever they are, the call ends, tokens of no request stay as they were, and the next call finds its workspace in order."""
+    dtype, u = TYPES["bf16"]
+    lengths = [400 + 37 * (i % 5) for i in range(batch)]
+    cache = Cache(2, lengths, kv, 16, 128, dtype)
+    q = randn(3, 8 + 40, heads, 128).to(dtype)
+    for window, sinks in ((None, 0), (150, 5)):
+        for cycle in ((0, 4), (4, 8, 0), (0, 8, 3, 8, -5), (8, 0, 10 ** 9, 5, -2 ** 31), (8, 7, 6, 5), (0, 48), (2, 40, 1)):
+            cu = [cycle[i % len(cycle)] for i in range(batch + 1)]
+            out = torch.full_like(q, 7.0)
+            hq.chunk_attention(q, cache.k, cache.v, cache.table, i32(lengths), i32(cu), window=window, sinks=sinks, out=out)
+            inside = {t for a, b in zip(cu, cu[1:]) for t in range(max(a, 0), min(b, len(q)))}
+            outside = [t for t in range(len(q)) if t not in inside]
+            assert (out[outside] == 7).all(), cycle
+            new = [1 + (i % 3 == 0) for i in range(batch)]
+            good, got = run_chunk(hq, cache, new, heads, 128, dtype, window, sinks)
+            check_chunk(good, got, cache, new, window, sinks, None, u)
