@@ -7,9 +7,12 @@
 // A lane holds two pieces of eight elements of a head, those that are rotated against each other, so that nothing but the sum of
 // the squares goes from lane to lane: D / 16 lanes a head, 64 * 16 / D heads of a token a wave, which are queries, keys or values (of several
 // sets of heads one after the other, whose cosines and sines would be read once: 62.0 us with two, 64.3 with three where 60.9 here), in the
-// order of memory (a token's sets in workgroups far from each other: 78 us).  Bound by the copy: 16384 tokens of 32 / 8 heads of 128 57.8 us,
-// 5.9 TB/s of data, where a plain copy of 512 MB reaches 6.5; short calls by the launch and the loads that wait for another (positions, then
-// the table's row; in the cache's form bounds and starts, then the table's row and the page): one token 4.4 us.
+// order of memory (a token's sets in workgroups far from each other: 78 us).  Memory sees whole heads all the same, half of the wave's an instruction
+// (exchange): stores of a lane's own two pieces are of half lines wherever they are not halves of a head of 128, and cost 16384 tokens of
+// 32 / 8 heads of 64 34.3 us by way of the L2, which puts them together, where it is 29.7 here, and with 64 of 128 elements rotated, past the L2,
+// 108 where it is 55.8.  Bound by the copy: of heads of 128 56.0 us, 6.1 TB/s of data, where a plain copy of 512 MB reaches 6.5; short calls by
+// the launch and the loads that wait for another (positions, then the table's row; in the cache's form bounds and starts, then the table's
+// row and the page): one token 4.4 us.
 #include <climits>
 #include <cmath>
 
@@ -56,6 +59,17 @@ __device__ __forceinline__ float head_sum(float v) {
   return LANES == 8 ? v + hq_dpp<0x141>(v) : v;  // row_half_mirror
 }
 
+// The upper lanes' first pieces against the lower lanes' second ones: what were two pieces of every lane is then the lower lanes' heads, whole, in one
+// register and the upper lanes' in the other; and back.
+__device__ __forceinline__ void exchange(hq_u4v& a, hq_u4v& b) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const auto s = __builtin_amdgcn_permlane32_swap(a[i], b[i], false, false);
+    a[i] = s[0];
+    b[i] = s[1];
+  }
+}
+
 // The first i with bounds[i + 1] > t, n if there is none: a wave halves the range sixty-four-fold a step.
 __device__ __forceinline__ int find_row(const int* bounds, int n, int t) {
   const int lane = threadIdx.x & 63;
@@ -83,10 +97,11 @@ __global__ __launch_bounds__(kThreads) void rotate_kernel(RotateArgs a) {
   const int lane = threadIdx.x & 63, l = lane % LANES, np = a.rotary / 16;
   const int pa = l < np ? l : 2 * l, pb = l < np ? l + np : 2 * l + 1;
   const bool query = set < a.q_sets, key = !query && (!CACHE || set < a.q_sets + a.k_sets);
-  const int heads = query ? a.heads : a.kv_heads, h = (set - (query ? 0 : key ? a.q_sets : a.q_sets + a.k_sets)) * HEADS + lane / LANES;
-  const hq_u4v* const from = (query ? a.q + t * a.qs : key ? a.k + t * a.ks : a.v + t * a.vs) + min(h, heads - 1) * CH;
+  const int heads = query ? a.heads : a.kv_heads, piece = lane < 32 ? pa : pb;
+  const int h = (set - (query ? 0 : key ? a.q_sets : a.q_sets + a.k_sets)) * HEADS + (lane & 31) / LANES, h2 = h + HEADS / 2;
+  const hq_u4v* const from = (query ? a.q + t * a.qs : key ? a.k + t * a.ks : a.v + t * a.vs) + piece;
   const hq_u4v* const weight = query ? a.qw : key ? a.kw : nullptr;
-  hq_u4v xa = from[pa], xb = from[pb], wa = {}, wb = {};
+  hq_u4v xa = from[min(h, heads - 1) * CH], xb = from[min(h2, heads - 1) * CH], wa = {}, wb = {};
   if (weight) {
     wa = weight[pa];
     wb = weight[pb];
@@ -119,20 +134,23 @@ __global__ __launch_bounds__(kThreads) void rotate_kernel(RotateArgs a) {
       sn[4 + i] = s1[i];
     }
   }
-  hq_u4v* to;
-  bool there = h < heads;
+  hq_u4v* to;  // of the token's head 0
+  int step = CH;
+  bool there = true;
   if (query) {
-    to = a.qo + t * a.qos + h * CH;
+    to = a.qo + t * a.qos;
   } else if (CACHE) {
     const bool within = place >= 0 && place < (int64_t)a.width << a.page_log;
     const int page = within ? a.table[(int64_t)row * a.width + (place >> a.page_log)] : -1;
-    there = there && (unsigned)page < (unsigned)a.pages;
-    to = (key ? a.ko : a.vo) + ((((int64_t)page * a.kv_heads + h) << a.page_log) + (place & ((1 << a.page_log) - 1))) * CH;
+    there = (unsigned)page < (unsigned)a.pages;
+    to = (key ? a.ko : a.vo) + (((int64_t)page * a.kv_heads << a.page_log) + (place & ((1 << a.page_log) - 1))) * CH;
+    step <<= a.page_log;
   } else {
-    to = a.ko + t * a.kos + h * CH;
+    to = a.ko + t * a.kos;
   }
   if (query || key) {
     float u[8], v[8];
+    exchange(xa, xb);
     wide<T>(u, xa);
     wide<T>(v, xb);
     if (weight) {
@@ -180,15 +198,12 @@ __global__ __launch_bounds__(kThreads) void rotate_kernel(RotateArgs a) {
     }
     xa = narrow<T>(u);
     xb = narrow<T>(v);
+    exchange(xa, xb);
   }
   if (!there) return;
-  if (D == 128) {  // whole lines, past the L2 (16384 tokens 60.9 -> 57.8 us); of heads of 64 they are halves, which the L2 puts together (33.5; past it 95)
-    hq_store_stream(to + pa, xa);
-    hq_store_stream(to + pb, xb);
-  } else {
-    to[pa] = xa;
-    to[pb] = xb;
-  }
+  to += piece;  // whole lines, past the L2 (by way of it 32.3 us and 60.0 where these are 29.7 and 56.0)
+  if (h < heads) hq_store_stream(to + (int64_t)h * step, xa);
+  if (h2 < heads) hq_store_stream(to + (int64_t)h2 * step, xb);
 }
 
 template <typename T, int D, bool CACHE>
