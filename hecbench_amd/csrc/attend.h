@@ -292,7 +292,7 @@ struct Places {
 };
 
 // The same tiles of pages.  Rows behind the last one are whatever its page holds.
-template <typename T, int D, bool WINDOW = false>
+template <typename T, int D, bool WINDOW = false, int SIDES = 1>
 struct PagedTiles {
   static constexpr int CH = D / 8, NL = 64 * CH / kThreads, RG = 64 / CH;  // RG: rows of an instruction, all in one page
   Pages<T, D> p;
@@ -303,7 +303,7 @@ struct PagedTiles {
   Skip skip;  // WINDOW
   __device__ __forceinline__ int place(int u) const { return WINDOW ? skip.key(u) : u; }
   __device__ PagedTiles(const Pages<T, D>& pages, int end) : p(pages), n(end) {}
-  __device__ __forceinline__ int key(int t) const { return first + t * 64 + (int)((threadIdx.x >> 6) * NL + threadIdx.x % NL) * RG; }
+  __device__ __forceinline__ int key(int t) const { return first + t * (64 * SIDES) + (int)((threadIdx.x >> 6) * NL + threadIdx.x % NL) * RG; }
   __device__ __forceinline__ void start(int f) {
     first = f;
     const int lane = threadIdx.x & 63, row = lane / CH;  // of a multiple of 16
@@ -335,12 +335,14 @@ struct PagedTiles {
 };
 
 // ---- many rows -----------------------------------------------------------------------------------------------------------
-// 128 rows of a workgroup, 32 a wave.  WINDOW: a row sees its first keys, and those from a key of its own on.
-template <typename T, int D, bool WINDOW = false>
+// 128 rows of a workgroup, 32 a wave.  WINDOW: a row sees its first keys, and those from a key of its own on.  SIDES 2: twice as many waves and
+// keys of a tile, of which four go through the first half and four through the other, and their sums meet at the end: one workgroup then
+// keeps a compute unit as busy as two do.
+template <typename T, int D, bool WINDOW = false, int SIDES = 1>
 struct Many {
   typedef typename Kind<T>::V8 V8;
-  static constexpr int NB = 2, TILE = 64;           // blocks of 32 keys, keys of a tile
-  static constexpr int CH = D / 8, NL = 64 * CH / kThreads;
+  static constexpr int NB = 2, TILE = 64 * SIDES;   // a wave's blocks of 32 keys, keys of a tile
+  static constexpr int THREADS = SIDES * kThreads, CH = D / 8, NL = TILE * CH / THREADS;
   static constexpr int HALF = TILE * D * 2, LDS = 4 * HALF;  // keys or values of a tile; two of each
   static constexpr bool K_AHEAD = D == 128;         // see run()
 
@@ -355,6 +357,8 @@ struct Many {
   // WINDOW: of those, the row sees the ones below `sinks` and those from `lo` on, `lo_most` at most among the wave's rows
   int lo = 0, lo_most = 0, sinks = 0;
 
+  // The first of the wave's keys of a tile.
+  static __device__ __forceinline__ int side() { return SIDES == 1 ? 0 : (int)(threadIdx.x / kThreads) * 64; }
   // Whether a tile holds keys that not every row of the wave sees.
   __device__ __forceinline__ bool partial(int base) const {
     return base + TILE > all_see || (WINDOW && base < lo_most && base + TILE > sinks);
@@ -367,7 +371,7 @@ struct Many {
     hq_u4v v[NL];
     uint32_t any = 0;
 #pragma unroll
-    for (int i = 0; i < NL; ++i) v[i] = vs[i * kThreads];
+    for (int i = 0; i < NL; ++i) v[i] = vs[i * THREADS];
 #pragma unroll
     for (int i = 0; i < NL; ++i)
 #pragma unroll
@@ -382,7 +386,7 @@ struct Many {
         bad |= ((e >> 15 & 1u) | (e >> 30 & 2u)) << (8 * i + 2 * w);
         v[i][w] &= ~((e >> 15) * 0xffffu);
       }
-      vs[i * kThreads] = v[i];
+      vs[i * THREADS] = v[i];
     }
   }
 
@@ -396,7 +400,7 @@ struct Many {
         const uint32_t b = bad >> (8 * i + 2 * j);
         w[j] = (b & 1 ? Kind<T>::kOne & 0xffffu : 0u) | (b & 2 ? Kind<T>::kOne & 0xffff0000u : 0u);
       }
-      reinterpret_cast<hq_u4v*>(values)[threadIdx.x + i * kThreads] = w;
+      reinterpret_cast<hq_u4v*>(values)[threadIdx.x + i * THREADS] = w;
     }
   }
 
@@ -404,7 +408,7 @@ struct Many {
   // the scores' registers hold them.
   static __device__ __forceinline__ V8 v_operand(const char* values, int b, int t, int d) {
     const int lane = threadIdx.x & 63;
-    const int row = 32 * b + 16 * t + 4 * (lane >> 5) + ((lane >> 2) & 3);
+    const int row = side() + 32 * b + 16 * t + 4 * (lane >> 5) + ((lane >> 2) & 3);
     const int ch = 4 * d + 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1);
     lds_char* vs = (lds_char*)values + (lane & 1) * 8;
     typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
@@ -426,13 +430,13 @@ struct Many {
       for (int r = 0; r < 16; ++r) s[b][r] = 0.f;
 #pragma unroll
       for (int kk = 0; kk < D / 16; ++kk) {
-        const int row = 32 * b + (lane & 31);
+        const int row = side() + 32 * b + (lane & 31);
         const V8 a = *reinterpret_cast<const V8*>(keys + row * D * 2 + k_piece<D>(row, 2 * kk + half) * 16);
         s[b] = Kind<T>::mfma(a, qf[kk], s[b]);
       }
     }
   }
-  // Which of the lane's registers are keys that the row sees; at: the tile's first key, 4 more in the upper lanes.
+  // Which of the lane's registers are keys that the row sees; at: the wave's first key of the tile, 4 more in the upper lanes.
   __device__ __forceinline__ void mask(f32x16 (&s)[NB], int at) const {
     const int left = lim - at;
 #pragma unroll
@@ -507,7 +511,7 @@ struct Many {
     const int lane = threadIdx.x & 63, half = lane >> 5;
     constexpr int STEPS = NB * D / 16, EACH = NB * 16 / STEPS, AHEAD = 4;
     auto operand = [&](int j) {
-      const int row = 32 * (j / (D / 16)) + (lane & 31);
+      const int row = side() + 32 * (j / (D / 16)) + (lane & 31);
       return *reinterpret_cast<const V8*>(keys + row * D * 2 + k_piece<D>(row, 2 * (j % (D / 16)) + half) * 16);
     };
     float sum[2] = {0.f, 0.f};
@@ -616,7 +620,7 @@ struct Many {
 #pragma unroll
       for (int r = 0; r < 16; ++r) o[d][r] = 0.f;
     if (first >= end) return;
-    const int nt = (end - first + TILE - 1) / TILE, half4 = 4 * ((threadIdx.x >> 5) & 1);
+    const int nt = (end - first + TILE - 1) / TILE, half4 = side() + 4 * ((threadIdx.x >> 5) & 1);
     f32x16 s0[NB], s1[NB];
     float top = 0.f;
     src.start(first);
@@ -683,6 +687,31 @@ struct Many {
       for (int t = 0; t < nt; ++t) step(t, t & 1, s0, s1);
     }
     l = pair_sum(l);
+  }
+
+  // SIDES 2: the first four waves' sums become those of both sides, by way of LDS, where nothing is needed any more.
+  __device__ __forceinline__ void meet() {
+    static_assert(D / 2 * kThreads * 4 <= LDS, "the sums of a side");
+    __shared__ float2 other[kThreads];
+    float* const sums = reinterpret_cast<float*>(sm) + threadIdx.x % kThreads;
+    __syncthreads();
+    if (threadIdx.x >= kThreads) {
+      other[threadIdx.x % kThreads] = float2{m, l};
+#pragma unroll
+      for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) sums[(16 * d + r) * kThreads] = o[d][r];
+    }
+    __syncthreads();
+    if (threadIdx.x >= kThreads) return;
+    const float2 of = other[threadIdx.x];
+    const float top = fmaxf(m, of.x), f = __builtin_amdgcn_exp2f(m - finite_or_zero(top)), g = __builtin_amdgcn_exp2f(of.x - finite_or_zero(top));
+    m = top;
+    l = l * f + of.y * g;
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[d][r] = o[d][r] * f + sums[(16 * d + r) * kThreads] * g;
   }
 
   // The row's result.  A lane and its partner hold every other four elements of their row; two exchanges a pair of fours make them eights,

@@ -227,11 +227,11 @@ __device__ __forceinline__ void few_rows(const ChunkArgs& a, char* sm, const Ite
 __device__ __forceinline__ int64_t many_place(const ChunkArgs& a, int share, int head) {
   return (int64_t)a.few * a.kv_heads * kFew + ((int64_t)share * a.kv_heads + head) * kRows;
 }
-template <typename T, int D, bool WINDOW>
+template <typename T, int D, bool WINDOW, int SIDES>
 __device__ __forceinline__ void many_rows(const ChunkArgs& a, char* sm, int* poison, const Item& item, int head) {
   typedef typename Kind<T>::V8 V8;
   const Request& r = item.r;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, rows = r.nq * a.ratio;
+  const int lane = threadIdx.x & 63, wave = (threadIdx.x >> 6) % kWaves, rows = r.nq * a.ratio;
   const uint32_t ratio = a.ratio;
   const int first_row = ((rows + kRows - 1) / kRows - 1 - item.tile) * kRows, last_row = min(first_row + kRows, rows) - 1;
   const int first_token = (uint32_t)first_row / ratio, last_token = (uint32_t)last_row / ratio;
@@ -240,7 +240,7 @@ __device__ __forceinline__ void many_rows(const ChunkArgs& a, char* sm, int* poi
   item.keys(uniform(sight.limit(last_token)), &first, &end);
   const int row = first_row + wave * 32 + (lane & 31), mine = min(row, last_row);
   const int token = (uint32_t)mine / ratio, h = head * ratio + (uint32_t)mine % ratio;
-  Many<T, D, WINDOW> w;
+  Many<T, D, WINDOW, SIDES> w;
   w.sm = sm;
   w.poison = poison;
   set_up(poison);
@@ -255,9 +255,13 @@ __device__ __forceinline__ void many_rows(const ChunkArgs& a, char* sm, int* poi
     w.sinks = a.sinks;
     w.lo_most = __builtin_amdgcn_readlane(w.lo, 31);
   }
-  PagedTiles<T, D, WINDOW> src(pages_of<T, D>(a, item.b, head), end);
+  PagedTiles<T, D, WINDOW, SIDES> src(pages_of<T, D>(a, item.b, head), end);
   src.skip = sight.skip;
   w.run(src, first, end, uniform(min(sight.limit(first_token), end)), a.c, uniform(sight.low(last_token)));
+  if (SIDES == 2) {
+    w.meet();
+    if (threadIdx.x >= kThreads) return;
+  }
   // the row, worked out once more: in the loop there is no register to spare
   int tid = threadIdx.x;
   asm volatile("" : "+v"(tid));
@@ -269,15 +273,16 @@ __device__ __forceinline__ void many_rows(const ChunkArgs& a, char* sm, int* poi
   else w.put_share(a.po, a.pm, many_place(a, item.first + item.share, head) + again - first_row, sees);
 }
 
-template <typename T, int D, bool WINDOW>
-__global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void chunk_kernel(ChunkArgs a) {
+template <typename T, int D, bool WINDOW, int SIDES>
+__global__ __launch_bounds__(SIDES * kThreads, D == 64 && SIDES == 1 ? 3 : 2) void chunk_kernel(ChunkArgs a) {
   extern __shared__ __align__(16) char sm[];
   __shared__ int poison;
   const uint32_t x = blockIdx.x / (uint32_t)a.kv_heads, head = blockIdx.x - x * (uint32_t)a.kv_heads;
   Item item;
   if (!item.find<D, WINDOW>(a, x, blockIdx.x == 0 && threadIdx.x < 64 && a.said)) return;
-  if (item.r.nq * a.ratio <= kFew) few_rows<T, D, WINDOW>(a, sm, item, head);
-  else many_rows<T, D, WINDOW>(a, sm, &poison, item, head);
+  if (item.r.nq * a.ratio <= kFew) {
+    if (SIDES == 1 || threadIdx.x < kThreads) few_rows<T, D, WINDOW>(a, sm, item, head);  // barriers wait for no wave that has ended
+  } else many_rows<T, D, WINDOW, SIDES>(a, sm, &poison, item, head);
 }
 
 // The shares of rows of many together, a row a wave (WAVES 1) or a workgroup, from row to row: where nothing was divided, which the host does
@@ -303,6 +308,17 @@ __global__ __launch_bounds__(kThreads) void join_chunk_kernel(ChunkArgs a) {
     if (WAVES > 1) __syncthreads();  // the row before has been put together
     join_shares<T, D, WAVES, PRE>(a.po, a.pm, row, many_place(a, (int)first, head) + mine % kRows, a.kv_heads * kRows, n, n, n, n, (T*)a.out);
   }
+}
+
+template <typename T, int D, bool WINDOW, int SIDES>
+int launch_sides(dim3 workgroups, hipStream_t stream, const ChunkArgs& a) {
+  constexpr int lds = std::max(Many<T, D, WINDOW, SIDES>::LDS, Few<T, D>::LDS);
+  if (lds > 65536) {
+    static const hipError_t attr =
+        hipFuncSetAttribute(reinterpret_cast<const void*>(&chunk_kernel<T, D, WINDOW, SIDES>), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    if (attr != hipSuccess) return (int)attr;
+  }
+  return hq_launch_as_is(chunk_kernel<T, D, WINDOW, SIDES>, workgroups, dim3(SIDES * kThreads), lds, stream, a);
 }
 
 template <typename T, int D, bool WINDOW>
@@ -357,9 +373,13 @@ int launch_chunk(ChunkArgs a, int cus, hipStream_t stream) {
     a.pm = a.po + places * D;
     if (many_divided) a.said = reinterpret_cast<int*>(a.pm + 2 * places);
   }
-  constexpr int lds = std::max(Many<T, D>::LDS, Few<T, D>::LDS);
-  static_assert(lds <= 65536, "no attribute to set");
-  const int rc = hq_launch_as_is(chunk_kernel<T, D, WINDOW>, dim3((unsigned)(grid * a.kv_heads)), dim3(kThreads), lds, stream, a);
+  const dim3 workgroups((unsigned)(grid * a.kv_heads));
+  // Undivided tiles, one to a compute unit at most: of twice the waves (SIDES in attend.h; 1024 tokens behind 3500, 32 / 8 heads of 128, 93 -> 77 us,
+  // 700 86 -> 69, of 64 84 -> 59 and 78 -> 52; behind nothing 28.6 -> 26.5 and 23.1 -> 18.1; up to 256 keys 8.6 and 9.6).  Not beside many
+  // requests, which then find no room next to the tiles: 8 of one token beside 900 106 -> 102, 16 of them 111 -> 117, 30 of up to 4000 117 -> 133
+  // (3 of 16000 beside 1000 tokens go 63 -> 77, which the host cannot tell).
+  const bool alone = tiles && units > 2 && !many_divided && ((rows - requests) / kRows + requests) * a.kv_heads <= cus && 4 * requests * a.kv_heads <= cus;
+  const int rc = alone ? launch_sides<T, D, WINDOW, 2>(workgroups, stream, a) : launch_sides<T, D, WINDOW, 1>(workgroups, stream, a);
   if (rc != HQ_OK || !a.said) return rc;
   const int64_t all = std::min((int64_t)a.total_q * a.heads, likely * kRows * a.kv_heads);
   if (std::min(room / likely, units / 2) <= 2 * kSharesOfAWave)

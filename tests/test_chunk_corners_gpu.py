@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from tests.test_attention_gpu import TYPES, bounds, i32, randn
-from tests.test_chunk_gpu import Cache, check, check_chunk, run_chunk
+from tests.test_chunk_gpu import Cache, check, check_chunk, run_chunk, seen_of
 
 pytestmark = pytest.mark.gpu
 
@@ -184,3 +184,74 @@ def test_bounds_that_do_not_ascend(hq, heads, kv, batch):
             new = [1 + (i % 3 == 0) for i in range(batch)]
             good, got = run_chunk(hq, cache, new, heads, 128, dtype, window, sinks)
             check_chunk(good, got, cache, new, window, sinks, None, u)
+
+
+# Tiles, undivided, of 170 to 256 workgroups: those of twice the waves.
+ALONE = [((64, 64), [350], [1500]), ((64, 16), [350], [901]), ((64, 16), [200, 150], [1300, 149]), ((64, 16), [340, 1, 9], [345, 700, 60]),
+         ((64, 32), [400, 0], [100, 50]), ((64, 16), [6, 360], [6, 2000]), ((60, 12), [450], [450])]
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("heads,new,lengths", ALONE)
+@pytest.mark.parametrize("window,sinks", [(None, 0), (1, 0), (100, 4), (700, 130)])
+def test_tiles_that_have_a_compute_unit_each(hq, kind, D, heads, new, lengths, window, sinks):
+    dtype, u = TYPES[kind]
+    cache = Cache(4, lengths, heads[1], 16, D, dtype)
+    q, out = run_chunk(hq, cache, new, heads[0], D, dtype, window, sinks, behind=2)
+    check_chunk(q, out, cache, new, window, sinks, None, u)
+    again = hq.chunk_attention(q, cache.k, cache.v, cache.table, i32(lengths), i32(bounds(new)), window=window, sinks=sinks)
+    assert torch.equal(again[:sum(new)], out[:sum(new)])
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("what", [math.nan, math.inf, -math.inf, "most"])
+@pytest.mark.parametrize("window,sinks", [(None, 0), (150, 6)])
+def test_tiles_that_have_a_compute_unit_each_and_what_is_not_seen(hq, kind, D, what, window, sinks):
+    """As test_what_is_not_seen_has_no_effect: pages of keys and values in both halves of a tile, a missing page among them."""
+    dtype, _ = TYPES[kind]
+    new, length, bad = 350, 800, torch.finfo(dtype).max if what == "most" else what
+    cache = Cache(6, [length], 16, 16, D, dtype)
+    q, want = run_chunk(hq, cache, [new], 64, D, dtype, window, sinks)
+    for key in (3, 6, 63, 64, 301, 450, 451, 512, 600, 640, 700, 799):
+        k, v = cache.k.clone(), cache.v.clone()
+        page = cache.rows[0][key // 16]
+        k[page, 1, key % 16, 3] = bad
+        v[page, 2, key % 16, 5] = bad
+        sees = seen_of(new, length, window, sinks)[:, key]
+        got = hq.chunk_attention(q, k, v, cache.table, i32([length]), i32([0, new]), window=window, sinks=sinks)
+        touched = torch.zeros_like(got, dtype=torch.bool)
+        touched[sees, 4:8] = True
+        touched[:, 8:12, 5] = sees[:, None].expand(-1, 4)
+        assert torch.equal(got[~touched], want[~touched]), key
+        if what != "most":
+            assert torch.isnan(got[sees][:, 8:12, 5]).all(), key
+    for missing in (0, 20, 38, 40):
+        table, k, v = cache.table.clone(), cache.k.clone(), cache.v.clone()
+        table[0, missing] = -1
+        k[cache.rows[0][missing]] = 0
+        v[cache.rows[0][missing]] = 0
+        args = (i32([length]), i32([0, new]), window, sinks)
+        assert torch.equal(hq.chunk_attention(q, cache.k, cache.v, table, *args), hq.chunk_attention(q, k, v, cache.table, *args))
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_tiles_that_have_a_compute_unit_each_in_a_graph(hq, D):
+    """Replayed with other lengths, beside eager calls; the stream's first call is the captured one."""
+    dtype, u = TYPES["bf16"]
+    cache = Cache(8, [1400], 16, 16, D, dtype)
+    q, cu, ln = randn(5, 350, 64, D).to(dtype), i32([0, 350]), i32([1400])
+    stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.graph(graph, stream=stream):
+        out = hq.chunk_attention(q, cache.k, cache.v, cache.table, ln, cu)
+    for length in (1400, 350, 777, 20):
+        ln.copy_(i32([length]))
+        out.fill_(7.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, hq.chunk_attention(q, cache.k, cache.v, cache.table, ln, cu))
+        n = min(length, 350)
+        assert (out[:350 - n] == 0).all()
+        check(out[350 - n:], q[350 - n:], *(x[:length] for x in cache.dense[0]), None, 0, 1 / math.sqrt(D), u)
