@@ -27,6 +27,11 @@ struct ChunkArgs {
 };
 
 constexpr int kFew = 16, kUnit = 128, kRows = 128;
+// Keys that are not divided, in kUnits: of a tile of few rows (147 take a workgroup 7.3 us, two 8.9), of more than 64 (256 tokens with 356 keys, 32 / 8
+// heads of 128, beside a joining launch that finds nothing 15.5 us, divided 17.8; 128 with 428 17.0 and 16.0), and of any of many where that saves the
+// joining launch (128 with 428 14.8, with 628 18.6 and 16.9).  (In between every 128 keys count: 12 requests of 5 tokens, 16 / 2 heads, up to 698
+// keys 15.7, 17.7 with up to 384 undivided.)
+constexpr int kShort = 3, kShortOfAll = 4;
 
 // A request: its new tokens and the tokens it has with them.
 struct Request {
@@ -86,14 +91,14 @@ struct Item {
     int keys = mine.length;
     if (WINDOW) keys = (int)min((int64_t)keys, (int64_t)min(a.sinks, keys) + a.window + 14 + (rows <= kFew ? mine.nq : kRows / a.ratio + 2));
     const unsigned few = rows <= kFew ? tiles : 0, many = tiles - few;
-    // (Few rows with up to 384 keys are not divided: 147 of them take a workgroup 7.3 us, two 8.9.)
-    const unsigned units = few && keys <= 3 * kUnit ? 1 : max((unsigned)(keys + kUnit - 1) / kUnit, 1u);
+    const unsigned units = few && keys <= kShort * kUnit ? 1 : max((unsigned)(keys + kUnit - 1) / kUnit, 1u);
     // Tiles of more than 64 rows are divided where three shares each, or more, find room, two workgroups a compute unit; where they do not, what
     // the shares' sums cost, which are written, read and joined, is more than it brings (behind 3500 keys, 32 / 8 heads of 128: 640 tokens 63 us
     // in three shares, 78 undivided; 768 in two 74 and 78, 896 78 and 78, 1024 82 and 78).  A few of them by themselves are as fast with half as
     // many shares (128 tokens 26.2 us, with all 28.2; 384 52.8 and 46.0).  Fewer rows, bound by memory, are divided in any case.
     const unsigned all_many = wave_sum(many), heavy = rows > 64 ? tiles : 0, all_heavy = wave_sum(heavy), groups = all_heavy * a.kv_heads;
-    const bool heavy_too = a.said && 3 * groups <= 2u * a.cus, divisible = ascend && a.arrived && (rows <= kFew || (a.said && (rows <= 64 || heavy_too)));
+    const bool heavy_too = a.said && 3 * groups <= 2u * a.cus;
+    const bool divisible = ascend && a.arrived && (rows <= kFew || (a.said && (rows <= 64 || (heavy_too && units > kShort))));
     const unsigned of = divisible ? tiles : 0, all_of = wave_sum(of);
     const bool half = heavy_too && all_of == all_heavy && 8 * groups <= (unsigned)a.cus;
     const unsigned room = half ? (a.room + 1) / 2 : a.room;
@@ -324,14 +329,22 @@ int launch_sides(dim3 workgroups, hipStream_t stream, const ChunkArgs& a) {
 template <typename T, int D, bool WINDOW>
 int launch_chunk(ChunkArgs a, int cus, hipStream_t stream) {
   const int64_t cap = (int64_t)a.width << a.page_log, rows = (int64_t)a.total_q * a.ratio, requests = std::min(a.batch, a.total_q);
-  const int64_t units = std::max<int64_t>((cap + kUnit - 1) / kUnit, 1), room = std::max<int64_t>(2 * (int64_t)cus / a.kv_heads, 1);
+  const int64_t keys = WINDOW ? std::min(cap, std::min<int64_t>(a.sinks, cap) + a.window + 14 + std::max(kFew, kRows / a.ratio + 2)) : cap;  // of a tile
+  const int64_t units = std::max<int64_t>((keys + kUnit - 1) / kUnit, 1), room = std::max<int64_t>(2 * (int64_t)cus / a.kv_heads, 1);
   // Tiles of many rows, at most, each of whose requests has more than kFew of them; and how many there are if all but a token a request are
   // theirs.
   const int64_t tiles = rows / kRows + std::min(requests, rows / (kFew + 1)), slots = rows / kRows + a.batch;
   const int64_t likely = (rows - requests * a.ratio + kRows - 1) / kRows;
+  // Tiles that a compute unit has one of, at most, and half of them has: undivided and of twice the waves (SIDES in attend.h; 1024 tokens behind 3500,
+  // 32 / 8 heads of 128, 93 -> 77 us, 700 86 -> 69, of 64 84 -> 59 and 78 -> 52, behind nothing 28.6 -> 26.5 and 23.1 -> 18.1; up to 256 keys 8.6 and
+  // 9.6; 640 tokens, which could be divided in three, behind 1000 40 -> 33, 3500 68 and 68, 16000 212 -> 240).  Not beside many requests, which
+  // then find no room next to the tiles: 8 of one token beside 900 106 -> 102, 16 of them 111 -> 117, 30 of up to 4000 117 -> 133 (3 of 16000
+  // beside 1000 tokens go 63 -> 77, which the host cannot tell).
+  const bool alone = tiles && units > 2 && 2 * likely * a.kv_heads > cus && ((rows - requests) / kRows + requests) * a.kv_heads <= cus &&
+                     4 * requests * a.kv_heads <= cus;
   a.cus = cus;
   a.room = (int)room;
-  bool divide = units > 1, many_divided;
+  bool divide = units > kShort, many_divided;
   size_t floats = 0, counters = 0;
   int64_t few, many, places;
   for (;;) {
@@ -345,8 +358,8 @@ int launch_chunk(ChunkArgs a, int cus, hipStream_t stream) {
     } else {
       few = divide ? std::min(std::max(room, requests), requests * units) : requests;
       many = tiles;
-      // (Where the likely ones are too many to be divided, nothing asks for room for their shares and a launch that joins them.)
-      if (divide && tiles && tiles < 2 * room && likely && 3 * likely * a.kv_heads <= 2 * cus) {  // more tiles than that fill the device
+      // (Where the likely ones are too many to be divided, or their keys too few, nothing asks for room for shares and a launch that joins them.)
+      if (divide && units > kShortOfAll && !alone && tiles && tiles < 2 * room && likely && 3 * likely * a.kv_heads <= 2 * cus) {  // more tiles than that fill the device
         many = tiles + std::min(room, tiles * units);  // some as they are, beside shares that fill the room
         many_divided = true;
       }
@@ -374,11 +387,6 @@ int launch_chunk(ChunkArgs a, int cus, hipStream_t stream) {
     if (many_divided) a.said = reinterpret_cast<int*>(a.pm + 2 * places);
   }
   const dim3 workgroups((unsigned)(grid * a.kv_heads));
-  // Undivided tiles, one to a compute unit at most: of twice the waves (SIDES in attend.h; 1024 tokens behind 3500, 32 / 8 heads of 128, 93 -> 77 us,
-  // 700 86 -> 69, of 64 84 -> 59 and 78 -> 52; behind nothing 28.6 -> 26.5 and 23.1 -> 18.1; up to 256 keys 8.6 and 9.6).  Not beside many
-  // requests, which then find no room next to the tiles: 8 of one token beside 900 106 -> 102, 16 of them 111 -> 117, 30 of up to 4000 117 -> 133
-  // (3 of 16000 beside 1000 tokens go 63 -> 77, which the host cannot tell).
-  const bool alone = tiles && units > 2 && !many_divided && ((rows - requests) / kRows + requests) * a.kv_heads <= cus && 4 * requests * a.kv_heads <= cus;
   const int rc = alone ? launch_sides<T, D, WINDOW, 2>(workgroups, stream, a) : launch_sides<T, D, WINDOW, 1>(workgroups, stream, a);
   if (rc != HQ_OK || !a.said) return rc;
   const int64_t all = std::min((int64_t)a.total_q * a.heads, likely * kRows * a.kv_heads);
