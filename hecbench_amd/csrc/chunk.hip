@@ -335,12 +335,13 @@ int launch_chunk(ChunkArgs a, int cus, hipStream_t stream) {
   // theirs.
   const int64_t tiles = rows / kRows + std::min(requests, rows / (kFew + 1)), slots = rows / kRows + a.batch;
   const int64_t likely = (rows - requests * a.ratio + kRows - 1) / kRows;
-  // Tiles that a compute unit has one of, at most, and half of them has: undivided and of twice the waves (SIDES in attend.h; 1024 tokens behind 3500,
-  // 32 / 8 heads of 128, 93 -> 77 us, 700 86 -> 69, of 64 84 -> 59 and 78 -> 52, behind nothing 28.6 -> 26.5 and 23.1 -> 18.1; up to 256 keys 8.6 and
-  // 9.6; 640 tokens, which could be divided in three, behind 1000 40 -> 33, 3500 68 and 68, 16000 212 -> 240).  Not beside many requests, which
-  // then find no room next to the tiles: 8 of one token beside 900 106 -> 102, 16 of them 111 -> 117, 30 of up to 4000 117 -> 133 (3 of 16000
-  // beside 1000 tokens go 63 -> 77, which the host cannot tell).
-  const bool alone = tiles && units > 2 && 2 * likely * a.kv_heads > cus && ((rows - requests) / kRows + requests) * a.kv_heads <= cus &&
+  // Tiles that a compute unit has one of, at most, and half of them has, or with up to 1024 keys a quarter: undivided and of twice the waves (SIDES
+  // in attend.h; 1024 tokens behind 3500, 32 / 8 heads of 128, 93 -> 77 us, 700 86 -> 69, of 64 84 -> 59 and 78 -> 52, behind nothing 28.6 -> 26.5
+  // and 23.1 -> 18.1; up to 256 keys 8.6 and 9.6; 640 tokens, which could be divided in three, behind 1000 40 -> 33, 3500 68 and 68, 16000 212 ->
+  // 240; 512 behind 500 29.3 -> 23.5, and 256 behind 700 would go 20.5 -> 23.2).  Not beside many requests, which then find no room next to the
+  // tiles: 8 of one token beside 900 106 -> 102, 16 of them 111 -> 117, 30 of up to 4000 117 -> 133 (3 of 16000 beside 1000 tokens go 63 -> 77,
+  // which the host cannot tell).
+  const bool alone = tiles && units > 2 && (units <= 8 ? 4 : 2) * likely * a.kv_heads > cus && ((rows - requests) / kRows + requests) * a.kv_heads <= cus &&
                      4 * requests * a.kv_heads <= cus;
   a.cus = cus;
   a.room = (int)room;
