@@ -186,9 +186,10 @@ def test_bounds_that_do_not_ascend(hq, heads, kv, batch):
             check_chunk(good, got, cache, new, window, sinks, None, u)
 
 
-# Tiles, undivided, of 170 to 256 workgroups: those of twice the waves.
+# Tiles, undivided, of 128 to 256 workgroups, or 64 with few keys: those of twice the waves, and some beside them.
 ALONE = [((64, 64), [350], [1500]), ((64, 16), [350], [901]), ((64, 16), [200, 150], [1300, 149]), ((64, 16), [340, 1, 9], [345, 700, 60]),
-         ((64, 32), [400, 0], [100, 50]), ((64, 16), [6, 360], [6, 2000]), ((60, 12), [450], [450])]
+         ((64, 32), [400, 0], [100, 50]), ((64, 16), [6, 360], [6, 2000]), ((60, 12), [450], [450]),
+         ((32, 8), [400], [900]), ((32, 8), [300, 90, 2], [700, 400, 500]), ((32, 8), [257], [300])]
 
 
 @pytest.mark.parametrize("kind", ["bf16", "f16"])
