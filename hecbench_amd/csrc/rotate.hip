@@ -115,13 +115,9 @@ __global__ __launch_bounds__(kThreads) void rotate_kernel(RotateArgs a) {
   } else {
     place = a.rotary ? a.positions[t] : 0;
   }
-  float cs[8], sn[8];  // of the lane's pairs
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    cs[i] = 1.f;
-    sn[i] = 0.f;
-  }
-  if (l < np && (query || key)) {
+  const bool rotated = l < np;
+  float cs[8] = {}, sn[8] = {};  // of the lane's pairs, if they are rotated
+  if (rotated && (query || key)) {
     const int at = (int)min(max(place, (int64_t)0), (int64_t)a.known - 1);
     const hq_f4v* const c = a.cs + (int64_t)at * (a.rotary / 4);
     const int i0 = a.interleaved ? l : 2 * l, i1 = a.interleaved ? l + np : 2 * l + 1, sines = a.rotary / 8;
@@ -179,7 +175,9 @@ __global__ __launch_bounds__(kThreads) void rotate_kernel(RotateArgs a) {
         v[j] = v[j] * r * wv[j];
       }
     }
-    if (a.interleaved) {
+    // The others are left out of it: turned by an angle of 0, they would take 0 times what is beside them, NaN where that is not finite, and
+    // lose the sign of a zero.
+    if (rotated && a.interleaved) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const float u0 = u[2 * j], v0 = v[2 * j];
@@ -188,7 +186,7 @@ __global__ __launch_bounds__(kThreads) void rotate_kernel(RotateArgs a) {
         v[2 * j] = v0 * cs[4 + j] - v[2 * j + 1] * sn[4 + j];
         v[2 * j + 1] = v[2 * j + 1] * cs[4 + j] + v0 * sn[4 + j];
       }
-    } else {
+    } else if (rotated) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const float u0 = u[j];
