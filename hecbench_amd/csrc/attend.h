@@ -208,6 +208,7 @@ struct PackedTiles {
     load_v(0, v0);
     if (two) load_k(1, k1);
   }
+  __device__ __forceinline__ void then(char*, bool) const {}
   // A tile on both sides of what is left out: every lane by an address of its own.
   template <typename F>
   __device__ __forceinline__ void load_across(const T* from, int64_t stride, int base, char* to, F piece) const {
@@ -291,8 +292,11 @@ struct Places {
   }
 };
 
-// The same tiles of pages.  Rows behind the last one are whatever its page holds.
-template <typename T, int D, bool WINDOW = false, int SIDES = 1>
+// The same tiles of pages.  Rows behind the last one are whatever its page holds.  AT_ONCE (heads of 128): keys of the first two tiles and values of
+// the first are asked for together, behind one trip for their pages, which long tiles gain from (2048 tokens behind 30000 1007 -> 985 us); or one
+// behind the other, with which a share of a few tiles has its first keys sooner (32 requests behind 8192 common keys, four tiles a share, 24.2 us, at
+// once 25.1).
+template <typename T, int D, bool WINDOW = false, int SIDES = 1, bool AT_ONCE = true>
 struct PagedTiles {
   static constexpr int CH = D / 8, NL = 64 * CH / kThreads, RG = 64 / CH;  // RG: rows of an instruction, all in one page
   Pages<T, D> p;
@@ -310,17 +314,27 @@ struct PagedTiles {
     koff = row * D * 2 + k_piece<D>(row, lane % CH) * 16;
     voff = row * D * 2 + v_piece<D>(row, lane % CH) * 16;
     ids = p.id(place(min(key(0), n - 1)));
-    if (D == 128) {  // the first two tiles' pages by one trip to memory
+    if (D == 128 && AT_ONCE) {  // the first two tiles' pages by one trip to memory
       const int then = p.id(place(min(key(1), n - 1)));
       now.set(p, ids, place(key(0)));
       next.set(p, then, place(key(1)));
       ids = p.id(place(min(key(2), n - 1)));
     }
   }
-  __device__ __forceinline__ void begin(char* k0, char* k1, char* v0, bool two) const {
+  __device__ __forceinline__ void begin(char* k0, char* k1, char* v0, bool two) {
+    if (!AT_ONCE) {
+      advance(0);
+      load_k(0, k0);
+      advance(1);
+      return load_v(0, v0);
+    }
     now.template load<D, false, NL>(p.k, 0, koff, k0 + (threadIdx.x >> 6) * (NL * 1024));
     load_v(0, v0);
     if (two) load_k(1, k1);
+  }
+  // With the first tile there.
+  __device__ __forceinline__ void then(char* k1, bool two) const {
+    if (!AT_ONCE && two) load_k(1, k1);
   }
   // Before the first load of tile t: its pages are there, those of the tile behind it are asked for.
   __device__ __forceinline__ void advance(int t) {
@@ -636,6 +650,7 @@ struct Many {
     if (K_AHEAD) {
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       __syncthreads();
+      src.then(sm + HALF, nt > 1);
       scores(s0, sm);
       if (partial(first)) mask(s0, first + half4);
       top = top_of(s0);

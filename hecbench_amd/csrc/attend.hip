@@ -262,7 +262,7 @@ __device__ __forceinline__ void many_rows(const PagedArgs& a, char* sm, int* poi
   if (lane == 0) seen[wave] = w.all_see;
   __syncthreads();
   const int whole = min(min(seen[0], seen[1]), min(seen[2], seen[3]));
-  PagedTiles<T, D> src(pages_of<T, D>(a, b0, head), end);
+  PagedTiles<T, D, false, 1, false> src(pages_of<T, D>(a, b0, head), end);
   w.run(src, first, end, uniform(whole), a.c);
   // the row, worked out once more: in the loop there is no register to spare
   int tid = threadIdx.x;
