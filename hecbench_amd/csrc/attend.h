@@ -1131,6 +1131,11 @@ __device__ __forceinline__ void join_here(const A& a, char* sm, int nrows, int64
 }
 
 constexpr int kJoin = 32, kTeam = 16;  // shares that are joined at once, of that many and of more
+// Shares that there is room for, two workgroups a compute unit (`side` of them for every one), and no more than two steps join: a team's counter is that
+// of its first share, and a third step's first team would count on the first one's, which others may still be at.  (256 compute units: 512,
+// just as many.)
+constexpr int64_t share_room(int64_t cus, int64_t side) { return std::max<int64_t>(std::min<int64_t>(2 * cus / side, kJoin * kTeam), 1); }
+static_assert(share_room(1024, 1) <= kJoin * kTeam, "joined in two steps on any device");
 constexpr int kApart = 16;  // counters, a line of 64 bytes each: atomics on one line wait for each other (64 shares: 17.7 us, apart 14.5)
 
 // The shares of a row together, by WAVES waves: their maxima and sums a lane each, then the sums of the values, 16 bytes a lane, several

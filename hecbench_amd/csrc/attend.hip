@@ -440,7 +440,7 @@ int launch_paged(PagedArgs a, int cus, hipStream_t stream) {
       joined = (rows >= 4096 ? a.likely : a.most_np) + a.ns;
     } else {
       a.per_row = 1;
-      const int64_t most = a.batch * std::max<int64_t>(1, (cap + kUnit - 1) / kUnit), room = divide ? 2 * (int64_t)cus / (a.kv_heads * tiles) : 1;
+      const int64_t most = a.batch * std::max<int64_t>(1, (cap + kUnit - 1) / kUnit), room = divide ? share_room(cus, a.kv_heads * tiles) : 1;
       a.ns = 0;
       if (a.batch == 1 || a.batch > 64 || a.batch >= room || a.batch == most) a.ns = (int)std::max<int64_t>(1, std::min(room, most) / a.batch);
       a.items = (int)(a.ns ? (int64_t)a.ns * a.batch : std::min(room, most));

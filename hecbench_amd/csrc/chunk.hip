@@ -330,7 +330,7 @@ template <typename T, int D, bool WINDOW>
 int launch_chunk(ChunkArgs a, int cus, hipStream_t stream) {
   const int64_t cap = (int64_t)a.width << a.page_log, rows = (int64_t)a.total_q * a.ratio, requests = std::min(a.batch, a.total_q);
   const int64_t keys = WINDOW ? std::min(cap, std::min<int64_t>(a.sinks, cap) + a.window + 14 + std::max(kFew, kRows / a.ratio + 2)) : cap;  // of a tile
-  const int64_t units = std::max<int64_t>((keys + kUnit - 1) / kUnit, 1), room = std::max<int64_t>(2 * (int64_t)cus / a.kv_heads, 1);
+  const int64_t units = std::max<int64_t>((keys + kUnit - 1) / kUnit, 1), room = share_room(cus, a.kv_heads);
   // Tiles of many rows, at most, each of whose requests has more than kFew of them; and how many there are if all but a token a request are
   // theirs.
   const int64_t tiles = rows / kRows + std::min(requests, rows / (kFew + 1)), slots = rows / kRows + a.batch;
