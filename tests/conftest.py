@@ -10,6 +10,19 @@ if ROOT not in sys.path:
 
 def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs a real MI355X (run with -m gpu)")
+    config.addinivalue_line("markers", "no_gpu: passes made-up addresses through all checks, which only a missing device stops; skipped where there is one")
+
+
+def devices():
+    import torch
+    return torch.cuda.device_count()
+
+
+def pytest_collection_modifyitems(items):
+    made_up = [item for item in items if item.get_closest_marker("no_gpu") or item.name == "test_columns_of_one_row_are_apart"]
+    if made_up and devices():
+        for item in made_up:
+            item.add_marker(pytest.mark.skip(reason="made-up addresses, and a device that would go there"))
 
 
 @pytest.fixture(scope="session")
