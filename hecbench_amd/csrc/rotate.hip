@@ -13,6 +13,7 @@
 // 108 where it is 55.8.  Bound by the copy: of heads of 128 56.0 us, 6.1 TB/s of data, where a plain copy of 512 MB reaches 6.5; short calls by
 // the launch and the loads that wait for another (positions, then the table's row; in the cache's form bounds and starts, then the table's
 // row and the page): one token 4.4 us.
+#include <algorithm>
 #include <climits>
 #include <cmath>
 
@@ -235,6 +236,26 @@ bool apart(const Region& x, const Region& y, int64_t tokens, bool same) {
   return d >= (uint64_t)x.bytes && d + (uint64_t)y.bytes <= (uint64_t)x.stride;
 }
 
+// One stretch of memory.  Two of them, and one and rows, have nothing in common, not even in the gaps between the rows' bytes.
+struct Stretch {
+  const void* p;
+  int64_t bytes;
+};
+bool apart(const Stretch& x, const Stretch& y) {
+  const uintptr_t a = (uintptr_t)x.p, b = (uintptr_t)y.p;
+  return !x.p || !y.p || x.bytes <= 0 || y.bytes <= 0 || a + x.bytes <= b || b + y.bytes <= a;
+}
+bool apart(const Region& x, int64_t tokens, const Stretch& y) {
+  if (apart(Stretch{x.p, (tokens - 1) * x.stride + x.bytes}, y)) return true;
+  if ((uintptr_t)y.p < (uintptr_t)x.p) return false;
+  const int64_t d = (int64_t)(((uintptr_t)y.p - (uintptr_t)x.p) % (uint64_t)x.stride);
+  return d >= x.bytes && y.bytes <= x.stride - d;
+}
+// Bytes of the pages, as far as any memory reaches.
+int64_t bytes_of_pages(int pages, int heads, int page, int head_dim) {
+  return (int64_t)std::min((double)(1ll << 60), 2.0 * pages * heads * page * head_dim);
+}
+
 int check(int dtype, int head_dim, int rotary, int num_positions, const float* cos_sin, int64_t tokens, int heads, int kv_heads, float eps) {
   if (tokens < 0 || heads < 1 || kv_heads < 1 || num_positions < 0 || rotary < 0 || rotary % 16 || rotary > head_dim) return HQ_ERR_BAD_SHAPE;
   if (head_dim != 64 && head_dim != 128) return HQ_ERR_BAD_SHAPE;
@@ -268,6 +289,10 @@ extern "C" int hq_norm_rotate(const void* q, const void* k, void* q_out, void* k
   if (!apart(qo, qi, tokens, true) || !apart(ko, ki, tokens, true) || !apart(qo, ki, tokens, false) || !apart(ko, qi, tokens, false) ||
       !apart(qo, ko, tokens, false))
     return HQ_ERR_BAD_SHAPE;
+  const Stretch read[] = {{q_weight, 2 * (int64_t)head_dim}, {k_weight, 2 * (int64_t)head_dim}, {rotary ? cos_sin : nullptr, 4 * (int64_t)num_positions * rotary},
+                          {rotary ? positions : nullptr, 4 * tokens}};
+  for (const Stretch& x : read)
+    if (!apart(qo, tokens, x) || !apart(ko, tokens, x)) return HQ_ERR_BAD_SHAPE;
   const HqDevice* dev = nullptr;
   const int dc = hq_current_device(&dev);
   if (dc != HQ_OK) return dc;
@@ -316,6 +341,15 @@ extern "C" int hq_cache_write_rotated(const void* q, const void* k, const void* 
   if (q_stride > kMost || k_stride > kMost || v_stride > kMost || q_out_stride > kMost) return HQ_ERR_TOO_LARGE;
   const Region qi{q, 2 * qn, 2 * q_stride}, ki{k, 2 * kn, 2 * k_stride}, vi{v, 2 * kn, 2 * v_stride}, qo{q_out, 2 * qn, 2 * q_out_stride};
   if (!apart(qo, qi, tokens, true) || !apart(qo, ki, tokens, false) || !apart(qo, vi, tokens, false)) return HQ_ERR_BAD_SHAPE;
+  const int64_t bytes = table_width ? bytes_of_pages(num_pages, kv_heads, page_size, head_dim) : 0;
+  const Stretch kp{k_pages, bytes}, vp{v_pages, bytes};
+  const Stretch read[] = {{q_weight, 2 * (int64_t)head_dim}, {k_weight, 2 * (int64_t)head_dim}, {rotary ? cos_sin : nullptr, 4 * (int64_t)num_positions * rotary},
+                          {table, 4 * (int64_t)rows * table_width}, {starts, 4 * (int64_t)rows}, {cu, 4 * ((int64_t)rows + 1)}};
+  for (const Stretch& x : read)
+    if (!apart(qo, tokens, x) || !apart(kp, x) || !apart(vp, x)) return HQ_ERR_BAD_SHAPE;
+  for (const Region& x : {qi, ki, vi, qo})
+    if (!apart(x, tokens, kp) || !apart(x, tokens, vp)) return HQ_ERR_BAD_SHAPE;
+  if (!apart(kp, vp)) return HQ_ERR_BAD_SHAPE;
   const HqDevice* dev = nullptr;
   const int dc = hq_current_device(&dev);
   if (dc != HQ_OK) return dc;
