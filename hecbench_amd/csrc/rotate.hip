@@ -256,11 +256,11 @@ int64_t bytes_of_pages(int pages, int heads, int page, int head_dim) {
   return (int64_t)std::min((double)(1ll << 60), 2.0 * pages * heads * page * head_dim);
 }
 
-int check(int dtype, int head_dim, int rotary, int num_positions, const float* cos_sin, int64_t tokens, int heads, int kv_heads, float eps) {
+int check(int dtype, int head_dim, int rotary, int num_positions, const float* cos_sin, int64_t tokens, int heads, int kv_heads, bool normed, float eps) {
   if (tokens < 0 || heads < 1 || kv_heads < 1 || num_positions < 0 || rotary < 0 || rotary % 16 || rotary > head_dim) return HQ_ERR_BAD_SHAPE;
   if (head_dim != 64 && head_dim != 128) return HQ_ERR_BAD_SHAPE;
   if (dtype != HQ_DTYPE_F16 && dtype != HQ_DTYPE_BF16) return HQ_ERR_BAD_ENUM;
-  if (!(eps >= 0x1p-126f) || std::isinf(eps)) return HQ_ERR_BAD_SHAPE;
+  if (normed && (!(eps >= 0x1p-126f) || std::isinf(eps))) return HQ_ERR_BAD_SHAPE;
   if (rotary && num_positions == 0 && tokens) return HQ_ERR_BAD_SHAPE;
   if (rotary && tokens && !cos_sin) return HQ_ERR_NULL_POINTER;
   if (tokens > INT_MAX || heads > 1 << 16 || kv_heads > 1 << 16) return HQ_ERR_TOO_LARGE;
@@ -274,7 +274,7 @@ extern "C" int hq_norm_rotate(const void* q, const void* k, void* q_out, void* k
                               const float* cos_sin, const int32_t* positions, int64_t tokens, int heads, int kv_heads, int head_dim, int rotary,
                               int num_positions, int64_t q_stride, int64_t k_stride, int64_t q_out_stride, int64_t k_out_stride, float eps,
                               int interleaved, void* stream) {
-  const int rc = check(dtype, head_dim, rotary, num_positions, cos_sin, tokens, heads, kv_heads, eps);
+  const int rc = check(dtype, head_dim, rotary, num_positions, cos_sin, tokens, heads, kv_heads, q_weight || k_weight, eps);
   if (rc != HQ_OK) return rc;
   if (tokens == 0) return HQ_OK;
   if (!q || !k || !q_out || !k_out || (rotary && !positions)) return HQ_ERR_NULL_POINTER;
@@ -325,7 +325,7 @@ extern "C" int hq_cache_write_rotated(const void* q, const void* k, const void* 
                                       const int32_t* starts, const int32_t* cu, int rows, int64_t tokens, int table_width, int num_pages,
                                       int page_size, int heads, int kv_heads, int head_dim, int rotary, int num_positions, int64_t q_stride,
                                       int64_t k_stride, int64_t v_stride, int64_t q_out_stride, float eps, int interleaved, void* stream) {
-  const int rc = check(dtype, head_dim, rotary, num_positions, cos_sin, tokens, heads, kv_heads, eps);
+  const int rc = check(dtype, head_dim, rotary, num_positions, cos_sin, tokens, heads, kv_heads, q_weight || k_weight, eps);
   if (rc != HQ_OK) return rc;
   if (rows < 0 || table_width < 0 || num_pages < 0) return HQ_ERR_BAD_SHAPE;
   if (page_size < 1 || page_size > 1024 || (page_size & (page_size - 1))) return HQ_ERR_BAD_SHAPE;

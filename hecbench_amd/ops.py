@@ -201,7 +201,8 @@ def rotary_table(positions, rotary, base=10000.0, device="cuda"):
 
 def norm_rotate(q, k, cos_sin, positions, q_weight=None, k_weight=None, eps=1e-6, interleaved=False, out=None):
     """Heads of queries and keys normed and rotated: each of q [tokens][heads][64 or 128] and k [tokens][kv_heads][head size], fp16 or bf16,
-    becomes x * rsqrt(mean(x^2) + eps) * weight (weight [head size] of their type; None: is not normed), and then its first cos_sin.size(1)
+    becomes x * rsqrt(mean(x^2) + eps) * weight (weight [head size] of their type; None: is not normed; eps at least
+    2 ** -126), and then its first cos_sin.size(1)
     elements (a multiple of 16) are rotated by row positions[t] of cos_sin, cosines and then sines of the angles (rotary_table; a position
     that is not in the table is cut to it): element i against element i + half of them, or, interleaved, 2 i against 2 i + 1.  cos_sin
     None: no rotation.  fp32, one rounding.  q and k may be parts of a fused projection's rows.  Returns (q, k), new tensors or

@@ -399,7 +399,7 @@ int hq_cache_compact(void* pool, int planes, int64_t page_bytes, const int32_t* 
  *   and every pair (a, b) of the first `rotary` elements of y
  *     (a * c - b * s, b * c + a * s)                 c = cos_sin[p][i], s = cos_sin[p][rotary / 2 + i], p = positions[t]
  *   pair i being elements i and i + rotary / 2, or (interleaved != 0) 2 i and 2 i + 1.  rotary a multiple of 16, at most head_dim, 0: none;
- *   cos_sin fp32 [num_positions][rotary]; a position outside it is cut to it; eps finite, 2^-126 at least.  Rows of q, k and the results are
+ *   cos_sin fp32 [num_positions][rotary]; a position outside it is cut to it; eps, where there is a weight, finite and 2^-126 at least.  Rows of q, k and the results are
  *   their strides (elements, multiples of 8) apart; q_out and k_out may be q and k themselves, or other columns of the same rows, and
  *   share no memory with each other or with the inputs otherwise, weights, angles and positions among them (HQ_ERR_BAD_SHAPE).  All data 16-byte aligned.
  * hq_cache_write_rotated: the same for tokens cu[s] ... cu[s+1]-1, at positions starts[s] ... : keys and values go to those tokens of row s
