@@ -193,7 +193,9 @@ def cache_compact(pool, table, refs, out=None):
 def rotary_table(positions, rotary, base=10000.0, device="cuda"):
     """Cosines and sines of a head's angles at positions 0 ... positions - 1, as norm_rotate takes them: fp32 [positions][rotary], the
     cosines of position * base ** (-2 i / rotary), i < rotary / 2, and then their sines.  Angles in 64 bits: in 32, those of far positions
-    are off by thousandths."""
+    are off by thousandths.  rotary: a multiple of 16."""
+    if rotary < 0 or rotary % 16:
+        raise ValueError(f"rotary must be a multiple of 16, got {rotary}")
     half = rotary // 2
     angle = torch.arange(positions, dtype=torch.float64)[:, None] * float(base) ** (-torch.arange(half, dtype=torch.float64) / half)
     return torch.cat([angle.cos(), angle.sin()], 1).float().to(device)
