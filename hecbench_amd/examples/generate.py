@@ -106,6 +106,8 @@ class Server:
         """prompts: embeddings [tokens][hidden] of each; every one is continued `samples` times by `tokens` tokens."""
         self.model, self.samples = model, samples
         self.lengths = [len(p) for p in prompts]
+        if model.angles is not None and max(self.lengths) + tokens > len(model.angles):
+            raise ValueError(f"{max(self.lengths)} tokens and {tokens} more, and the model knows {len(model.angles)} positions")
         rows = len(prompts) * samples
         width = max(self.lengths) // page + tokens // page + 3
         # a prompt's pages once, and for every sample its tail, its tokens and a page to begin
@@ -201,9 +203,10 @@ def main():
     ap.add_argument("--sinks", type=int, default=0, help="first tokens that stay visible behind the window")
     a = ap.parse_args()
     hq.init()
-    model = Decoder(a.layers, rotary=10000.0, window=a.window, sinks=a.sinks)
+    lengths = [200 + 173 * i for i in range(a.prompts)]
+    model = Decoder(a.layers, rotary=10000.0, longest=max(lengths) + max(a.tokens, 2), window=a.window, sinks=a.sinks)
     gen = torch.Generator(device="cuda").manual_seed(2)
-    prompts = [torch.randn((200 + 173 * i, model.hidden), generator=gen, device="cuda").half() for i in range(a.prompts)]
+    prompts = [torch.randn((n, model.hidden), generator=gen, device="cuda").half() for n in lengths]
     Server(model, prompts, a.samples, 2).run(2, piece=a.piece)  # the first calls size the stream's workspace
     server = Server(model, prompts, a.samples, a.tokens)
     torch.cuda.synchronize()
