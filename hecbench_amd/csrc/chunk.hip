@@ -331,17 +331,19 @@ int launch_chunk(ChunkArgs a, int cus, hipStream_t stream) {
   const int64_t cap = (int64_t)a.width << a.page_log, rows = (int64_t)a.total_q * a.ratio, requests = std::min(a.batch, a.total_q);
   const int64_t keys = WINDOW ? std::min(cap, std::min<int64_t>(a.sinks, cap) + a.window + 14 + std::max(kFew, kRows / a.ratio + 2)) : cap;  // of a tile
   const int64_t units = std::max<int64_t>((keys + kUnit - 1) / kUnit, 1), room = share_room(cus, a.kv_heads);
-  // Tiles of many rows, at most, each of whose requests has more than kFew of them; and how many there are if all but a token a request are
-  // theirs.
+  // Tiles of many rows, at most, each of whose requests has more than kFew of them; how many there are if all but a token a request are theirs; and
+  // how many are counted on, all tokens' where one by itself has more than kFew rows (one of 30000 keys, 32 / 1 heads of 128: undivided, as if there
+  // were no tile, 552 us, divided 17.3).
   const int64_t tiles = rows / kRows + std::min(requests, rows / (kFew + 1)), slots = rows / kRows + a.batch;
-  const int64_t likely = (rows - requests * a.ratio + kRows - 1) / kRows;
+  const int64_t of_chunks = (rows - requests * a.ratio + kRows - 1) / kRows;
+  const int64_t likely = a.ratio > kFew ? std::max((rows + kRows - 1) / kRows, requests) : of_chunks;
   // Tiles that a compute unit has one of, at most, and half of them has, or with up to 1024 keys a quarter: undivided and of twice the waves (SIDES
   // in attend.h; 1024 tokens behind 3500, 32 / 8 heads of 128, 93 -> 77 us, 700 86 -> 69, of 64 84 -> 59 and 78 -> 52, behind nothing 28.6 -> 26.5
   // and 23.1 -> 18.1; up to 256 keys 8.6 and 9.6; 640 tokens, which could be divided in three, behind 1000 40 -> 33, 3500 68 and 68, 16000 212 ->
   // 240; 512 behind 500 29.3 -> 23.5, and 256 behind 700 would go 20.5 -> 23.2).  Not beside many requests, which then find no room next to the
   // tiles: 8 of one token beside 900 106 -> 102, 16 of them 111 -> 117, 30 of up to 4000 117 -> 133 (3 of 16000 beside 1000 tokens go 63 -> 77,
   // which the host cannot tell).
-  const bool alone = tiles && units > 2 && (units <= 8 ? 4 : 2) * likely * a.kv_heads > cus && ((rows - requests) / kRows + requests) * a.kv_heads <= cus &&
+  const bool alone = tiles && units > 2 && (units <= 8 ? 4 : 2) * of_chunks * a.kv_heads > cus && ((rows - requests) / kRows + requests) * a.kv_heads <= cus &&
                      4 * requests * a.kv_heads <= cus;
   a.cus = cus;
   a.room = (int)room;
