@@ -11,15 +11,13 @@
 // transposed, S^T = K Q^T: the matrix core leaves a row's scores in one lane and its partner 32 lanes on, so maximum and sum are
 // sums within a lane and one exchange, and the same registers are, rounded, the operand of O^T = V^T P^T without another move: the
 // order of the keys in that sum is free, and the transposing LDS read fetches V's rows in the order in which S^T left them.
-#include <algorithm>
 #pragma once
 
+#include <algorithm>
 #include <cfloat>
 #include <climits>
 #include <cmath>
 #include <type_traits>
-
-#include "hq_internal.h"
 
 #include "hq_internal.h"
 
@@ -115,7 +113,6 @@ __device__ __forceinline__ const P* uniform(const P* p) {
 }
 
 constexpr int kThreads = 256, kWaves = 4;
-
 
 __device__ __forceinline__ int wave_min(int v) {
 #pragma unroll
@@ -573,7 +570,7 @@ struct Many {
       if (j + AHEAD < STEPS) a[j % AHEAD] = operand(j + AHEAD);
 #pragma unroll
       for (int i = j * EACH; i < (j + 1) * EACH; ++i) top = fmaxf(top, n[i / 16][i % 16]);
-            asm volatile("" : "+v"(top));
+      asm volatile("" : "+v"(top));
       __builtin_amdgcn_sched_barrier(0);
     }
     return pair_max(top);
@@ -1233,6 +1230,17 @@ bool bad_scale(float s) { return !(s >= 0.f) || std::isinf(s); }
 // Keys of a row are numbered in 32 bits, as are the ends of loads and shares behind the last one: up to 512 shares rounded up to 128 keys, page
 // numbers up to 2048 keys ahead.
 constexpr int kMostKeys = INT_MAX - (1 << 17);
+// One of the four kernels by type and head size: f of a Form.
+template <typename T_, int D_>
+struct Form {
+  typedef T_ T;
+  static constexpr int D = D_;
+};
+template <typename F>
+int by_type(int dtype, int head_dim, F f) {
+  if (dtype == HQ_DTYPE_F16) return head_dim == 64 ? f(Form<_Float16, 64>()) : f(Form<_Float16, 128>());
+  return head_dim == 64 ? f(Form<__bf16, 64>()) : f(Form<__bf16, 128>());
+}
 bool misaligned(const void* p, int64_t stride) { return ((uintptr_t)p & 15) || stride % 8; }
 
 }  // namespace

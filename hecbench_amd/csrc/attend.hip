@@ -414,7 +414,7 @@ int launch_prompt(PromptArgs a, int cus, hipStream_t stream) {
 // Common keys: a workgroup a compute unit for them, two for heads of 64, and the requests' own keys divided until they fill as many (64
 // requests in 4 groups behind 15000 keys, 32 / 8 heads, own up to 500: heads of 128 72.9 us, with two 78.1; of 64 50.0, with two 43.2).
 // Nothing common: two workgroups a compute unit, of shares by length (Share).
-template <typename T, int D, bool>
+template <typename T, int D>
 int launch_paged(PagedArgs a, int cus, hipStream_t stream) {
   const int64_t cap = (int64_t)a.width << a.page_log, rows = (int64_t)a.batch * a.heads, tiles = a.ratio <= 16 ? 1 : (a.ratio + 127) / 128;
   const int64_t own = (int64_t)a.batch * a.kv_heads * tiles;
@@ -476,11 +476,6 @@ int launch_paged(PagedArgs a, int cus, hipStream_t stream) {
                                       join_paged_kernel<T, D, kWaves, 8>},
                      rows, joined, stream, a);
 }
-
-// One of the four kernels by type and head size.
-#define HQ_BY_TYPE(fn, window, ...)                                                                                     \
-  (dtype == HQ_DTYPE_F16 ? (head_dim == 64 ? fn<_Float16, 64, window>(__VA_ARGS__) : fn<_Float16, 128, window>(__VA_ARGS__)) \
-                         : (head_dim == 64 ? fn<__bf16, 64, window>(__VA_ARGS__) : fn<__bf16, 128, window>(__VA_ARGS__)))
 }  // namespace
 
 // window 0: none.
@@ -507,8 +502,11 @@ static int prompt_attention(const void* q, const void* k, const void* v, void* o
   const PromptArgs a{q, k, v, out, cu_q, cu_k ? cu_k : cu_q, q_stride, k_stride, v_stride, nullptr, nullptr, seqs, (int)total_q, (int)total_k, heads, kv_heads,
                      heads / kv_heads, causal != 0, 1, exponent_scale(scale), window, sinks};
   const hipStream_t s = (hipStream_t)stream;
-  if (window && window < total_k) return HQ_BY_TYPE(launch_prompt, true, a, dev->cus, s);
-  return HQ_BY_TYPE(launch_prompt, false, a, dev->cus, s);
+  return by_type(dtype, head_dim, [&](auto f) {
+    typedef decltype(f) F;
+    if (window && window < total_k) return launch_prompt<typename F::T, F::D, true>(a, dev->cus, s);
+    return launch_prompt<typename F::T, F::D, false>(a, dev->cus, s);
+  });
 }
 
 extern "C" int hq_prompt_attention(const void* q, const void* k, const void* v, void* out, int dtype, const int32_t* cu_q,
@@ -569,5 +567,5 @@ extern "C" int hq_paged_attention(const void* q, const void* k_pages, const void
   a.kv_heads = kv_heads;
   a.ratio = heads / kv_heads;
   a.c = exponent_scale(scale);
-  return HQ_BY_TYPE(launch_paged, false, a, dev->cus, (hipStream_t)stream);
+  return by_type(dtype, head_dim, [&](auto f) { return launch_paged<typename decltype(f)::T, decltype(f)::D>(a, dev->cus, (hipStream_t)stream); });
 }

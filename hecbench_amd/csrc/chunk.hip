@@ -397,10 +397,6 @@ int launch_chunk(ChunkArgs a, int cus, hipStream_t stream) {
     return hq_launch_as_is(join_chunk_kernel<T, D, 1, 0>, dim3((unsigned)((all + kWaves - 1) / kWaves)), dim3(kThreads), 0, stream, a);
   return hq_launch_as_is(join_chunk_kernel<T, D, kWaves, 8>, dim3((unsigned)all), dim3(kThreads), 0, stream, a);
 }
-#define HQ_BY_TYPE(fn, window, ...)                                                                                     \
-  (dtype == HQ_DTYPE_F16 ? (head_dim == 64 ? fn<_Float16, 64, window>(__VA_ARGS__) : fn<_Float16, 128, window>(__VA_ARGS__)) \
-                         : (head_dim == 64 ? fn<__bf16, 64, window>(__VA_ARGS__) : fn<__bf16, 128, window>(__VA_ARGS__)))
-
 }  // namespace
 
 extern "C" int hq_chunk_attention(const void* q, const void* k_pages, const void* v_pages, void* out, int dtype, const int32_t* table,
@@ -447,6 +443,9 @@ extern "C" int hq_chunk_attention(const void* q, const void* k_pages, const void
   a.sinks = sinks;
   a.c = exponent_scale(scale);
   const hipStream_t s = (hipStream_t)stream;
-  if (window && window < (int64_t)table_width * page_size) return HQ_BY_TYPE(launch_chunk, true, a, dev->cus, s);
-  return HQ_BY_TYPE(launch_chunk, false, a, dev->cus, s);
+  return by_type(dtype, head_dim, [&](auto f) {
+    typedef decltype(f) F;
+    if (window && window < (int64_t)table_width * page_size) return launch_chunk<typename F::T, F::D, true>(a, dev->cus, s);
+    return launch_chunk<typename F::T, F::D, false>(a, dev->cus, s);
+  });
 }

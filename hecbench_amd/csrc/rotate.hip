@@ -35,7 +35,7 @@ struct RotateArgs {
   int rows, width, pages, page_log, interleaved;
   float eps;
   int q_sets, k_sets;          // sets of heads
-  unsigned sets, reciprocal;   // of a token, all; 2^32 / sets, rounded up
+  unsigned sets, reciprocal;   // of a token, all, two at least; 2^32 / sets, rounded up
 };
 
 template <typename T>
@@ -91,7 +91,7 @@ template <typename T, int D, bool CACHE>
 __global__ __launch_bounds__(kThreads) void rotate_kernel(RotateArgs a) {
   constexpr int LANES = D / 16, HEADS = 64 / LANES, CH = D / 8;
   const unsigned wave = __builtin_amdgcn_readfirstlane(blockIdx.x * kWaves + (threadIdx.x >> 6));
-  unsigned token = a.sets == 1 ? wave : __umulhi(wave, a.reciprocal);  // or one more
+  unsigned token = __umulhi(wave, a.reciprocal);  // or one more
   if (token * a.sets > wave) --token;
   const int t = token, set = wave - token * a.sets;
   if (t >= a.tokens) return;
