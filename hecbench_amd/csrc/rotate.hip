@@ -236,7 +236,7 @@ bool apart(const Region& x, const Region& y, int64_t tokens, bool same) {
   return d >= (uint64_t)x.bytes && d + (uint64_t)y.bytes <= (uint64_t)x.stride;
 }
 
-// One stretch of memory.  Two of them, and one and rows, have nothing in common, not even in the gaps between the rows' bytes.
+// One stretch of memory; apart from another, or from rows, of which what lies in the gaps between them is apart too.
 struct Stretch {
   const void* p;
   int64_t bytes;
